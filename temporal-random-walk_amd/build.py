@@ -4,6 +4,8 @@ Produces, inside ``temporal-random-walk_amd/temporal_random_walk/``:
 
 * ``libtrw_engine.so`` -- the HIP engine (gfx950 code objects) behind the
   C ABI of ``include/trw_engine.h``;
+* ``libtrw_operators.so`` -- the operators on walks (attention, its
+  single-event form, the distance bias) behind ``include/trw_operators.h``;
 * ``_temporal_random_walk*.so`` -- the pybind11 module that mirrors the
   reference's Python surface on top of the C++ ``TemporalRandomWalk`` class,
   which calls the C ABI;
@@ -47,6 +49,8 @@ HIP_FLAGS = [
 ]
 
 HIP_SOURCES = ["primitives.hip", "build.hip", "walk.hip", "handoff.hip", "pickers.hip", "capi.hip"]
+OPERATOR_SOURCES = ["walk_mask.hip", "attention.hip", "attention_backward.hip",
+                    "attention_step.hip", "relative_bias.hip", "operators_capi.hip"]
 PROBE_DIR = os.path.join(PKG_ROOT, "probe")
 
 
@@ -59,7 +63,7 @@ def _run(cmd):
     return out
 
 
-def build_engine() -> str:
+def _compile(sources):
     os.makedirs(BUILD_DIR, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
 
@@ -68,11 +72,35 @@ def build_engine() -> str:
         _run([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj])
         return obj
 
-    with ThreadPoolExecutor(max_workers=min(6, len(HIP_SOURCES))) as ex:
-        objs = list(ex.map(compile_one, HIP_SOURCES))
+    with ThreadPoolExecutor(max_workers=min(6, len(sources))) as ex:
+        return list(ex.map(compile_one, sources))
+
+
+def build_engine() -> str:
+    objs = _compile(HIP_SOURCES)
     lib = os.path.join(OUT_DIR, "libtrw_engine.so")
     tmp = lib + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", *objs, "-o", tmp])
+    os.replace(tmp, lib)
+    return lib
+
+
+def build_operators() -> str:
+    """The operators' library.  They run on the caller's streams, which belong
+    to one copy of the HIP runtime: the one that PyTorch loads from its own
+    folder under the name libamdhip64.so.  The library asks for that name (a
+    stub that carries it stands in at link time), not for the versioned one
+    that the engine names and that would bring in the system's copy beside
+    PyTorch's.  Without PyTorch, /opt/rocm/lib has the name too."""
+    objs = _compile(OPERATOR_SOURCES)
+    stub = os.path.join(BUILD_DIR, "stub", "libamdhip64.so")
+    os.makedirs(os.path.dirname(stub), exist_ok=True)
+    _run(["g++", "-shared", "-nostdlib", "-x", "c", "/dev/null", "-Wl,-soname,libamdhip64.so",
+          "-o", stub])
+    lib = os.path.join(OUT_DIR, "libtrw_operators.so")
+    tmp = lib + ".tmp"
+    _run(["g++", "-shared", "-fPIC", *objs, "-Wl,--no-as-needed", stub, "-Wl,--as-needed",
+          "-Wl,-rpath,/opt/rocm/lib", "-o", tmp])
     os.replace(tmp, lib)
     return lib
 
@@ -110,6 +138,7 @@ def build_probe() -> str:
 
 def build_all() -> None:
     build_engine()
+    build_operators()
     build_python_module()
     build_probe()
 

@@ -1,0 +1,341 @@
+// attention_step.hip -- one new event of each walk over its cache.
+//
+// Per walk and key head: read the cache once, at memory speed.  The query
+// heads that share a key head are the columns of the products (up to 32 of
+// them; the matrix instructions are idle most of the time either way), a wave
+// takes blocks of 32 positions, and four waves and, where walks are few, many
+// workgroups share a walk: each keeps a maximum, a sum and an output of its
+// own, joined at the end.  Positions past the walk's length are never read.
+//
+// The new key and value are taken from the call's arguments, not from the
+// cache, by the workgroup whose positions include them, and written to the
+// cache by the walk's first workgroup: no launch and no wait between the two.
+#include "operators.h"
+
+namespace trw {
+namespace ops {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kKeys = 32;  // positions of a wave's block
+
+struct StepArgs {
+    Rows q, k, v, out;
+    char *k_cache, *v_cache;
+    int64_t k_batch, k_pos, k_head, v_batch, v_pos, v_head;
+    const int64_t* lens;
+    float* k_times;
+    Score score;
+    int64_t capacity;
+    int batch, heads, kv_heads, group, columns, dim, splits;
+    float* partial;  // [batch, heads, splits, dim]
+    float2* part_stats;  // [batch, heads, splits]
+};
+
+// Rows first .. of a cache [positions, dim] into registers; row `last` is the
+// call's own; rows past it are zeros.
+template <typename T, int DB>
+struct CacheRows {
+    typedef Tile<T, DB> G;
+    static constexpr int kMine = kKeys * G::kUsed / 64;
+    u32x4 r[kMine];
+    __device__ __forceinline__ void load(const T* cache, int64_t stride, const T* fresh, int dim,
+                                         int64_t first, int64_t last, int lane) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int at = lane + n * 64;
+            const int64_t row = first + at / G::kUsed;
+            const int col = (at % G::kUsed) * G::kElems;
+            const T* from = row == last ? fresh : cache + row * stride;
+            r[n] = row <= last && col < dim ? *reinterpret_cast<const u32x4*>(from + col)
+                                            : u32x4{0, 0, 0, 0};
+        }
+    }
+    __device__ __forceinline__ void store(u32x4* lds, int lane) const {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int at = lane + n * 64;
+            lds[G::slot(at / G::kUsed, at % G::kUsed)] = r[n];
+        }
+    }
+};
+
+template <typename T, int DB>
+__global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
+    typedef Tile<T, DB> G;
+    constexpr size_t kTileBytes = G::bytes(kKeys);
+    constexpr size_t kJoinBytes = kWaves * 32 * 33 * sizeof(float);
+    constexpr size_t kBytes = kWaves * kTileBytes > kJoinBytes ? kWaves * kTileBytes : kJoinBytes;
+    __shared__ u32x4 s_mem[kBytes / 16];
+    __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+
+    const int split = blockIdx.x % a.splits;
+    int rest = blockIdx.x / a.splits;
+    const int col_group = rest % a.columns;
+    rest /= a.columns;
+    const int kv_head = rest % a.kv_heads;
+    const int b = rest / a.kv_heads;
+    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, half = lane >> 5;
+    const Score& sc = a.score;
+
+    const int64_t n = a.lens[b];  // position of the new event
+    const bool idle = n < 0 || n >= a.capacity;
+    const int col = col_group * 32 + (lane & 31);
+    const int head = kv_head * a.group + col;
+    const bool any = !idle && col < a.group;
+    const T* fresh_k = row_of<const T>(a.k, b, kv_head);
+    const T* fresh_v = row_of<const T>(a.v, b, kv_head);
+    T* cache_k = reinterpret_cast<T*>(a.k_cache) + b * a.k_batch + kv_head * a.k_head;
+    T* cache_v = reinterpret_cast<T*>(a.v_cache) + b * a.v_batch + kv_head * a.v_head;
+    const float q_time = sc.q_times ? sc.q_times[b] : 0.0f;
+
+    if (!idle && split == 0 && col_group == 0) {
+        constexpr int kElems = G::kElems;
+        const int at = thread * kElems;
+        if (at < a.dim) {
+            *reinterpret_cast<u32x4*>(cache_k + n * a.k_pos + at) =
+                *reinterpret_cast<const u32x4*>(fresh_k + at);
+            *reinterpret_cast<u32x4*>(cache_v + n * a.v_pos + at) =
+                *reinterpret_cast<const u32x4*>(fresh_v + at);
+        }
+        if (a.k_times && kv_head == 0 && thread == 0) a.k_times[b * a.capacity + n] = q_time;
+    }
+
+    // this workgroup's blocks of positions
+    const int64_t blocks = idle ? 0 : n / kKeys + 1;
+    const int64_t block_begin = blocks * split / a.splits;
+    const int64_t block_end = blocks * (split + 1) / a.splits;
+
+    Frag<T> q[G::kSteps];
+    load_operand<T, DB>(q, row_of<const T>(a.q, b, any ? head : 0), any, a.dim, half);
+    const float slope = sc.slopes && any ? sc.slopes[head] * kLog2e : 0.0f;
+    const float far_bias = sc.table && any ? table_entry(sc, head, 2 * sc.reach) : 0.0f;
+    const float* k_times = sc.k_times ? sc.k_times + b * a.capacity : nullptr;
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int c = 0; c < DB; ++c) o[c] = zero16();
+    float m = kFloor, l = 0.0f;
+    u32x4* s_tile = s_mem + wave * (kTileBytes / 16);
+    CacheRows<T, DB> k, v;
+    int64_t block = block_begin + wave;
+    if (block < block_end) {
+        k.load(cache_k, a.k_pos, fresh_k, a.dim, block * kKeys, n, lane);
+        v.load(cache_v, a.v_pos, fresh_v, a.dim, block * kKeys, n, lane);
+    }
+    for (; block < block_end; block += kWaves) {
+        const int64_t j0 = block * kKeys;
+        const bool more = block + kWaves < block_end;
+        const int64_t j1 = j0 + kWaves * kKeys;
+        k.store(s_tile, lane);
+        if (more) k.load(cache_k, a.k_pos, fresh_k, a.dim, j1, n, lane);
+        f32x16 x = zero16();
+#pragma unroll
+        for (int st = 0; st < G::kSteps; ++st) x = mma(G::row(s_tile, lane & 31, st, half), q[st], x);
+        float s[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float unused;
+            s[r] = sc.softcap > 0 ? capped<T>(sc, x[r], unused) : x[r] * sc.scale2;
+        }
+        // distances from the new event of register r's position: last_d - acc_row(r)
+        const int64_t last_d = n - j0 - 4 * half;
+        if (sc.table) {
+            if (n - (j0 + kKeys - 1) >= sc.reach) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] += far_bias;
+            } else if (any) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t d = min(max(last_d - acc_row(r), int64_t{0}), int64_t{sc.reach});
+                    s[r] += table_entry(sc, head, static_cast<int>(d) + sc.reach);
+                }
+            }
+        }
+        if (sc.slopes) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float gap = static_cast<float>(last_d - acc_row(r));
+                if (k_times)
+                    gap = last_d > acc_row(r) ? q_time - k_times[n - (last_d - acc_row(r))] : 0.0f;
+                s[r] = fmaf(-slope, fabsf(gap), s[r]);
+            }
+        }
+        if (j0 + kKeys > n + 1) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (acc_row(r) > last_d) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m)) {
+            const float grown = fmaxf(m, top);
+            const float by = exp2_fast(m - grown);
+            m = grown;
+            l *= by;
+#pragma unroll
+            for (int c = 0; c < DB; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[c][r] *= by;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2_fast(s[r] - m);
+            l += s[r];
+        }
+        v.store(s_tile, lane);
+        if (more) v.load(cache_v, a.v_pos, fresh_v, a.dim, j1, n, lane);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            Frag<T> p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = static_cast<T>(s[8 * t + e]);
+#pragma unroll
+            for (int c = 0; c < DB; ++c) o[c] = mma(G::columns(s_tile, 16 * t, c, lane), p, o[c]);
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    // join the waves
+    if (half == 0) {
+        s_m[wave][lane] = m;
+        s_l[wave][lane] = l;
+    }
+    __syncthreads();  // also: the tiles are done with
+    float* s_join = reinterpret_cast<float*>(s_mem);
+    const int jc = thread >> 3, jd = (thread & 7) * 4;  // a column and four of its elements
+    float top = s_m[0][jc], by[kWaves], total = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][jc]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        by[w] = exp2_fast(s_m[w][jc] - top);
+        total += by[w] * s_l[w][jc];
+    }
+    const int join_col = col_group * 32 + jc;
+    const int join_head = kv_head * a.group + join_col;
+    const int64_t part = (static_cast<int64_t>(b) * a.heads + join_head) * a.splits + split;
+    const float scale = a.splits > 1 ? 1.0f : 1.0f / total;
+#pragma unroll
+    for (int c = 0; c < DB; ++c) {
+        if (c) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            s_join[(wave * 32 + (lane & 31)) * 33 + acc_row(r) + 4 * half] = o[c][r];
+        __syncthreads();
+        const int d = 32 * c + jd;
+        if (join_col < a.group && d < a.dim) {
+            f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    sum[e] = fmaf(by[w], s_join[(w * 32 + jc) * 33 + jd + e], sum[e]);
+            if (a.splits > 1) {
+                *reinterpret_cast<f32x4*>(a.partial + part * a.dim + d) = sum;
+            } else {
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                t4 out;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float value = n < 0 ? 0.0f : idle ? NAN : sum[e] * scale;
+                    out[e] = static_cast<T>(value);
+                }
+                *reinterpret_cast<t4*>(row_of<T>(a.out, b, join_head) + d) = out;
+            }
+        }
+    }
+    if (a.splits > 1 && jd == 0 && join_col < a.group)
+        a.part_stats[part] = make_float2(top, total);
+}
+
+// Joins the workgroups of one walk and head: a thread for each element.
+template <typename T>
+__global__ __launch_bounds__(128) void join_step_kernel(StepArgs a) {
+    const int head = blockIdx.x % a.heads;
+    const int b = blockIdx.x / a.heads;
+    const int d = threadIdx.x;
+    const int64_t part = (static_cast<int64_t>(b) * a.heads + head) * a.splits;
+    float top = kFloor;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[part + s].x);
+    float total = 0.0f, sum = 0.0f;
+    if (d < a.dim)
+        for (int s = 0; s < a.splits; ++s) {
+            const float2 st = a.part_stats[part + s];
+            const float by = exp2_fast(st.x - top);
+            total = fmaf(by, st.y, total);
+            sum = fmaf(by, a.partial[(part + s) * a.dim + d], sum);
+        }
+    if (d >= a.dim) return;
+    const int64_t n = a.lens[b];
+    const float value = n < 0 ? 0.0f : n >= a.capacity ? NAN : sum / total;
+    row_of<T>(a.out, b, head)[d] = static_cast<T>(value);
+}
+
+// Workgroups of one walk and key head: enough for four on each of the 256
+// compute units, each with at least four blocks a wave where the cache is full.
+int splits_of(const trw_attention_step_params& p) {
+    const int group = p.heads / p.kv_heads;
+    const int64_t items = p.batch * p.kv_heads * ((group + 31) / 32);
+    const int64_t most = (p.capacity + 4 * kWaves * kKeys - 1) / (4 * kWaves * kKeys);
+    const int64_t want = (1024 + items - 1) / (items > 0 ? items : 1);
+    return static_cast<int>(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+}
+
+}  // namespace
+
+uint64_t attention_step_workspace(const trw_attention_step_params& p) {
+    const int splits = splits_of(p);
+    if (splits == 1) return 0;
+    return static_cast<uint64_t>(p.batch) * p.heads * splits * (p.dim + 2) * sizeof(float);
+}
+
+void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
+    if (p.batch == 0) return;
+    require(p.workspace_bytes >= attention_step_workspace(p), "workspace is too small");
+    StepArgs a;
+    a.q = make_rows(p.q);
+    a.k = make_rows(p.k);
+    a.v = make_rows(p.v);
+    a.out = make_rows(p.out);
+    a.k_cache = static_cast<char*>(p.k_cache);
+    a.v_cache = static_cast<char*>(p.v_cache);
+    a.k_batch = p.k_batch_stride;
+    a.k_pos = p.k_pos_stride;
+    a.k_head = p.k_head_stride;
+    a.v_batch = p.v_batch_stride;
+    a.v_pos = p.v_pos_stride;
+    a.v_head = p.v_head_stride;
+    a.lens = p.lens;
+    a.k_times = const_cast<float*>(p.score.k_times);
+    a.score = make_score(p.score);
+    a.capacity = p.capacity;
+    a.batch = static_cast<int>(p.batch);
+    a.heads = p.heads;
+    a.kv_heads = p.kv_heads;
+    a.group = p.heads / p.kv_heads;
+    a.columns = (a.group + 31) / 32;
+    a.dim = p.dim;
+    a.splits = splits_of(p);
+    a.partial = static_cast<float*>(p.workspace);
+    a.part_stats = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(p.batch) * p.heads *
+                                                             a.splits * p.dim);
+    const int64_t grid = p.batch * p.kv_heads * a.columns * a.splits;
+    require(grid < (int64_t{1} << 31), "too many walks and heads");
+    dispatch(p.dtype, p.dim, [&](auto t, auto db) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((attention_step_kernel<T, decltype(db)::value>),
+                           dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+        check_launch("attention_step");
+        if (a.splits > 1)
+            hipLaunchKernelGGL((join_step_kernel<T>), dim3(static_cast<unsigned>(a.batch * a.heads)),
+                               dim3(128), 0, stream, a);
+        check_launch("attention_step");
+    });
+}
+
+}  // namespace ops
+}  // namespace trw

@@ -1,0 +1,390 @@
+// operators.h -- what the operator kernels share: element types, matrix
+// instructions, tiles in LDS, scores.
+//
+// All attention kernels hold the matrix products the same way round.  A wave
+// owns 32 columns (query rows in the forward and dQ kernels, keys in the dK/dV
+// kernel), one per lane of each half wave, whose vectors stay in registers as
+// the B operand; the other side's rows pass through LDS and are the A operand.
+// v_mfma_f32_32x32x16 then leaves lane l with 16 rows of column l & 31 (and
+// lane l ^ 32 with the other 16), so a softmax over rows is a sum over a
+// lane's own registers and one exchange with lane l ^ 32, and the 16 values
+// are, two by two, the B operand of the next product without moving: register
+// 8 t + e is row 16 t + 8 (e / 4) + 4 (l / 32) + e % 4, and the A operand of
+// that product is read from LDS in the same order of rows.
+#ifndef TRW_OPERATORS_KERNELS_H
+#define TRW_OPERATORS_KERNELS_H
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "trw_operators.h"
+
+namespace trw {
+namespace ops {
+
+struct InvalidArgument : std::invalid_argument {
+    using std::invalid_argument::invalid_argument;
+};
+inline void require(bool ok, const char* message) {
+    if (!ok) throw InvalidArgument(message);
+}
+inline void check_launch(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// Where a running maximum starts: below every finite score (scores are clamped
+// to kLowest), above the -inf of masked ones, so that exp2(score - maximum) is
+// 0 for those and never NaN.
+constexpr float kFloor = -3.0e38f;
+constexpr float kLowest = -1.0e38f;
+
+// Eight values of one lane: one operand of a product over 16.
+template <typename T>
+struct Lane8;
+template <>
+struct Lane8<__bf16> {
+    typedef bf16x8 vec;
+};
+template <>
+struct Lane8<_Float16> {
+    typedef f16x8 vec;
+};
+template <>
+struct Lane8<float> {
+    typedef f32x8 vec;
+};
+template <typename T>
+using Frag = typename Lane8<T>::vec;
+
+// c += A B over 16: lane l holds elements 8 (l / 32) .. + 8 of row (column)
+// l & 31 of A (B).
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Row of accumulator register r: 8 (r / 4) + 4 (lane / 32) + r % 4.
+__device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// ---- tiles of rows in LDS --------------------------------------------------------------------
+//
+// Rows of 32, 64 or 128 elements as 16-byte chunks, chunk c of row r in slot
+// c ^ swizzle(r) of the row.  Both ways the tiles are read then touch every
+// bank once: 16 consecutive rows' chunk c (row reads) lie in 16 slots of the
+// 256 bytes that the banks span, and so do 4 consecutive rows' 64-byte pieces
+// (transposing reads).
+template <typename T, int DB>
+struct Tile {
+    static constexpr int kElems = 16 / sizeof(T);  // of a chunk
+    static constexpr int kWidth = DB == 1 ? 32 : DB == 2 ? 64 : 128;
+    static constexpr int kSlots = kWidth / kElems;    // per row
+    static constexpr int kUsed = DB * 32 / kElems;    // chunks per row that are read
+    static constexpr int kSteps = DB * 2;             // products over 16 in a row
+
+    static constexpr size_t bytes(int rows) { return size_t(rows) * kSlots * 16; }
+
+    __device__ static __forceinline__ int swizzle(int r) {
+        if (kSlots == 4) return (r >> 2) & 3;
+        if (kSlots == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+    __device__ static __forceinline__ int slot(int row, int chunk) {
+        return row * kSlots + (chunk ^ swizzle(row));
+    }
+
+    // Elements 16 step + 8 half .. + 8 of a row.
+    __device__ static __forceinline__ Frag<T> row(const u32x4* lds, int row, int step, int half) {
+        union {
+            u32x4 u[sizeof(T) / 2];
+            Frag<T> f;
+        } x;
+        if constexpr (sizeof(T) == 2) {
+            x.u[0] = lds[slot(row, 2 * step + half)];
+        } else {
+            x.u[0] = lds[slot(row, 4 * step + 2 * half)];
+            x.u[1] = lds[slot(row, 4 * step + 2 * half + 1)];
+        }
+        return x.f;
+    }
+
+    // The transposed operand: column 32 block + (lane & 31) of the rows first
+    // + 8 (e / 4) + 4 (lane / 32) + e % 4, e = 0..7 -- the order in which an
+    // accumulator's registers hold them.
+    __device__ static __forceinline__ Frag<T> columns(const u32x4* lds, int first, int block,
+                                                      int lane) {
+        if constexpr (sizeof(T) == 2) {
+            // Each group of 16 lanes reads 4 rows of 16 columns, lane s
+            // addressing columns 4 (s % 4) .. + 4 of row s / 4, and receives
+            // its own column of the 4 rows.
+            const int s = lane & 15;
+            const int r = first + 4 * (lane >> 5) + (s >> 2);
+            const int col = 32 * block + 16 * ((lane >> 4) & 1) + 4 * (s & 3);
+            union {
+                s16x4 s[2];
+                Frag<T> f;
+            } x;
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const char* at = reinterpret_cast<const char*>(lds);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int byte = slot(r + 8 * h, col >> 3) * 16 + (col & 7) * 2;
+                x.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds4)(const_cast<char*>(at) + byte));
+            }
+            return x.f;
+        } else {
+            const float* at = reinterpret_cast<const float*>(lds);
+            const int col = 32 * block + (lane & 31);
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = first + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                f[e] = at[slot(r, col >> 2) * 4 + (col & 3)];
+            }
+            return f;
+        }
+    }
+};
+
+// A tile on its way from global memory to LDS: kRows rows over kThreads
+// threads, in registers, so that the loads of one tile run beside the products
+// of the tile before it.
+template <typename T, int DB, int kRows, int kThreads>
+struct Staged {
+    typedef Tile<T, DB> G;
+    static constexpr int kChunks = kRows * G::kUsed;
+    static constexpr int kMine = (kChunks + kThreads - 1) / kThreads;
+    u32x4 r[kMine];
+
+    // Rows first .. of [rows, dim]; rows outside [begin, end) and columns from
+    // dim on are zeros.
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int dim, int first,
+                                         int begin, int end, int thread) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int i = thread + n * kThreads;
+            const int row = first + i / G::kUsed;
+            const int col = (i % G::kUsed) * G::kElems;
+            const bool in = (kChunks % kThreads == 0 || i < kChunks) && row >= begin &&
+                            row < end && col < dim;
+            r[n] = in ? *reinterpret_cast<const u32x4*>(base + row * row_stride + col)
+                      : u32x4{0, 0, 0, 0};
+        }
+    }
+    __device__ __forceinline__ void store(u32x4* lds, int thread) const {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int i = thread + n * kThreads;
+            if (kChunks % kThreads == 0 || i < kChunks)
+                lds[G::slot(i / G::kUsed, i % G::kUsed)] = r[n];
+        }
+    }
+};
+
+// A row of global memory as B operands: lane's elements 16 s + 8 half .. + 8
+// for every step s; zeros where `in` is false and from column dim on.
+template <typename T, int DB>
+__device__ __forceinline__ void load_operand(Frag<T> (&f)[2 * DB], const T* row, bool in, int dim,
+                                             int half) {
+#pragma unroll
+    for (int s = 0; s < 2 * DB; ++s) {
+        union {
+            u32x4 u[sizeof(T) / 2];
+            Frag<T> f;
+        } x;
+        const int col = 16 * s + 8 * half;
+#pragma unroll
+        for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h)
+            x.u[h] = in && col < dim
+                         ? *reinterpret_cast<const u32x4*>(row + col + h * (16 / sizeof(T)))
+                         : u32x4{0, 0, 0, 0};
+        f[s] = x.f;
+    }
+}
+
+// Writes a column's accumulators (rows of the transposed product = elements of
+// the row) as a row of global memory, times `by`.
+template <typename T, int DB>
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], float by, int dim,
+                                          int half) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * b + 8 * g + 4 * half;
+            if (col >= dim) continue;
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            t4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(acc[b][4 * g + e] * by);
+            *reinterpret_cast<t4*>(row + col) = v;
+        }
+}
+
+// ---- reductions -------------------------------------------------------------------------------
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x = min(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
+    return x;
+}
+
+// ---- scores -----------------------------------------------------------------------------------
+// What a kernel needs of trw_score, everything in base 2 (exp2 of it is the
+// softmax's numerator).
+struct Score {
+    float scale2;    // scale log2 e
+    float softcap;   // 0: none
+    float cap_in;    // 2 scale log2 e / softcap: tanh(x) = 1 - 2 / (1 + exp2(2 log2 e x))
+    float cap_out;   // softcap log2 e
+    float scale;
+    const float* table;
+    const int32_t* buckets;
+    int num_buckets, reach;
+    const float* slopes;
+    const float *q_times, *k_times;
+};
+
+inline Score make_score(const trw_score& s) {
+    Score r;
+    r.scale = s.scale;
+    r.scale2 = s.scale * kLog2e;
+    r.softcap = s.softcap;
+    r.cap_in = s.softcap > 0 ? 2.0f * kLog2e * s.scale / s.softcap : 0.0f;
+    r.cap_out = s.softcap * kLog2e;
+    r.table = s.table;
+    r.buckets = s.buckets;
+    r.num_buckets = s.num_buckets;
+    r.reach = s.table ? s.reach : 0;
+    r.slopes = s.slopes;
+    r.q_times = s.q_times;
+    r.k_times = s.k_times;
+    return r;
+}
+
+// The biases of distances -reach..reach of one head, in base 2.  The type's
+// lowest value and its like stay finite (a row of nothing else is a uniform
+// row); -inf masks.
+__device__ __forceinline__ float table_entry(const Score& s, int head, int at) {
+    const int b = min(max(s.buckets[at], 0), s.num_buckets - 1);
+    const float raw = s.table[static_cast<int64_t>(head) * s.num_buckets + b];
+    const float t = raw * kLog2e;
+    return raw != -INFINITY && t < kLowest ? kLowest : t;
+}
+__device__ __forceinline__ void fill_bias(float* lut, const Score& s, int head, int thread,
+                                          int threads) {
+    for (int i = thread; i < 2 * s.reach + 1; i += threads) lut[i] = table_entry(s, head, i);
+}
+
+// log2 e softcap tanh(scale x / softcap), and 1 - tanh^2.  The 16-bit types
+// take tanh from exp2 and a reciprocal: its error of some 1e-7 is absolute, far
+// below what their scores carry; float32 calls tanhf.
+template <typename T>
+__device__ __forceinline__ float capped(const Score& s, float x, float& slope) {
+    if constexpr (sizeof(T) == 4) {
+        const float t = tanhf(x * s.scale / s.softcap);
+        slope = 1.0f - t * t;
+        return s.cap_out * t;
+    } else {
+        const float u = __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * s.cap_in));
+        slope = 4.0f * u * (1.0f - u);
+        return fmaf(-2.0f * s.cap_out, u, s.cap_out);
+    }
+}
+
+struct Rows {
+    char* data;
+    int64_t row, head;  // strides in elements
+};
+inline Rows make_rows(const trw_rows& r) {
+    return Rows{static_cast<char*>(r.data), r.row_stride, r.head_stride};
+}
+template <typename T>
+__device__ __forceinline__ T* row_of(const Rows& r, int64_t row, int head) {
+    return reinterpret_cast<T*>(r.data) + row * r.row + head * r.head;
+}
+
+// Consecutive workgroup ids go to the eight XCDs in turn, each with an L2 of
+// its own: XCD x takes the x-th eighth of the items, so that workgroups that
+// read the same keys share one.
+__device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t items) {
+    const int64_t per = (items + 7) / 8;
+    return (id & 7) * per + (id >> 3);
+}
+inline int64_t xcd_grid(int64_t items) { return (items + 7) / 8 * 8; }
+
+// f<T, DB>() for a dtype and a head size.
+template <typename F>
+void dispatch(int dtype, int dim, F&& f) {
+    const int db = (dim + 31) / 32;
+    auto by_dim = [&](auto t) {
+        switch (db) {
+            case 1: f(t, std::integral_constant<int, 1>()); break;
+            case 2: f(t, std::integral_constant<int, 2>()); break;
+            case 3: f(t, std::integral_constant<int, 3>()); break;
+            default: f(t, std::integral_constant<int, 4>()); break;
+        }
+    };
+    if (dtype == TRW_F32)
+        by_dim(float{});
+    else if (dtype == TRW_F16)
+        by_dim(_Float16{});
+    else
+        by_dim(__bf16{});
+}
+
+inline size_t element_size(int dtype) { return dtype == TRW_F32 ? 4 : 2; }
+
+// Implementations behind the C ABI (operators_capi.hip checks the arguments).
+void walk_mask(const trw_walk_mask_params& p, hipStream_t stream);
+uint64_t attention_workspace(const trw_attention_params& p, bool backward);
+void attention_forward(const trw_attention_params& p, hipStream_t stream);
+void attention_backward(const trw_attention_params& p, hipStream_t stream);
+// d_table [heads, num_buckets] of `dtype` from partial [heads, tiles, num_buckets].
+void join_table(const float* partial, int64_t tiles, int heads, int num_buckets, int dtype,
+                void* d_table, hipStream_t stream);
+uint64_t attention_step_workspace(const trw_attention_step_params& p);
+void attention_step(const trw_attention_step_params& p, hipStream_t stream);
+uint64_t relative_bias_workspace(const trw_relative_bias_params& p);
+void relative_bias(const trw_relative_bias_params& p, hipStream_t stream);
+void relative_bias_backward(const trw_relative_bias_params& p, hipStream_t stream);
+
+}  // namespace ops
+}  // namespace trw
+#endif  // TRW_OPERATORS_KERNELS_H
