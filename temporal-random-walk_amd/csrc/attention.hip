@@ -60,8 +60,8 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
     const bool any = lo < hi;
 
     // the wave's and the workgroup's intervals
-    int w_lo = wave_min(any ? lo : INT_MAX), w_hi = wave_max(any ? hi : 0);
-    const int w_diag_lo = wave_min(any ? diag : INT_MAX), w_diag_hi = wave_max(any ? diag : INT_MIN);
+    int w_lo = wave_min(any ? lo : kNone), w_hi = wave_max(any ? hi : 0);
+    const int w_diag_lo = wave_min(any ? diag : kNone), w_diag_hi = wave_max(any ? diag : -kNone);
     const int w_last_lo = wave_max(any ? lo : 0);
     if (lane == 0) {
         s_reduce[wave][0] = w_lo;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
     }
     if (sc.table) fill_bias(s_lut, sc, head, thread, kThreads);
     __syncthreads();
-    int k_begin = INT_MAX, k_end = 0, last_lo = 0;
+    int k_begin = kNone, k_end = 0, last_lo = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         k_begin = min(k_begin, s_reduce[w][0]);
@@ -87,18 +87,19 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
     const T* v_base = row_of<const T>(a.v, 0, kv_head);
 
     int only = -1;  // -1: every row; else the rows whose keys begin there, again
+    int j_first = k_begin;
     for (;;) {
         f32x16 o[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b) o[b] = zero16();
         float m = kFloor, l = 0.0f;
         // Every row must be inside a tile for it to go unmasked
-        const int full_lo = wave_max(any ? lo : INT_MAX), full_hi = wave_min(any ? hi : 0);
+        const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
 
         Staged<T, DB, kKeys, kThreads> next_k, next_v;
-        next_k.load(k_base, a.k.row, a.dim, k_begin, k_begin, k_end, thread);
-        next_v.load(v_base, a.v.row, a.dim, k_begin, k_begin, k_end, thread);
-        for (int j0 = k_begin; j0 < k_end; j0 += kKeys) {
+        next_k.load(k_base, a.k.row, a.dim, j_first, k_begin, k_end, thread);
+        next_v.load(v_base, a.v.row, a.dim, j_first, k_begin, k_end, thread);
+        for (int j0 = j_first; j0 < k_end; j0 += kKeys) {
             __syncthreads();  // the tile before is done with
             next_k.store(s_k, thread);
             next_v.store(s_v, thread);
@@ -213,10 +214,11 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
         l += __shfl_xor(l, 32);
         const bool mine = i < a.q_rows && (only < 0 || (any && info.x == only));
         if (mine) {
-            store_row<T, DB>(row_of<T>(a.out, i, head), o, any ? 1.0f / l : 0.0f, a.dim, half);
+            const bool seen = any && l != 0.0f;  // 0: the bias masks every key
+            store_row<T, DB>(row_of<T>(a.out, i, head), o, seen, 1.0f / l, a.dim, half);
             if (a.stats && half == 0)
                 a.stats[static_cast<int64_t>(head) * a.q_rows + i] =
-                    any ? make_float2(m, __builtin_amdgcn_logf(l)) : make_float2(0.0f, INFINITY);
+                    seen ? make_float2(m, __builtin_amdgcn_logf(l)) : make_float2(0.0f, INFINITY);
         }
         if (!mixed) break;
 
@@ -234,22 +236,23 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
             off = only < 0 ? sum != 0.0f : true;
         }
         if (only < 0 && !__syncthreads_or(off)) break;
-        int w_next = wave_min(any && info.x > only ? info.x : INT_MAX);
+        int w_next = wave_min(any && info.x > only ? info.x : kNone);
         __syncthreads();
         if (lane == 0) s_reduce[wave][0] = w_next;
         __syncthreads();
-        int seg = INT_MAX;
+        int seg = kNone;
 #pragma unroll
         for (int w = 0; w < 4; ++w) seg = min(seg, s_reduce[w][0]);
-        if (seg == INT_MAX) break;
+        if (seg == kNone) break;
         only = seg;
         const bool in_seg = any && info.x == only;
         lo = in_seg ? info.x : 0;
         hi = in_seg ? max(info.x, min(info.y, a.k_rows)) : 0;
-        w_lo = wave_min(in_seg ? lo : INT_MAX);
+        w_lo = wave_min(in_seg ? lo : kNone);
         w_hi = wave_max(in_seg ? hi : 0);
         if (lane == 0) s_reduce[wave][1] = w_hi;
         __syncthreads();
+        j_first += (only - j_first) / kKeys * kKeys;  // the same tiles: the same bits
         k_begin = only;
         k_end = 0;
 #pragma unroll

@@ -83,8 +83,8 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
     int lo = info.x, hi = max(info.x, min(info.y, a.k_rows));
     const int diag = info.z;
     const bool any = lo < hi;
-    int w_lo = wave_min(any ? lo : INT_MAX), w_hi = wave_max(any ? hi : 0);
-    const int w_diag_lo = wave_min(any ? diag : INT_MAX), w_diag_hi = wave_max(any ? diag : INT_MIN);
+    int w_lo = wave_min(any ? lo : kNone), w_hi = wave_max(any ? hi : 0);
+    const int w_diag_lo = wave_min(any ? diag : kNone), w_diag_hi = wave_max(any ? diag : -kNone);
     const int w_last_lo = wave_max(any ? lo : 0);
     if (lane == 0) {
         s_reduce[wave][0] = w_lo;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
         for (int n = thread; n < 8 * line; n += kThreads) s_dyn[line + n] = 0.0f;
     }
     __syncthreads();
-    int k_begin = INT_MAX, k_end = 0, last_lo = 0;
+    int k_begin = kNone, k_end = 0, last_lo = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         k_begin = min(k_begin, s_reduce[w][0]);
@@ -134,15 +134,16 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
     float far_before = 0.0f, far_after = 0.0f;  // dS past the reach, either way
 
     int only = -1;
+    int j_first = k_begin;
     for (;;) {
         f32x16 dq[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b) dq[b] = zero16();
-        const int full_lo = wave_max(any ? lo : INT_MAX), full_hi = wave_min(any ? hi : 0);
+        const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
         Staged<T, DB, kKeys, kThreads> next_k, next_v;
-        next_k.load(k_base, a.k.row, a.dim, k_begin, k_begin, k_end, thread);
-        next_v.load(v_base, a.v.row, a.dim, k_begin, k_begin, k_end, thread);
-        for (int j0 = k_begin; j0 < k_end; j0 += kKeys) {
+        next_k.load(k_base, a.k.row, a.dim, j_first, k_begin, k_end, thread);
+        next_v.load(v_base, a.v.row, a.dim, j_first, k_begin, k_end, thread);
+        for (int j0 = j_first; j0 < k_end; j0 += kKeys) {
             __syncthreads();
             next_k.store(s_k, thread);
             next_v.store(s_v, thread);
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
             }
         }
         if (i < a.q_rows && (only < 0 || (any && info.x == only)))
-            store_row<T, DB>(row_of<T>(a.d_q, i, head), dq, any ? sc.scale : 0.0f, a.dim, half);
+            store_row<T, DB>(row_of<T>(a.d_q, i, head), dq, any, sc.scale, a.dim, half);
         if (!mixed) break;
 
         // As in the forward kernel: what is not finite stays in its walk.
@@ -249,22 +250,23 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
             off = sum != 0.0f;
         }
         if (only < 0 && !__syncthreads_or(off)) break;
-        const int w_next = wave_min(any && info.x > only ? info.x : INT_MAX);
+        const int w_next = wave_min(any && info.x > only ? info.x : kNone);
         __syncthreads();
         if (lane == 0) s_reduce[wave][0] = w_next;
         __syncthreads();
-        int seg = INT_MAX;
+        int seg = kNone;
 #pragma unroll
         for (int w = 0; w < 4; ++w) seg = min(seg, s_reduce[w][0]);
-        if (seg == INT_MAX) break;
+        if (seg == kNone) break;
         only = seg;
         const bool in_seg = any && info.x == only;
         lo = in_seg ? info.x : 0;
         hi = in_seg ? max(info.x, min(info.y, a.k_rows)) : 0;
-        w_lo = wave_min(in_seg ? lo : INT_MAX);
+        w_lo = wave_min(in_seg ? lo : kNone);
         w_hi = wave_max(in_seg ? hi : 0);
         if (lane == 0) s_reduce[wave][1] = w_hi;
         __syncthreads();
+        j_first += (only - j_first) / kKeys * kKeys;  // the same tiles: the same bits
         k_begin = only;
         k_end = 0;
 #pragma unroll
@@ -337,15 +339,15 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
     int first = info.x, last = max(info.x, min(info.y, a.q_rows));
     const bool any = first < last;
     const int doc = last;  // no two walks with pairs end at one query
-    int w_lo = wave_min(any ? first : INT_MAX), w_hi = wave_max(any ? last : 0);
-    const int w_first_doc = wave_min(any ? doc : INT_MAX);
+    int w_lo = wave_min(any ? first : kNone), w_hi = wave_max(any ? last : 0);
+    const int w_first_doc = wave_min(any ? doc : kNone);
     if (lane == 0) {
         s_reduce[wave][0] = w_lo;
         s_reduce[wave][1] = w_hi;
         s_reduce[wave][2] = w_first_doc;
     }
     __syncthreads();
-    int q_begin = INT_MAX, q_end = 0, first_doc = INT_MAX;
+    int q_begin = kNone, q_end = 0, first_doc = kNone;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         q_begin = min(q_begin, s_reduce[w][0]);
@@ -363,6 +365,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
     const int head_end = min(head_begin + heads_each, (kv_head + 1) * a.group);
 
     int only = -1;
+    int i_first = q_begin;
     for (;;) {
         f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
             dk[b] = zero16();
             dv[b] = zero16();
         }
-        const int full_lo = wave_max(any ? first : INT_MAX), full_hi = wave_min(any ? last : 0);
+        const int full_lo = wave_max(any ? first : kNone), full_hi = wave_min(any ? last : 0);
         for (int head = head_begin; head < head_end; ++head) {
             const T* q_base = row_of<const T>(a.q, 0, head);
             const T* do_base = row_of<const T>(a.d_out, 0, head);
@@ -381,9 +384,9 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
                 fill_bias(s_lut, sc, head, thread, kThreads);
             }
             Staged<T, DB, kRows, kThreads> next_q, next_do;
-            next_q.load(q_base, a.q.row, a.dim, q_begin, q_begin, q_end, thread);
-            next_do.load(do_base, a.d_out.row, a.dim, q_begin, q_begin, q_end, thread);
-            for (int i0 = q_begin; i0 < q_end; i0 += kRows) {
+            next_q.load(q_base, a.q.row, a.dim, i_first, q_begin, q_end, thread);
+            next_do.load(do_base, a.d_out.row, a.dim, i_first, q_begin, q_end, thread);
+            for (int i0 = i_first; i0 < q_end; i0 += kRows) {
                 __syncthreads();
                 next_q.store(s_q, thread);
                 next_do.store(s_do, thread);
@@ -471,12 +474,12 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
             if (a.splits > 1) {
                 const int64_t at =
                     ((static_cast<int64_t>(split) * a.k_rows + j) * kv_heads + kv_head) * a.dim;
-                store_row<float, DB>(a.part_k + at, dk, any ? sc.scale : 0.0f, a.dim, half);
-                store_row<float, DB>(a.part_v + at, dv, any ? 1.0f : 0.0f, a.dim, half);
+                store_row<float, DB>(a.part_k + at, dk, any, sc.scale, a.dim, half);
+                store_row<float, DB>(a.part_v + at, dv, any, 1.0f, a.dim, half);
             } else {
-                store_row<T, DB>(row_of<T>(a.d_k, j, kv_head), dk, any ? sc.scale : 0.0f, a.dim,
+                store_row<T, DB>(row_of<T>(a.d_k, j, kv_head), dk, any, sc.scale, a.dim,
                                  half);
-                store_row<T, DB>(row_of<T>(a.d_v, j, kv_head), dv, any ? 1.0f : 0.0f, a.dim, half);
+                store_row<T, DB>(row_of<T>(a.d_v, j, kv_head), dv, any, 1.0f, a.dim, half);
             }
         }
         if (!mixed) break;
@@ -492,26 +495,27 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
             off = sum != 0.0f;
         }
         if (only < 0 && !__syncthreads_or(off)) break;
-        const int w_next = wave_min(any && doc > only ? doc : INT_MAX);
+        const int w_next = wave_min(any && doc > only ? doc : kNone);
         __syncthreads();
         if (lane == 0) s_reduce[wave][0] = w_next;
         __syncthreads();
-        int seg = INT_MAX;
+        int seg = kNone;
 #pragma unroll
         for (int w = 0; w < 4; ++w) seg = min(seg, s_reduce[w][0]);
-        if (seg == INT_MAX) break;
+        if (seg == kNone) break;
         only = seg;
         const bool in_seg = any && doc == only;
         first = in_seg ? info.x : 0;
         last = in_seg ? doc : 0;
-        w_lo = wave_min(in_seg ? first : INT_MAX);
+        w_lo = wave_min(in_seg ? first : kNone);
         w_hi = wave_max(in_seg ? last : 0);
         if (lane == 0) s_reduce[wave][1] = w_lo;
         __syncthreads();
-        q_begin = INT_MAX;
+        q_begin = kNone;
         q_end = only;
 #pragma unroll
         for (int w = 0; w < 4; ++w) q_begin = min(q_begin, s_reduce[w][1]);
+        i_first += (q_begin - i_first) / kRows * kRows;  // the same tiles: the same bits
     }
 }
 

@@ -54,6 +54,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -3.0e38f;
 constexpr float kLowest = -1.0e38f;
 
+// The first row of an interval that has none: past every row (rows are below
+// 2^30), and row indices counted up from it do not overflow.
+constexpr int kNone = 1 << 30;
+
 // Eight values of one lane: one operand of a product over 16.
 template <typename T>
 struct Lane8;
@@ -235,10 +239,11 @@ __device__ __forceinline__ void load_operand(Frag<T> (&f)[2 * DB], const T* row,
 }
 
 // Writes a column's accumulators (rows of the transposed product = elements of
-// the row) as a row of global memory, times `by`.
+// the row) as a row of global memory, times `by`; zeros where `any` is false,
+// whatever was accumulated.
 template <typename T, int DB>
-__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], float by, int dim,
-                                          int half) {
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], bool any, float by,
+                                          int dim, int half) {
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -248,7 +253,7 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], float
             typedef T t4 __attribute__((ext_vector_type(4)));
             t4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(acc[b][4 * g + e] * by);
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(any ? acc[b][4 * g + e] * by : 0.0f);
             *reinterpret_cast<t4*>(row + col) = v;
         }
 }
