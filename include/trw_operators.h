@@ -21,7 +21,8 @@
  *    the device knows (offsets, lengths, bucket ids) are clamped there, so
  *    that wrong ones give wrong results and never an access out of range.
  *  - Strides are in elements.  A row of D values is contiguous and 16-byte
- *    aligned, D is a multiple of 8 up to 128.
+ *    aligned, D is a multiple of 8 up to 128; rows lie at most 2^22 elements
+ *    apart.
  */
 #ifndef TRW_OPERATORS_H
 #define TRW_OPERATORS_H
@@ -100,8 +101,8 @@ typedef struct trw_attention_params {
     const int32_t *q_rows_info, *k_rows_info; /* of trw_ops_walk_mask */
     trw_score score;
     trw_rows q, k, v, out;
-    float* stats; /* [heads, q_rows, 2]: largest score and log of the sum (base 2); written by
-                     the forward pass where not NULL, read by the backward pass */
+    float* stats; /* [2, heads, q_rows], of the rows' softmax (base 2); written by the forward
+                     pass where not NULL, read by the backward pass */
     /* backward */
     trw_rows d_out, d_q, d_k, d_v;
     float* d_table; /* [heads, num_buckets], where score.table is given */

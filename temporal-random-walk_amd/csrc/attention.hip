@@ -14,6 +14,8 @@
 // Scores, maxima, sums and the output accumulate in float32; P is rounded to
 // the inputs' type for the product with V (as the matrix instructions take
 // it), the sum l is of the unrounded values.
+#include <algorithm>
+
 #include "operators.h"
 
 namespace trw {
@@ -24,32 +26,55 @@ constexpr int kThreads = 256;
 constexpr int kRowsPerWave = 32;
 constexpr int kTileRows = 128;
 
+// A running maximum is raised once a score passes it by this much (base 2):
+// P is then at most 2^8, which every type holds as well as 1, and the output is
+// rarely scaled.
+constexpr float kSlack = 8.0f;
+
 struct ForwardArgs {
     Rows q, k, v, out;
     const int4* q_info;
-    float2* stats;
+    float* stats;
     Score score;
     int q_rows, k_rows, heads, group, dim;
-    int tiles;
+    int tiles, splits;
+    float* part_out;     // [splits, heads, q_rows, dim], where splits > 1
+    float2* part_stats;  // [splits, heads, q_rows]
 };
 
+// What the backward pass takes from a score to have log2 P: m + log2 l at once,
+// or in two where a bias can make scores so low that log2 l would be lost in
+// the sum.
+__device__ __forceinline__ void store_stats(const ForwardArgs& a, int64_t stat, bool seen, float m,
+                                            float l) {
+    if (!a.stats) return;
+    const float log_l = seen ? __builtin_amdgcn_logf(l) : INFINITY;
+    const bool apart = a.score.biased();
+    a.stats[stat] = apart ? m : m + log_l;
+    if (apart) a.stats[static_cast<int64_t>(a.heads) * a.q_rows + stat] = log_l;
+}
+
 template <typename T, int DB>
-__global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // of a tile
     constexpr int kBlocks = kKeys / 32;
-    __shared__ u32x4 s_k[G::bytes(kKeys) / 16], s_v[G::bytes(kKeys) / 16];
-    __shared__ float s_time[kKeys];
+    constexpr int kTileChunks = kKeys * G::kSlots;
+    __shared__ u32x4 s_kv[2][2][kTileChunks];  // two tiles of keys and values
+    __shared__ float s_times[2][64];
     __shared__ int s_reduce[4][4];
     extern __shared__ float s_lut[];
 
-    const int64_t item = xcd_item(blockIdx.x, static_cast<int64_t>(a.tiles) * a.heads);
-    if (item >= static_cast<int64_t>(a.tiles) * a.heads) return;
-    const int head = static_cast<int>(item / a.tiles);
+    const int64_t items = static_cast<int64_t>(a.tiles) * a.heads * a.splits;
+    const int64_t item = xcd_item(blockIdx.x, items);
+    if (item >= items) return;
+    const int split = static_cast<int>(item % a.splits);
+    const int head = static_cast<int>(item / a.splits / a.tiles);
     // the last rows of a causal walk see most: first
-    const int tile = a.tiles - 1 - static_cast<int>(item % a.tiles);
+    const int tile = a.tiles - 1 - static_cast<int>(item / a.splits % a.tiles);
     const int kv_head = head / a.group;
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, half = lane >> 5;
+    const int thread = threadIdx.x, lane = thread & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const Score& sc = a.score;
 
     const int i = tile * kTileRows + wave * kRowsPerWave + (lane & 31);
@@ -58,6 +83,9 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
     int lo = info.x, hi = max(info.x, min(info.y, a.k_rows));
     const int diag = info.z;
     const bool any = lo < hi;
+
+    Frag<T> q[G::kSteps];
+    load_operand<T, DB>(q, row_of<const T>(a.q, i, head), any, a.dim, half);
 
     // the wave's and the workgroup's intervals
     int w_lo = wave_min(any ? lo : kNone), w_hi = wave_max(any ? hi : 0);
@@ -77,17 +105,31 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
         k_end = max(k_end, s_reduce[w][1]);
         last_lo = max(last_lo, s_reduce[w][2]);
     }
+    k_begin = __builtin_amdgcn_readfirstlane(k_begin);
+    k_end = __builtin_amdgcn_readfirstlane(k_end);
     const bool mixed = k_begin < last_lo;  // rows of more than one walk
+    // this split's tiles of the workgroup's keys
+    int j_first = k_begin, j_last = k_end;
+    if (a.splits > 1 && k_begin < k_end) {
+        const int count = (k_end - k_begin + kKeys - 1) / kKeys;
+        j_first = k_begin + static_cast<int>(static_cast<int64_t>(count) * split / a.splits) * kKeys;
+        j_last = min(k_end, k_begin + static_cast<int>(static_cast<int64_t>(count) * (split + 1) /
+                                                       a.splits) * kKeys);
+    }
 
-    Frag<T> q[G::kSteps];
-    load_operand<T, DB>(q, row_of<const T>(a.q, i, head), any, a.dim, half);
     const float slope = sc.slopes ? sc.slopes[head] * kLog2e : 0.0f;
     const float q_time = sc.q_times && any ? sc.q_times[i] : 0.0f;
     const T* k_base = row_of<const T>(a.k, 0, kv_head);
     const T* v_base = row_of<const T>(a.v, 0, kv_head);
+    const Loader<T, DB, kKeys, kThreads> k_load(a.k.row, a.dim, thread);
+    const Loader<T, DB, kKeys, kThreads> v_load(a.v.row, a.dim, thread);
+    // Scores that are only products are scaled inside the exponential
+    const bool plain = !sc.biased() && !(sc.softcap > 0) && sc.scale2 > 0;
+    const float in_exp = plain ? sc.scale2 : 1.0f;
+
+    const int j_begin = j_first, j_end = j_last;
 
     int only = -1;  // -1: every row; else the rows whose keys begin there, again
-    int j_first = k_begin;
     for (;;) {
         f32x16 o[DB];
 #pragma unroll
@@ -96,21 +138,21 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
         // Every row must be inside a tile for it to go unmasked
         const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
 
-        Staged<T, DB, kKeys, kThreads> next_k, next_v;
-        next_k.load(k_base, a.k.row, a.dim, j_first, k_begin, k_end, thread);
-        next_v.load(v_base, a.v.row, a.dim, j_first, k_begin, k_end, thread);
-        for (int j0 = j_first; j0 < k_end; j0 += kKeys) {
-            __syncthreads();  // the tile before is done with
-            next_k.store(s_k, thread);
-            next_v.store(s_v, thread);
-            if (sc.k_times && thread < kKeys)
-                s_time[thread] = j0 + thread < k_end ? sc.k_times[j0 + thread] : 0.0f;
-            __syncthreads();
-            if (j0 + kKeys < k_end) {
-                next_k.load(k_base, a.k.row, a.dim, j0 + kKeys, k_begin, k_end, thread);
-                next_v.load(v_base, a.v.row, a.dim, j0 + kKeys, k_begin, k_end, thread);
-            }
+        auto fetch = [&](int j0, int buffer) {
+            k_load.load(k_base, j0, k_begin, k_end, s_kv[buffer][0], thread);
+            v_load.load(v_base, j0, k_begin, k_end, s_kv[buffer][1], thread);
+            if (sc.k_times && wave == 0)
+                load_floats(sc.k_times, j0, k_begin, k_end, s_times[buffer], lane);
+        };
+        int buffer = 0;
+        if (j_first < j_last) fetch(j_first, 0);
+        for (int j0 = j_first; j0 < j_last; j0 += kKeys, buffer ^= 1) {
+            landed();  // and the other buffer is done with
+            if (j0 + kKeys < j_last) fetch(j0 + kKeys, buffer ^ 1);
             if (j0 >= w_hi || j0 + kKeys <= w_lo) continue;
+            const u32x4* s_k = s_kv[buffer][0];
+            const u32x4* s_v = s_kv[buffer][1];
+            const float* s_time = s_times[buffer];
 
             float s[kBlocks][16];
 #pragma unroll
@@ -122,50 +164,10 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[b][r] = x[r];
             }
-            if (sc.softcap > 0) {
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float unused;
-                        s[b][r] = capped<T>(sc, s[b][r], unused);
-                    }
-            } else {
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[b][r] *= sc.scale2;
-            }
             const int j_lane = j0 + 4 * half;  // register r's key: + 32 b + acc_row(r)
-            if (sc.table) {
-                const int far_lo = w_diag_lo - (j0 + kKeys - 1), far_hi = w_diag_hi - j0;
-                if (far_lo >= sc.reach || far_hi <= -sc.reach) {
-                    const float bias = s_lut[far_lo >= sc.reach ? 2 * sc.reach : 0];
-#pragma unroll
-                    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[b][r] += bias;
-                } else {
-#pragma unroll
-                    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int d = diag - (j_lane + 32 * b + acc_row(r));
-                            s[b][r] += s_lut[min(max(d, -sc.reach), sc.reach) + sc.reach];
-                        }
-                }
-            }
-            if (sc.slopes) {
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int at = 32 * b + acc_row(r);
-                        const float gap = sc.k_times
-                                              ? q_time - s_time[at + 4 * half]
-                                              : static_cast<float>(diag - (j_lane + at));
-                        s[b][r] = fmaf(-slope, fabsf(gap), s[b][r]);
-                    }
+            if (!plain) {
+                cap_scores<T>(sc, s);
+                add_biases(sc, s, s_lut, slope, diag, w_diag_lo, w_diag_hi, q_time, s_time, j0, half);
             }
             if (j0 < full_lo || j0 + kKeys > full_hi) {
                 const unsigned span = static_cast<unsigned>(hi - lo);
@@ -182,9 +184,10 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m)) {
-                const float grown = fmaxf(m, top);
+            top = fmaxf(top, __shfl_xor(top, 32)) * in_exp;
+            if (__any(top > m + kSlack)) {
+                // by its own scores alone: a row's bits do not depend on its neighbours
+                const float grown = top > m + kSlack ? top : m;
                 const float by = exp2_fast(m - grown);
                 m = grown;
                 l *= by;
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
             for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[b][r] = exp2_fast(s[b][r] - m);
+                    s[b][r] = exp2_fast(fmaf(s[b][r], in_exp, -m));
                     l += s[b][r];
                 }
             }
@@ -215,10 +218,15 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
         const bool mine = i < a.q_rows && (only < 0 || (any && info.x == only));
         if (mine) {
             const bool seen = any && l != 0.0f;  // 0: the bias masks every key
-            store_row<T, DB>(row_of<T>(a.out, i, head), o, seen, 1.0f / l, a.dim, half);
-            if (a.stats && half == 0)
-                a.stats[static_cast<int64_t>(head) * a.q_rows + i] =
-                    seen ? make_float2(m, __builtin_amdgcn_logf(l)) : make_float2(0.0f, INFINITY);
+            const int64_t stat = static_cast<int64_t>(head) * a.q_rows + i;
+            if (a.splits > 1) {
+                const int64_t part = static_cast<int64_t>(split) * a.heads * a.q_rows + stat;
+                store_row<float, DB>(a.part_out + part * a.dim, o, seen, 1.0f, a.dim, half);
+                if (half == 0) a.part_stats[part] = make_float2(m, seen ? l : 0.0f);
+            } else {
+                store_row<T, DB>(row_of<T>(a.out, i, head), o, seen, 1.0f / l, a.dim, half);
+                if (half == 0) store_stats(a, stat, seen, m, l);
+            }
         }
         if (!mixed) break;
 
@@ -252,12 +260,61 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
         w_hi = wave_max(in_seg ? hi : 0);
         if (lane == 0) s_reduce[wave][1] = w_hi;
         __syncthreads();
-        j_first += (only - j_first) / kKeys * kKeys;  // the same tiles: the same bits
         k_begin = only;
         k_end = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) k_end = max(k_end, s_reduce[w][1]);
+        k_begin = __builtin_amdgcn_readfirstlane(k_begin);
+        k_end = __builtin_amdgcn_readfirstlane(k_end);
+        // the same tiles: the same bits
+        j_first = j_begin + max(k_begin - j_begin, 0) / kKeys * kKeys;
+        j_last = min(j_end, k_end);
     }
+}
+
+// Joins the splits of a row: four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
+    const int64_t t = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
+    const int pieces = a.dim / 4;
+    const int64_t rows = static_cast<int64_t>(a.heads) * a.q_rows;
+    if (t >= rows * pieces) return;
+    const int64_t stat = t / pieces;  // head, row
+    const int col = static_cast<int>(t % pieces) * 4;
+    float m = kFloor;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 st = a.part_stats[s * rows + stat];
+        m = st.y != 0.0f ? fmaxf(m, st.x) : m;
+    }
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 st = a.part_stats[s * rows + stat];
+        if (st.y == 0.0f) continue;
+        const float by = exp2_fast(st.x - m);
+        const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_out + (s * rows + stat) * a.dim + col);
+        l = fmaf(by, st.y, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(by, part[e], o[e]);
+    }
+    const bool seen = l != 0.0f;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(seen ? o[e] / l : 0.0f);
+    const int head = static_cast<int>(stat / a.q_rows);
+    *reinterpret_cast<t4*>(row_of<T>(a.out, stat % a.q_rows, head) + col) = out;
+    if (col == 0) store_stats(a, stat, seen, m, l);
+}
+
+// Workgroups that share the keys of one: where the tiles of query rows are
+// fewer than two for each of the 256 compute units, up to that many, each with
+// 256 keys or more if one walk has them all.
+int splits_of(const trw_attention_params& p) {
+    const int64_t items = (p.q_rows + kTileRows - 1) / kTileRows * p.heads;
+    if (items == 0) return 1;
+    const int64_t splits = std::min<int64_t>({512 / items, p.k_rows / 256, 16});
+    return static_cast<int>(std::max<int64_t>(splits, 1));
 }
 
 }  // namespace
@@ -265,18 +322,22 @@ __global__ __launch_bounds__(kThreads) void attention_forward_kernel(ForwardArgs
 uint64_t attention_backward_workspace(const trw_attention_params& p);
 
 uint64_t attention_workspace(const trw_attention_params& p, bool backward) {
-    return backward ? attention_backward_workspace(p) : 0;
+    if (backward) return attention_backward_workspace(p);
+    const int splits = splits_of(p);
+    if (splits == 1) return 0;
+    return static_cast<uint64_t>(splits) * p.heads * p.q_rows * (p.dim + 2) * sizeof(float);
 }
 
 void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     if (p.q_rows == 0) return;
+    require(p.workspace_bytes >= attention_workspace(p, false), "workspace is too small");
     ForwardArgs a;
     a.q = make_rows(p.q);
     a.k = make_rows(p.k);
     a.v = make_rows(p.v);
     a.out = make_rows(p.out);
     a.q_info = reinterpret_cast<const int4*>(p.q_rows_info);
-    a.stats = reinterpret_cast<float2*>(p.stats);
+    a.stats = p.stats;
     a.score = make_score(p.score);
     a.q_rows = static_cast<int>(p.q_rows);
     a.k_rows = static_cast<int>(p.k_rows);
@@ -284,13 +345,24 @@ void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     a.group = p.heads / p.kv_heads;
     a.dim = p.dim;
     a.tiles = static_cast<int>((p.q_rows + kTileRows - 1) / kTileRows);
-    const int64_t grid = xcd_grid(static_cast<int64_t>(a.tiles) * a.heads);
+    a.splits = splits_of(p);
+    const int64_t rows = static_cast<int64_t>(a.heads) * a.q_rows;
+    a.part_out = static_cast<float*>(p.workspace);
+    a.part_stats = reinterpret_cast<float2*>(a.part_out + a.splits * rows * a.dim);
+    const int64_t grid = xcd_grid(static_cast<int64_t>(a.tiles) * a.heads * a.splits);
     const size_t lds = p.score.table ? (2 * a.score.reach + 1) * sizeof(float) : 0;
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {
         hipLaunchKernelGGL((attention_forward_kernel<decltype(t), decltype(db)::value>),
                            dim3(static_cast<unsigned>(grid)), dim3(kThreads), lds, stream, a);
+        check_launch("attention_forward");
+        if (a.splits > 1) {
+            const int64_t threads = rows * (a.dim / 4);
+            hipLaunchKernelGGL((join_forward_kernel<decltype(t)>),
+                               dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)),
+                               dim3(kThreads), 0, stream, a);
+            check_launch("attention_forward");
+        }
     });
-    check_launch("attention_forward");
 }
 
 }  // namespace ops

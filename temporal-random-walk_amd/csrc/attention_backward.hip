@@ -24,7 +24,7 @@ struct BackwardArgs {
     Rows q, k, v, out, d_out, d_q, d_k, d_v;
     const int4* q_info;
     const int2* k_info;
-    const float2* stats;
+    const float* stats;
     float* delta;    // [heads, q_rows] D
     float* partial;  // [heads, q tiles, num_buckets]
     Score score;
@@ -34,16 +34,17 @@ struct BackwardArgs {
     float *part_k, *part_v;  // [splits, k_rows, kv_heads, dim], where splits > 1
 };
 
-// Scores of 16 pairs in base 2 from their products, and the slope the cap left.
+// Scores in base 2 of one block's products, and the slope that the cap left.
 template <typename T>
-__device__ __forceinline__ void score_block(const Score& sc, float (&x)[16], float (&slope)[16]) {
+__device__ __forceinline__ void score_block(const Score& sc, const f32x16& product,
+                                            float (&x)[1][16], float (&slope)[16]) {
     if (sc.softcap > 0) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = capped<T>(sc, x[r], slope[r]);
+        for (int r = 0; r < 16; ++r) x[0][r] = capped<T>(sc, product[r], slope[r]);
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            x[r] *= sc.scale2;
+            x[0][r] = product[r] * sc.scale2;
             slope[r] = 1.0f;
         }
     }
@@ -57,11 +58,11 @@ __device__ __forceinline__ void score_block(const Score& sc, float (&x)[16], flo
 // sums of its own and adds to it without two lanes meeting; pairs past the
 // reach, which share two buckets, are summed in registers.
 template <typename T, int DB>
-__global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(BackwardArgs a) {
     typedef Tile<T, DB> G;
-    constexpr int kKeys = 32;
-    __shared__ u32x4 s_k[G::bytes(kKeys) / 16], s_v[G::bytes(kKeys) / 16];
-    __shared__ float s_time[kKeys];
+    constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
+    __shared__ u32x4 s_kv[2][2][kKeys * G::kSlots];
+    __shared__ float s_times[2][64];
     __shared__ int s_reduce[4][4];
     extern __shared__ float s_dyn[];  // bias by distance, then 8 lines of its gradient
 
@@ -71,7 +72,8 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
     const int head = static_cast<int>(item / a.q_tiles);
     const int tile = a.q_tiles - 1 - static_cast<int>(item % a.q_tiles);
     const int kv_head = head / a.group;
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, half = lane >> 5;
+    const int thread = threadIdx.x, lane = thread & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const Score& sc = a.score;
     const int line = 2 * sc.reach + 1;
     float* s_lut = s_dyn;
@@ -83,6 +85,11 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
     int lo = info.x, hi = max(info.x, min(info.y, a.k_rows));
     const int diag = info.z;
     const bool any = lo < hi;
+
+    Frag<T> q[G::kSteps], d_o[G::kSteps];
+    load_operand<T, DB>(q, row_of<const T>(a.q, i, head), any, a.dim, half);
+    load_operand<T, DB>(d_o, row_of<const T>(a.d_out, i, head), any, a.dim, half);
+
     int w_lo = wave_min(any ? lo : kNone), w_hi = wave_max(any ? hi : 0);
     const int w_diag_lo = wave_min(any ? diag : kNone), w_diag_hi = wave_max(any ? diag : -kNone);
     const int w_last_lo = wave_max(any ? lo : 0);
@@ -103,11 +110,10 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
         k_end = max(k_end, s_reduce[w][1]);
         last_lo = max(last_lo, s_reduce[w][2]);
     }
+    k_begin = __builtin_amdgcn_readfirstlane(k_begin);
+    k_end = __builtin_amdgcn_readfirstlane(k_end);
     const bool mixed = k_begin < last_lo;
 
-    Frag<T> q[G::kSteps], d_o[G::kSteps];
-    load_operand<T, DB>(q, row_of<const T>(a.q, i, head), any, a.dim, half);
-    load_operand<T, DB>(d_o, row_of<const T>(a.d_out, i, head), any, a.dim, half);
     float delta = 0.0f;
     {
         Frag<T> o[G::kSteps];
@@ -120,119 +126,105 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
         delta += __shfl_xor(delta, 32);
     }
     const int64_t stat = static_cast<int64_t>(head) * a.q_rows + i;
-    float m = 0.0f, log_l = INFINITY;
+    float m = INFINITY, log_l = INFINITY;
     if (any) {
-        const float2 st = a.stats[stat];
-        m = st.x;
-        log_l = st.y;
+        m = a.stats[stat];
+        log_l = sc.biased() ? a.stats[static_cast<int64_t>(a.heads) * a.q_rows + stat] : 0.0f;
     }
     if (i < a.q_rows && half == 0) a.delta[stat] = delta;
     const float slope = sc.slopes ? sc.slopes[head] * kLog2e : 0.0f;
     const float q_time = sc.q_times && any ? sc.q_times[i] : 0.0f;
     const T* k_base = row_of<const T>(a.k, 0, kv_head);
     const T* v_base = row_of<const T>(a.v, 0, kv_head);
+    const Loader<T, DB, kKeys, kThreads> k_load(a.k.row, a.dim, thread);
+    const Loader<T, DB, kKeys, kThreads> v_load(a.v.row, a.dim, thread);
     float far_before = 0.0f, far_after = 0.0f;  // dS past the reach, either way
 
     int only = -1;
+    const int j_begin = k_begin;
     int j_first = k_begin;
     for (;;) {
         f32x16 dq[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b) dq[b] = zero16();
         const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
-        Staged<T, DB, kKeys, kThreads> next_k, next_v;
-        next_k.load(k_base, a.k.row, a.dim, j_first, k_begin, k_end, thread);
-        next_v.load(v_base, a.v.row, a.dim, j_first, k_begin, k_end, thread);
-        for (int j0 = j_first; j0 < k_end; j0 += kKeys) {
-            __syncthreads();
-            next_k.store(s_k, thread);
-            next_v.store(s_v, thread);
-            if (sc.k_times && thread < kKeys)
-                s_time[thread] = j0 + thread < k_end ? sc.k_times[j0 + thread] : 0.0f;
-            __syncthreads();
-            if (j0 + kKeys < k_end) {
-                next_k.load(k_base, a.k.row, a.dim, j0 + kKeys, k_begin, k_end, thread);
-                next_v.load(v_base, a.v.row, a.dim, j0 + kKeys, k_begin, k_end, thread);
-            }
-            if (j0 >= w_hi || j0 + kKeys <= w_lo) continue;
+        auto fetch = [&](int j0, int buffer) {
+            k_load.load(k_base, j0, k_begin, k_end, s_kv[buffer][0], thread);
+            v_load.load(v_base, j0, k_begin, k_end, s_kv[buffer][1], thread);
+            if (sc.k_times && wave == 0)
+                load_floats(sc.k_times, j0, k_begin, k_end, s_times[buffer], lane);
+        };
+        int buffer = 0;
+        if (j_first < k_end) fetch(j_first, 0);
+        for (int jt = j_first; jt < k_end; jt += kKeys, buffer ^= 1) {
+            landed();
+            if (jt + kKeys < k_end) fetch(jt + kKeys, buffer ^ 1);
+#pragma unroll 1
+            for (int sub = 0; sub < kKeys; sub += 32) {
+                const int j0 = jt + sub;
+                if (j0 >= w_hi || j0 + 32 <= w_lo) continue;
+                const u32x4* s_k = s_kv[buffer][0] + sub * G::kSlots;
+                const u32x4* s_v = s_kv[buffer][1] + sub * G::kSlots;
 
-            f32x16 x16 = zero16(), dp = zero16();
+                f32x16 product = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < G::kSteps; ++st) {
-                x16 = mma(G::row(s_k, lane & 31, st, half), q[st], x16);
-                dp = mma(G::row(s_v, lane & 31, st, half), d_o[st], dp);
-            }
-            float x[16], cap_slope[16];
+                for (int st = 0; st < G::kSteps; ++st) {
+                    product = mma(G::row(s_k, lane & 31, st, half), q[st], product);
+                    dp = mma(G::row(s_v, lane & 31, st, half), d_o[st], dp);
+                }
+                float x[1][16], cap_slope[16];
+                score_block<T>(sc, product, x, cap_slope);
+                const int j_lane = j0 + 4 * half;
+                if (sc.biased()) {
+                    add_biases(sc, x, s_lut, slope, diag, w_diag_lo, w_diag_hi, q_time,
+                               s_times[buffer] + sub, j0, half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = x16[r];
-            score_block<T>(sc, x, cap_slope);
-            const int j_lane = j0 + 4 * half;
-            const int far_lo = w_diag_lo - (j0 + kKeys - 1), far_hi = w_diag_hi - j0;
-            const bool far = far_lo >= sc.reach || far_hi <= -sc.reach;
-            if (sc.table) {
-                if (far) {
-                    const float bias = s_lut[far_lo >= sc.reach ? 2 * sc.reach : 0];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] += bias;
+                    for (int r = 0; r < 16; ++r) x[0][r] = (x[0][r] - m) - log_l;
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int d = diag - (j_lane + acc_row(r));
-                        x[r] += s_lut[min(max(d, -sc.reach), sc.reach) + sc.reach];
-                    }
+                    for (int r = 0; r < 16; ++r) x[0][r] -= m;
                 }
-            }
-            if (sc.slopes) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float gap = sc.k_times
-                                          ? q_time - s_time[acc_row(r) + 4 * half]
-                                          : static_cast<float>(diag - (j_lane + acc_row(r)));
-                    x[r] = fmaf(-slope, fabsf(gap), x[r]);
-                }
-            }
-            // m apart from log l: next to a score near the type's lowest, log l
-            // would be lost
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                x[r] = exp2_fast((x[r] - m) - log_l) * (dp[r] - delta);
-            }
-            if (j0 < full_lo || j0 + kKeys > full_hi) {
-                const unsigned span = static_cast<unsigned>(hi - lo);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = j_lane + acc_row(r);
-                    if (static_cast<unsigned>(j - lo) >= span) x[r] = 0.0f;
-                }
-            }
-            if (sc.table && only < 0) {
-                if (far) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += x[r];
-                    if (far_lo >= sc.reach) far_before += sum;
-                    else far_after += sum;
-                } else {
+                for (int r = 0; r < 16; ++r) x[0][r] = exp2_fast(x[0][r]) * (dp[r] - delta);
+                if (j0 < full_lo || j0 + 32 > full_hi) {
+                    const unsigned span = static_cast<unsigned>(hi - lo);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int d = diag - (j_lane + acc_row(r));
-                        if (d >= sc.reach) far_before += x[r];
-                        else if (d <= -sc.reach) far_after += x[r];
-                        else if (any) atomicAdd(&s_sum[d + sc.reach], x[r]);
+                        const int j = j_lane + acc_row(r);
+                        if (static_cast<unsigned>(j - lo) >= span) x[0][r] = 0.0f;
                     }
                 }
-            }
-            if (sc.softcap > 0) {
+                if (sc.table && only < 0) {
+                    const int far_lo = w_diag_lo - (j0 + 31), far_hi = w_diag_hi - j0;
+                    if (far_lo >= sc.reach || far_hi <= -sc.reach) {
+                        float sum = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] *= cap_slope[r];
-            }
+                        for (int r = 0; r < 16; ++r) sum += x[0][r];
+                        if (far_lo >= sc.reach) far_before += sum;
+                        else far_after += sum;
+                    } else {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                Frag<T> ds;
+                        for (int r = 0; r < 16; ++r) {
+                            const int d = diag - (j_lane + acc_row(r));
+                            if (d >= sc.reach) far_before += x[0][r];
+                            else if (d <= -sc.reach) far_after += x[0][r];
+                            else if (any) atomicAdd(&s_sum[d + sc.reach], x[0][r]);
+                        }
+                    }
+                }
+                if (sc.softcap > 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ds[e] = static_cast<T>(x[8 * t + e]);
+                    for (int r = 0; r < 16; ++r) x[0][r] *= cap_slope[r];
+                }
 #pragma unroll
-                for (int b = 0; b < DB; ++b) dq[b] = mma(G::columns(s_k, 16 * t, b, lane), ds, dq[b]);
+                for (int t = 0; t < 2; ++t) {
+                    Frag<T> ds;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ds[e] = static_cast<T>(x[0][8 * t + e]);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b)
+                        dq[b] = mma(G::columns(s_k, 16 * t, b, lane), ds, dq[b]);
+                }
             }
         }
         if (i < a.q_rows && (only < 0 || (any && info.x == only)))
@@ -266,11 +258,13 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
         w_hi = wave_max(in_seg ? hi : 0);
         if (lane == 0) s_reduce[wave][1] = w_hi;
         __syncthreads();
-        j_first += (only - j_first) / kKeys * kKeys;  // the same tiles: the same bits
         k_begin = only;
         k_end = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) k_end = max(k_end, s_reduce[w][1]);
+        k_begin = __builtin_amdgcn_readfirstlane(k_begin);
+        k_end = __builtin_amdgcn_readfirstlane(k_end);
+        j_first = j_begin + (k_begin - j_begin) / kKeys * kKeys;  // the same tiles: the same bits
     }
 
     if (!sc.table) return;
@@ -314,12 +308,13 @@ __global__ __launch_bounds__(kThreads) void attention_backward_q_kernel(Backward
 // A lane holds one key (column) and 16 query rows at a time; q and dO pass
 // through LDS and are read both ways.
 template <typename T, int DB>
-__global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_kv_kernel(
+    BackwardArgs a) {
     typedef Tile<T, DB> G;
-    constexpr int kRows = 32;
-    __shared__ u32x4 s_q[G::bytes(kRows) / 16], s_do[G::bytes(kRows) / 16];
-    __shared__ float s_m[kRows], s_log_l[kRows], s_delta[kRows], s_time[kRows];
-    __shared__ int s_diag[kRows];
+    constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
+    __shared__ u32x4 s_rows[2][2][kRows * G::kSlots];  // q and dO
+    __shared__ float s_stats[2][4][64];                // m, log l, D, times
+    __shared__ int4 s_infos[2][64];
     __shared__ int s_reduce[4][4];
     extern __shared__ float s_lut[];
 
@@ -330,7 +325,8 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
     const int split = static_cast<int>(item / a.k_tiles) % a.splits;
     const int kv_head = static_cast<int>(item / a.k_tiles) / a.splits;
     const int tile = static_cast<int>(item % a.k_tiles);  // the first keys are seen most: first
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, half = lane >> 5;
+    const int thread = threadIdx.x, lane = thread & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const Score& sc = a.score;
 
     const int j = tile * kTileRows + wave * 32 + (lane & 31);
@@ -339,6 +335,11 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
     int first = info.x, last = max(info.x, min(info.y, a.q_rows));
     const bool any = first < last;
     const int doc = last;  // no two walks with pairs end at one query
+
+    Frag<T> k[G::kSteps], v[G::kSteps];
+    load_operand<T, DB>(k, row_of<const T>(a.k, j, kv_head), any, a.dim, half);
+    load_operand<T, DB>(v, row_of<const T>(a.v, j, kv_head), any, a.dim, half);
+
     int w_lo = wave_min(any ? first : kNone), w_hi = wave_max(any ? last : 0);
     const int w_first_doc = wave_min(any ? doc : kNone);
     if (lane == 0) {
@@ -354,17 +355,20 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
         q_end = max(q_end, s_reduce[w][1]);
         first_doc = min(first_doc, s_reduce[w][2]);
     }
+    q_begin = __builtin_amdgcn_readfirstlane(q_begin);
+    q_end = __builtin_amdgcn_readfirstlane(q_end);
     const bool mixed = q_begin < q_end && first_doc < q_end;
 
-    Frag<T> k[G::kSteps], v[G::kSteps];
-    load_operand<T, DB>(k, row_of<const T>(a.k, j, kv_head), any, a.dim, half);
-    load_operand<T, DB>(v, row_of<const T>(a.v, j, kv_head), any, a.dim, half);
     const float k_time = sc.k_times && any ? sc.k_times[j] : 0.0f;
     const int heads_each = (a.group + a.splits - 1) / a.splits;
     const int head_begin = kv_head * a.group + split * heads_each;
     const int head_end = min(head_begin + heads_each, (kv_head + 1) * a.group);
+    const Loader<T, DB, kRows, kThreads> q_load(a.q.row, a.dim, thread);
+    const Loader<T, DB, kRows, kThreads> do_load(a.d_out.row, a.dim, thread);
+    const bool positions = sc.table || (sc.slopes && !sc.k_times);
 
     int only = -1;
+    const int i_begin = q_begin;
     int i_first = q_begin;
     for (;;) {
         f32x16 dk[DB], dv[DB];
@@ -374,98 +378,127 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
             dv[b] = zero16();
         }
         const int full_lo = wave_max(any ? first : kNone), full_hi = wave_min(any ? last : 0);
+#pragma unroll 1
         for (int head = head_begin; head < head_end; ++head) {
             const T* q_base = row_of<const T>(a.q, 0, head);
             const T* do_base = row_of<const T>(a.d_out, 0, head);
-            const int64_t stat = static_cast<int64_t>(head) * a.q_rows;
+            const float* m_base = a.stats + static_cast<int64_t>(head) * a.q_rows;
+            const float* log_l_base = m_base + static_cast<int64_t>(a.heads) * a.q_rows;
+            const float* delta_base = a.delta + static_cast<int64_t>(head) * a.q_rows;
             const float slope = sc.slopes ? sc.slopes[head] * kLog2e : 0.0f;
-            if (sc.table) {
-                __syncthreads();
-                fill_bias(s_lut, sc, head, thread, kThreads);
-            }
-            Staged<T, DB, kRows, kThreads> next_q, next_do;
-            next_q.load(q_base, a.q.row, a.dim, i_first, q_begin, q_end, thread);
-            next_do.load(do_base, a.d_out.row, a.dim, i_first, q_begin, q_end, thread);
-            for (int i0 = i_first; i0 < q_end; i0 += kRows) {
-                __syncthreads();
-                next_q.store(s_q, thread);
-                next_do.store(s_do, thread);
-                if (thread < kRows) {
-                    const int i = i0 + thread;
-                    const bool in = i < q_end;
-                    const float2 st = in ? a.stats[stat + i] : make_float2(0.0f, INFINITY);
-                    s_m[thread] = st.x;
-                    s_log_l[thread] = st.y;
-                    s_delta[thread] = in ? a.delta[stat + i] : 0.0f;
-                    s_time[thread] = in && sc.q_times ? sc.q_times[i] : 0.0f;
-                    s_diag[thread] = in ? a.q_info[i].z : 0;
+            __syncthreads();  // the head before is done with its biases and tiles
+            if (sc.table) fill_bias(s_lut, sc, head, thread, kThreads);
+            auto fetch = [&](int i0, int buffer) {
+                q_load.load(q_base, i0, q_begin, q_end, s_rows[buffer][0], thread);
+                do_load.load(do_base, i0, q_begin, q_end, s_rows[buffer][1], thread);
+                if (wave == 0) {
+                    load_floats(m_base, i0, q_begin, q_end, s_stats[buffer][0], lane);
+                    if (sc.biased())
+                        load_floats(log_l_base, i0, q_begin, q_end, s_stats[buffer][1], lane);
+                } else if (wave == 1) {
+                    load_floats(delta_base, i0, q_begin, q_end, s_stats[buffer][2], lane);
+                } else if (wave == 2) {
+                    if (sc.q_times)
+                        load_floats(sc.q_times, i0, q_begin, q_end, s_stats[buffer][3], lane);
+                } else if (positions) {
+                    const int from = min(max(i0, q_begin), q_end - 1);
+                    const int at = min(max(i0 + lane, q_begin), q_end - 1) - from;
+                    copy_to_lds(a.q_info + from, static_cast<uint32_t>(at) * 16,
+                                lds_address(s_infos[buffer]));
                 }
-                __syncthreads();
-                if (i0 + kRows < q_end) {
-                    next_q.load(q_base, a.q.row, a.dim, i0 + kRows, q_begin, q_end, thread);
-                    next_do.load(do_base, a.d_out.row, a.dim, i0 + kRows, q_begin, q_end, thread);
-                }
-                if (i0 >= w_hi || i0 + kRows <= w_lo) continue;
+            };
+            int buffer = 0;
+            if (i_first < q_end) fetch(i_first, 0);
+            for (int it = i_first; it < q_end; it += kRows, buffer ^= 1) {
+                landed();
+                if (it + kRows < q_end) fetch(it + kRows, buffer ^ 1);
+#pragma unroll 1
+                for (int sub = 0; sub < kRows; sub += 32) {
+                    const int i0 = it + sub;
+                    if (i0 >= w_hi || i0 + 32 <= w_lo) continue;
+                    const u32x4* s_q = s_rows[buffer][0] + sub * G::kSlots;
+                    const u32x4* s_do = s_rows[buffer][1] + sub * G::kSlots;
+                    // row of register r: acc_row(r) of these
+                    const float* s_m = s_stats[buffer][0] + sub + 4 * half;
+                    const float* s_log_l = s_stats[buffer][1] + sub + 4 * half;
+                    const float* s_delta = s_stats[buffer][2] + sub + 4 * half;
+                    const float* s_time = s_stats[buffer][3] + sub + 4 * half;
+                    const int4* s_info = s_infos[buffer] + sub + 4 * half;
 
-                f32x16 x16 = zero16(), dp = zero16();
+                    f32x16 product = zero16(), dp = zero16();
 #pragma unroll
-                for (int st = 0; st < G::kSteps; ++st) {
-                    x16 = mma(G::row(s_q, lane & 31, st, half), k[st], x16);
-                    dp = mma(G::row(s_do, lane & 31, st, half), v[st], dp);
-                }
-                float x[16], cap_slope[16];
+                    for (int st = 0; st < G::kSteps; ++st) {
+                        product = mma(G::row(s_q, lane & 31, st, half), k[st], product);
+                        dp = mma(G::row(s_do, lane & 31, st, half), v[st], dp);
+                    }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = x16[r];
-                score_block<T>(sc, x, cap_slope);
-                if (sc.table) {
+                    for (int r = 0; r < 16; ++r) dp[r] -= s_delta[acc_row(r)];
+                    float x[16];
+                    if (sc.softcap > 0) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            float cap_slope;
+                            x[r] = capped<T>(sc, product[r], cap_slope);
+                            dp[r] *= cap_slope;
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] = product[r] * sc.scale2;
+                    }
+                    if (sc.table) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int d = s_info[acc_row(r)].z - j;
+                            x[r] += s_lut[min(max(d, -sc.reach), sc.reach) + sc.reach];
+                        }
+                    }
+                    if (sc.slopes) {
+                        if (sc.k_times) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                x[r] = fmaf(-slope, fabsf(s_time[acc_row(r)] - k_time), x[r]);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                x[r] = fmaf(-slope,
+                                            fabsf(static_cast<float>(s_info[acc_row(r)].z - j)),
+                                            x[r]);
+                        }
+                    }
+                    if (sc.biased()) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            x[r] = (x[r] - s_m[acc_row(r)]) - s_log_l[acc_row(r)];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] -= s_m[acc_row(r)];
+                    }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int d = s_diag[acc_row(r) + 4 * half] - j;
-                        x[r] += s_lut[min(max(d, -sc.reach), sc.reach) + sc.reach];
+                        x[r] = exp2_fast(x[r]);
+                        dp[r] *= x[r];
                     }
-                }
-                if (sc.slopes) {
+                    if (i0 < full_lo || i0 + 32 > full_hi) {
+                        const unsigned span = static_cast<unsigned>(last - first);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int at = acc_row(r) + 4 * half;
-                        const float gap = sc.k_times ? s_time[at] - k_time
-                                                     : static_cast<float>(s_diag[at] - j);
-                        x[r] = fmaf(-slope, fabsf(gap), x[r]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int at = acc_row(r) + 4 * half;
-                    x[r] = exp2_fast((x[r] - s_m[at]) - s_log_l[at]);
-                }
-                float ds[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    ds[r] = x[r] * (dp[r] - s_delta[acc_row(r) + 4 * half]);
-                if (i0 < full_lo || i0 + kRows > full_hi) {
-                    const unsigned span = static_cast<unsigned>(last - first);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = i0 + acc_row(r) + 4 * half;
-                        if (static_cast<unsigned>(i - first) >= span) x[r] = ds[r] = 0.0f;
-                    }
-                }
-                if (sc.softcap > 0) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ds[r] *= cap_slope[r];
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    Frag<T> p, s;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        p[e] = static_cast<T>(x[8 * t + e]);
-                        s[e] = static_cast<T>(ds[8 * t + e]);
+                        for (int r = 0; r < 16; ++r) {
+                            const int i = i0 + acc_row(r) + 4 * half;
+                            if (static_cast<unsigned>(i - first) >= span) x[r] = dp[r] = 0.0f;
+                        }
                     }
 #pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        dv[b] = mma(G::columns(s_do, 16 * t, b, lane), p, dv[b]);
-                        dk[b] = mma(G::columns(s_q, 16 * t, b, lane), s, dk[b]);
+                    for (int t = 0; t < 2; ++t) {
+                        Frag<T> p, ds;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            p[e] = static_cast<T>(x[8 * t + e]);
+                            ds[e] = static_cast<T>(dp[8 * t + e]);
+                        }
+#pragma unroll
+                        for (int b = 0; b < DB; ++b) {
+                            dv[b] = mma(G::columns(s_do, 16 * t, b, lane), p, dv[b]);
+                            dk[b] = mma(G::columns(s_q, 16 * t, b, lane), ds, dk[b]);
+                        }
                     }
                 }
             }
@@ -477,8 +510,7 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
                 store_row<float, DB>(a.part_k + at, dk, any, sc.scale, a.dim, half);
                 store_row<float, DB>(a.part_v + at, dv, any, 1.0f, a.dim, half);
             } else {
-                store_row<T, DB>(row_of<T>(a.d_k, j, kv_head), dk, any, sc.scale, a.dim,
-                                 half);
+                store_row<T, DB>(row_of<T>(a.d_k, j, kv_head), dk, any, sc.scale, a.dim, half);
                 store_row<T, DB>(row_of<T>(a.d_v, j, kv_head), dv, any, 1.0f, a.dim, half);
             }
         }
@@ -512,10 +544,11 @@ __global__ __launch_bounds__(kThreads) void attention_backward_kv_kernel(Backwar
         if (lane == 0) s_reduce[wave][1] = w_lo;
         __syncthreads();
         q_begin = kNone;
-        q_end = only;
+        q_end = __builtin_amdgcn_readfirstlane(only);
 #pragma unroll
         for (int w = 0; w < 4; ++w) q_begin = min(q_begin, s_reduce[w][1]);
-        i_first += (q_begin - i_first) / kRows * kRows;  // the same tiles: the same bits
+        q_begin = __builtin_amdgcn_readfirstlane(q_begin);
+        i_first = i_begin + (q_begin - i_begin) / kRows * kRows;  // the same tiles: the same bits
     }
 }
 
@@ -609,7 +642,7 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
     a.d_v = make_rows(p.d_v);
     a.q_info = reinterpret_cast<const int4*>(p.q_rows_info);
     a.k_info = reinterpret_cast<const int2*>(p.k_rows_info);
-    a.stats = reinterpret_cast<const float2*>(p.stats);
+    a.stats = p.stats;
     a.delta = reinterpret_cast<float*>(ws + l.delta);
     a.partial = reinterpret_cast<float*>(ws + l.partial);
     a.part_k = reinterpret_cast<float*>(ws + l.part_k);

@@ -182,37 +182,92 @@ struct Tile {
     }
 };
 
-// A tile on its way from global memory to LDS: kRows rows over kThreads
-// threads, in registers, so that the loads of one tile run beside the products
-// of the tile before it.
-template <typename T, int DB, int kRows, int kThreads>
-struct Staged {
-    typedef Tile<T, DB> G;
-    static constexpr int kChunks = kRows * G::kUsed;
-    static constexpr int kMine = (kChunks + kThreads - 1) / kThreads;
-    u32x4 r[kMine];
+// 16 bytes a lane from global memory to LDS at `lds` + 16 lane, past the
+// registers.  Written as text because the compiler, given its builtin, waits for
+// the copy before the next LDS read of any address, which is what copying
+// beside the products is to avoid.  It has no register to write; landed() waits
+// for it, and the statements around stay in order.
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(base)
+                 : "memory");
+}
+// The same of 4 bytes a lane.
+__device__ __forceinline__ void copy_word_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dword %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(base)
+                 : "memory");
+}
+// A wave's scalar: the LDS address of what it points to.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    typedef __attribute__((address_space(3))) const void* lds_ptr;
+    return __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(p))));
+}
+// Every copy of this wave has landed, and every wave is here.
+__device__ __forceinline__ void landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+}
+// floats first .. first + 63 of [begin, end), the nearest for those outside, by
+// one wave.
+__device__ __forceinline__ void load_floats(const float* base, int first, int begin, int end,
+                                            const float* lds, int lane) {
+    const int from = min(max(first, begin), end - 1);
+    const int at = min(max(first + lane, begin), end - 1) - from;
+    copy_word_to_lds(base + from, static_cast<uint32_t>(at) * 4, lds_address(lds));
+}
 
-    // Rows first .. of [rows, dim]; rows outside [begin, end) and columns from
-    // dim on are zeros.
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int dim, int first,
-                                         int begin, int end, int thread) {
+// A tile's way from global memory to LDS beside the products of the tile before
+// it: each lane names the 16 bytes that land in its slot, which is where the
+// swizzle is made.  Rows outside [begin, end) repeat its nearest row, columns
+// from `dim` on the row's first ones: they meet a P of 0, a q of 0 or an output
+// that is not stored, and hold nothing that the interval does not hold itself.
+template <typename T, int DB, int kRows, int kThreads>
+struct Loader {
+    typedef Tile<T, DB> G;
+    static constexpr int kSlots = kRows * G::kSlots;
+    static constexpr int kMine = kSlots / kThreads;
+    static_assert(kSlots % kThreads == 0, "whole waves fill a tile");
+    uint32_t pitch;          // bytes of a row: 64 of them fit 31 bits (checked on the host)
+    uint32_t offset[kMine];  // bytes from the tile's first row
+
+    __device__ __forceinline__ int row_of(int n, int thread) const {
+        return (thread + n * kThreads) / G::kSlots;
+    }
+    __device__ __forceinline__ Loader(int64_t row_stride, int dim, int thread)
+        : pitch(static_cast<uint32_t>(row_stride * sizeof(T))) {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
-            const int i = thread + n * kThreads;
-            const int row = first + i / G::kUsed;
-            const int col = (i % G::kUsed) * G::kElems;
-            const bool in = (kChunks % kThreads == 0 || i < kChunks) && row >= begin &&
-                            row < end && col < dim;
-            r[n] = in ? *reinterpret_cast<const u32x4*>(base + row * row_stride + col)
-                      : u32x4{0, 0, 0, 0};
+            const int row = row_of(n, thread);
+            const int chunk = ((thread + n * kThreads) % G::kSlots) ^ G::swizzle(row);
+            const int col = chunk * G::kElems < dim ? chunk * G::kElems : 0;
+            offset[n] = row * pitch + col * static_cast<uint32_t>(sizeof(T));
         }
     }
-    __device__ __forceinline__ void store(u32x4* lds, int thread) const {
+    // begin < end, first a wave's scalar
+    __device__ __forceinline__ void load(const T* base, int first, int begin, int end,
+                                         const u32x4* lds, int thread) const {
+        const int from = min(max(first, begin), end - 1);
+        const char* at = reinterpret_cast<const char*>(base) + static_cast<int64_t>(from) * pitch;
+        const uint32_t to = lds_address(lds + (thread & ~63));
+        if (first >= begin && first + kRows <= end) {
 #pragma unroll
-        for (int n = 0; n < kMine; ++n) {
-            const int i = thread + n * kThreads;
-            if (kChunks % kThreads == 0 || i < kChunks)
-                lds[G::slot(i / G::kUsed, i % G::kUsed)] = r[n];
+            for (int n = 0; n < kMine; ++n) copy_to_lds(at, offset[n], to + n * kThreads * 16);
+        } else {
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) {
+                const int row = row_of(n, thread);
+                const int near = min(max(first + row, begin), end - 1) - from;  // 0 .. kRows - 1
+                copy_to_lds(at, offset[n] + (near - row) * pitch, to + n * kThreads * 16);
+            }
         }
     }
 };
@@ -284,6 +339,8 @@ struct Score {
     int num_buckets, reach;
     const float* slopes;
     const float *q_times, *k_times;
+
+    __device__ __forceinline__ bool biased() const { return table || slopes; }
 };
 
 inline Score make_score(const trw_score& s) {
@@ -330,6 +387,71 @@ __device__ __forceinline__ float capped(const Score& s, float x, float& slope) {
         const float u = __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * s.cap_in));
         slope = 4.0f * u * (1.0f - u);
         return fmaf(-2.0f * s.cap_out, u, s.cap_out);
+    }
+}
+
+// Products to scores in base 2, without biases and mask.
+template <typename T, int kBlocks>
+__device__ __forceinline__ void cap_scores(const Score& sc, float (&s)[kBlocks][16]) {
+    if (sc.softcap > 0) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float unused;
+                s[b][r] = capped<T>(sc, s[b][r], unused);
+            }
+    } else {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] *= sc.scale2;
+    }
+}
+
+// Adds table and slope terms where a lane's column is a query (position `diag`
+// among the keys, time q_time; the wave's positions lie in [diag_lo, diag_hi])
+// and register (b, r) is key j0 + 32 b + acc_row(r) + 4 half.
+template <int kBlocks>
+__device__ __forceinline__ void add_biases(const Score& sc, float (&s)[kBlocks][16],
+                                           const float* lut, float slope, int diag, int diag_lo,
+                                           int diag_hi, float q_time, const float* k_time, int j0,
+                                           int half) {
+    const int at = diag - (j0 + 4 * half);  // distance of register (b, r): at - 32 b - acc_row(r)
+    if (sc.table) {
+        const int far_lo = diag_lo - (j0 + 32 * kBlocks - 1), far_hi = diag_hi - j0;
+        if (far_lo >= sc.reach || far_hi <= -sc.reach) {
+            const float bias = lut[far_lo >= sc.reach ? 2 * sc.reach : 0];
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] += bias;
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = at - (32 * b + acc_row(r));
+                    s[b][r] += lut[min(max(d, -sc.reach), sc.reach) + sc.reach];
+                }
+        }
+    }
+    if (sc.slopes) {
+        if (sc.k_times) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[b][r] = fmaf(-slope, fabsf(q_time - k_time[32 * b + acc_row(r) + 4 * half]),
+                                   s[b][r]);
+        } else {
+            const float from = static_cast<float>(at);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[b][r] = fmaf(-slope, fabsf(from - (32 * b + acc_row(r))), s[b][r]);
+        }
     }
 }
 

@@ -64,6 +64,8 @@ void check_rows(const trw_rows& r, int dtype, int64_t rows, const char* null_mes
     check_aligned(r.data, "rows must be 16-byte aligned");
     require(r.row_stride % piece == 0 && r.head_stride % piece == 0,
             "row and head strides must be multiples of 16 bytes");
+    require(r.row_stride >= 0 && r.row_stride <= (int64_t{1} << 22) && r.head_stride >= 0,
+            "row strides must be 0 to 2^22 elements");
 }
 
 void check_buckets(const float* table, const int32_t* buckets, int num_buckets, int reach) {

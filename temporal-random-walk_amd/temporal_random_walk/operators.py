@@ -29,6 +29,7 @@ LIB_PATH = os.path.join(HERE, "libtrw_operators.so")
 ABI_VERSION = 1  # TRW_OPS_ABI_VERSION of include/trw_operators.h
 MAX_REACH = 1024
 MAX_BUCKETS = 256
+MAX_ROW_STRIDE = 1 << 22  # elements
 
 # every symbol include/trw_operators.h declares
 EXPORTS = [
@@ -170,8 +171,11 @@ def _pieces(x):
 
 
 def _readable(x):
-    """The tensor, or a copy where its rows are not 16-byte pieces."""
-    return x if x.numel() == 0 or _pieces(x) else x.clone(memory_format=torch.contiguous_format)
+    """The tensor, or a copy where its rows are not 16-byte pieces (or lie further apart than the
+    kernels count)."""
+    if x.numel() == 0 or (_pieces(x) and x.stride(0) <= MAX_ROW_STRIDE):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _rows(x):
@@ -375,7 +379,7 @@ class _WalkAttention(torch.autograd.Function):
         p = _attention_params(q, k, v, out, table, mask, terms)
         stats = None
         if any(ctx.needs_input_grad[:4]):
-            stats = torch.empty(q.shape[1], q.shape[0], 2, dtype=torch.float32, device=device)
+            stats = torch.empty(2, q.shape[1], q.shape[0], dtype=torch.float32, device=device)
             p.stats = stats.data_ptr()
         with torch.cuda.device(device):
             space = _workspace(p, 0, device)  # noqa: F841  (held until the call has queued)
