@@ -26,7 +26,7 @@ struct BackwardArgs {
     const int2* k_info;
     const float* stats;
     float* delta;    // [heads, q_rows] D
-    float* partial;  // [heads, q tiles, num_buckets]
+    float* partial;  // [heads, q tiles, 2 reach + 1] dS by distance
     Score score;
     int q_rows, k_rows, heads, group, dim;
     int q_tiles, k_tiles;
@@ -53,10 +53,17 @@ __device__ __forceinline__ void score_block(const Score& sc, const f32x16& produ
 // ---- over query rows: dq, D, the table -------------------------------------------------------
 //
 // A lane holds one query row (column) and 16 keys at a time.  The table's
-// gradient is summed by distance in LDS: the rows of a half wave lie at
-// distinct distances from one key, so each half of each wave has a line of
-// sums of its own and adds to it without two lanes meeting; pairs past the
-// reach, which share two buckets, are summed in registers.
+// gradient needs dS summed by distance, along the diagonals of a block.  Float
+// atomics of LDS take some 100 cycles an instruction, so a wave writes 16 keys
+// of a block to a square of its own, each row followed by zeros, and every lane
+// reads one diagonal (rows kPitch + 1 apart, at constant offsets) and adds its
+// sum to the wave's line of distances.  Pairs past the reach, which share two
+// buckets, are summed in registers.  Rows whose walks' queries and keys are not
+// one distance apart (prompts of several walks) have no common diagonals and
+// take the atomics.
+constexpr int kPitch = 72;  // 32 values and zeros; two half waves' rows in other banks
+constexpr int kSquare = 17 * kPitch;
+
 template <typename T, int DB>
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(BackwardArgs a) {
     typedef Tile<T, DB> G;
@@ -64,7 +71,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     __shared__ u32x4 s_kv[2][2][kKeys * G::kSlots];
     __shared__ float s_times[2][64];
     __shared__ int s_reduce[4][4];
-    extern __shared__ float s_dyn[];  // bias by distance, then 8 lines of its gradient
+    extern __shared__ float s_dyn[];  // bias by distance; 4 lines of its gradient, 4 squares
 
     const int64_t items = static_cast<int64_t>(a.q_tiles) * a.heads;
     const int64_t item = xcd_item(blockIdx.x, items);
@@ -77,7 +84,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     const Score& sc = a.score;
     const int line = 2 * sc.reach + 1;
     float* s_lut = s_dyn;
-    float* s_sum = s_dyn + line + (wave * 2 + half) * line;
+    float* s_sum = s_dyn + line + wave * line;
+    float* s_square = s_dyn + 5 * line + wave * kSquare;
 
     const int i = tile * kTileRows + wave * 32 + (lane & 31);
     int4 info = {0, 0, 0, 0};
@@ -92,6 +100,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
 
     int w_lo = wave_min(any ? lo : kNone), w_hi = wave_max(any ? hi : 0);
     const int w_diag_lo = wave_min(any ? diag : kNone), w_diag_hi = wave_max(any ? diag : -kNone);
+    // distance of lane's row from key j: apart + i - j, where all rows agree
+    const int apart = wave_min(any ? diag - i : kNone);
+    const bool diagonal = apart == wave_max(any ? diag - i : -kNone);
     const int w_last_lo = wave_max(any ? lo : 0);
     if (lane == 0) {
         s_reduce[wave][0] = w_lo;
@@ -100,7 +111,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     }
     if (sc.table) {
         fill_bias(s_lut, sc, head, thread, kThreads);
-        for (int n = thread; n < 8 * line; n += kThreads) s_dyn[line + n] = 0.0f;
+        for (int n = thread; n < 4 * (line + kSquare); n += kThreads) s_dyn[line + n] = 0.0f;
     }
     __syncthreads();
     int k_begin = kNone, k_end = 0, last_lo = 0;
@@ -202,13 +213,31 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                         for (int r = 0; r < 16; ++r) sum += x[0][r];
                         if (far_lo >= sc.reach) far_before += sum;
                         else far_after += sum;
+                    } else if (diagonal) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                s_square[(1 + acc_row(r) + 4 * half) * kPitch + (lane & 31)] =
+                                    x[0][8 * t + r];
+                            // lane's diagonal: its rows less its keys are lane - 15 (0 .. 46)
+                            const int at = min(lane, 47) - 15;
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                sum += s_square[(1 + r) * kPitch + r + at];
+                            const int d = tile * kTileRows + wave * 32 + apart - (j0 + 16 * t) + at;
+                            far_before += d >= sc.reach ? sum : 0.0f;
+                            far_after += d <= -sc.reach ? sum : 0.0f;
+                            if (abs(d) < sc.reach && lane < 47) s_sum[d + sc.reach] += sum;
+                        }
                     } else {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int d = diag - (j_lane + acc_row(r));
-                            if (d >= sc.reach) far_before += x[0][r];
-                            else if (d <= -sc.reach) far_after += x[0][r];
-                            else if (any) atomicAdd(&s_sum[d + sc.reach], x[0][r]);
+                            far_before += d >= sc.reach ? x[0][r] : 0.0f;
+                            far_after += d <= -sc.reach ? x[0][r] : 0.0f;
+                            if (abs(d) < sc.reach) atomicAdd(&s_sum[d + sc.reach], x[0][r]);
                         }
                     }
                 }
@@ -268,7 +297,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     }
 
     if (!sc.table) return;
-    // this tile's sums by bucket: lanes' far sums first
+    // this tile's line: lanes' far sums first
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         far_before += __shfl_xor(far_before, o);
@@ -280,26 +309,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     }
     __syncthreads();
     float* s_line = s_dyn + line;
+    float* out = a.partial + (static_cast<int64_t>(head) * a.q_tiles + tile) * line;
     for (int n = thread; n < line; n += kThreads) {
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) sum += s_line[w * line + n];
-        s_line[n] = sum;
-    }
-    __syncthreads();
-    // buckets in any order: 8 threads look through the distances for each
-    const int part = thread & 7;
-    for (int b = thread >> 3; b < sc.num_buckets; b += kThreads / 8) {
-        float sum = 0.0f;
-        for (int n = part; n < line; n += 8) {
-            const int of = min(max(sc.buckets[n], 0), sc.num_buckets - 1);
-            if (of == b) sum += s_line[n];
-        }
-        sum += __shfl_xor(sum, 1);
-        sum += __shfl_xor(sum, 2);
-        sum += __shfl_xor(sum, 4);
-        if (part == 0)
-            a.partial[(static_cast<int64_t>(head) * a.q_tiles + tile) * sc.num_buckets + b] = sum;
+        for (int w = 0; w < 4; ++w) sum += s_line[w * line + n];
+        out[n] = sum;
     }
 }
 
@@ -611,9 +626,8 @@ Layout layout_of(const trw_attention_params& p) {
         return here;
     };
     l.delta = take(static_cast<uint64_t>(p.heads) * p.q_rows);
-    l.partial = take(p.score.table ? static_cast<uint64_t>(p.heads) * tiles_of(p.q_rows) *
-                                         p.score.num_buckets
-                                   : 0);
+    l.partial =
+        take(p.score.table ? join_table_floats(tiles_of(p.q_rows), p.heads, p.score.reach) : 0);
     const int splits = splits_of(p);
     const uint64_t part =
         splits > 1 ? static_cast<uint64_t>(splits) * p.k_rows * p.kv_heads * p.dim : 0;
@@ -664,7 +678,7 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
             hipLaunchKernelGGL(
                 (attention_backward_q_kernel<T, DB>),
                 dim3(static_cast<unsigned>(xcd_grid(static_cast<int64_t>(a.q_tiles) * a.heads))),
-                dim3(kThreads), 9 * line, stream, a);
+                dim3(kThreads), line ? 5 * line + 4 * kSquare * sizeof(float) : 0, stream, a);
         check_launch("attention_backward");
         if (a.k_tiles)
             hipLaunchKernelGGL((attention_backward_kv_kernel<T, DB>),
@@ -681,7 +695,8 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
         }
     });
     if (p.score.table) {
-        join_table(a.partial, a.q_tiles, p.heads, p.score.num_buckets, TRW_F32, p.d_table, stream);
+        join_table(a.partial, a.q_tiles, p.heads, p.score.buckets, a.score.reach,
+                   p.score.num_buckets, TRW_F32, p.d_table, stream);
     }
 }
 

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
     constexpr size_t kJoinBytes = kWaves * 32 * 33 * sizeof(float);
     constexpr size_t kBytes = kWaves * kTileBytes > kJoinBytes ? kWaves * kTileBytes : kJoinBytes;
     __shared__ u32x4 s_mem[kBytes / 16];
-    __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+    __shared__ float s_m[kWaves][32], s_l[kWaves][32], s_times[kWaves][32];
 
     const int split = blockIdx.x % a.splits;
     int rest = blockIdx.x / a.splits;
@@ -119,8 +119,12 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
     float m = kFloor, l = 0.0f;
     u32x4* s_tile = s_mem + wave * (kTileBytes / 16);
     CacheRows<T, DB> k, v;
+    // time of position j0 + (lane & 31), the nearest of the cache past its end
+    auto time_at = [&](int64_t j0) { return k_times[min(j0 + (lane & 31), max(n - 1, int64_t{0}))]; };
+    float next_time = 0.0f;
     int64_t block = block_begin + wave;
     if (block < block_end) {
+        if (k_times) next_time = time_at(block * kKeys);
         k.load(cache_k, a.k_pos, fresh_k, a.dim, block * kKeys, n, lane);
         v.load(cache_v, a.v_pos, fresh_v, a.dim, block * kKeys, n, lane);
     }
@@ -128,6 +132,10 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
         const int64_t j0 = block * kKeys;
         const bool more = block + kWaves < block_end;
         const int64_t j1 = j0 + kWaves * kKeys;
+        if (k_times) {
+            s_times[wave][lane & 31] = next_time;
+            if (more) next_time = time_at(j1);
+        }
         k.store(s_tile, lane);
         if (more) k.load(cache_k, a.k_pos, fresh_k, a.dim, j1, n, lane);
         f32x16 x = zero16();
@@ -154,12 +162,17 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
             }
         }
         if (sc.slopes) {
+            if (k_times) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float gap = static_cast<float>(last_d - acc_row(r));
-                if (k_times)
-                    gap = last_d > acc_row(r) ? q_time - k_times[n - (last_d - acc_row(r))] : 0.0f;
-                s[r] = fmaf(-slope, fabsf(gap), s[r]);
+                for (int r = 0; r < 16; ++r) {
+                    // the new event's own time is not in the cache yet: it is 0 away
+                    const float gap = q_time - s_times[wave][acc_row(r) + 4 * half];
+                    s[r] = fmaf(-slope, last_d == acc_row(r) ? 0.0f : fabsf(gap), s[r]);
+                }
+            } else {
+                const float from = static_cast<float>(last_d);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(from - acc_row(r)), s[r]);
             }
         }
         if (j0 + kKeys > n + 1) {
@@ -252,27 +265,53 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
         a.part_stats[part] = make_float2(top, total);
 }
 
-// Joins the workgroups of one walk and head: a thread for each element.
+// Joins the workgroups of one walk and head: 32 threads for the elements, four
+// each, and eight shares of the workgroups.
 template <typename T>
-__global__ __launch_bounds__(128) void join_step_kernel(StepArgs a) {
+__global__ __launch_bounds__(kThreads) void join_step_kernel(StepArgs a) {
+    __shared__ f32x4 s_sum[8][32];
+    __shared__ float s_total[8], s_top[4];
     const int head = blockIdx.x % a.heads;
     const int b = blockIdx.x / a.heads;
-    const int d = threadIdx.x;
+    const int thread = threadIdx.x, share = thread >> 5, d = (thread & 31) * 4;
     const int64_t part = (static_cast<int64_t>(b) * a.heads + head) * a.splits;
     float top = kFloor;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[part + s].x);
-    float total = 0.0f, sum = 0.0f;
-    if (d < a.dim)
-        for (int s = 0; s < a.splits; ++s) {
-            const float2 st = a.part_stats[part + s];
-            const float by = exp2_fast(st.x - top);
-            total = fmaf(by, st.y, total);
-            sum = fmaf(by, a.partial[(part + s) * a.dim + d], sum);
+    for (int s = thread; s < a.splits; s += kThreads) top = fmaxf(top, a.part_stats[part + s].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((thread & 63) == 0) s_top[thread >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    float total = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = share; s < a.splits; s += 8) {
+        const float2 st = a.part_stats[part + s];
+        const float by = exp2_fast(st.x - top);
+        total = fmaf(by, st.y, total);
+        if (d < a.dim) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.partial + (part + s) * a.dim + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, x[e], sum[e]);
         }
-    if (d >= a.dim) return;
+    }
+    s_sum[share][thread & 31] = sum;
+    if ((thread & 31) == 0) s_total[share] = total;
+    __syncthreads();
+    if (share || d >= a.dim) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+        total += s_total[w];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += s_sum[w][thread & 31][e];
+    }
     const int64_t n = a.lens[b];
-    const float value = n < 0 ? 0.0f : n >= a.capacity ? NAN : sum / total;
-    row_of<T>(a.out, b, head)[d] = static_cast<T>(value);
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        out[e] = static_cast<T>(n < 0 ? 0.0f : n >= a.capacity ? NAN : sum[e] / total);
+    *reinterpret_cast<t4*>(row_of<T>(a.out, b, head) + d) = out;
 }
 
 // Workgroups of one walk and key head: enough for four on each of the 256
@@ -332,7 +371,7 @@ void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
         check_launch("attention_step");
         if (a.splits > 1)
             hipLaunchKernelGGL((join_step_kernel<T>), dim3(static_cast<unsigned>(a.batch * a.heads)),
-                               dim3(128), 0, stream, a);
+                               dim3(kThreads), 0, stream, a);
         check_launch("attention_step");
     });
 }

@@ -503,9 +503,11 @@ void walk_mask(const trw_walk_mask_params& p, hipStream_t stream);
 uint64_t attention_workspace(const trw_attention_params& p, bool backward);
 void attention_forward(const trw_attention_params& p, hipStream_t stream);
 void attention_backward(const trw_attention_params& p, hipStream_t stream);
-// d_table [heads, num_buckets] of `dtype` from partial [heads, tiles, num_buckets].
-void join_table(const float* partial, int64_t tiles, int heads, int num_buckets, int dtype,
-                void* d_table, hipStream_t stream);
+// d_table [heads, num_buckets] of `dtype` from sums by distance, partial
+// [heads, tiles, 2 reach + 1]; what partial has room for: join_table_floats.
+uint64_t join_table_floats(int64_t tiles, int heads, int reach);
+void join_table(float* partial, int64_t tiles, int heads, const int32_t* buckets, int reach,
+                int num_buckets, int dtype, void* d_table, hipStream_t stream);
 uint64_t attention_step_workspace(const trw_attention_step_params& p);
 void attention_step(const trw_attention_step_params& p, hipStream_t stream);
 uint64_t relative_bias_workspace(const trw_relative_bias_params& p);

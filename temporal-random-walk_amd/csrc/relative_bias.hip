@@ -10,10 +10,9 @@
 // modulo a chunk, so a workgroup keeps the line once for each such place in
 // LDS, and every chunk is one aligned 16-byte read of the right copy.
 //
-// Backward: a wave walks down the rows with its lanes at fixed distances, eight
-// (float32: four) consecutive ones each, and sums them in registers; the loads
-// slide by one element a row.  The sums are taken to buckets once per tile of
-// rows, and the tiles' sums added in a fixed order.
+// Backward: sums by distance first, in lanes' registers and lines of LDS that
+// one wave adds to in its own order; workgroups' lines are joined in a fixed
+// order, and distances become buckets once, at the end.
 #include "operators.h"
 
 namespace trw {
@@ -21,14 +20,11 @@ namespace ops {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowsPerWave = 64;  // backward: of one tile
 
 struct BiasArgs {
     trw_relative_bias_params p;
-    int rows_per_group;  // forward
-    int row_tiles, bands;
-    int64_t first_distance;  // of band 0
-    float* partial;
+    int rows_per_group;
+    float* partial;  // backward: [heads, workgroups, 2 reach + 1]
 };
 
 // Chunks of a copy of the line: the first and the last are the ends alone, in
@@ -90,94 +86,182 @@ __global__ __launch_bounds__(kThreads) void relative_bias_kernel(BiasArgs a) {
     }
 }
 
+// Sums by distance: wave w walks down every fourth row of the workgroup's, its
+// lanes at consecutive 16-byte pieces.  Past the reach a sum in
+// registers is enough.  Within it a piece's elements go to the wave's own line
+// in LDS, distance d of it in slot (d % kElems) (line / kElems) + d / kElems, so
+// that lanes (kElems apart in distance) meet neither in a slot nor in a bank.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void relative_bias_backward_kernel(BiasArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void relative_bias_backward_kernel(BiasArgs a) {
     constexpr int kElems = 16 / sizeof(T);
-    constexpr int kBand = 64 * kElems;  // distances of a wave
-    __shared__ float s_sum[4][kBand];
+    constexpr int kAhead = 2;  // pieces of a lane in flight
+    extern __shared__ float s_lines[];  // [4][kElems * pieces]
     const trw_relative_bias_params& p = a.p;
-    const int band = blockIdx.x % a.bands;
-    const int tile = blockIdx.x / a.bands;
+    const int reach = p.reach, line = 2 * reach + 1;
+    const int pieces = (line + kElems - 1) / kElems;
     const int head = blockIdx.y;
     const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
+    for (int n = thread; n < 4 * kElems * pieces; n += kThreads) s_lines[n] = 0.0f;
+    __syncthreads();
+    float* s = s_lines + wave * kElems * pieces;
 
-    // this lane's elements of row i: columns i + j0 .., distances falling
-    const int64_t top_d = a.first_distance + static_cast<int64_t>(band + 1) * kBand - 1;
-    const int64_t j0 = p.q_offset - top_d + lane * kElems;
-    float sum[kElems];
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) sum[e] = 0.0f;
+    // Pieces begin at multiples of kElems whatever the rows' alignment, so that
+    // a gradient's layout does not change its bits.
+    typedef u32x4 loose __attribute__((aligned(2)));
+    union Piece {
+        u32x4 u;
+        T t[kElems];
+    };
     const T* base = static_cast<const T*>(p.d_out) + head * p.d_out_head_stride;
-    const int64_t row0 = (static_cast<int64_t>(tile) * 4 + wave) * kRowsPerWave;
-    const int64_t row1 = min(row0 + kRowsPerWave, p.q_len);
-    typedef u32x4 loose __attribute__((aligned(2)));  // slides by one element a row
-#pragma unroll 4
-    for (int64_t i = row0; i < row1; ++i) {
-        const int64_t j = i + j0;
+    const int k_len = static_cast<int>(p.k_len);
+    const int row0 = static_cast<int>(blockIdx.x * static_cast<int64_t>(a.rows_per_group)) + wave;
+    const int row1 = static_cast<int>(min((blockIdx.x + int64_t{1}) * a.rows_per_group, p.q_len));
+    auto fetch = [&](int i, int j) {
+        Piece x;
         const T* at = base + i * p.d_out_row_stride + j;
-        union {
-            u32x4 u;
-            T t[kElems];
-        } x;
-        if (j >= 0 && j + kElems <= p.k_len) {
+        if (j + kElems <= k_len) {
             x.u = *reinterpret_cast<const loose*>(at);
         } else {
+            x.u = u32x4{0, 0, 0, 0};
+            if (j < k_len) {
 #pragma unroll
-            for (int e = 0; e < kElems; ++e)
-                x.t[e] = j + e >= 0 && j + e < p.k_len ? at[e] : static_cast<T>(0.0f);
+                for (int e = 0; e < kElems; ++e)
+                    if (j + e < k_len) x.t[e] = at[e];
+            }
         }
+        return x;
+    };
+    // A wave's pieces in order, the next kAhead of them on their way
+    Piece x[kAhead];
+    int load_i = row0, load_g = 0;
+    auto advance = [&](int& i, int& g) {
+        g += 64 * kElems;
+        if (g >= k_len) {
+            g = 0;
+            i += kThreads / 64;
+        }
+    };
 #pragma unroll
-        for (int e = 0; e < kElems; ++e) sum[e] += static_cast<float>(x.t[e]);
+    for (int n = 0; n < kAhead; ++n)
+        if (load_i < row1) {
+            x[n] = fetch(load_i, load_g + lane * kElems);
+            advance(load_i, load_g);
+        }
+    float before = 0.0f, after = 0.0f;
+    for (int i = row0, g = 0; i < row1;) {
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            if (i >= row1) break;
+            const Piece now = x[n];
+            if (load_i < row1) {
+                x[n] = fetch(load_i, load_g + lane * kElems);
+                advance(load_i, load_g);
+            }
+            // distances of the wave's pieces: first .. first - 64 kElems + 1
+            const int first = i + static_cast<int>(p.q_offset) - g;
+            if (first - 64 * kElems + 1 >= reach || first <= -reach) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) sum += static_cast<float>(now.t[e]);
+                if (first <= -reach) after += sum;
+                else before += sum;
+            } else {
+                // Read, add, write: no two elements of a wave's pieces share a
+                // slot, and float atomics of LDS take 100 cycles an instruction.
+                const int mine = first - lane * kElems + reach;  // slot of element 0
+                float line_value[kElems];
+                int slot[kElems];
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) {
+                    const int at = mine - e;
+                    const float value = static_cast<float>(now.t[e]);
+                    before += at >= 2 * reach ? value : 0.0f;
+                    after += at <= 0 && reach > 0 ? value : 0.0f;
+                    const unsigned in = at > 0 && at < 2 * reach ? at : 0;  // 0: read only
+                    slot[e] = in % kElems * pieces + in / kElems;
+                    line_value[e] = s[slot[e]] + value;
+                }
+#pragma unroll
+                for (int e = 0; e < kElems; ++e)
+                    if (slot[e]) s[slot[e]] = line_value[e];
+            }
+            advance(i, g);
+        }
     }
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) s_sum[wave][lane * kElems + e] = sum[e];
+    for (int o = 32; o; o >>= 1) {
+        before += __shfl_xor(before, o);
+        after += __shfl_xor(after, o);
+    }
     __syncthreads();
-    for (int n = thread; n < kBand; n += kThreads)
-        s_sum[0][n] += s_sum[1][n] + s_sum[2][n] + s_sum[3][n];
+    if (lane == 0) {
+        const int at = 2 * reach;
+        s[at % kElems * pieces + at / kElems] += before;
+        s[0] += after;
+    }
     __syncthreads();
-    // to buckets, each by 8 threads; entry n is distance top_d - n
-    const int part = thread & 7;
-    for (int b = thread >> 3; b < p.num_buckets; b += kThreads / 8) {
-        float total = 0.0f;
-        for (int n = part; n < kBand; n += 8) {
-            const int64_t d =
-                min(max(top_d - n, -static_cast<int64_t>(p.reach)), static_cast<int64_t>(p.reach));
-            const int of = min(max(p.buckets[d + p.reach], 0), p.num_buckets - 1);
-            if (of == b) total += s_sum[0][n];
-        }
-        total += __shfl_xor(total, 1);
-        total += __shfl_xor(total, 2);
-        total += __shfl_xor(total, 4);
-        if (part == 0)
-            a.partial[(static_cast<int64_t>(head) * gridDim.x + blockIdx.x) * p.num_buckets + b] =
-                total;
+    float* out = a.partial + (static_cast<int64_t>(head) * gridDim.x + blockIdx.x) * line;
+    for (int n = thread; n < line; n += kThreads) {
+        const int at = n % kElems * pieces + n / kElems;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += s_lines[w * kElems * pieces + at];
+        out[n] = sum;
     }
 }
 
-// One workgroup per entry of the table sums the tiles' sums.
+// Sums tiles' lines into `groups` lines per head: a thread per distance, every
+// groups-th tile.
+__global__ __launch_bounds__(kThreads) void join_lines_kernel(const float* partial, int64_t tiles,
+                                                              int line, int groups, float* out) {
+    const int group = blockIdx.x % groups;
+    const int64_t head = blockIdx.x / groups;
+    for (int n = threadIdx.x; n < line; n += kThreads) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int64_t t = group; t < tiles; t += groups)
+            sum += partial[(head * tiles + t) * line + n];
+        out[(head * groups + group) * line + n] = sum;
+    }
+}
+
+// A head's lines to its table: distances first, in float64, then each bucket's
+// by eight threads (bucket ids may come in any order).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_table_kernel(const float* partial, int64_t tiles,
+__global__ __launch_bounds__(kThreads) void join_table_kernel(const float* lines, int64_t count,
+                                                              const int32_t* buckets, int line,
                                                               int num_buckets, T* d_table) {
-    const int bucket = blockIdx.x % num_buckets;
-    const int64_t head = blockIdx.x / num_buckets;
-    double sum = 0.0;
-    for (int64_t t = threadIdx.x; t < tiles; t += kThreads)
-        sum += partial[(head * tiles + t) * num_buckets + bucket];
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    __shared__ double s[4];
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
+    extern __shared__ double s_sum[];  // [line], then the ids
+    int* s_id = reinterpret_cast<int*>(s_sum + line);
+    const int64_t head = blockIdx.x;
+    for (int n = threadIdx.x; n < line; n += kThreads) {
+        double sum = 0.0;
+#pragma unroll 8
+        for (int64_t t = 0; t < count; ++t) sum += lines[(head * count + t) * line + n];
+        s_sum[n] = sum;
+        s_id[n] = min(max(buckets[n], 0), num_buckets - 1);
+    }
     __syncthreads();
-    if (threadIdx.x == 0)
-        d_table[head * num_buckets + bucket] =
-            static_cast<T>(static_cast<float>(s[0] + s[1] + s[2] + s[3]));
+    const int part = threadIdx.x & 7;
+    for (int b = threadIdx.x >> 3; b < num_buckets; b += kThreads / 8) {
+        double sum = 0.0;
+        for (int n = part; n < line; n += 8)
+            if (s_id[n] == b) sum += s_sum[n];
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        sum += __shfl_xor(sum, 4);
+        if (part == 0) d_table[head * num_buckets + b] = static_cast<T>(static_cast<float>(sum));
+    }
 }
 
-void shape_backward(BiasArgs& a) {
-    const int band = 64 * 16 / static_cast<int>(element_size(a.p.dtype));
-    a.first_distance = a.p.q_offset - a.p.k_len + 1;
-    a.bands = static_cast<int>((a.p.q_len + a.p.k_len - 1 + band - 1) / band);
-    a.row_tiles = static_cast<int>((a.p.q_len + 4 * kRowsPerWave - 1) / (4 * kRowsPerWave));
+constexpr int kGroups = 64;  // lines of a head that one workgroup still sums alone
+
+int64_t row_groups(const trw_relative_bias_params& p, int* rows_per_group) {
+    // as many rows as leave 2048 workgroups, in whole rounds of the four waves
+    int64_t rows = (p.q_len * p.heads + 2047) / 2048;
+    rows = (rows + 3) / 4 * 4;
+    *rows_per_group = static_cast<int>(rows);
+    return (p.q_len + rows - 1) / rows;
 }
 
 template <typename F>
@@ -189,13 +273,29 @@ void by_type(int dtype, F&& f) {
 
 }  // namespace
 
-void join_table(const float* partial, int64_t tiles, int heads, int num_buckets, int dtype,
-                void* d_table, hipStream_t stream) {
+uint64_t join_table_floats(int64_t tiles, int heads, int reach) {
+    const uint64_t line = 2 * static_cast<uint64_t>(reach) + 1;
+    return heads * line * (tiles + (tiles > kGroups ? kGroups : 0));
+}
+
+void join_table(float* partial, int64_t tiles, int heads, const int32_t* buckets, int reach,
+                int num_buckets, int dtype, void* d_table, hipStream_t stream) {
+    const int line = 2 * reach + 1;
+    const float* lines = partial;
+    int64_t count = tiles;
+    if (tiles > kGroups) {
+        float* grouped = partial + static_cast<int64_t>(heads) * tiles * line;
+        hipLaunchKernelGGL(join_lines_kernel, dim3(static_cast<unsigned>(heads * kGroups)),
+                           dim3(kThreads), 0, stream, partial, tiles, line, kGroups, grouped);
+        check_launch("join_lines");
+        lines = grouped;
+        count = kGroups;
+    }
     by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((join_table_kernel<T>), dim3(static_cast<unsigned>(heads * num_buckets)),
-                           dim3(kThreads), 0, stream, partial, tiles, num_buckets,
-                           static_cast<T*>(d_table));
+        hipLaunchKernelGGL((join_table_kernel<T>), dim3(static_cast<unsigned>(heads)),
+                           dim3(kThreads), line * (sizeof(double) + sizeof(int)), stream, lines,
+                           count, buckets, line, num_buckets, static_cast<T*>(d_table));
     });
     check_launch("join_table");
 }
@@ -226,30 +326,29 @@ void relative_bias(const trw_relative_bias_params& p, hipStream_t stream) {
 
 uint64_t relative_bias_workspace(const trw_relative_bias_params& p) {
     if (p.q_len == 0 || p.k_len == 0) return 0;
-    BiasArgs a{};
-    a.p = p;
-    shape_backward(a);
-    return static_cast<uint64_t>(p.heads) * a.bands * a.row_tiles * p.num_buckets * sizeof(float);
+    int rows;
+    return join_table_floats(row_groups(p, &rows), p.heads, p.reach) * sizeof(float);
 }
 
 void relative_bias_backward(const trw_relative_bias_params& p, hipStream_t stream) {
     require(p.workspace_bytes >= relative_bias_workspace(p), "workspace is too small");
-    if (p.heads == 0) return;
     BiasArgs a{};
     a.p = p;
     a.partial = static_cast<float*>(p.workspace);
-    int64_t tiles = 0;
+    int64_t groups = 0;
     if (p.q_len && p.k_len) {
-        shape_backward(a);
-        tiles = static_cast<int64_t>(a.bands) * a.row_tiles;
+        groups = row_groups(p, &a.rows_per_group);
         by_type(p.dtype, [&](auto t) {
+            constexpr int kElems = 16 / sizeof(t);
+            const int pieces = (2 * p.reach + 1 + kElems - 1) / kElems;
             hipLaunchKernelGGL((relative_bias_backward_kernel<decltype(t)>),
-                               dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(p.heads)),
-                               dim3(kThreads), 0, stream, a);
+                               dim3(static_cast<unsigned>(groups), static_cast<unsigned>(p.heads)),
+                               dim3(kThreads), 4 * kElems * pieces * sizeof(float), stream, a);
         });
         check_launch("relative_bias_backward");
     }
-    join_table(a.partial, tiles, p.heads, p.num_buckets, p.dtype, p.d_table, stream);
+    join_table(a.partial, groups, p.heads, p.buckets, p.reach, p.num_buckets, p.dtype, p.d_table,
+               stream);
 }
 
 }  // namespace ops
