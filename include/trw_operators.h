@@ -72,8 +72,11 @@ typedef struct trw_walk_mask_params {
     const int64_t *q_offsets, *k_offsets; /* packed: [docs + 1], ascending */
     const int64_t* prefix;              /* TRW_MASK_PREFIX: [docs] */
     int32_t kind;
-    int32_t* q_rows_info; /* out: [q_rows, 4] first key, end key, key at the row's own position, 0 */
-    int32_t* k_rows_info; /* out: [k_rows, 2] first query, end query */
+    int32_t* q_rows_info; /* out: [q_rows, 4] first key, end key, key at the row's own position,
+                             rows of its document (of queries or keys, whichever has more) */
+    int32_t* k_rows_info; /* out: [k_rows, 4] first query, end query, 0, rows of its document */
+    int32_t* docs_info;   /* out: [docs, 8] first query, queries, their rows with padding, first
+                             key, keys, their rows with padding, prefix, kind */
 } trw_walk_mask_params;
 trw_status trw_ops_walk_mask(const trw_walk_mask_params* params, void* stream);
 
@@ -98,7 +101,10 @@ typedef struct trw_attention_params {
     int32_t dtype; /* of q, k, v, out and their gradients */
     int32_t heads, kv_heads, dim; /* heads: a multiple of kv_heads, which it shares in order */
     int64_t q_rows, k_rows;
-    const int32_t *q_rows_info, *k_rows_info; /* of trw_ops_walk_mask */
+    const int32_t *q_rows_info, *k_rows_info, *docs_info; /* of trw_ops_walk_mask */
+    int64_t docs;
+    int64_t longest; /* no document has more queries or keys than this; 0: not known */
+    int32_t own_causal; /* 1: the mask is causal, over the queries' own rows as keys */
     trw_score score;
     trw_rows q, k, v, out;
     float* stats; /* [2, heads, q_rows], of the rows' softmax (base 2); written by the forward

@@ -50,7 +50,7 @@ HIP_FLAGS = [
 
 HIP_SOURCES = ["primitives.hip", "build.hip", "walk.hip", "handoff.hip", "pickers.hip", "capi.hip"]
 OPERATOR_SOURCES = ["walk_mask.hip", "attention.hip", "attention_backward.hip",
-                    "attention_step.hip", "relative_bias.hip", "operators_capi.hip"]
+                    "attention_walks.hip", "attention_step.hip", "relative_bias.hip", "operators_capi.hip"]
 PROBE_DIR = os.path.join(PKG_ROOT, "probe")
 
 

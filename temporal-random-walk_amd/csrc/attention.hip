@@ -38,6 +38,7 @@ struct ForwardArgs {
     Score score;
     int q_rows, k_rows, heads, group, dim;
     int tiles, splits;
+    int walk_limit;      // documents up to here go a wave each (attention_walks.hip)
     float* part_out;     // [splits, heads, q_rows, dim], where splits > 1
     float2* part_stats;  // [splits, heads, q_rows]
 };
@@ -80,7 +81,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
     const int i = tile * kTileRows + wave * kRowsPerWave + (lane & 31);
     int4 info = {0, 0, 0, 0};
     if (i < a.q_rows) info = a.q_info[i];
-    int lo = info.x, hi = max(info.x, min(info.y, a.k_rows));
+    const bool tiled_row = i < a.q_rows && tiled(info.w, a.walk_limit);
+    if (!__syncthreads_or(tiled_row)) return;
+    int lo = info.x, hi = tiled_row ? max(info.x, min(info.y, a.k_rows)) : info.x;
     const int diag = info.z;
     const bool any = lo < hi;
 
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
         }
 
         l += __shfl_xor(l, 32);
-        const bool mine = i < a.q_rows && (only < 0 || (any && info.x == only));
+        const bool mine = tiled_row && (only < 0 || (any && info.x == only));
         if (mine) {
             const bool seen = any && l != 0.0f;  // 0: the bias masks every key
             const int64_t stat = static_cast<int64_t>(head) * a.q_rows + i;
@@ -280,6 +283,7 @@ __global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
     const int64_t rows = static_cast<int64_t>(a.heads) * a.q_rows;
     if (t >= rows * pieces) return;
     const int64_t stat = t / pieces;  // head, row
+    if (!tiled(a.q_info[stat % a.q_rows].w, a.walk_limit)) return;
     const int col = static_cast<int>(t % pieces) * 4;
     float m = kFloor;
     for (int s = 0; s < a.splits; ++s) {
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
 // 256 keys or more if one walk has them all.
 int splits_of(const trw_attention_params& p) {
     const int64_t items = (p.q_rows + kTileRows - 1) / kTileRows * p.heads;
-    if (items == 0) return 1;
+    if (items == 0 || walk_blocks(p)) return 1;
     const int64_t splits = std::min<int64_t>({512 / items, p.k_rows / 256, 16});
     return static_cast<int>(std::max<int64_t>(splits, 1));
 }
@@ -331,7 +335,13 @@ uint64_t attention_workspace(const trw_attention_params& p, bool backward) {
 void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     if (p.q_rows == 0) return;
     require(p.workspace_bytes >= attention_workspace(p, false), "workspace is too small");
+    const int blocks = walk_blocks(p);
+    if (blocks) {
+        walk_forward(p, blocks, stream);
+        if (!walk_rest(p, blocks)) return;
+    }
     ForwardArgs a;
+    a.walk_limit = 32 * blocks;
     a.q = make_rows(p.q);
     a.k = make_rows(p.k);
     a.v = make_rows(p.v);

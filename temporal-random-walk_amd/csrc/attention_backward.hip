@@ -11,6 +11,8 @@
 // products of seven, and no sum is shared between workgroups, so nothing
 // depends on the order they run in and no float32 copy of a gradient goes
 // through memory.  Heads that share keys are one sum in registers.
+#include <algorithm>
+
 #include "operators.h"
 
 namespace trw {
@@ -23,7 +25,7 @@ constexpr int kTileRows = 128;  // query rows or keys of a workgroup
 struct BackwardArgs {
     Rows q, k, v, out, d_out, d_q, d_k, d_v;
     const int4* q_info;
-    const int2* k_info;
+    const int4* k_info;
     const float* stats;
     float* delta;    // [heads, q_rows] D
     float* partial;  // [heads, q tiles, 2 reach + 1] dS by distance
@@ -31,6 +33,7 @@ struct BackwardArgs {
     int q_rows, k_rows, heads, group, dim;
     int q_tiles, k_tiles;
     int splits;          // workgroups that share a key head's query heads
+    int walk_limit;      // documents up to here go a wave each (attention_walks.hip)
     float *part_k, *part_v;  // [splits, k_rows, kv_heads, dim], where splits > 1
 };
 
@@ -53,17 +56,10 @@ __device__ __forceinline__ void score_block(const Score& sc, const f32x16& produ
 // ---- over query rows: dq, D, the table -------------------------------------------------------
 //
 // A lane holds one query row (column) and 16 keys at a time.  The table's
-// gradient needs dS summed by distance, along the diagonals of a block.  Float
-// atomics of LDS take some 100 cycles an instruction, so a wave writes 16 keys
-// of a block to a square of its own, each row followed by zeros, and every lane
-// reads one diagonal (rows kPitch + 1 apart, at constant offsets) and adds its
-// sum to the wave's line of distances.  Pairs past the reach, which share two
-// buckets, are summed in registers.  Rows whose walks' queries and keys are not
-// one distance apart (prompts of several walks) have no common diagonals and
-// take the atomics.
-constexpr int kPitch = 72;  // 32 values and zeros; two half waves' rows in other banks
-constexpr int kSquare = 17 * kPitch;
-
+// gradient is dS by distance, along a block's diagonals (add_diagonals); pairs
+// past the reach are summed in registers.  Rows whose walks' queries and keys
+// are not one distance apart (prompts of several walks) have no common diagonals
+// and take float atomics on the wave's own line.
 template <typename T, int DB>
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(BackwardArgs a) {
     typedef Tile<T, DB> G;
@@ -90,7 +86,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     const int i = tile * kTileRows + wave * 32 + (lane & 31);
     int4 info = {0, 0, 0, 0};
     if (i < a.q_rows) info = a.q_info[i];
-    int lo = info.x, hi = max(info.x, min(info.y, a.k_rows));
+    const bool mine = i < a.q_rows && tiled(info.w, a.walk_limit);
+    int lo = info.x, hi = mine ? max(info.x, min(info.y, a.k_rows)) : info.x;
     const int diag = info.z;
     const bool any = lo < hi;
 
@@ -108,6 +105,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
         s_reduce[wave][0] = w_lo;
         s_reduce[wave][1] = w_hi;
         s_reduce[wave][2] = w_last_lo;
+    }
+    if (!__syncthreads_or(mine)) {
+        if (sc.table)
+            for (int n = thread; n < line; n += kThreads)
+                a.partial[(static_cast<int64_t>(head) * a.q_tiles + tile) * line + n] = 0.0f;
+        return;
     }
     if (sc.table) {
         fill_bias(s_lut, sc, head, thread, kThreads);
@@ -142,7 +145,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
         m = a.stats[stat];
         log_l = sc.biased() ? a.stats[static_cast<int64_t>(a.heads) * a.q_rows + stat] : 0.0f;
     }
-    if (i < a.q_rows && half == 0) a.delta[stat] = delta;
+    if (mine && half == 0) a.delta[stat] = delta;
     const float slope = sc.slopes ? sc.slopes[head] * kLog2e : 0.0f;
     const float q_time = sc.q_times && any ? sc.q_times[i] : 0.0f;
     const T* k_base = row_of<const T>(a.k, 0, kv_head);
@@ -214,23 +217,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                         if (far_lo >= sc.reach) far_before += sum;
                         else far_after += sum;
                     } else if (diagonal) {
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                s_square[(1 + acc_row(r) + 4 * half) * kPitch + (lane & 31)] =
-                                    x[0][8 * t + r];
-                            // lane's diagonal: its rows less its keys are lane - 15 (0 .. 46)
-                            const int at = min(lane, 47) - 15;
-                            float sum = 0.0f;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                sum += s_square[(1 + r) * kPitch + r + at];
-                            const int d = tile * kTileRows + wave * 32 + apart - (j0 + 16 * t) + at;
-                            far_before += d >= sc.reach ? sum : 0.0f;
-                            far_after += d <= -sc.reach ? sum : 0.0f;
-                            if (abs(d) < sc.reach && lane < 47) s_sum[d + sc.reach] += sum;
-                        }
+                        const int at = tile * kTileRows + wave * 32 + apart - j0;
+                        add_diagonals(x[0], s_square, s_sum, sc.reach, at, at + 31, lane, half);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
@@ -256,7 +244,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                 }
             }
         }
-        if (i < a.q_rows && (only < 0 || (any && info.x == only)))
+        if (mine && (only < 0 || (any && info.x == only)))
             store_row<T, DB>(row_of<T>(a.d_q, i, head), dq, any, sc.scale, a.dim, half);
         if (!mixed) break;
 
@@ -345,9 +333,11 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
     const Score& sc = a.score;
 
     const int j = tile * kTileRows + wave * 32 + (lane & 31);
-    int2 info = {0, 0};
+    int4 info = {0, 0, 0, 0};
     if (j < a.k_rows) info = a.k_info[j];
-    int first = info.x, last = max(info.x, min(info.y, a.q_rows));
+    const bool mine = j < a.k_rows && tiled(info.w, a.walk_limit);
+    if (!__syncthreads_or(mine)) return;
+    int first = info.x, last = mine ? max(info.x, min(info.y, a.q_rows)) : info.x;
     const bool any = first < last;
     const int doc = last;  // no two walks with pairs end at one query
 
@@ -518,7 +508,7 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
                 }
             }
         }
-        if (j < a.k_rows && (only < 0 || (any && doc == only))) {
+        if (mine && (only < 0 || (any && doc == only))) {
             if (a.splits > 1) {
                 const int64_t at =
                     ((static_cast<int64_t>(split) * a.k_rows + j) * kv_heads + kv_head) * a.dim;
@@ -578,6 +568,7 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(BackwardArgs a) {
     const int64_t rest = t / (a.dim / 4);
     const int head = static_cast<int>(rest % kv_heads);
     const int64_t row = rest / kv_heads;
+    if (!tiled(a.k_info[row].w, a.walk_limit)) return;
     const int64_t step = static_cast<int64_t>(a.k_rows) * kv_heads * a.dim;
     f32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
     for (int s = 0; s < a.splits; ++s) {
@@ -615,7 +606,7 @@ int splits_of(const trw_attention_params& p) {
 uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-    uint64_t delta, partial, part_k, part_v, bytes;
+    uint64_t delta, partial = 0, walk_partial = 0, lines = 0, part_k, part_v, bytes;
 };
 Layout layout_of(const trw_attention_params& p) {
     Layout l;
@@ -626,8 +617,13 @@ Layout layout_of(const trw_attention_params& p) {
         return here;
     };
     l.delta = take(static_cast<uint64_t>(p.heads) * p.q_rows);
-    l.partial =
-        take(p.score.table ? join_table_floats(tiles_of(p.q_rows), p.heads, p.score.reach) : 0);
+    if (p.score.table) {
+        const uint64_t heads = p.heads, line = 2 * static_cast<uint64_t>(p.score.reach) + 1;
+        const int blocks = walk_blocks(p);
+        l.partial = take(heads * tiles_of(p.q_rows) * line);
+        l.walk_partial = take(blocks ? heads * p.docs * walk_line(p, blocks) : 0);
+        l.lines = take(heads * 2 * kJoinGroups * line);
+    }
     const int splits = splits_of(p);
     const uint64_t part =
         splits > 1 ? static_cast<uint64_t>(splits) * p.k_rows * p.kv_heads * p.dim : 0;
@@ -655,7 +651,7 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
     a.d_k = make_rows(p.d_k);
     a.d_v = make_rows(p.d_v);
     a.q_info = reinterpret_cast<const int4*>(p.q_rows_info);
-    a.k_info = reinterpret_cast<const int2*>(p.k_rows_info);
+    a.k_info = reinterpret_cast<const int4*>(p.k_rows_info);
     a.stats = p.stats;
     a.delta = reinterpret_cast<float*>(ws + l.delta);
     a.partial = reinterpret_cast<float*>(ws + l.partial);
@@ -670,34 +666,58 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
     a.q_tiles = tiles_of(p.q_rows);
     a.k_tiles = tiles_of(p.k_rows);
     a.splits = splits_of(p);
+    const int blocks = walk_blocks(p);
+    const bool tiles = blocks == 0 || walk_rest(p, blocks);
+    a.walk_limit = 32 * blocks;
+    float* walk_partial = reinterpret_cast<float*>(ws + l.walk_partial);
+    if (blocks) walk_backward(p, blocks, walk_partial, stream);
     const size_t line = p.score.table ? (2 * a.score.reach + 1) * sizeof(float) : 0;
-    dispatch(p.dtype, p.dim, [&](auto t, auto db) {
-        typedef decltype(t) T;
-        constexpr int DB = decltype(db)::value;
-        if (a.q_tiles)
-            hipLaunchKernelGGL(
-                (attention_backward_q_kernel<T, DB>),
-                dim3(static_cast<unsigned>(xcd_grid(static_cast<int64_t>(a.q_tiles) * a.heads))),
-                dim3(kThreads), line ? 5 * line + 4 * kSquare * sizeof(float) : 0, stream, a);
-        check_launch("attention_backward");
-        if (a.k_tiles)
-            hipLaunchKernelGGL((attention_backward_kv_kernel<T, DB>),
-                               dim3(static_cast<unsigned>(xcd_grid(
-                                   static_cast<int64_t>(a.k_tiles) * p.kv_heads * a.splits))),
-                               dim3(kThreads), line, stream, a);
-        check_launch("attention_backward");
-        if (a.k_tiles && a.splits > 1) {
-            const int64_t n = p.k_rows * p.kv_heads * (p.dim / 4);
-            hipLaunchKernelGGL((join_splits_kernel<T>),
-                               dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)),
-                               dim3(kThreads), 0, stream, a);
+    if (tiles)
+        dispatch(p.dtype, p.dim, [&](auto t, auto db) {
+            typedef decltype(t) T;
+            constexpr int DB = decltype(db)::value;
+            if (a.q_tiles)
+                hipLaunchKernelGGL((attention_backward_q_kernel<T, DB>),
+                                   dim3(static_cast<unsigned>(
+                                       xcd_grid(static_cast<int64_t>(a.q_tiles) * a.heads))),
+                                   dim3(kThreads),
+                                   line ? 5 * line + 4 * kSquare * sizeof(float) : 0, stream, a);
             check_launch("attention_backward");
-        }
-    });
-    if (p.score.table) {
-        join_table(a.partial, a.q_tiles, p.heads, p.score.buckets, a.score.reach,
-                   p.score.num_buckets, TRW_F32, p.d_table, stream);
+            if (a.k_tiles)
+                hipLaunchKernelGGL((attention_backward_kv_kernel<T, DB>),
+                                   dim3(static_cast<unsigned>(xcd_grid(
+                                       static_cast<int64_t>(a.k_tiles) * p.kv_heads * a.splits))),
+                                   dim3(kThreads), line, stream, a);
+            check_launch("attention_backward");
+            if (a.k_tiles && a.splits > 1) {
+                const int64_t n = p.k_rows * p.kv_heads * (p.dim / 4);
+                hipLaunchKernelGGL((join_splits_kernel<T>),
+                                   dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)),
+                                   dim3(kThreads), 0, stream, a);
+                check_launch("attention_backward");
+            }
+        });
+    if (!p.score.table) return;
+    // the table: tiles' and walks' lines, in up to 64 sums of each
+    const int reach = a.score.reach;
+    const int64_t walks = blocks ? p.docs : 0, q_tiles = tiles ? a.q_tiles : 0;
+    const float* lines = a.partial;
+    int count = static_cast<int>(q_tiles);
+    if (walks || q_tiles > kJoinGroups) {
+        float* joined = reinterpret_cast<float*>(ws + l.lines);
+        const int tile_groups = static_cast<int>(std::min<int64_t>(q_tiles, kJoinGroups));
+        const int walk_groups = static_cast<int>(std::min<int64_t>(walks, kJoinGroups));
+        count = tile_groups + walk_groups;
+        if (tile_groups)
+            join_lines(a.partial, q_tiles, 2 * reach + 1, p.heads, tile_groups, joined, 0, count,
+                       reach, stream);
+        if (walk_groups)
+            join_lines(walk_partial, walks, walk_line(p, blocks), p.heads, walk_groups, joined,
+                       tile_groups, count, reach, stream);
+        lines = joined;
     }
+    join_table(lines, count, p.heads, p.score.buckets, reach, p.score.num_buckets, TRW_F32,
+               p.d_table, stream);
 }
 
 }  // namespace ops

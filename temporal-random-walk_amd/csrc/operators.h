@@ -455,6 +455,52 @@ __device__ __forceinline__ void add_biases(const Score& sc, float (&s)[kBlocks][
     }
 }
 
+// Sums of a block's dS by distance, along its diagonals.  Float atomics of LDS
+// take some 100 cycles an instruction (counted), so a wave writes 16 keys at a
+// time to a square of its own, each row followed by zeros, and every lane reads
+// one diagonal (rows kPitch + 1 apart, at constant offsets) and adds its sum to
+// the wave's line of distances -reach .. reach.  Pairs past the reach share the
+// line's ends: sums over lanes.
+constexpr int kPitch = 72;  // 32 values and zeros; two half waves' rows in other banks
+constexpr int kSquare = 17 * kPitch;
+
+// v: register r is key acc_row(r) + 4 half, the lane's column a query row; lo,
+// hi: distances of the first and last row from the block's first key.
+__device__ __forceinline__ void add_diagonals(const float (&v)[16], float* square, float* line,
+                                              int reach, int lo, int hi, int lane, int half) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            square[(1 + acc_row(r) + 4 * half) * kPitch + (lane & 31)] = v[8 * t + r];
+        // lane's diagonal: its row less its key is lane - 15 (lanes 0 .. 46)
+        const int at = min(lane, 47) - 15;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += square[(1 + r) * kPitch + r + at];
+        const int d = lo - 16 * t + at;
+        const bool mine = lane < 47;
+        if (mine && abs(d) < reach) line[d + reach] += sum;
+        if (hi - 16 * t >= reach || lo - 16 * t - 15 <= -reach) {
+            float before = mine && d >= reach ? sum : 0.0f;
+            float after = mine && d <= -reach && reach ? sum : 0.0f;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) {
+                before += __shfl_xor(before, o);
+                after += __shfl_xor(after, o);
+            }
+            if (lane == 0) {
+                line[2 * reach] += before;
+                line[0] += after;
+            }
+        }
+    }
+}
+
+// Whether a document of `size` rows (0: a row of no document) belongs to the
+// kernels of tiles, when documents up to `limit` go a wave each.
+__device__ __forceinline__ bool tiled(int size, int limit) { return size == 0 || size > limit; }
+
 struct Rows {
     char* data;
     int64_t row, head;  // strides in elements
@@ -501,13 +547,25 @@ inline size_t element_size(int dtype) { return dtype == TRW_F32 ? 4 : 2; }
 // Implementations behind the C ABI (operators_capi.hip checks the arguments).
 void walk_mask(const trw_walk_mask_params& p, hipStream_t stream);
 uint64_t attention_workspace(const trw_attention_params& p, bool backward);
+// Short walks (attention_walks.hip): how many blocks of 32 rows one may have
+// (0: none go there), whether longer ones may be in the batch, floats of one
+// line of the table's gradient.
+int walk_blocks(const trw_attention_params& p);
+bool walk_rest(const trw_attention_params& p, int blocks);
+int walk_line(const trw_attention_params& p, int blocks);
+void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream);
+void walk_backward(const trw_attention_params& p, int blocks, float* partial, hipStream_t stream);
 void attention_forward(const trw_attention_params& p, hipStream_t stream);
 void attention_backward(const trw_attention_params& p, hipStream_t stream);
-// d_table [heads, num_buckets] of `dtype` from sums by distance, partial
-// [heads, tiles, 2 reach + 1]; what partial has room for: join_table_floats.
-uint64_t join_table_floats(int64_t tiles, int heads, int reach);
-void join_table(float* partial, int64_t tiles, int heads, const int32_t* buckets, int reach,
+// A table's gradient from sums by distance: join_lines adds up to `groups`
+// lines per head from `partial` [heads, tiles, short_line] (distances
+// -short_line / 2 ..) at line `first` of `lines` [heads, count, 2 reach + 1];
+// join_table makes d_table [heads, num_buckets] of `dtype` of those.
+void join_lines(const float* partial, int64_t tiles, int short_line, int heads, int groups,
+                float* lines, int first, int count, int reach, hipStream_t stream);
+void join_table(const float* lines, int count, int heads, const int32_t* buckets, int reach,
                 int num_buckets, int dtype, void* d_table, hipStream_t stream);
+constexpr int kJoinGroups = 64;
 uint64_t attention_step_workspace(const trw_attention_step_params& p);
 void attention_step(const trw_attention_step_params& p, hipStream_t stream);
 uint64_t relative_bias_workspace(const trw_relative_bias_params& p);

@@ -92,6 +92,9 @@ const trw_attention_params& checked(const trw_attention_params* p) {
     require(((p->q_rows + 127) / 128 + 8) * p->heads < (int64_t{1} << 31) &&
                 ((p->k_rows + 127) / 128 + 8) * p->heads < (int64_t{1} << 31),
             "too many rows and heads");
+    require(p->docs >= 0 && p->docs < kMaxRows && p->longest >= 0,
+            "docs must be 0 to 2^30 - 1, longest not negative");
+    require(p->docs * p->kv_heads < (int64_t{1} << 31), "too many documents and heads");
     check_score(p->score);
     return *p;
 }
@@ -103,6 +106,8 @@ void check_forward(const trw_attention_params& p) {
     check_rows(p.out, p.dtype, p.q_rows, "out is null");
     require(p.q_rows == 0 || p.q_rows_info, "q_rows_info is null");
     check_aligned(p.q_rows_info, "q_rows_info must be 16-byte aligned");
+    require(p.docs == 0 || p.docs_info, "docs_info is null");
+    check_aligned(p.docs_info, "docs_info must be 16-byte aligned");
     require(reinterpret_cast<uintptr_t>(p.stats) % 8 == 0, "stats must be 8-byte aligned");
 }
 
@@ -159,8 +164,9 @@ trw_status trw_ops_walk_mask(const trw_walk_mask_params* params, void* stream) {
         require((p.q_rows == 0 || p.q_rows_info) && (p.k_rows == 0 || p.k_rows_info),
                 "the rows' info is null");
         check_aligned(p.q_rows_info, "q_rows_info must be 16-byte aligned");
-        require(reinterpret_cast<uintptr_t>(p.k_rows_info) % 8 == 0,
-                "k_rows_info must be 8-byte aligned");
+        check_aligned(p.k_rows_info, "k_rows_info must be 16-byte aligned");
+        require(p.docs == 0 || p.docs_info, "docs_info is null");
+        check_aligned(p.docs_info, "docs_info must be 16-byte aligned");
         trw::ops::walk_mask(p, static_cast<hipStream_t>(stream));
     });
 }
@@ -193,8 +199,7 @@ trw_status trw_ops_attention_backward(const trw_attention_params* params, void* 
         require(p.q_rows == 0 || p.stats, "stats is null");
         require(p.k_rows == 0 || p.k_rows_info, "k_rows_info is null");
         require(!p.score.table || p.d_table, "d_table is null");
-        require(reinterpret_cast<uintptr_t>(p.k_rows_info) % 8 == 0,
-                "k_rows_info must be 8-byte aligned");
+        check_aligned(p.k_rows_info, "k_rows_info must be 16-byte aligned");
         check_aligned(p.workspace, "workspace must be 16-byte aligned");
         trw::ops::attention_backward(p, static_cast<hipStream_t>(stream));
     });

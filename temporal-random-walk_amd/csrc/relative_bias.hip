@@ -213,15 +213,21 @@ __global__ __launch_bounds__(kThreads, 6) void relative_bias_backward_kernel(Bia
 // Sums tiles' lines into `groups` lines per head: a thread per distance, every
 // groups-th tile.
 __global__ __launch_bounds__(kThreads) void join_lines_kernel(const float* partial, int64_t tiles,
-                                                              int line, int groups, float* out) {
+                                                              int short_line, int groups,
+                                                              float* lines, int first, int count,
+                                                              int line) {
     const int group = blockIdx.x % groups;
     const int64_t head = blockIdx.x / groups;
+    float* out = lines + (head * count + first + group) * line;
     for (int n = threadIdx.x; n < line; n += kThreads) {
+        const int at = n - (line - short_line) / 2;
         float sum = 0.0f;
-#pragma unroll 4
-        for (int64_t t = group; t < tiles; t += groups)
-            sum += partial[(head * tiles + t) * line + n];
-        out[(head * groups + group) * line + n] = sum;
+        if (at >= 0 && at < short_line) {
+#pragma unroll 8
+            for (int64_t t = group; t < tiles; t += groups)
+                sum += partial[(head * tiles + t) * short_line + at];
+        }
+        out[n] = sum;
     }
 }
 
@@ -254,8 +260,6 @@ __global__ __launch_bounds__(kThreads) void join_table_kernel(const float* lines
     }
 }
 
-constexpr int kGroups = 64;  // lines of a head that one workgroup still sums alone
-
 int64_t row_groups(const trw_relative_bias_params& p, int* rows_per_group) {
     // as many rows as leave 2048 workgroups, in whole rounds of the four waves
     int64_t rows = (p.q_len * p.heads + 2047) / 2048;
@@ -273,24 +277,17 @@ void by_type(int dtype, F&& f) {
 
 }  // namespace
 
-uint64_t join_table_floats(int64_t tiles, int heads, int reach) {
-    const uint64_t line = 2 * static_cast<uint64_t>(reach) + 1;
-    return heads * line * (tiles + (tiles > kGroups ? kGroups : 0));
+void join_lines(const float* partial, int64_t tiles, int short_line, int heads, int groups,
+                float* lines, int first, int count, int reach, hipStream_t stream) {
+    hipLaunchKernelGGL(join_lines_kernel, dim3(static_cast<unsigned>(heads * groups)),
+                       dim3(kThreads), 0, stream, partial, tiles, short_line, groups, lines, first,
+                       count, 2 * reach + 1);
+    check_launch("join_lines");
 }
 
-void join_table(float* partial, int64_t tiles, int heads, const int32_t* buckets, int reach,
+void join_table(const float* lines, int count, int heads, const int32_t* buckets, int reach,
                 int num_buckets, int dtype, void* d_table, hipStream_t stream) {
     const int line = 2 * reach + 1;
-    const float* lines = partial;
-    int64_t count = tiles;
-    if (tiles > kGroups) {
-        float* grouped = partial + static_cast<int64_t>(heads) * tiles * line;
-        hipLaunchKernelGGL(join_lines_kernel, dim3(static_cast<unsigned>(heads * kGroups)),
-                           dim3(kThreads), 0, stream, partial, tiles, line, kGroups, grouped);
-        check_launch("join_lines");
-        lines = grouped;
-        count = kGroups;
-    }
     by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         hipLaunchKernelGGL((join_table_kernel<T>), dim3(static_cast<unsigned>(heads)),
@@ -327,7 +324,9 @@ void relative_bias(const trw_relative_bias_params& p, hipStream_t stream) {
 uint64_t relative_bias_workspace(const trw_relative_bias_params& p) {
     if (p.q_len == 0 || p.k_len == 0) return 0;
     int rows;
-    return join_table_floats(row_groups(p, &rows), p.heads, p.reach) * sizeof(float);
+    const uint64_t groups = row_groups(p, &rows);
+    return (groups + kJoinGroups) * p.heads * (2 * static_cast<uint64_t>(p.reach) + 1) *
+           sizeof(float);
 }
 
 void relative_bias_backward(const trw_relative_bias_params& p, hipStream_t stream) {
@@ -347,8 +346,16 @@ void relative_bias_backward(const trw_relative_bias_params& p, hipStream_t strea
         });
         check_launch("relative_bias_backward");
     }
-    join_table(a.partial, groups, p.heads, p.buckets, p.reach, p.num_buckets, p.dtype, p.d_table,
-               stream);
+    const int line = 2 * p.reach + 1;
+    float* lines = a.partial;
+    if (groups > kJoinGroups) {
+        lines = a.partial + groups * p.heads * line;
+        join_lines(a.partial, groups, line, p.heads, kJoinGroups, lines, 0, kJoinGroups, p.reach,
+                   stream);
+        groups = kJoinGroups;
+    }
+    join_table(lines, static_cast<int>(groups), p.heads, p.buckets, p.reach, p.num_buckets, p.dtype,
+               p.d_table, stream);
 }
 
 }  // namespace ops

@@ -4,7 +4,8 @@
 // Every mask here (a walk's own keys, causal, prefix, padding) leaves a query
 // an interval of key rows, and, the documents being in order in both, leaves a
 // key an interval of query rows.  The attention kernels work from these
-// intervals alone.  One thread per row of either side; a packed row finds its
+// intervals alone (a wave with a walk of its own, from the walk's spans).  One
+// thread per row of either side and per document; a packed row finds its
 // document by a binary search of the offsets.
 #include "operators.h"
 
@@ -54,7 +55,8 @@ struct MaskArgs {
     }
 };
 
-__global__ __launch_bounds__(kB) void walk_mask_kernel(MaskArgs a, unsigned q_blocks) {
+__global__ __launch_bounds__(kB) void walk_mask_kernel(MaskArgs a, unsigned q_blocks,
+                                                            unsigned k_blocks) {
     const trw_walk_mask_params& p = a.p;
     if (blockIdx.x < q_blocks) {
         const int64_t i = blockIdx.x * static_cast<int64_t>(kB) + threadIdx.x;
@@ -73,12 +75,14 @@ __global__ __launch_bounds__(kB) void walk_mask_kernel(MaskArgs a, unsigned q_bl
                 info.y = static_cast<int>(k.begin + seen);
                 info.z = static_cast<int>(k.begin + pos);
             }
+            if (local >= 0 && (local < q.len || !p.q_offsets))
+                info.w = static_cast<int>(max(max(q.len, k.len), int64_t{1}));
         }
         reinterpret_cast<int4*>(p.q_rows_info)[i] = info;
-    } else {
+    } else if (blockIdx.x < q_blocks + k_blocks) {
         const int64_t j = (blockIdx.x - q_blocks) * static_cast<int64_t>(kB) + threadIdx.x;
         if (j >= p.k_rows) return;
-        int2 info = {0, 0};
+        int4 info = {0, 0, 0, 0};
         if (p.docs > 0) {
             const int64_t w = a.doc_of(j, p.k_offsets, p.k_length);
             const Span q = a.q_span(w), k = a.k_span(w);
@@ -90,8 +94,21 @@ __global__ __launch_bounds__(kB) void walk_mask_kernel(MaskArgs a, unsigned q_bl
                 info.x = static_cast<int>(q.begin + first);
                 info.y = static_cast<int>(q.begin + q.len);
             }
+            if (local >= 0 && (local < k.len || !p.k_offsets))
+                info.w = static_cast<int>(max(max(q.len, k.len), int64_t{1}));
         }
-        reinterpret_cast<int2*>(p.k_rows_info)[j] = info;
+        reinterpret_cast<int4*>(p.k_rows_info)[j] = info;
+    } else {
+        const int64_t w = (blockIdx.x - q_blocks - k_blocks) * static_cast<int64_t>(kB) + threadIdx.x;
+        if (w >= p.docs) return;
+        const Span q = a.q_span(w), k = a.k_span(w);
+        int4* out = reinterpret_cast<int4*>(p.docs_info) + 2 * w;
+        // rows of padding are the document's as well
+        out[0] = int4{static_cast<int>(q.begin), static_cast<int>(q.len),
+                      static_cast<int>(p.q_offsets ? q.len : p.q_length),
+                      static_cast<int>(k.begin)};
+        out[1] = int4{static_cast<int>(k.len), static_cast<int>(p.k_offsets ? k.len : p.k_length),
+                      static_cast<int>(a.prefix_of(w, k.len)), p.kind};
     }
 }
 
@@ -106,8 +123,9 @@ void walk_mask(const trw_walk_mask_params& p, hipStream_t stream) {
     }
     const unsigned qb = static_cast<unsigned>((p.q_rows + kB - 1) / kB);
     const unsigned kb = static_cast<unsigned>((p.k_rows + kB - 1) / kB);
-    if (qb + kb == 0) return;
-    hipLaunchKernelGGL(walk_mask_kernel, dim3(qb + kb), dim3(kB), 0, stream, a, qb);
+    const unsigned db = static_cast<unsigned>((p.docs + kB - 1) / kB);
+    if (qb + kb + db == 0) return;
+    hipLaunchKernelGGL(walk_mask_kernel, dim3(qb + kb + db), dim3(kB), 0, stream, a, qb, kb);
     check_launch("walk_mask");
 }
 

@@ -52,7 +52,8 @@ class _MaskParams(C.Structure):
                 ("q_length", C.c_int64), ("k_length", C.c_int64),
                 ("q_lens", C.c_void_p), ("k_lens", C.c_void_p),
                 ("q_offsets", C.c_void_p), ("k_offsets", C.c_void_p), ("prefix", C.c_void_p),
-                ("kind", C.c_int32), ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p)]
+                ("kind", C.c_int32), ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
+                ("docs_info", C.c_void_p)]
 
 
 class _Score(C.Structure):
@@ -64,7 +65,10 @@ class _Score(C.Structure):
 class _AttentionParams(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
                 ("dim", C.c_int32), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
-                ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p), ("score", _Score),
+                ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
+                ("docs_info", C.c_void_p), ("docs", C.c_int64), ("longest", C.c_int64),
+                ("own_causal", C.c_int32),
+                ("score", _Score),
                 ("q", _Rows), ("k", _Rows), ("v", _Rows), ("out", _Rows), ("stats", C.c_void_p),
                 ("d_out", _Rows), ("d_q", _Rows), ("d_k", _Rows), ("d_v", _Rows),
                 ("d_table", C.c_void_p), ("workspace", C.c_void_p),
@@ -239,10 +243,16 @@ class WalkMask:
         self.q_shape, self.k_shape = q_shape, k_shape  # leading dimensions of q; of k and v
         self.device = device
         self.q_info = torch.empty(q_rows, 4, dtype=torch.int32, device=device)
-        self.k_info = torch.empty(k_rows, 2, dtype=torch.int32, device=device)
+        self.k_info = torch.empty(k_rows, 4, dtype=torch.int32, device=device)
+        self.docs_info = torch.empty(docs, 8, dtype=torch.int32, device=device)
+        self.docs = docs
+        # of any document, where the host knows it
+        self.longest = max(q_length, k_length) if q_offsets is None else 0
+        self.own_causal = kind == "causal" and k_lens is None and k_offsets is None
         p = _MaskParams(docs, q_rows, k_rows, q_length, k_length, _ptr(q_lens), _ptr(k_lens),
                         _ptr(q_offsets), _ptr(k_offsets), _ptr(prefix), _KINDS[kind],
-                        self.q_info.data_ptr(), self.k_info.data_ptr())
+                        self.q_info.data_ptr(), self.k_info.data_ptr(),
+                        self.docs_info.data_ptr())
         with torch.cuda.device(device):
             _call(lib().trw_ops_walk_mask, C.byref(p), _stream(device))
 
@@ -356,8 +366,10 @@ def _attention_params(q, k, v, out, table, mask, terms):
     return _AttentionParams(
         dtype=_DTYPES[q.dtype], heads=q.shape[1], kv_heads=k.shape[1], dim=q.shape[2],
         q_rows=mask.q_rows, k_rows=mask.k_rows, q_rows_info=mask.q_info.data_ptr(),
-        k_rows_info=mask.k_info.data_ptr(), score=terms.struct(table), q=_rows(q), k=_rows(k),
-        v=_rows(v), out=_rows(out))
+        k_rows_info=mask.k_info.data_ptr(), docs_info=mask.docs_info.data_ptr(), docs=mask.docs,
+        longest=mask.longest, own_causal=mask.own_causal,
+        score=terms.struct(table), q=_rows(q), k=_rows(k), v=_rows(v),
+        out=_rows(out))
 
 
 def _workspace(p, backward, device):
