@@ -124,6 +124,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
     const float q_time = sc.q_times && any ? sc.q_times[i] : 0.0f;
     const T* k_base = row_of<const T>(a.k, 0, kv_head);
     const T* v_base = row_of<const T>(a.v, 0, kv_head);
+    const uint32_t at_kv = lds_address(s_kv), at_times = lds_address(s_times);
     const Loader<T, DB, kKeys, kThreads> k_load(a.k.row, a.dim, thread);
     const Loader<T, DB, kKeys, kThreads> v_load(a.v.row, a.dim, thread);
     // Scores that are only products are scaled inside the exponential
@@ -142,10 +143,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
         const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
 
         auto fetch = [&](int j0, int buffer) {
-            k_load.load(k_base, j0, k_begin, k_end, s_kv[buffer][0], thread);
-            v_load.load(v_base, j0, k_begin, k_end, s_kv[buffer][1], thread);
+            k_load.load(k_base, j0, k_begin, k_end, at_kv + buffer * 2 * kTileChunks * 16, thread);
+            v_load.load(v_base, j0, k_begin, k_end, at_kv + (buffer * 2 + 1) * kTileChunks * 16, thread);
             if (sc.k_times && wave == 0)
-                load_floats(sc.k_times, j0, k_begin, k_end, s_times[buffer], lane);
+                load_floats(sc.k_times, j0, k_begin, k_end, at_times + buffer * 256, lane);
         };
         int buffer = 0;
         if (j_first < j_last) fetch(j_first, 0);

@@ -150,6 +150,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     const float q_time = sc.q_times && any ? sc.q_times[i] : 0.0f;
     const T* k_base = row_of<const T>(a.k, 0, kv_head);
     const T* v_base = row_of<const T>(a.v, 0, kv_head);
+    constexpr int kTileBytes = kKeys * G::kSlots * 16;
+    const uint32_t at_kv = lds_address(s_kv), at_times = lds_address(s_times);
     const Loader<T, DB, kKeys, kThreads> k_load(a.k.row, a.dim, thread);
     const Loader<T, DB, kKeys, kThreads> v_load(a.v.row, a.dim, thread);
     float far_before = 0.0f, far_after = 0.0f;  // dS past the reach, either way
@@ -163,10 +165,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
         for (int b = 0; b < DB; ++b) dq[b] = zero16();
         const int full_lo = wave_max(any ? lo : kNone), full_hi = wave_min(any ? hi : 0);
         auto fetch = [&](int j0, int buffer) {
-            k_load.load(k_base, j0, k_begin, k_end, s_kv[buffer][0], thread);
-            v_load.load(v_base, j0, k_begin, k_end, s_kv[buffer][1], thread);
+            k_load.load(k_base, j0, k_begin, k_end, at_kv + buffer * 2 * kTileBytes, thread);
+            v_load.load(v_base, j0, k_begin, k_end, at_kv + (buffer * 2 + 1) * kTileBytes, thread);
             if (sc.k_times && wave == 0)
-                load_floats(sc.k_times, j0, k_begin, k_end, s_times[buffer], lane);
+                load_floats(sc.k_times, j0, k_begin, k_end, at_times + buffer * 256, lane);
         };
         int buffer = 0;
         if (j_first < k_end) fetch(j_first, 0);
@@ -368,6 +370,9 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
     const int heads_each = (a.group + a.splits - 1) / a.splits;
     const int head_begin = kv_head * a.group + split * heads_each;
     const int head_end = min(head_begin + heads_each, (kv_head + 1) * a.group);
+    constexpr int kTileBytes = kRows * G::kSlots * 16;
+    const uint32_t at_rows = lds_address(s_rows), at_stats = lds_address(s_stats),
+                   at_infos = lds_address(s_infos);
     const Loader<T, DB, kRows, kThreads> q_load(a.q.row, a.dim, thread);
     const Loader<T, DB, kRows, kThreads> do_load(a.d_out.row, a.dim, thread);
     const bool positions = sc.table || (sc.slopes && !sc.k_times);
@@ -394,22 +399,23 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
             __syncthreads();  // the head before is done with its biases and tiles
             if (sc.table) fill_bias(s_lut, sc, head, thread, kThreads);
             auto fetch = [&](int i0, int buffer) {
-                q_load.load(q_base, i0, q_begin, q_end, s_rows[buffer][0], thread);
-                do_load.load(do_base, i0, q_begin, q_end, s_rows[buffer][1], thread);
+                q_load.load(q_base, i0, q_begin, q_end, at_rows + buffer * 2 * kTileBytes, thread);
+                do_load.load(do_base, i0, q_begin, q_end, at_rows + (buffer * 2 + 1) * kTileBytes,
+                             thread);
                 if (wave == 0) {
-                    load_floats(m_base, i0, q_begin, q_end, s_stats[buffer][0], lane);
+                    load_floats(m_base, i0, q_begin, q_end, at_stats + (buffer * 4 + 0) * 256, lane);
                     if (sc.biased())
-                        load_floats(log_l_base, i0, q_begin, q_end, s_stats[buffer][1], lane);
+                        load_floats(log_l_base, i0, q_begin, q_end, at_stats + (buffer * 4 + 1) * 256, lane);
                 } else if (wave == 1) {
-                    load_floats(delta_base, i0, q_begin, q_end, s_stats[buffer][2], lane);
+                    load_floats(delta_base, i0, q_begin, q_end, at_stats + (buffer * 4 + 2) * 256, lane);
                 } else if (wave == 2) {
                     if (sc.q_times)
-                        load_floats(sc.q_times, i0, q_begin, q_end, s_stats[buffer][3], lane);
+                        load_floats(sc.q_times, i0, q_begin, q_end, at_stats + (buffer * 4 + 3) * 256, lane);
                 } else if (positions) {
                     const int from = min(max(i0, q_begin), q_end - 1);
                     const int at = min(max(i0 + lane, q_begin), q_end - 1) - from;
                     copy_to_lds(a.q_info + from, static_cast<uint32_t>(at) * 16,
-                                lds_address(s_infos[buffer]));
+                                at_infos + buffer * 1024);
                 }
             };
             int buffer = 0;

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
     __shared__ float s_time[128];
     __shared__ float s_lut[64 * kNB + 1];
 
-    const int lane = threadIdx.x, half = lane >> 5;
+    int lane = threadIdx.x;
     const int kv_head = blockIdx.x % a.kv_heads;
     const Doc d = load_doc(a.docs, blockIdx.x / a.kv_heads);
     if (max(d.q_len, d.k_len) > a.limit) return;  // the tiles' kernel has it
@@ -120,23 +120,28 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
     auto load_q = [&](Frag<T>(&f)[G::kSteps], int step) {
         const int i = step % q_blocks * 32 + (lane & 31);
         load_operand<T, DB>(f, row_of<const T>(a.q, d.q_begin + i, first_head + step / q_blocks),
-                            i < d.q_len, a.dim, half);
+                            i < d.q_len, a.dim, lane >> 5);
     };
     if (steps > 0 && k_blocks > 0) {
         const Loader<T, DB, 32, 64> k_load(a.k.row, a.dim, lane), v_load(a.v.row, a.dim, lane);
         const T* k_base = row_of<const T>(a.k, d.k_begin, kv_head);
         const T* v_base = row_of<const T>(a.v, d.k_begin, kv_head);
         for (int b = 0; b < k_blocks; ++b) {
-            k_load.load(k_base, 32 * b, 0, d.k_len, s_k + b * kBlock, lane);
-            v_load.load(v_base, 32 * b, 0, d.k_len, s_v + b * kBlock, lane);
+            k_load.load(k_base, 32 * b, 0, d.k_len, lds_address(s_k) + b * kBlock * 16, lane);
+            v_load.load(v_base, 32 * b, 0, d.k_len, lds_address(s_v) + b * kBlock * 16, lane);
         }
         if (sc.k_times)
             for (int j = 0; j < d.k_len; j += 64)
-                load_floats(sc.k_times + d.k_begin, j, 0, d.k_len, s_time + j, lane);
+                load_floats(sc.k_times + d.k_begin, j, 0, d.k_len, lds_address(s_time) + j * 4,
+                            lane);
         load_q(next, 0);
     }
     for (int step = 0; step < steps; ++step) {
         const int head = first_head + step / q_blocks, i0 = step % q_blocks * 32;
+        // What follows from the lane is worked out for every step: held over the
+        // loop, it would take the registers that the scores need.
+        asm volatile("" : "+v"(lane));
+        const int half = lane >> 5;
         if (sc.table && i0 == 0) fill_walk_bias<kNB>(s_lut, a.score, head, lane);
 #pragma unroll
         for (int s = 0; s < G::kSteps; ++s) q[s] = next[s];
@@ -221,14 +226,14 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
 // in the first half and the most in the second, the last wave the other way
 // round.  P and dS lie where the keys and values were.
 template <typename T, int DB, int kNB, bool kShared>
-__global__ __launch_bounds__(64 * kNB, kShared ? 1 : 2) void walk_backward_kernel(WalkArgs a) {
+__global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 : 2) void walk_backward_kernel(WalkArgs a) {
     typedef Tile<T, DB> G;
     typedef Tile<T, 1> S;  // P and dS of a block: rows of queries, columns of keys
     constexpr int kBlock = 32 * G::kSlots;
     constexpr int kTile = 32 * S::kSlots;
     extern __shared__ u32x4 s_mem[];
 
-    const int lane = threadIdx.x & 63, half = lane >> 5;
+    int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.x % a.kv_heads;
     const int doc = blockIdx.x / a.kv_heads;
@@ -244,6 +249,7 @@ __global__ __launch_bounds__(64 * kNB, kShared ? 1 : 2) void walk_backward_kerne
                     a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * line + n] = 0.0f;
         return;
     }
+    const uint32_t at_mem = lds_address(s_mem);
     u32x4* s_q = s_mem;
     u32x4* s_do = s_q + kNB * kBlock;
     u32x4* s_k = s_do + kNB * kBlock;
@@ -261,15 +267,10 @@ __global__ __launch_bounds__(64 * kNB, kShared ? 1 : 2) void walk_backward_kerne
     };
     auto most_of = [&](int q) { return d.seen(min(32 * q + 31, d.q_len - 1)); };
     const bool q_mine = wave < q_blocks && k_blocks > 0;
-    const int i0 = 32 * wave, i = i0 + (lane & 31);
-    const bool in = i < d.q_len;
-    const int row = min(i, d.q_len - 1);
-    const int seen = in && q_mine ? d.seen(row) : 0;  // rows past the end have no part in dk, dv
+    const int i0 = 32 * wave;
     const int least = i0 + 32 <= d.q_len ? d.seen(i0) : 0;
     const int most = q_mine ? most_of(wave) : 0;
-    const int diag = d.k_len - d.q_len + row;
     const int diag_lo = d.k_len - d.q_len + i0, diag_hi = diag_lo + 31;
-    const int j = 32 * wave + (lane & 31);
 
     const T* k_base = row_of<const T>(a.k, d.k_begin, kv_head);
     const T* v_base = row_of<const T>(a.v, d.k_begin, kv_head);
@@ -286,21 +287,33 @@ __global__ __launch_bounds__(64 * kNB, kShared ? 1 : 2) void walk_backward_kerne
 #pragma unroll 1
     for (int g = 0; g < heads; ++g) {
         const int head = first_head + g;
+        // What follows from the lane is worked out for every head: held over
+        // the loop, it would take the registers that the scores need.
+        if (kShared) asm volatile("" : "+v"(lane));
+        const int half = lane >> 5;
+        const int i = i0 + (lane & 31);
+        const bool in = i < d.q_len;
+        const int row = min(i, d.q_len - 1);
+        const int seen = in && q_mine ? d.seen(row) : 0;  // rows past the end have no part in dk, dv
+        const int diag = d.k_len - d.q_len + row;
         if (kShared && g) __syncthreads();  // the head before is done with its tiles
         if (q_mine) {
             const Loader<T, DB, 32, 64> q_load(a.q.row, a.dim, lane);
             const Loader<T, DB, 32, 64> do_load(a.d_out.row, a.dim, lane);
-            q_load.load(row_of<const T>(a.q, d.q_begin, head), i0, 0, d.q_len, s_q + wave * kBlock,
-                        lane);
+            q_load.load(row_of<const T>(a.q, d.q_begin, head), i0, 0, d.q_len,
+                        at_mem + wave * kBlock * 16, lane);
             do_load.load(row_of<const T>(a.d_out, d.q_begin, head), i0, 0, d.q_len,
-                         s_do + wave * kBlock, lane);
+                         at_mem + (kNB + wave) * kBlock * 16, lane);
         }
         if (wave < k_blocks) {
             const Loader<T, DB, 32, 64> k_load(a.k.row, a.dim, lane), v_load(a.v.row, a.dim, lane);
-            k_load.load(k_base, 32 * wave, 0, d.k_len, s_k + wave * kBlock, lane);
-            v_load.load(v_base, 32 * wave, 0, d.k_len, s_v + wave * kBlock, lane);
+            k_load.load(k_base, 32 * wave, 0, d.k_len, at_mem + (2 * kNB + wave) * kBlock * 16,
+                        lane);
+            v_load.load(v_base, 32 * wave, 0, d.k_len, at_mem + (3 * kNB + wave) * kBlock * 16,
+                        lane);
             if (sc.k_times)
-                load_floats(sc.k_times + d.k_begin, 32 * wave, 0, d.k_len, s_time + 32 * wave, lane);
+                load_floats(sc.k_times + d.k_begin, 32 * wave, 0, d.k_len,
+                            at_mem + a.time_at * 16 + 128 * wave, lane);
         }
         float m = 0.0f, log_l = 0.0f, q_time = 0.0f;
         if (q_mine) {
@@ -463,6 +476,7 @@ __global__ __launch_bounds__(64 * kNB, kShared ? 1 : 2) void walk_backward_kerne
             }
         }
     }
+    const int half = lane >> 5, j = 32 * wave + (lane & 31);
     if (j < d.k_len) {
         const bool any = heads > 0 && d.first(j) < d.q_len;
         store_row<T, DB>(row_of<T>(a.d_k, d.k_begin + j, kv_head), dk, any, sc.scale, a.dim, half);

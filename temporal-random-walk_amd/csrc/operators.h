@@ -204,11 +204,11 @@ __device__ __forceinline__ void copy_word_to_lds(const void* base, uint32_t offs
                  : "s"(lds), "v"(offset), "s"(base)
                  : "memory");
 }
-// A wave's scalar: the LDS address of what it points to.
+// The LDS address of a __shared__ array (pass the array itself: of a pointer
+// that came a longer way the compiler does not know that it is one).
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     typedef __attribute__((address_space(3))) const void* lds_ptr;
-    return __builtin_amdgcn_readfirstlane(
-        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(p))));
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(p)));
 }
 // Every copy of this wave has landed, and every wave is here.
 __device__ __forceinline__ void landed() {
@@ -219,10 +219,10 @@ __device__ __forceinline__ void landed() {
 // floats first .. first + 63 of [begin, end), the nearest for those outside, by
 // one wave.
 __device__ __forceinline__ void load_floats(const float* base, int first, int begin, int end,
-                                            const float* lds, int lane) {
+                                            uint32_t lds, int lane) {
     const int from = min(max(first, begin), end - 1);
     const int at = min(max(first + lane, begin), end - 1) - from;
-    copy_word_to_lds(base + from, static_cast<uint32_t>(at) * 4, lds_address(lds));
+    copy_word_to_lds(base + from, static_cast<uint32_t>(at) * 4, lds);
 }
 
 // A tile's way from global memory to LDS beside the products of the tile before
@@ -252,12 +252,12 @@ struct Loader {
             offset[n] = row * pitch + col * static_cast<uint32_t>(sizeof(T));
         }
     }
-    // begin < end, first a wave's scalar
-    __device__ __forceinline__ void load(const T* base, int first, int begin, int end,
-                                         const u32x4* lds, int thread) const {
+    // To the LDS address `lds`.  begin < end; first and lds are a wave's scalars.
+    __device__ __forceinline__ void load(const T* base, int first, int begin, int end, uint32_t lds,
+                                         int thread) const {
         const int from = min(max(first, begin), end - 1);
         const char* at = reinterpret_cast<const char*>(base) + static_cast<int64_t>(from) * pitch;
-        const uint32_t to = lds_address(lds + (thread & ~63));
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (thread & ~63) * 16);
         if (first >= begin && first + kRows <= end) {
 #pragma unroll
             for (int n = 0; n < kMine; ++n) copy_to_lds(at, offset[n], to + n * kThreads * 16);
