@@ -157,7 +157,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
             const u32x4* s_k = s_kv[buffer][0];
             const u32x4* s_v = s_kv[buffer][1];
             const float* s_time = s_times[buffer];
-
             float s[kBlocks][16];
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {

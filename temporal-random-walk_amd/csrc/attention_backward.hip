@@ -181,6 +181,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                 if (j0 >= w_hi || j0 + 32 <= w_lo) continue;
                 const u32x4* s_k = s_kv[buffer][0] + sub * G::kSlots;
                 const u32x4* s_v = s_kv[buffer][1] + sub * G::kSlots;
+                // LDS addresses are worked out for each block: held over the
+                // loop, they would take the registers of the sums
+                int at_lane = lane;
+                asm volatile("" : "+v"(at_lane));
 
                 f32x16 product = zero16(), dp = zero16();
 #pragma unroll
@@ -242,7 +246,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                     for (int e = 0; e < 8; ++e) ds[e] = static_cast<T>(x[0][8 * t + e]);
 #pragma unroll
                     for (int b = 0; b < DB; ++b)
-                        dq[b] = mma(G::columns(s_k, 16 * t, b, lane), ds, dq[b]);
+                        dq[b] = mma(G::columns(s_k, 16 * t, b, at_lane), ds, dq[b]);
                 }
             }
         }
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
 // A lane holds one key (column) and 16 query rows at a time; q and dO pass
 // through LDS and are read both ways.
 template <typename T, int DB>
-__global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_kv_kernel(
+__global__ __launch_bounds__(kThreads, DB < 4 ? 2 : 1) void attention_backward_kv_kernel(
     BackwardArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
@@ -429,6 +433,8 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
                     if (i0 >= w_hi || i0 + 32 <= w_lo) continue;
                     const u32x4* s_q = s_rows[buffer][0] + sub * G::kSlots;
                     const u32x4* s_do = s_rows[buffer][1] + sub * G::kSlots;
+                    int at_lane = lane;  // as above
+                    if (DB == 3) asm volatile("" : "+v"(at_lane));
                     // row of register r: acc_row(r) of these
                     const float* s_m = s_stats[buffer][0] + sub + 4 * half;
                     const float* s_log_l = s_stats[buffer][1] + sub + 4 * half;
@@ -439,8 +445,9 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
                     f32x16 product = zero16(), dp = zero16();
 #pragma unroll
                     for (int st = 0; st < G::kSteps; ++st) {
-                        product = mma(G::row(s_q, lane & 31, st, half), k[st], product);
-                        dp = mma(G::row(s_do, lane & 31, st, half), v[st], dp);
+                        product = mma(G::row(s_q, at_lane & 31, st, at_lane >> 5), k[st], product);
+                        dp = mma(G::row(s_do, at_lane & 31, st, at_lane >> 5), v[st], dp);
+                        if (DB == 3 && st % 2) hold_reads();
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dp[r] -= s_delta[acc_row(r)];
@@ -507,8 +514,9 @@ __global__ __launch_bounds__(kThreads, DB < 3 ? 2 : 1) void attention_backward_k
                         }
 #pragma unroll
                         for (int b = 0; b < DB; ++b) {
-                            dv[b] = mma(G::columns(s_do, 16 * t, b, lane), p, dv[b]);
-                            dk[b] = mma(G::columns(s_q, 16 * t, b, lane), ds, dk[b]);
+                            dv[b] = mma(G::columns(s_do, 16 * t, b, at_lane), p, dv[b]);
+                            dk[b] = mma(G::columns(s_q, 16 * t, b, at_lane), ds, dk[b]);
+                            if (DB == 3) hold_reads();
                         }
                     }
                 }

@@ -33,42 +33,35 @@ struct StepArgs {
     float2* part_stats;  // [batch, heads, splits]
 };
 
-// Rows first .. of a cache [positions, dim] into registers; row `last` is the
-// call's own; rows past it are zeros.
+// All but this wave's last kLater copies to LDS have landed.
+template <int kLater>
+__device__ __forceinline__ void copies_landed() {
+    static_assert(kLater < 64, "counted in six bits");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | (kLater >> 4 << 14));
+    asm volatile("" ::: "memory");
+}
+
+// The call's own row, in every row of a tile from `from` on.
 template <typename T, int DB>
-struct CacheRows {
+__device__ __forceinline__ void put_row(u32x4* tile, const T* row, int from, int dim, int lane) {
     typedef Tile<T, DB> G;
-    static constexpr int kMine = kKeys * G::kUsed / 64;
-    u32x4 r[kMine];
-    __device__ __forceinline__ void load(const T* cache, int64_t stride, const T* fresh, int dim,
-                                         int64_t first, int64_t last, int lane) {
-#pragma unroll
-        for (int n = 0; n < kMine; ++n) {
-            const int at = lane + n * 64;
-            const int64_t row = first + at / G::kUsed;
-            const int col = (at % G::kUsed) * G::kElems;
-            const T* from = row == last ? fresh : cache + row * stride;
-            r[n] = row <= last && col < dim ? *reinterpret_cast<const u32x4*>(from + col)
-                                            : u32x4{0, 0, 0, 0};
-        }
+    for (int n = from * G::kUsed + lane; n < kKeys * G::kUsed; n += 64) {
+        const int col = n % G::kUsed * G::kElems;
+        tile[G::slot(n / G::kUsed, n % G::kUsed)] =
+            col < dim ? *reinterpret_cast<const u32x4*>(row + col) : u32x4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void store(u32x4* lds, int lane) const {
-#pragma unroll
-        for (int n = 0; n < kMine; ++n) {
-            const int at = lane + n * 64;
-            lds[G::slot(at / G::kUsed, at % G::kUsed)] = r[n];
-        }
-    }
-};
+}
 
 template <typename T, int DB>
 __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
     typedef Tile<T, DB> G;
     constexpr size_t kTileBytes = G::bytes(kKeys);
     constexpr size_t kJoinBytes = kWaves * 32 * 33 * sizeof(float);
-    constexpr size_t kBytes = kWaves * kTileBytes > kJoinBytes ? kWaves * kTileBytes : kJoinBytes;
+    constexpr size_t kBytes =
+        2 * kWaves * kTileBytes > kJoinBytes ? 2 * kWaves * kTileBytes : kJoinBytes;
     __shared__ u32x4 s_mem[kBytes / 16];
-    __shared__ float s_m[kWaves][32], s_l[kWaves][32], s_times[kWaves][32];
+    __shared__ float s_m[kWaves][32], s_l[kWaves][32], s_times[kWaves][64];
 
     const int split = blockIdx.x % a.splits;
     int rest = blockIdx.x / a.splits;
@@ -76,7 +69,8 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
     rest /= a.columns;
     const int kv_head = rest % a.kv_heads;
     const int b = rest / a.kv_heads;
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, half = lane >> 5;
+    const int thread = threadIdx.x, lane = thread & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const Score& sc = a.score;
 
     const int64_t n = a.lens[b];  // position of the new event
@@ -117,47 +111,67 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
 #pragma unroll
     for (int c = 0; c < DB; ++c) o[c] = zero16();
     float m = kFloor, l = 0.0f;
-    u32x4* s_tile = s_mem + wave * (kTileBytes / 16);
-    CacheRows<T, DB> k, v;
-    // time of position j0 + (lane & 31), the nearest of the cache past its end
-    auto time_at = [&](int64_t j0) { return k_times[min(j0 + (lane & 31), max(n - 1, int64_t{0}))]; };
-    float next_time = 0.0f;
-    int64_t block = block_begin + wave;
-    if (block < block_end) {
-        if (k_times) next_time = time_at(block * kKeys);
-        k.load(cache_k, a.k_pos, fresh_k, a.dim, block * kKeys, n, lane);
-        v.load(cache_v, a.v_pos, fresh_v, a.dim, block * kKeys, n, lane);
+    // The wave's tile of keys and of values.  The next keys are on their way
+    // while this block's softmax and values are worked on, the next values
+    // while the next scores are: each is waited for by the number of copies
+    // asked for after it.
+    u32x4* s_k = s_mem + wave * 2 * (kTileBytes / 16);
+    u32x4* s_v = s_k + kTileBytes / 16;
+    const uint32_t at_k = lds_address(s_mem) + wave * 2 * kTileBytes;
+    const Loader<T, DB, kKeys, 64> k_load(a.k_pos, a.dim, lane), v_load(a.v_pos, a.dim, lane);
+    constexpr int kCopies = Loader<T, DB, kKeys, 64>::kMine;
+    const int length = static_cast<int>(n);  // rows of the cache
+    auto fetch_k = [&](int j) {
+        k_load.load(cache_k, j, 0, length, at_k, lane);
+        if (k_times) load_floats(k_times, j, 0, length, lds_address(s_times) + wave * 256, lane);
+    };
+    auto fetch_v = [&](int j) { v_load.load(cache_v, j, 0, length, at_k + kTileBytes, lane); };
+    int block = static_cast<int>(block_begin) + wave;
+    if (block < block_end && block * kKeys < length) {
+        fetch_k(block * kKeys);
+        fetch_v(block * kKeys);
     }
+#pragma unroll 1
     for (; block < block_end; block += kWaves) {
-        const int64_t j0 = block * kKeys;
-        const bool more = block + kWaves < block_end;
-        const int64_t j1 = j0 + kWaves * kKeys;
-        if (k_times) {
-            s_times[wave][lane & 31] = next_time;
-            if (more) next_time = time_at(j1);
+        const int j0 = block * kKeys;
+        const int j1 = j0 + kWaves * kKeys;
+        const bool more = block + kWaves < block_end && j1 < length;
+        int at_lane = lane;  // LDS addresses are not held over the loop
+        asm volatile("" : "+v"(at_lane));
+        copies_landed<kCopies>();  // keys; the values, asked for last, may be on their way
+        if (j0 + kKeys > length) {
+            copies_landed<0>();
+            put_row<T, DB>(s_k, fresh_k, length - j0, a.dim, at_lane);
+            put_row<T, DB>(s_v, fresh_v, length - j0, a.dim, at_lane);
         }
-        k.store(s_tile, lane);
-        if (more) k.load(cache_k, a.k_pos, fresh_k, a.dim, j1, n, lane);
         f32x16 x = zero16();
 #pragma unroll
-        for (int st = 0; st < G::kSteps; ++st) x = mma(G::row(s_tile, lane & 31, st, half), q[st], x);
+        for (int st = 0; st < G::kSteps; ++st)
+            x = mma(G::row(s_k, at_lane & 31, st, at_lane >> 5), q[st], x);
         float s[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float unused;
             s[r] = sc.softcap > 0 ? capped<T>(sc, x[r], unused) : x[r] * sc.scale2;
         }
+        float time[16];
+        if (k_times) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) time[r] = s_times[wave][acc_row(r) + 4 * half];
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): read, so the next keys may come
+        if (more) fetch_k(j1);
         // distances from the new event of register r's position: last_d - acc_row(r)
-        const int64_t last_d = n - j0 - 4 * half;
+        const int last_d = length - j0 - 4 * half;
         if (sc.table) {
-            if (n - (j0 + kKeys - 1) >= sc.reach) {
+            if (length - (j0 + kKeys - 1) >= sc.reach) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] += far_bias;
             } else if (any) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t d = min(max(last_d - acc_row(r), int64_t{0}), int64_t{sc.reach});
-                    s[r] += table_entry(sc, head, static_cast<int>(d) + sc.reach);
+                    const int d = min(max(last_d - acc_row(r), 0), sc.reach);
+                    s[r] += table_entry(sc, head, d + sc.reach);
                 }
             }
         }
@@ -166,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     // the new event's own time is not in the cache yet: it is 0 away
-                    const float gap = q_time - s_times[wave][acc_row(r) + 4 * half];
+                    const float gap = q_time - time[r];
                     s[r] = fmaf(-slope, last_d == acc_row(r) ? 0.0f : fabsf(gap), s[r]);
                 }
             } else {
@@ -175,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
                 for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(from - acc_row(r)), s[r]);
             }
         }
-        if (j0 + kKeys > n + 1) {
+        if (j0 + kKeys > length + 1) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if (acc_row(r) > last_d) s[r] = -INFINITY;
@@ -199,16 +213,18 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
             s[r] = exp2_fast(s[r] - m);
             l += s[r];
         }
-        v.store(s_tile, lane);
-        if (more) v.load(cache_v, a.v_pos, fresh_v, a.dim, j1, n, lane);
+        if (more) copies_landed<kCopies>();  // values; the next keys may be on their way
+        else copies_landed<0>();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             Frag<T> p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = static_cast<T>(s[8 * t + e]);
 #pragma unroll
-            for (int c = 0; c < DB; ++c) o[c] = mma(G::columns(s_tile, 16 * t, c, lane), p, o[c]);
+            for (int c = 0; c < DB; ++c) o[c] = mma(G::columns(s_v, 16 * t, c, at_lane), p, o[c]);
         }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        if (more) fetch_v(j1);
     }
     l += __shfl_xor(l, 32);
 

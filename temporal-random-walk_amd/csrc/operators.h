@@ -99,6 +99,10 @@ __device__ __forceinline__ f32x16 zero16() {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// No LDS read moves across: where the compiler would read all operands of a
+// chain of products ahead and run out of registers for them.
+__device__ __forceinline__ void hold_reads() { asm volatile("" ::: "memory"); }
+
 // Row of accumulator register r: 8 (r / 4) + 4 (lane / 32) + r % 4.
 __device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
@@ -456,32 +460,32 @@ __device__ __forceinline__ void add_biases(const Score& sc, float (&s)[kBlocks][
 }
 
 // Sums of a block's dS by distance, along its diagonals.  Float atomics of LDS
-// take some 100 cycles an instruction (counted), so a wave writes 16 keys at a
+// take some 100 cycles an instruction (counted), so a wave writes 8 keys at a
 // time to a square of its own, each row followed by zeros, and every lane reads
 // one diagonal (rows kPitch + 1 apart, at constant offsets) and adds its sum to
 // the wave's line of distances -reach .. reach.  Pairs past the reach share the
 // line's ends: sums over lanes.
-constexpr int kPitch = 72;  // 32 values and zeros; two half waves' rows in other banks
-constexpr int kSquare = 17 * kPitch;
+constexpr int kPitch = 40;  // 32 values and 8 zeros; two half waves' rows in other banks
+constexpr int kSquare = 9 * kPitch;
 
 // v: register r is key acc_row(r) + 4 half, the lane's column a query row; lo,
 // hi: distances of the first and last row from the block's first key.
 __device__ __forceinline__ void add_diagonals(const float (&v)[16], float* square, float* line,
                                               int reach, int lo, int hi, int lane, int half) {
+    // lane's diagonal: its row less its key is at (lanes 0 .. 38)
+    const int at = min(lane, 39) - 7;
+    const bool mine = lane < 39;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int g = 0; g < 4; ++g) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-            square[(1 + acc_row(r) + 4 * half) * kPitch + (lane & 31)] = v[8 * t + r];
-        // lane's diagonal: its row less its key is lane - 15 (lanes 0 .. 46)
-        const int at = min(lane, 47) - 15;
+        for (int r = 0; r < 4; ++r)
+            square[(1 + r + 4 * half) * kPitch + (lane & 31)] = v[4 * g + r];
         float sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += square[(1 + r) * kPitch + r + at];
-        const int d = lo - 16 * t + at;
-        const bool mine = lane < 47;
+        for (int r = 0; r < 8; ++r) sum += square[(1 + r) * kPitch + r + at];
+        const int d = lo - 8 * g + at;
         if (mine && abs(d) < reach) line[d + reach] += sum;
-        if (hi - 16 * t >= reach || lo - 16 * t - 15 <= -reach) {
+        if (hi - 8 * g >= reach || lo - 8 * g - 7 <= -reach) {
             float before = mine && d >= reach ? sum : 0.0f;
             float after = mine && d <= -reach && reach ? sum : 0.0f;
 #pragma unroll

@@ -115,7 +115,7 @@ const trw_attention_step_params& checked(const trw_attention_step_params* p) {
     require(p != nullptr, "null argument");
     check_heads(p->dtype, p->heads, p->kv_heads, p->dim);
     require(p->batch >= 0 && p->batch < kMaxRows, "batch must be 0 to 2^30 - 1");
-    require(p->capacity >= 0, "capacity must not be negative");
+    require(p->capacity >= 0 && p->capacity < kMaxRows, "capacity must be 0 to 2^30 - 1");
     require(p->batch * p->heads < (int64_t{1} << 31) / 1024, "too many walks and heads");
     check_score(p->score);
     return *p;
