@@ -30,6 +30,8 @@ constexpr int kTileRows = 128;
 // P is then at most 2^8, which every type holds as well as 1, and the output is
 // rarely scaled.
 constexpr float kSlack = 8.0f;
+// Keys that a workgroup takes at least, where several share a tile's.
+constexpr int kShare = 512;
 
 struct ForwardArgs {
     Rows q, k, v, out;
@@ -39,8 +41,10 @@ struct ForwardArgs {
     int q_rows, k_rows, heads, group, dim;
     int tiles, splits;
     int walk_limit;      // documents up to here go a wave each (attention_walks.hip)
-    float* part_out;     // [splits, heads, q_rows, dim], where splits > 1
+    // where splits > 1
+    float* part_out;     // [splits, heads, q_rows, dim]
     float2* part_stats;  // [splits, heads, q_rows]
+    int* part_count;     // [tiles] workgroups that a tile's keys were shared by
 };
 
 // What the backward pass takes from a score to have log2 P: m + log2 l at once,
@@ -111,13 +115,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
     k_begin = __builtin_amdgcn_readfirstlane(k_begin);
     k_end = __builtin_amdgcn_readfirstlane(k_end);
     const bool mixed = k_begin < last_lo;  // rows of more than one walk
-    // this split's tiles of the workgroup's keys
+    // this split's tiles of the workgroup's keys: as many splits as have kShare
+    // tiles each
     int j_first = k_begin, j_last = k_end;
-    if (a.splits > 1 && k_begin < k_end) {
-        const int count = (k_end - k_begin + kKeys - 1) / kKeys;
-        j_first = k_begin + static_cast<int>(static_cast<int64_t>(count) * split / a.splits) * kKeys;
-        j_last = min(k_end, k_begin + static_cast<int>(static_cast<int64_t>(count) * (split + 1) /
-                                                       a.splits) * kKeys);
+    bool shared = false;
+    if (a.splits > 1) {
+        const int count = k_begin < k_end ? (k_end - k_begin + kKeys - 1) / kKeys : 0;
+        const int used = min(a.splits, max((count * kKeys + kShare - 1) / kShare, 1));
+        if (split >= used) return;
+        if (split == 0 && head == 0 && thread == 0) a.part_count[tile] = used;
+        shared = used > 1;
+        if (shared) {
+            j_first = k_begin + static_cast<int>(static_cast<int64_t>(count) * split / used) * kKeys;
+            j_last = min(k_end, k_begin + static_cast<int>(static_cast<int64_t>(count) *
+                                                           (split + 1) / used) * kKeys);
+        }
     }
 
     const float slope = sc.slopes ? sc.slopes[head] * kLog2e : 0.0f;
@@ -222,7 +234,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
         if (mine) {
             const bool seen = any && l != 0.0f;  // 0: the bias masks every key
             const int64_t stat = static_cast<int64_t>(head) * a.q_rows + i;
-            if (a.splits > 1) {
+            if (shared) {
                 const int64_t part = static_cast<int64_t>(split) * a.heads * a.q_rows + stat;
                 store_row<float, DB>(a.part_out + part * a.dim, o, seen, 1.0f, a.dim, half);
                 if (half == 0) a.part_stats[part] = make_float2(m, seen ? l : 0.0f);
@@ -283,16 +295,17 @@ __global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
     const int64_t rows = static_cast<int64_t>(a.heads) * a.q_rows;
     if (t >= rows * pieces) return;
     const int64_t stat = t / pieces;  // head, row
-    if (!tiled(a.q_info[stat % a.q_rows].w, a.walk_limit)) return;
+    const int count = a.part_count[stat % a.q_rows / kTileRows];
+    if (count == 1) return;  // written by its one workgroup
     const int col = static_cast<int>(t % pieces) * 4;
     float m = kFloor;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < count; ++s) {
         const float2 st = a.part_stats[s * rows + stat];
         m = st.y != 0.0f ? fmaxf(m, st.x) : m;
     }
     f32x4 o = {0, 0, 0, 0};
     float l = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < count; ++s) {
         const float2 st = a.part_stats[s * rows + stat];
         if (st.y == 0.0f) continue;
         const float by = exp2_fast(st.x - m);
@@ -311,13 +324,13 @@ __global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
     if (col == 0) store_stats(a, stat, seen, m, l);
 }
 
-// Workgroups that share the keys of one: where the tiles of query rows are
-// fewer than two for each of the 256 compute units, up to that many, each with
-// 256 keys or more if one walk has them all.
+// Workgroups that may share one tile's keys: where tiles and heads are fewer
+// than four workgroups for each of the 256 compute units, enough for eight, for
+// each tile as its keys (which the device knows) allow.
 int splits_of(const trw_attention_params& p) {
     const int64_t items = (p.q_rows + kTileRows - 1) / kTileRows * p.heads;
-    if (items == 0 || walk_blocks(p)) return 1;
-    const int64_t splits = std::min<int64_t>({512 / items, p.k_rows / 256, 16});
+    if (items == 0 || items > 1024 || walk_blocks(p)) return 1;
+    const int64_t splits = std::min<int64_t>({2048 / items, p.k_rows / kShare, 32});
     return static_cast<int>(std::max<int64_t>(splits, 1));
 }
 
@@ -329,7 +342,8 @@ uint64_t attention_workspace(const trw_attention_params& p, bool backward) {
     if (backward) return attention_backward_workspace(p);
     const int splits = splits_of(p);
     if (splits == 1) return 0;
-    return static_cast<uint64_t>(splits) * p.heads * p.q_rows * (p.dim + 2) * sizeof(float);
+    return static_cast<uint64_t>(splits) * p.heads * p.q_rows * (p.dim + 2) * sizeof(float) +
+           (p.q_rows + kTileRows - 1) / kTileRows * sizeof(int);
 }
 
 void attention_forward(const trw_attention_params& p, hipStream_t stream) {
@@ -359,6 +373,7 @@ void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.heads) * a.q_rows;
     a.part_out = static_cast<float*>(p.workspace);
     a.part_stats = reinterpret_cast<float2*>(a.part_out + a.splits * rows * a.dim);
+    a.part_count = reinterpret_cast<int*>(a.part_stats + a.splits * rows);
     const int64_t grid = xcd_grid(static_cast<int64_t>(a.tiles) * a.heads * a.splits);
     const size_t lds = p.score.table ? (2 * a.score.reach + 1) * sizeof(float) : 0;
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {

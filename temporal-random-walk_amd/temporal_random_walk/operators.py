@@ -134,6 +134,17 @@ def _call(function, *args):
         raise {1: ValueError, 3: MemoryError}.get(rc, RuntimeError)(message)
 
 
+def _queue(device, function, *args):
+    """The call with the current stream of a device, on that device."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        _call(function, *args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            _call(function, *args, torch.cuda.current_stream(index).cuda_stream)
+
+
+# Messages are put together only where a check fails: a small call's time is the host's.
 def _require(ok, message):
     if not ok:
         raise ValueError(message)
@@ -142,36 +153,45 @@ def _require(ok, message):
 def _on_gpu(name, x, device=None):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    _require(x.is_cuda, f"{name} must be on the GPU")
-    _require(device is None or x.device == device, f"{name} is on another device")
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    if device is not None and x.device != device:
+        raise ValueError(f"{name} is on another device")
 
 
 def _ints(name, x, shape, device):
     """An int64 tensor of one shape (a view or a copy of what was given)."""
     _on_gpu(name, x, device)
-    _require(not x.is_floating_point() and not x.is_complex() and x.dtype != torch.bool,
-             f"{name} must hold whole numbers")
-    _require(tuple(x.shape) == shape, f"{name} must have the shape {shape}")
-    return x.to(torch.int64).contiguous()
+    if x.dtype is not torch.int64:
+        if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
+            raise ValueError(f"{name} must hold whole numbers")
+        x = x.to(torch.int64)
+    if x.shape != shape:
+        raise ValueError(f"{name} must have the shape {shape}")
+    return x.contiguous()
 
 
 def _floats(name, x, shape, device):
     _on_gpu(name, x, device)
-    _require(x.dtype == torch.float32, f"{name} must be float32")
-    _require(tuple(x.shape) == shape, f"{name} must have the shape {shape}")
-    _require(not (x.requires_grad and torch.is_grad_enabled()), f"{name} has no gradient here")
+    if x.dtype is not torch.float32:
+        raise ValueError(f"{name} must be float32")
+    if x.shape != shape:
+        raise ValueError(f"{name} must have the shape {shape}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no gradient here")
     return x.contiguous()
 
 
 def _pieces(x):
     """Whether rows of the last dimension can be read 16 bytes at a time."""
+    *outer, last = x.stride()
+    if last != 1 or x.data_ptr() % 16:
+        return False
     per = 16 // x.element_size()
-    return (x.stride(-1) == 1 and x.data_ptr() % 16 == 0
-            and all(s % per == 0 for s in x.stride()[:-1]))
+    for s in outer:
+        if s % per:
+            return False
+    return True
 
 
 def _readable(x):
@@ -242,19 +262,20 @@ class WalkMask:
         self.q_rows, self.k_rows = q_rows, k_rows
         self.q_shape, self.k_shape = q_shape, k_shape  # leading dimensions of q; of k and v
         self.device = device
-        self.q_info = torch.empty(q_rows, 4, dtype=torch.int32, device=device)
-        self.k_info = torch.empty(k_rows, 4, dtype=torch.int32, device=device)
-        self.docs_info = torch.empty(docs, 8, dtype=torch.int32, device=device)
+        # rows' and documents' intervals, one after another
+        self._info = torch.empty(4 * (q_rows + k_rows) + 8 * docs, dtype=torch.int32,
+                                 device=device)
+        self.q_info = self._info.data_ptr()
+        self.k_info = self.q_info + 16 * q_rows
+        self.docs_info = self.k_info + 16 * k_rows
         self.docs = docs
         # of any document, where the host knows it
         self.longest = max(q_length, k_length) if q_offsets is None else 0
         self.own_causal = kind == "causal" and k_lens is None and k_offsets is None
         p = _MaskParams(docs, q_rows, k_rows, q_length, k_length, _ptr(q_lens), _ptr(k_lens),
                         _ptr(q_offsets), _ptr(k_offsets), _ptr(prefix), _KINDS[kind],
-                        self.q_info.data_ptr(), self.k_info.data_ptr(),
-                        self.docs_info.data_ptr())
-        with torch.cuda.device(device):
-            _call(lib().trw_ops_walk_mask, C.byref(p), _stream(device))
+                        self.q_info, self.k_info, self.docs_info)
+        _queue(device, lib().trw_ops_walk_mask, C.byref(p))
 
     @classmethod
     def padded(cls, lens, length, *, k_lens=None, k_length=None, kind="causal", prefix=None):
@@ -315,8 +336,8 @@ class _Terms:
             self.times = _floats("times", times, time_shapes[0], device)
             self.k_times = (self.times if k_times is None or k_times is times
                             else _floats("k_times", k_times, time_shapes[1], device))
-            _require(tuple(self.k_times.shape) == time_shapes[1],
-                     f"k_times must have the shape {time_shapes[1]}")
+            if self.k_times.shape != time_shapes[1]:
+                raise ValueError(f"k_times must have the shape {time_shapes[1]}")
 
     def struct(self, table):
         b = self.buckets
@@ -335,7 +356,8 @@ def _bias_arguments(table, buckets, heads, device):
     _require(table.dim() == 2 and table.shape[0] == heads,
              "bias_table must be [heads, num_buckets]")
     _require(table.dtype in _DTYPES, "bias_table must be float32, float16 or bfloat16")
-    _require(1 <= table.shape[1] <= MAX_BUCKETS, f"1 to {MAX_BUCKETS} buckets")
+    if not 1 <= table.shape[1] <= MAX_BUCKETS:
+        raise ValueError(f"1 to {MAX_BUCKETS} buckets")
     _check_ids(buckets)
     return table.float().contiguous(), buckets.contiguous(), table.shape[1]
 
@@ -343,14 +365,16 @@ def _bias_arguments(table, buckets, heads, device):
 def _check_ids(buckets):
     _require(buckets.dtype == torch.int32 and buckets.dim() == 1 and buckets.shape[0] % 2 == 1,
              "buckets must be an int32 tensor of 2 reach + 1 ids")
-    _require(buckets.shape[0] // 2 <= MAX_REACH, f"reach must be 0 to {MAX_REACH}")
+    if buckets.shape[0] // 2 > MAX_REACH:
+        raise ValueError(f"reach must be 0 to {MAX_REACH}")
 
 
 def _check_qkv(q, k, v, dims):
     _on_gpu("q", q)
     _on_gpu("k", k, q.device)
     _on_gpu("v", v, q.device)
-    _require(q.dim() == dims, f"q must have {dims} dimensions")
+    if q.dim() != dims:
+        raise ValueError(f"q must have {dims} dimensions")
     _require(k.shape == v.shape, "k and v must have the same shape")
     _require(k.dim() == dims and q.shape[-1] == k.shape[-1], "q and k must have the same head size")
     _require(q.dtype in _DTYPES, "q must be float32, float16 or bfloat16")
@@ -360,16 +384,6 @@ def _check_qkv(q, k, v, dims):
              "heads must be a positive multiple of the key heads")
     _require(0 < dim <= 128 and dim % 8 == 0, "the head size must be a multiple of 8 up to 128")
     return heads, kv_heads, dim
-
-
-def _attention_params(q, k, v, out, table, mask, terms):
-    return _AttentionParams(
-        dtype=_DTYPES[q.dtype], heads=q.shape[1], kv_heads=k.shape[1], dim=q.shape[2],
-        q_rows=mask.q_rows, k_rows=mask.k_rows, q_rows_info=mask.q_info.data_ptr(),
-        k_rows_info=mask.k_info.data_ptr(), docs_info=mask.docs_info.data_ptr(), docs=mask.docs,
-        longest=mask.longest, own_causal=mask.own_causal,
-        score=terms.struct(table), q=_rows(q), k=_rows(k), v=_rows(v),
-        out=_rows(out))
 
 
 def _workspace(p, backward, device):
@@ -383,40 +397,50 @@ def _workspace(p, backward, device):
 
 
 class _WalkAttention(torch.autograd.Function):
+    """q, k, v: [walks, length, heads, dim] or [rows, heads, dim]."""
+
     @staticmethod
     def forward(ctx, q, k, v, table, mask, terms):
+        shapes = q.shape, k.shape
+        if q.dim() == 4:
+            q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
         q, k, v = _readable(q), _readable(k), _readable(v)
         device = q.device
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        p = _attention_params(q, k, v, out, table, mask, terms)
+        _, heads, dim = q.shape
+        p = _AttentionParams(
+            _DTYPES[q.dtype], heads, k.shape[1], dim, mask.q_rows, mask.k_rows, mask.q_info,
+            mask.k_info, mask.docs_info, mask.docs, mask.longest, mask.own_causal,
+            terms.struct(table), _rows(q), _rows(k), _rows(v), _rows(out))
         stats = None
         if any(ctx.needs_input_grad[:4]):
-            stats = torch.empty(2, q.shape[1], q.shape[0], dtype=torch.float32, device=device)
+            stats = torch.empty(2, heads, mask.q_rows, dtype=torch.float32, device=device)
             p.stats = stats.data_ptr()
-        with torch.cuda.device(device):
-            space = _workspace(p, 0, device)  # noqa: F841  (held until the call has queued)
-            _call(lib().trw_ops_attention_forward, C.byref(p), _stream(device))
+        space = _workspace(p, 0, device)  # held until the call has queued
+        _queue(device, lib().trw_ops_attention_forward, C.byref(p))
+        del space
         if stats is not None:
             ctx.save_for_backward(q, k, v, table, out, stats)
-            ctx.mask, ctx.terms = mask, terms
-        return out
+            ctx.mask, ctx.terms, ctx.params, ctx.shapes = mask, terms, p, shapes
+        return out.view(shapes[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, table, out, stats = ctx.saved_tensors
+        q, k, v, table, _, _ = ctx.saved_tensors
         device = q.device
-        d_out = _readable(d_out)
+        d_out = _readable(d_out.flatten(0, 1) if d_out.dim() == 4 else d_out)
         d_q, d_k, d_v = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
         d_table = None if table is None else torch.empty_like(table)
-        p = _attention_params(q, k, v, out, table, ctx.mask, ctx.terms)
-        p.stats = stats.data_ptr()
+        p = _AttentionParams.from_buffer_copy(ctx.params)
         p.d_out, p.d_q, p.d_k, p.d_v = _rows(d_out), _rows(d_q), _rows(d_k), _rows(d_v)
         p.d_table = _ptr(d_table)
-        with torch.cuda.device(device):
-            space = _workspace(p, 1, device)  # noqa: F841
-            _call(lib().trw_ops_attention_backward, C.byref(p), _stream(device))
-        return d_q, d_k, d_v, d_table, None, None
+        p.workspace, p.workspace_bytes = None, 0
+        space = _workspace(p, 1, device)
+        _queue(device, lib().trw_ops_attention_backward, C.byref(p))
+        del space
+        q_shape, k_shape = ctx.shapes
+        return d_q.view(q_shape), d_k.view(k_shape), d_v.view(k_shape), d_table, None, None
 
 
 def walk_attention(q, k, v, mask, *, scale=None, softcap=0.0, bias_table=None, buckets=None,
@@ -444,15 +468,14 @@ def walk_attention(q, k, v, mask, *, scale=None, softcap=0.0, bias_table=None, b
     _require(isinstance(mask, WalkMask), "mask must be a WalkMask")
     heads, _, dim = _check_qkv(q, k, v, len(mask.q_shape) + 2)
     _require(q.device == mask.device, "q is on another device than the mask")
-    _require(tuple(q.shape[:-2]) == mask.q_shape, f"q must be {mask.q_shape} rows of heads")
-    _require(tuple(k.shape[:-2]) == mask.k_shape, f"k must be {mask.k_shape} rows of heads")
+    if q.shape[:-2] != mask.q_shape:
+        raise ValueError(f"q must be {mask.q_shape} rows of heads")
+    if k.shape[:-2] != mask.k_shape:
+        raise ValueError(f"k must be {mask.k_shape} rows of heads")
     table, buckets, num_buckets = _bias_arguments(bias_table, buckets, heads, q.device)
     terms = _Terms(heads, q.device, dim, scale, softcap, buckets, num_buckets, slopes, times,
                    k_times, (mask.q_shape, mask.k_shape))
-    shape = q.shape
-    if len(mask.q_shape) == 2:
-        q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
-    return _WalkAttention.apply(q, k, v, table, mask, terms).view(shape)
+    return _WalkAttention.apply(q, k, v, table, mask, terms)
 
 
 @torch.no_grad()
@@ -476,10 +499,11 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
     _require(k.shape[0] == batch, "q and k must have the same batch")
     for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
         _on_gpu(name, x, device)
-        _require(x.dtype == q.dtype and x.dim() == 4 and x.shape[0] == batch
-                 and tuple(x.shape[2:]) == (kv_heads, dim),
-                 f"{name} must be [batch, capacity, kv_heads, dim] of q's type")
-        _require(x.numel() == 0 or _pieces(x), f"{name}'s rows must be 16-byte pieces")
+        if (x.dtype is not q.dtype or x.dim() != 4 or x.shape[0] != batch
+                or x.shape[2:] != (kv_heads, dim)):
+            raise ValueError(f"{name} must be [batch, capacity, kv_heads, dim] of q's type")
+        if x.numel() and not _pieces(x):
+            raise ValueError(f"{name}'s rows must be 16-byte pieces")
     _require(k_cache.shape == v_cache.shape, "k_cache and v_cache must have the same shape")
     capacity = k_cache.shape[1]
     lens = _ints("lens", lens, (batch,), device)
@@ -494,13 +518,12 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
         _DTYPES[q.dtype], heads, kv_heads, dim, batch, capacity, lens.data_ptr(),
         terms.struct(table), _rows(q), _rows(k), _rows(v), _rows(out), k_cache.data_ptr(),
         v_cache.data_ptr(), *k_cache.stride()[:3], *v_cache.stride()[:3])
-    with torch.cuda.device(device):
-        size = C.c_uint64()
-        _call(lib().trw_ops_attention_step_workspace, C.byref(p), C.byref(size))
-        if size.value:
-            space = torch.empty(size.value, dtype=torch.uint8, device=device)
-            p.workspace, p.workspace_bytes = space.data_ptr(), size.value
-        _call(lib().trw_ops_attention_step, C.byref(p), _stream(device))
+    size = C.c_uint64()
+    _call(lib().trw_ops_attention_step_workspace, C.byref(p), C.byref(size))
+    if size.value:
+        space = torch.empty(size.value, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = space.data_ptr(), size.value
+    _queue(device, lib().trw_ops_attention_step, C.byref(p))
     return out
 
 
@@ -512,8 +535,7 @@ class _RelativeBias(torch.autograd.Function):
         out = torch.empty(heads, q_len, k_len, dtype=table.dtype, device=table.device)
         p = _BiasParams(_DTYPES[table.dtype], heads, num_buckets, buckets.shape[0] // 2, q_len,
                         k_len, q_offset, table.data_ptr(), buckets.data_ptr(), out.data_ptr())
-        with torch.cuda.device(table.device):
-            _call(lib().trw_ops_relative_bias, C.byref(p), _stream(table.device))
+        _queue(table.device, lib().trw_ops_relative_bias, C.byref(p))
         ctx.save_for_backward(table, buckets)
         ctx.q_offset = q_offset
         return out
@@ -529,12 +551,11 @@ class _RelativeBias(torch.autograd.Function):
                         d_out.shape[1], d_out.shape[2], ctx.q_offset, table.data_ptr(),
                         buckets.data_ptr(), None, d_out.data_ptr(), d_out.stride(0),
                         d_out.stride(1), d_table.data_ptr())
-        with torch.cuda.device(table.device):
-            size = C.c_uint64()
-            _call(lib().trw_ops_relative_bias_workspace, C.byref(p), C.byref(size))
-            space = torch.empty(max(16, size.value), dtype=torch.uint8, device=table.device)
-            p.workspace, p.workspace_bytes = space.data_ptr(), size.value
-            _call(lib().trw_ops_relative_bias_backward, C.byref(p), _stream(table.device))
+        size = C.c_uint64()
+        _call(lib().trw_ops_relative_bias_workspace, C.byref(p), C.byref(size))
+        space = torch.empty(max(16, size.value), dtype=torch.uint8, device=table.device)
+        p.workspace, p.workspace_bytes = space.data_ptr(), size.value
+        _queue(table.device, lib().trw_ops_relative_bias_backward, C.byref(p))
         return d_table, None, None, None, None
 
 
@@ -547,7 +568,8 @@ def relative_bias(table, buckets, q_len, k_len, q_offset=0):
     _on_gpu("buckets", buckets, table.device)
     _require(table.dim() == 2 and table.shape[0] > 0, "table must be [heads, num_buckets]")
     _require(table.dtype in _DTYPES, "table must be float32, float16 or bfloat16")
-    _require(1 <= table.shape[1] <= MAX_BUCKETS, f"1 to {MAX_BUCKETS} buckets")
+    if not 1 <= table.shape[1] <= MAX_BUCKETS:
+        raise ValueError(f"1 to {MAX_BUCKETS} buckets")
     _check_ids(buckets)
     q_len, k_len, q_offset = int(q_len), int(k_len), int(q_offset)
     _require(q_len >= 0 and k_len >= 0, "lengths must not be negative")
