@@ -68,14 +68,41 @@ __device__ __forceinline__ Doc load_doc(const int4* docs, int doc) {
 }
 
 // Zeros in rows [from, to) of one head, which nobody else writes.
-template <typename T>
+template <typename T, int DB>
 __device__ __forceinline__ void zero_rows(const Rows& r, int64_t begin, int from, int to, int head,
                                           int dim, int lane) {
-    constexpr int kElems = 16 / sizeof(T);
-    const int pieces = dim / kElems;
-    for (int n = lane; n < (to - from) * pieces; n += 64)
-        *reinterpret_cast<u32x4*>(row_of<T>(r, begin + from + n / pieces, head) +
-                                  n % pieces * kElems) = u32x4{0, 0, 0, 0};
+    typedef Tile<T, DB> G;
+    constexpr int kRows = 64 / G::kUsed;  // at a time
+    const int col = lane % G::kUsed * G::kElems;
+    if (col >= dim || lane >= kRows * G::kUsed) return;
+    T* row = row_of<T>(r, begin + from + lane / G::kUsed, head) + col;
+    for (int i = from + lane / G::kUsed; i < to; i += kRows, row += kRows * r.row)
+        *reinterpret_cast<u32x4*>(row) = u32x4{0, 0, 0, 0};
+}
+
+// A row as B operands, as load_operand, of a row that is there: columns from
+// `dim` on are zeros.
+template <typename T, int DB>
+__device__ __forceinline__ void load_whole_operand(Frag<T> (&f)[2 * DB], const T* row, int dim,
+                                                   int half) {
+#pragma unroll
+    for (int s = 0; s < 2 * DB; ++s) {
+        union {
+            u32x4 u;
+            Frag<T> f;
+        } x;
+        const int col = 16 * s + 8 * half;
+        x.u = *reinterpret_cast<const u32x4*>(row + (col < dim ? col : 0));
+        f[s] = x.f;
+    }
+    if (dim < 32 * DB) {
+#pragma unroll
+        for (int s = 0; s < 2 * DB; ++s)
+            if (16 * s + 8 * half >= dim) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[s][e] = static_cast<T>(0.0f);
+            }
+    }
 }
 
 // All copies of this wave have landed (the tiles are the wave's own).
@@ -118,9 +145,9 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
     const int steps = q_blocks * a.group;
     Frag<T> q[G::kSteps], next[G::kSteps];
     auto load_q = [&](Frag<T>(&f)[G::kSteps], int step) {
-        const int i = step % q_blocks * 32 + (lane & 31);
-        load_operand<T, DB>(f, row_of<const T>(a.q, d.q_begin + i, first_head + step / q_blocks),
-                            i < d.q_len, a.dim, lane >> 5);
+        const int i = min(step % q_blocks * 32 + (lane & 31), d.q_len - 1);
+        load_whole_operand<T, DB>(
+            f, row_of<const T>(a.q, d.q_begin + i, first_head + step / q_blocks), a.dim, lane >> 5);
     };
     if (steps > 0 && k_blocks > 0) {
         const Loader<T, DB, 32, 64> k_load(a.k.row, a.dim, lane), v_load(a.v.row, a.dim, lane);
@@ -217,7 +244,7 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
         }
     }
     for (int h = first_head; h < first_head + a.group; ++h)
-        zero_rows<T>(a.out, d.q_begin, d.q_len, d.q_rows, h, a.dim, lane);
+        zero_rows<T, DB>(a.out, d.q_begin, d.q_len, d.q_rows, h, a.dim, lane);
 }
 
 // Backward: a wave for each 32 rows of the walk.  First the wave owns query
@@ -482,12 +509,12 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 
         store_row<T, DB>(row_of<T>(a.d_k, d.k_begin + j, kv_head), dk, any, sc.scale, a.dim, half);
         store_row<T, DB>(row_of<T>(a.d_v, d.k_begin + j, kv_head), dv, any, 1.0f, a.dim, half);
     }
-    if (wave == 0) zero_rows<T>(a.d_k, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
-    if (wave == kNB - 1) zero_rows<T>(a.d_v, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
+    if (wave == 0) zero_rows<T, DB>(a.d_k, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
+    if (wave == kNB - 1) zero_rows<T, DB>(a.d_v, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
     for (int h = first_head; h < first_head + a.group; ++h) {
         // queries over no keys at all, and padding
         if (wave == kNB / 2)
-            zero_rows<T>(a.d_q, d.q_begin, heads > 0 ? d.q_len : 0, d.q_rows, h, a.dim, lane);
+            zero_rows<T, DB>(a.d_q, d.q_begin, heads > 0 ? d.q_len : 0, d.q_rows, h, a.dim, lane);
         if (sc.table && heads == 0)
             for (int n = threadIdx.x; n < line; n += 64 * kNB)
                 a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * line + n] = 0.0f;

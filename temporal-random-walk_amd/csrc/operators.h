@@ -240,20 +240,21 @@ struct Loader {
     static constexpr int kSlots = kRows * G::kSlots;
     static constexpr int kMine = kSlots / kThreads;
     static_assert(kSlots % kThreads == 0, "whole waves fill a tile");
-    uint32_t pitch;          // bytes of a row: 64 of them fit 31 bits (checked on the host)
-    uint32_t offset[kMine];  // bytes from the tile's first row
+    static constexpr int kStep = kThreads / G::kSlots;  // rows from one copy of a lane to the next
+    int pitch;                // bytes of a row: 64 of them fit 31 bits (checked on the host)
+    int first_row;            // bytes from the tile's first row to that of copy 0
+    uint32_t offset[kMine];   // bytes from the tile's first row to copy n
 
-    __device__ __forceinline__ int row_of(int n, int thread) const {
-        return (thread + n * kThreads) / G::kSlots;
-    }
+    // row_stride * kRows elements fit 31 bits of bytes (checked on the host)
     __device__ __forceinline__ Loader(int64_t row_stride, int dim, int thread)
-        : pitch(static_cast<uint32_t>(row_stride * sizeof(T))) {
+        : pitch(static_cast<int>(row_stride * sizeof(T))),
+          first_row(thread / G::kSlots * pitch) {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
-            const int row = row_of(n, thread);
+            const int row = thread / G::kSlots + n * kStep;
             const int chunk = ((thread + n * kThreads) % G::kSlots) ^ G::swizzle(row);
             const int col = chunk * G::kElems < dim ? chunk * G::kElems : 0;
-            offset[n] = row * pitch + col * static_cast<uint32_t>(sizeof(T));
+            offset[n] = first_row + n * kStep * pitch + col * static_cast<int>(sizeof(T));
         }
     }
     // To the LDS address `lds`.  begin < end; first and lds are a wave's scalars.
@@ -266,11 +267,13 @@ struct Loader {
 #pragma unroll
             for (int n = 0; n < kMine; ++n) copy_to_lds(at, offset[n], to + n * kThreads * 16);
         } else {
+            // rows as bytes from row `from`, kept between it and the last one
+            const int before = (from - first) * pitch, last = (end - 1 - from) * pitch;
 #pragma unroll
             for (int n = 0; n < kMine; ++n) {
-                const int row = row_of(n, thread);
-                const int near = min(max(first + row, begin), end - 1) - from;  // 0 .. kRows - 1
-                copy_to_lds(at, offset[n] + (near - row) * pitch, to + n * kThreads * 16);
+                const int row = first_row + n * kStep * pitch;
+                const int near = min(max(row - before, 0), last);
+                copy_to_lds(at, offset[n] + (near - row), to + n * kThreads * 16);
             }
         }
     }
