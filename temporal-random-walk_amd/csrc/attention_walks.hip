@@ -126,10 +126,10 @@ __device__ __forceinline__ void fill_walk_bias(float* lut, const Score& sc, int 
 }
 
 template <typename T, int DB, int kNB>
-__global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
+__global__ __launch_bounds__(64, DB < 3 ? 2 : 1) void walk_forward_kernel(WalkArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kBlock = 32 * G::kSlots;
-    __shared__ u32x4 s_k[kNB * kBlock], s_v[kNB * kBlock];
+    __shared__ u32x4 s_v[kNB * kBlock];
     __shared__ float s_time[128];
     __shared__ float s_lut[64 * kNB + 1];
 
@@ -143,20 +143,26 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
 
     const int q_blocks = (d.q_len + 31) / 32, k_blocks = (d.k_len + 31) / 32;
     const int steps = q_blocks * a.group;
-    Frag<T> q[G::kSteps], next[G::kSteps];
+    // Keys stay in registers for all query rows and heads, values, which are
+    // read transposed, in LDS.
+    Frag<T> k[kNB][G::kSteps], q[G::kSteps], next[G::kSteps];
     auto load_q = [&](Frag<T>(&f)[G::kSteps], int step) {
         const int i = min(step % q_blocks * 32 + (lane & 31), d.q_len - 1);
         load_whole_operand<T, DB>(
             f, row_of<const T>(a.q, d.q_begin + i, first_head + step / q_blocks), a.dim, lane >> 5);
     };
     if (steps > 0 && k_blocks > 0) {
-        const Loader<T, DB, 32, 64> k_load(a.k.row, a.dim, lane), v_load(a.v.row, a.dim, lane);
-        const T* k_base = row_of<const T>(a.k, d.k_begin, kv_head);
+#pragma unroll
+        for (int b = 0; b < kNB; ++b)
+            if (b < k_blocks)
+                load_whole_operand<T, DB>(
+                    k[b],
+                    row_of<const T>(a.k, d.k_begin + min(32 * b + (lane & 31), d.k_len - 1), kv_head),
+                    a.dim, lane >> 5);
+        const Loader<T, DB, 32, 64> v_load(a.v.row, a.dim, lane);
         const T* v_base = row_of<const T>(a.v, d.k_begin, kv_head);
-        for (int b = 0; b < k_blocks; ++b) {
-            k_load.load(k_base, 32 * b, 0, d.k_len, lds_address(s_k) + b * kBlock * 16, lane);
+        for (int b = 0; b < k_blocks; ++b)
             v_load.load(v_base, 32 * b, 0, d.k_len, lds_address(s_v) + b * kBlock * 16, lane);
-        }
         if (sc.k_times)
             for (int j = 0; j < d.k_len; j += 64)
                 load_floats(sc.k_times + d.k_begin, j, 0, d.k_len, lds_address(s_time) + j * 4,
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(64) void walk_forward_kernel(WalkArgs a) {
             f32x16 x = zero16();
 #pragma unroll
             for (int st = 0; st < G::kSteps; ++st)
-                x = mma(G::row(s_k + b * kBlock, lane & 31, st, half), q[st], x);
+                x = mma(k[b][st], q[st], x);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][0][r] = x[r];
             cap_scores<T>(sc, s[b]);
