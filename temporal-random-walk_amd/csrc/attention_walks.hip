@@ -53,6 +53,16 @@ struct Doc {
     }
 };
 
+// Consecutive workgroups go to the eight XCDs in turn: each takes all key heads
+// of a walk, whose rows lie side by side.
+__device__ __forceinline__ int head_of(const WalkArgs& a, int id) { return id / 8 % a.kv_heads; }
+__device__ __forceinline__ int doc_of(const WalkArgs& a, int id) {
+    return id / (8 * a.kv_heads) * 8 + id % 8;
+}
+inline unsigned walk_grid(const trw_attention_params& p) {
+    return static_cast<unsigned>((p.docs + 7) / 8 * 8 * p.kv_heads);
+}
+
 __device__ __forceinline__ Doc load_doc(const int4* docs, int doc) {
     const int4 a = docs[2 * doc], b = docs[2 * doc + 1];
     Doc d;
@@ -134,8 +144,9 @@ __global__ __launch_bounds__(64, DB < 3 ? 2 : 1) void walk_forward_kernel(WalkAr
     __shared__ float s_lut[64 * kNB + 1];
 
     int lane = threadIdx.x;
-    const int kv_head = blockIdx.x % a.kv_heads;
-    const Doc d = load_doc(a.docs, blockIdx.x / a.kv_heads);
+    const int kv_head = head_of(a, blockIdx.x), doc = doc_of(a, blockIdx.x);
+    if (doc >= a.doc_count) return;
+    const Doc d = load_doc(a.docs, doc);
     if (max(d.q_len, d.k_len) > a.limit) return;  // the tiles' kernel has it
     const int first_head = kv_head * a.group;
     Score sc = a.score;
@@ -268,8 +279,8 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 
 
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv_head = blockIdx.x % a.kv_heads;
-    const int doc = blockIdx.x / a.kv_heads;
+    const int kv_head = head_of(a, blockIdx.x), doc = doc_of(a, blockIdx.x);
+    if (doc >= a.doc_count) return;
     const Doc d = load_doc(a.docs, doc);
     const int first_head = kv_head * a.group;
     Score sc = a.score;
@@ -603,7 +614,7 @@ bool walk_rest(const trw_attention_params& p, int blocks) {
 
 void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream) {
     const WalkArgs a = make_args(p, 32 * blocks);
-    const unsigned grid = static_cast<unsigned>(p.docs * p.kv_heads);
+    const unsigned grid = walk_grid(p);
     walk_dispatch(p.dtype, p.dim, blocks, [&](auto t, auto db, auto nb) {
         hipLaunchKernelGGL(
             (walk_forward_kernel<decltype(t), decltype(db)::value, decltype(nb)::value>),
@@ -620,7 +631,7 @@ void walk_backward(const trw_attention_params& p, int blocks, float* partial, hi
     WalkArgs a = make_args(p, 32 * blocks);
     a.partial = partial;
     a.triangle = p.own_causal;
-    const unsigned grid = static_cast<unsigned>(p.docs * p.kv_heads);
+    const unsigned grid = walk_grid(p);
     const int line = walk_line(p, blocks);
     walk_dispatch(p.dtype, p.dim, blocks, [&](auto t, auto db, auto nb) {
         typedef decltype(t) T;

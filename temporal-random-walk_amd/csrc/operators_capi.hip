@@ -94,7 +94,7 @@ const trw_attention_params& checked(const trw_attention_params* p) {
             "too many rows and heads");
     require(p->docs >= 0 && p->docs < kMaxRows && p->longest >= 0,
             "docs must be 0 to 2^30 - 1, longest not negative");
-    require(p->docs * p->kv_heads < (int64_t{1} << 31), "too many documents and heads");
+    require((p->docs + 7) * p->kv_heads < (int64_t{1} << 31), "too many documents and heads");
     check_score(p->score);
     return *p;
 }
