@@ -115,6 +115,37 @@ __device__ __forceinline__ void load_whole_operand(Frag<T> (&f)[2 * DB], const T
     }
 }
 
+// A block's accumulators (a column each a row of the output) as rows of global
+// memory, times `by`, zeros where a lane's row has nothing: through a tile of
+// the wave's own in LDS, so that a store instruction writes whole rows and not
+// 16 bytes of each of 32.
+template <typename T, int DB>
+__device__ __forceinline__ void store_rows(u32x4* tile, const f32x16 (&acc)[DB], bool any, float by,
+                                           const Rows& r, int64_t begin, int count, int head,
+                                           int dim, int lane) {
+    typedef Tile<T, DB> G;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const int half = lane >> 5;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            t4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = static_cast<T>(any ? acc[b][4 * g + e] * by : 0.0f);
+            *reinterpret_cast<t4*>(reinterpret_cast<char*>(tile) +
+                                   G::slot(lane & 31, 4 * b + g) * 16 + half * 8) = v;
+        }
+    T* base = row_of<T>(r, begin, head);
+#pragma unroll
+    for (int n = 0; n < (32 * G::kUsed + 63) / 64; ++n) {
+        const int at = lane + 64 * n, row = at / G::kUsed, col = at % G::kUsed * G::kElems;
+        if (row < count && col < dim)
+            *reinterpret_cast<u32x4*>(base + row * r.row + col) = tile[G::slot(row, at % G::kUsed)];
+    }
+}
+
 // All copies of this wave have landed (the tiles are the wave's own).
 __device__ __forceinline__ void wave_landed() {
     asm volatile("" ::: "memory");
@@ -139,7 +170,7 @@ template <typename T, int DB, int kNB>
 __global__ __launch_bounds__(64, DB < 3 ? 2 : 1) void walk_forward_kernel(WalkArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kBlock = 32 * G::kSlots;
-    __shared__ u32x4 s_v[kNB * kBlock];
+    __shared__ u32x4 s_v[kNB * kBlock], s_out[kBlock];
     __shared__ float s_time[128];
     __shared__ float s_lut[64 * kNB + 1];
 
@@ -249,10 +280,11 @@ __global__ __launch_bounds__(64, DB < 3 ? 2 : 1) void walk_forward_kernel(WalkAr
             }
         }
         l += __shfl_xor(l, 32);
-        if (in) {
+        {
             const bool any = l != 0.0f;
-            store_row<T, DB>(row_of<T>(a.out, d.q_begin + i, head), o, any, 1.0f / l, a.dim, half);
-            if (a.stats && half == 0) {
+            store_rows<T, DB>(s_out, o, any, 1.0f / l, a.out, d.q_begin + i0, d.q_len - i0, head,
+                              a.dim, lane);
+            if (a.stats && in && half == 0) {
                 const int64_t at = static_cast<int64_t>(head) * a.q_rows + d.q_begin + i;
                 const float log_l = any ? __builtin_amdgcn_logf(l) : INFINITY;
                 a.stats[at] = sc.biased() ? m : m + log_l;
@@ -520,11 +552,15 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 
             }
         }
     }
-    const int half = lane >> 5, j = 32 * wave + (lane & 31);
-    if (j < d.k_len) {
+    const int j = 32 * wave + (lane & 31);
+    __syncthreads();  // queries are done with
+    {
         const bool any = heads > 0 && d.first(j) < d.q_len;
-        store_row<T, DB>(row_of<T>(a.d_k, d.k_begin + j, kv_head), dk, any, sc.scale, a.dim, half);
-        store_row<T, DB>(row_of<T>(a.d_v, d.k_begin + j, kv_head), dv, any, 1.0f, a.dim, half);
+        u32x4* s_out = s_q + wave * kBlock;
+        store_rows<T, DB>(s_out, dk, any, sc.scale, a.d_k, d.k_begin + i0, d.k_len - i0, kv_head,
+                          a.dim, lane);
+        store_rows<T, DB>(s_out, dv, any, 1.0f, a.d_v, d.k_begin + i0, d.k_len - i0, kv_head, a.dim,
+                          lane);
     }
     if (wave == 0) zero_rows<T, DB>(a.d_k, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
     if (wave == kNB - 1) zero_rows<T, DB>(a.d_v, d.k_begin, d.k_len, d.k_rows, kv_head, a.dim, lane);
