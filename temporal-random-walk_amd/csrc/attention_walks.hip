@@ -82,6 +82,7 @@ template <typename T, int DB>
 __device__ __forceinline__ void zero_rows(const Rows& r, int64_t begin, int from, int to, int head,
                                           int dim, int lane) {
     typedef Tile<T, DB> G;
+    static_assert(G::kUsed <= 64, "a row at a time at least");
     constexpr int kRows = 64 / G::kUsed;  // at a time
     const int col = lane % G::kUsed * G::kElems;
     if (col >= dim || lane >= kRows * G::kUsed) return;
@@ -95,14 +96,17 @@ __device__ __forceinline__ void zero_rows(const Rows& r, int64_t begin, int from
 template <typename T, int DB>
 __device__ __forceinline__ void load_whole_operand(Frag<T> (&f)[2 * DB], const T* row, int dim,
                                                    int half) {
+    typedef Tile<T, DB> G;
 #pragma unroll
     for (int s = 0; s < 2 * DB; ++s) {
         union {
-            u32x4 u;
+            u32x4 u[sizeof(T) / 2];
             Frag<T> f;
         } x;
-        const int col = 16 * s + 8 * half;
-        x.u = *reinterpret_cast<const u32x4*>(row + (col < dim ? col : 0));
+        const int col = 16 * s + 8 * half < dim ? 16 * s + 8 * half : 0;
+#pragma unroll
+        for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h)
+            x.u[h] = *reinterpret_cast<const u32x4*>(row + col + h * G::kElems);
         f[s] = x.f;
     }
     if (dim < 32 * DB) {
@@ -113,6 +117,13 @@ __device__ __forceinline__ void load_whole_operand(Frag<T> (&f)[2 * DB], const T
                 for (int e = 0; e < 8; ++e) f[s][e] = static_cast<T>(0.0f);
             }
     }
+}
+
+// Byte of elements 8 g + 4 half .. + 4 of a row of a tile.
+template <typename G, typename T>
+__device__ __forceinline__ int four_at(int row, int g, int half) {
+    if (sizeof(T) == 4) return G::slot(row, 2 * g + half) * 16;
+    return G::slot(row, g) * 16 + half * 8;
 }
 
 // A block's accumulators (a column each a row of the output) as rows of global
@@ -135,7 +146,7 @@ __device__ __forceinline__ void store_rows(u32x4* tile, const f32x16 (&acc)[DB],
             for (int e = 0; e < 4; ++e)
                 v[e] = static_cast<T>(any ? acc[b][4 * g + e] * by : 0.0f);
             *reinterpret_cast<t4*>(reinterpret_cast<char*>(tile) +
-                                   G::slot(lane & 31, 4 * b + g) * 16 + half * 8) = v;
+                                   four_at<G, T>(lane & 31, 4 * b + g, half)) = v;
         }
     T* base = row_of<T>(r, begin, head);
 #pragma unroll
@@ -302,7 +313,8 @@ __global__ __launch_bounds__(64, DB < 3 ? 2 : 1) void walk_forward_kernel(WalkAr
 // in the first half and the most in the second, the last wave the other way
 // round.  P and dS lie where the keys and values were.
 template <typename T, int DB, int kNB, bool kShared>
-__global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 : 2) void walk_backward_kernel(WalkArgs a) {
+__global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > (sizeof(T) == 4 ? 2 : 4) || DB == 4) ? 1
+                                                                              : 2) void walk_backward_kernel(WalkArgs a) {
     typedef Tile<T, DB> G;
     typedef Tile<T, 1> S;  // P and dS of a block: rows of queries, columns of keys
     constexpr int kBlock = 32 * G::kSlots;
@@ -512,7 +524,7 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > 4 || DB == 4) ? 1 
                 char* at = reinterpret_cast<char*>(tile_of(wave, b));
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int byte = S::slot(lane & 31, c) * 16 + half * 8;
+                    const int byte = four_at<S, T>(lane & 31, c, half);
                     t4 vp, vs;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -620,7 +632,9 @@ void walk_dispatch(int dtype, int dim, int blocks, F&& f) {
             default: by_blocks(t, std::integral_constant<int, 4>(), std::integral_constant<int, 2>()); break;
         }
     };
-    if (dtype == TRW_F16)
+    if (dtype == TRW_F32)
+        by_dim(float{});
+    else if (dtype == TRW_F16)
         by_dim(_Float16{});
     else
         by_dim(__bf16{});
@@ -633,7 +647,7 @@ void walk_dispatch(int dtype, int dim, int blocks, F&& f) {
 // knows the padded length, or the mean of packed walks, whose double should
 // fit.  Longer walks of such a batch still go to the tiles.
 int walk_blocks(const trw_attention_params& p) {
-    if (p.dtype == TRW_F32 || p.docs == 0) return 0;  // float32 products are the bound there
+    if (p.docs == 0) return 0;
     const int db = (p.dim + 31) / 32;
     const int most = db <= 2 ? 3 : 2;
     const int64_t rows = std::max(p.q_rows, p.k_rows);
