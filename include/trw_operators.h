@@ -109,6 +109,8 @@ typedef struct trw_attention_params {
     trw_rows q, k, v, out;
     float* stats; /* [2, heads, q_rows], of the rows' softmax (base 2); written by the forward
                      pass where not NULL, read by the backward pass */
+    trw_rows out_low; /* what rounding took from out, in the same type, for a backward pass that
+                         takes sums of the output's products more exactly; data NULL: not kept */
     /* backward */
     trw_rows d_out, d_q, d_k, d_v;
     float* d_table; /* [heads, num_buckets], where score.table is given */

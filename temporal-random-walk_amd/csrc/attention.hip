@@ -34,7 +34,7 @@ constexpr float kSlack = 8.0f;
 constexpr int kShare = 512;
 
 struct ForwardArgs {
-    Rows q, k, v, out;
+    Rows q, k, v, out, out_low;
     const int4* q_info;
     float* stats;
     Score score;
@@ -239,7 +239,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
                 store_row<float, DB>(a.part_out + part * a.dim, o, seen, 1.0f, a.dim, half);
                 if (half == 0) a.part_stats[part] = make_float2(m, seen ? l : 0.0f);
             } else {
-                store_row<T, DB>(row_of<T>(a.out, i, head), o, seen, 1.0f / l, a.dim, half);
+                store_row<T, DB>(row_of<T>(a.out, i, head), o, seen, 1.0f / l, a.dim, half,
+                                 a.out_low.data ? row_of<T>(a.out_low, i, head) : nullptr);
                 if (half == 0) store_stats(a, stat, seen, m, l);
             }
         }
@@ -316,20 +317,26 @@ __global__ __launch_bounds__(kThreads) void join_forward_kernel(ForwardArgs a) {
     }
     const bool seen = l != 0.0f;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 out;
+    t4 out, low;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(seen ? o[e] / l : 0.0f);
+    for (int e = 0; e < 4; ++e) {
+        const float x = seen ? o[e] / l : 0.0f;
+        out[e] = static_cast<T>(x);
+        low[e] = static_cast<T>(x - static_cast<float>(out[e]));
+    }
     const int head = static_cast<int>(stat / a.q_rows);
     *reinterpret_cast<t4*>(row_of<T>(a.out, stat % a.q_rows, head) + col) = out;
+    if (a.out_low.data)
+        *reinterpret_cast<t4*>(row_of<T>(a.out_low, stat % a.q_rows, head) + col) = low;
     if (col == 0) store_stats(a, stat, seen, m, l);
 }
 
-// Workgroups that may share one tile's keys: where tiles and heads are fewer
-// than four workgroups for each of the 256 compute units, enough for eight, for
+// Workgroups that may share one tile's keys: where tiles and heads are no more
+// than two workgroups for each of the 256 compute units, enough for eight, for
 // each tile as its keys (which the device knows) allow.
 int splits_of(const trw_attention_params& p) {
     const int64_t items = (p.q_rows + kTileRows - 1) / kTileRows * p.heads;
-    if (items == 0 || items > 1024 || walk_blocks(p)) return 1;
+    if (items == 0 || items > 512 || walk_blocks(p)) return 1;
     const int64_t splits = std::min<int64_t>({2048 / items, p.k_rows / kShare, 32});
     return static_cast<int>(std::max<int64_t>(splits, 1));
 }
@@ -360,6 +367,7 @@ void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     a.k = make_rows(p.k);
     a.v = make_rows(p.v);
     a.out = make_rows(p.out);
+    a.out_low = make_rows(p.out_low);
     a.q_info = reinterpret_cast<const int4*>(p.q_rows_info);
     a.stats = p.stats;
     a.score = make_score(p.score);

@@ -23,7 +23,7 @@ constexpr int kThreads = 256;
 constexpr int kTileRows = 128;  // query rows or keys of a workgroup
 
 struct BackwardArgs {
-    Rows q, k, v, out, d_out, d_q, d_k, d_v;
+    Rows q, k, v, out, out_low, d_out, d_q, d_k, d_v;
     const int4* q_info;
     const int4* k_info;
     const float* stats;
@@ -137,6 +137,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 delta = fmaf(static_cast<float>(o[s][e]), static_cast<float>(d_o[s][e]), delta);
+        if (a.out_low.data) {
+            // of o before it was rounded: an error of D is one of every dS of
+            // its row, all of one sign, which a table's sums would keep
+            load_operand<T, DB>(o, row_of<const T>(a.out_low, i, head), any, a.dim, half);
+#pragma unroll
+            for (int s = 0; s < G::kSteps; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    delta = fmaf(static_cast<float>(o[s][e]), static_cast<float>(d_o[s][e]), delta);
+        }
         delta += __shfl_xor(delta, 32);
     }
     const int64_t stat = static_cast<int64_t>(head) * a.q_rows + i;
@@ -660,6 +670,7 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
     a.k = make_rows(p.k);
     a.v = make_rows(p.v);
     a.out = make_rows(p.out);
+    a.out_low = make_rows(p.out_low);
     a.d_out = make_rows(p.d_out);
     a.d_q = make_rows(p.d_q);
     a.d_k = make_rows(p.d_k);

@@ -302,21 +302,27 @@ __device__ __forceinline__ void load_operand(Frag<T> (&f)[2 * DB], const T* row,
 
 // Writes a column's accumulators (rows of the transposed product = elements of
 // the row) as a row of global memory, times `by`; zeros where `any` is false,
-// whatever was accumulated.
+// whatever was accumulated.  low: a row for what rounding took from each, or
+// null.
 template <typename T, int DB>
 __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DB], bool any, float by,
-                                          int dim, int half) {
+                                          int dim, int half, T* low = nullptr) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int col = 32 * b + 8 * g + 4 * half;
             if (col >= dim) continue;
-            typedef T t4 __attribute__((ext_vector_type(4)));
-            t4 v;
+            t4 v, l;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(any ? acc[b][4 * g + e] * by : 0.0f);
+            for (int e = 0; e < 4; ++e) {
+                const float x = any ? acc[b][4 * g + e] * by : 0.0f;
+                v[e] = static_cast<T>(x);
+                l[e] = static_cast<T>(x - static_cast<float>(v[e]));
+            }
             *reinterpret_cast<t4*>(row + col) = v;
+            if (low) *reinterpret_cast<t4*>(low + col) = l;
         }
 }
 

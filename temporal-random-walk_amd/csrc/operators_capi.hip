@@ -104,6 +104,7 @@ void check_forward(const trw_attention_params& p) {
     check_rows(p.k, p.dtype, p.k_rows, "k is null");
     check_rows(p.v, p.dtype, p.k_rows, "v is null");
     check_rows(p.out, p.dtype, p.q_rows, "out is null");
+    if (p.out_low.data) check_rows(p.out_low, p.dtype, p.q_rows, "out_low is null");
     require(p.q_rows == 0 || p.q_rows_info, "q_rows_info is null");
     check_aligned(p.q_rows_info, "q_rows_info must be 16-byte aligned");
     require(p.docs == 0 || p.docs_info, "docs_info is null");

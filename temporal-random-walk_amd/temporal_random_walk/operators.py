@@ -70,7 +70,7 @@ class _AttentionParams(C.Structure):
                 ("own_causal", C.c_int32),
                 ("score", _Score),
                 ("q", _Rows), ("k", _Rows), ("v", _Rows), ("out", _Rows), ("stats", C.c_void_p),
-                ("d_out", _Rows), ("d_q", _Rows), ("d_k", _Rows), ("d_v", _Rows),
+                ("out_low", _Rows), ("d_out", _Rows), ("d_q", _Rows), ("d_k", _Rows), ("d_v", _Rows),
                 ("d_table", C.c_void_p), ("workspace", C.c_void_p),
                 ("workspace_bytes", C.c_uint64)]
 
@@ -412,22 +412,26 @@ class _WalkAttention(torch.autograd.Function):
             _DTYPES[q.dtype], heads, k.shape[1], dim, mask.q_rows, mask.k_rows, mask.q_info,
             mask.k_info, mask.docs_info, mask.docs, mask.longest, mask.own_causal,
             terms.struct(table), _rows(q), _rows(k), _rows(v), _rows(out))
-        stats = None
+        stats = low = None
         if any(ctx.needs_input_grad[:4]):
             stats = torch.empty(2, heads, mask.q_rows, dtype=torch.float32, device=device)
             p.stats = stats.data_ptr()
+            # Walks that go a wave each sum what the backward pass needs of the output there
+            if q.dtype is not torch.float32 and not 0 < mask.longest <= (96 if dim <= 64 else 64):
+                low = torch.empty_like(out)
+                p.out_low = _rows(low)
         space = _workspace(p, 0, device)  # held until the call has queued
         _queue(device, lib().trw_ops_attention_forward, C.byref(p))
         del space
         if stats is not None:
-            ctx.save_for_backward(q, k, v, table, out, stats)
+            ctx.save_for_backward(q, k, v, table, out, stats, low)
             ctx.mask, ctx.terms, ctx.params, ctx.shapes = mask, terms, p, shapes
         return out.view(shapes[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, table, _, _ = ctx.saved_tensors
+        q, k, v, table, *_ = ctx.saved_tensors
         device = q.device
         d_out = _readable(d_out.flatten(0, 1) if d_out.dim() == 4 else d_out)
         d_q, d_k, d_v = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
