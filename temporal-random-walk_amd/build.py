@@ -6,6 +6,8 @@ Produces, inside ``temporal-random-walk_amd/temporal_random_walk/``:
   C ABI of ``include/trw_engine.h``;
 * ``libtrw_operators.so`` -- the operators on walks (attention, its
   single-event form, the distance bias) behind ``include/trw_operators.h``;
+* ``_operators*.so`` -- the same operators on PyTorch tensors (only where
+  PyTorch is installed);
 * ``_temporal_random_walk*.so`` -- the pybind11 module that mirrors the
   reference's Python surface on top of the C++ ``TemporalRandomWalk`` class,
   which calls the C ABI;
@@ -126,6 +128,33 @@ def build_python_module() -> str:
     return target
 
 
+def build_operators_module():
+    """The operators on PyTorch tensors; nothing where PyTorch is missing."""
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError:
+        return None
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    target = os.path.join(OUT_DIR, "_operators" + suffix)
+    tmp = target + ".tmp"
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+        "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_operators",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        f"-I{INCLUDE}", *(f"-I{d}" for d in include_paths()), "-I/opt/rocm/include",
+        f"-I{sysconfig.get_paths()['include']}",
+        os.path.join(HOST, "operators_module.cpp"),
+        f"-L{OUT_DIR}", "-ltrw_operators", "-Wl,-rpath,$ORIGIN",
+        f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+        "-o", tmp,
+    ]
+    _run(cmd)
+    os.replace(tmp, target)
+    return target
+
+
 def build_probe() -> str:
     """bench.py's random-gather probe: its own library beside probe.hip, not
     part of the engine."""
@@ -139,8 +168,10 @@ def build_probe() -> str:
 def build_all() -> None:
     build_engine()
     build_operators()
-    build_python_module()
-    build_probe()
+    with ThreadPoolExecutor(max_workers=3) as ex:
+        for built in [ex.submit(build) for build in (build_python_module, build_operators_module,
+                                                     build_probe)]:
+            built.result()
 
 
 if __name__ == "__main__":

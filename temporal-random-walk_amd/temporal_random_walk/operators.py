@@ -11,199 +11,32 @@ spends its time in:
   table itself).
 
 They run hand-written gfx950 kernels (``libtrw_operators.so``, whose C ABI is
-``include/trw_operators.h``) on the current stream of the tensors' device, wait
-for nothing, and follow PyTorch's rules for tensors used on several streams.
-There is no CPU path.  Import ``torch`` before the engine in one process:
+``include/trw_operators.h``; ``operators_capi`` has it by ctypes) on the current
+stream of the tensors' device, wait for nothing, and follow PyTorch's rules for
+tensors used on several streams.  There is no CPU path.  Import ``torch`` before the engine in one process:
 PyTorch brings a HIP runtime of its own, which has to come up first.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 import os
 
 import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-LIB_PATH = os.path.join(HERE, "libtrw_operators.so")
-ABI_VERSION = 1  # TRW_OPS_ABI_VERSION of include/trw_operators.h
+if not os.path.exists(os.path.join(HERE, "libtrw_operators.so")):
+    raise ImportError("libtrw_operators.so is missing: build it first "
+                      "(python temporal-random-walk_amd/build.py)")
+
+from . import _operators  # noqa: E402
+
 MAX_REACH = 1024
 MAX_BUCKETS = 256
-MAX_ROW_STRIDE = 1 << 22  # elements
-
-# every symbol include/trw_operators.h declares
-EXPORTS = [
-    "trw_ops_walk_mask", "trw_ops_attention_workspace", "trw_ops_attention_forward",
-    "trw_ops_attention_backward", "trw_ops_attention_step_workspace", "trw_ops_attention_step",
-    "trw_ops_relative_bias", "trw_ops_relative_bias_workspace", "trw_ops_relative_bias_backward",
-    "trw_ops_last_error", "trw_ops_abi_version",
-]
-
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_KINDS = {"full": 0, "causal": 1, "prefix": 2}
 
 
-class _Rows(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
-
-
-class _MaskParams(C.Structure):
-    _fields_ = [("docs", C.c_int64), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
-                ("q_length", C.c_int64), ("k_length", C.c_int64),
-                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p),
-                ("q_offsets", C.c_void_p), ("k_offsets", C.c_void_p), ("prefix", C.c_void_p),
-                ("kind", C.c_int32), ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
-                ("docs_info", C.c_void_p)]
-
-
-class _Score(C.Structure):
-    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("table", C.c_void_p),
-                ("buckets", C.c_void_p), ("num_buckets", C.c_int32), ("reach", C.c_int32),
-                ("slopes", C.c_void_p), ("q_times", C.c_void_p), ("k_times", C.c_void_p)]
-
-
-class _AttentionParams(C.Structure):
-    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
-                ("dim", C.c_int32), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
-                ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
-                ("docs_info", C.c_void_p), ("docs", C.c_int64), ("longest", C.c_int64),
-                ("own_causal", C.c_int32),
-                ("score", _Score),
-                ("q", _Rows), ("k", _Rows), ("v", _Rows), ("out", _Rows), ("stats", C.c_void_p),
-                ("out_low", _Rows), ("d_out", _Rows), ("d_q", _Rows), ("d_k", _Rows), ("d_v", _Rows),
-                ("d_table", C.c_void_p), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_uint64)]
-
-
-class _StepParams(C.Structure):
-    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
-                ("dim", C.c_int32), ("batch", C.c_int64), ("capacity", C.c_int64),
-                ("lens", C.c_void_p), ("score", _Score),
-                ("q", _Rows), ("k", _Rows), ("v", _Rows), ("out", _Rows),
-                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
-                ("k_batch_stride", C.c_int64), ("k_pos_stride", C.c_int64),
-                ("k_head_stride", C.c_int64), ("v_batch_stride", C.c_int64),
-                ("v_pos_stride", C.c_int64), ("v_head_stride", C.c_int64),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
-class _BiasParams(C.Structure):
-    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("num_buckets", C.c_int32),
-                ("reach", C.c_int32), ("q_len", C.c_int64), ("k_len", C.c_int64),
-                ("q_offset", C.c_int64), ("table", C.c_void_p), ("buckets", C.c_void_p),
-                ("out", C.c_void_p), ("d_out", C.c_void_p), ("d_out_head_stride", C.c_int64),
-                ("d_out_row_stride", C.c_int64), ("d_table", C.c_void_p),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
-_lib = None
-
-
-def lib():
-    """Load libtrw_operators.so (raises if it has not been built)."""
-    global _lib
-    if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise ImportError(f"{LIB_PATH} is missing: build it first "
-                              "(python temporal-random-walk_amd/build.py)")
-        L = C.CDLL(LIB_PATH)
-        P = C.c_void_p
-        size = C.POINTER(C.c_uint64)
-        L.trw_ops_walk_mask.argtypes = [C.POINTER(_MaskParams), P]
-        L.trw_ops_attention_workspace.argtypes = [C.POINTER(_AttentionParams), C.c_int32, size]
-        L.trw_ops_attention_forward.argtypes = [C.POINTER(_AttentionParams), P]
-        L.trw_ops_attention_backward.argtypes = [C.POINTER(_AttentionParams), P]
-        L.trw_ops_attention_step_workspace.argtypes = [C.POINTER(_StepParams), size]
-        L.trw_ops_attention_step.argtypes = [C.POINTER(_StepParams), P]
-        L.trw_ops_relative_bias.argtypes = [C.POINTER(_BiasParams), P]
-        L.trw_ops_relative_bias_workspace.argtypes = [C.POINTER(_BiasParams), size]
-        L.trw_ops_relative_bias_backward.argtypes = [C.POINTER(_BiasParams), P]
-        L.trw_ops_last_error.restype = C.c_char_p
-        L.trw_ops_abi_version.restype = C.c_int32
-        if L.trw_ops_abi_version() != ABI_VERSION:
-            raise ImportError(f"{LIB_PATH} has ABI {L.trw_ops_abi_version()}, these bindings "
-                              f"expect {ABI_VERSION}: rebuild it")
-        _lib = L
-    return _lib
-
-
-def _call(function, *args):
-    rc = function(*args)
-    if rc != 0:
-        message = lib().trw_ops_last_error().decode()
-        raise {1: ValueError, 3: MemoryError}.get(rc, RuntimeError)(message)
-
-
-def _queue(device, function, *args):
-    """The call with the current stream of a device, on that device."""
-    index = device.index
-    if torch.cuda.current_device() == index:
-        _call(function, *args, torch.cuda.current_stream(index).cuda_stream)
-    else:
-        with torch.cuda.device(index):
-            _call(function, *args, torch.cuda.current_stream(index).cuda_stream)
-
-
-# Messages are put together only where a check fails: a small call's time is the host's.
 def _require(ok, message):
     if not ok:
         raise ValueError(message)
-
-
-def _on_gpu(name, x, device=None):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor")
-    if not x.is_cuda:
-        raise ValueError(f"{name} must be on the GPU")
-    if device is not None and x.device != device:
-        raise ValueError(f"{name} is on another device")
-
-
-def _ints(name, x, shape, device):
-    """An int64 tensor of one shape (a view or a copy of what was given)."""
-    _on_gpu(name, x, device)
-    if x.dtype is not torch.int64:
-        if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
-            raise ValueError(f"{name} must hold whole numbers")
-        x = x.to(torch.int64)
-    if x.shape != shape:
-        raise ValueError(f"{name} must have the shape {shape}")
-    return x.contiguous()
-
-
-def _floats(name, x, shape, device):
-    _on_gpu(name, x, device)
-    if x.dtype is not torch.float32:
-        raise ValueError(f"{name} must be float32")
-    if x.shape != shape:
-        raise ValueError(f"{name} must have the shape {shape}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} has no gradient here")
-    return x.contiguous()
-
-
-def _pieces(x):
-    """Whether rows of the last dimension can be read 16 bytes at a time."""
-    *outer, last = x.stride()
-    if last != 1 or x.data_ptr() % 16:
-        return False
-    per = 16 // x.element_size()
-    for s in outer:
-        if s % per:
-            return False
-    return True
-
-
-def _readable(x):
-    """The tensor, or a copy where its rows are not 16-byte pieces (or lie further apart than the
-    kernels count)."""
-    if x.numel() == 0 or (_pieces(x) and x.stride(0) <= MAX_ROW_STRIDE):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _rows(x):
-    return _Rows(x.data_ptr(), x.stride(0), x.stride(1))
 
 
 def distance_buckets(num_buckets, reach, bidirectional=False, device="cuda"):
@@ -249,202 +82,34 @@ class WalkMask:
     nothing: their output and gradients are zero.
 
     Lengths and offsets stay on the device and are not read back; values out of
-    range are clamped."""
+    range are clamped.
 
-    def __init__(self, *, docs, q_rows, k_rows, q_shape, k_shape, device, kind, q_lens=None,
-                 k_lens=None, q_length=0, k_length=0, q_offsets=None, k_offsets=None,
-                 prefix=None):
-        _require(kind in _KINDS, f"kind must be one of {', '.join(_KINDS)}")
-        _require((prefix is not None) == (kind == "prefix"), "prefix is for the prefix mask")
-        if prefix is not None:
-            prefix = _ints("prefix", prefix, (docs,), device)
+    :meth:`record_stream` is for a mask that is used on another stream than the
+    one that was current when it was made, as a tensor's is."""
+
+    def __init__(self, mask, kind):
+        self._mask = mask
         self.kind = kind
-        self.q_rows, self.k_rows = q_rows, k_rows
-        self.q_shape, self.k_shape = q_shape, k_shape  # leading dimensions of q; of k and v
-        self.device = device
-        # rows' and documents' intervals, one after another
-        self._info = torch.empty(4 * (q_rows + k_rows) + 8 * docs, dtype=torch.int32,
-                                 device=device)
-        self.q_info = self._info.data_ptr()
-        self.k_info = self.q_info + 16 * q_rows
-        self.docs_info = self.k_info + 16 * k_rows
-        self.docs = docs
-        # of any document, where the host knows it
-        self.longest = max(q_length, k_length) if q_offsets is None else 0
-        self.own_causal = kind == "causal" and k_lens is None and k_offsets is None
-        p = _MaskParams(docs, q_rows, k_rows, q_length, k_length, _ptr(q_lens), _ptr(k_lens),
-                        _ptr(q_offsets), _ptr(k_offsets), _ptr(prefix), _KINDS[kind],
-                        self.q_info, self.k_info, self.docs_info)
-        _queue(device, lib().trw_ops_walk_mask, C.byref(p))
+        self.q_rows, self.k_rows = mask.q_rows, mask.k_rows
+        # leading dimensions of q; of k and v
+        self.q_shape, self.k_shape = tuple(mask.q_shape), tuple(mask.k_shape)
+        self.device = mask.info.device
+
+    def record_stream(self, stream):
+        self._mask.info.record_stream(stream)
 
     @classmethod
     def padded(cls, lens, length, *, k_lens=None, k_length=None, kind="causal", prefix=None):
         """Walks as the sampler leaves them: ``[walks, length]`` rows, of which
         the first ``lens[w]`` are walk w's.  ``k_lens``/``k_length``: keys that
         are not the queries' own rows."""
-        _on_gpu("lens", lens)
-        _require(lens.dim() == 1, "lens must have one dimension")
-        docs, length = lens.shape[0], int(length)
-        _require(length >= 0, "length must not be negative")
-        _require((k_lens is None) == (k_length is None), "k_lens and k_length go together")
-        lens = _ints("lens", lens, (docs,), lens.device)
-        own = k_lens is None
-        if not own:
-            k_lens, k_length = _ints("k_lens", k_lens, (docs,), lens.device), int(k_length)
-            _require(k_length >= 0, "k_length must not be negative")
-        kl = length if own else k_length
-        return cls(docs=docs, q_rows=docs * length, k_rows=docs * kl, q_shape=(docs, length),
-                   k_shape=(docs, kl), device=lens.device, kind=kind, q_lens=lens,
-                   k_lens=k_lens, q_length=length, k_length=kl, prefix=prefix)
+        return cls(_operators.padded_mask(lens, length, k_lens, k_length, kind, prefix), kind)
 
     @classmethod
     def packed(cls, offsets, rows, *, k_offsets=None, k_rows=None, kind="causal", prefix=None):
         """Documents one after another: document w has the rows
         ``offsets[w]`` up to ``offsets[w + 1]`` of ``rows``."""
-        _on_gpu("offsets", offsets)
-        _require(offsets.dim() == 1 and offsets.shape[0] >= 1,
-                 "offsets must have one dimension and an entry more than documents")
-        _require((k_offsets is None) == (k_rows is None), "k_offsets and k_rows go together")
-        offsets = _ints("offsets", offsets, tuple(offsets.shape), offsets.device)
-        rows = int(rows)
-        if k_offsets is not None:
-            k_offsets = _ints("k_offsets", k_offsets, tuple(offsets.shape), offsets.device)
-        kr = rows if k_rows is None else int(k_rows)
-        _require(rows >= 0 and kr >= 0, "rows must not be negative")
-        return cls(docs=offsets.shape[0] - 1, q_rows=rows, k_rows=kr, q_shape=(rows,),
-                   k_shape=(kr,), device=offsets.device, kind=kind, q_offsets=offsets,
-                   k_offsets=k_offsets, prefix=prefix)
-
-
-def _ptr(x):
-    return None if x is None else x.data_ptr()
-
-
-class _Terms:
-    """The checked terms of a score besides the products; holds its tensors."""
-
-    def __init__(self, heads, device, dim, scale, softcap, buckets, num_buckets, slopes, times,
-                 k_times, time_shapes):
-        self.scale = dim ** -0.5 if scale is None else float(scale)
-        self.softcap = float(softcap)
-        self.buckets, self.num_buckets = buckets, num_buckets
-        self.slopes = None if slopes is None else _floats("slopes", slopes, (heads,), device)
-        _require(times is None or slopes is not None, "times are for slopes")
-        _require(k_times is None or times is not None, "k_times go with times")
-        self.times = self.k_times = None
-        if times is not None:
-            self.times = _floats("times", times, time_shapes[0], device)
-            self.k_times = (self.times if k_times is None or k_times is times
-                            else _floats("k_times", k_times, time_shapes[1], device))
-            if self.k_times.shape != time_shapes[1]:
-                raise ValueError(f"k_times must have the shape {time_shapes[1]}")
-
-    def struct(self, table):
-        b = self.buckets
-        return _Score(self.scale, self.softcap, _ptr(table), _ptr(b),
-                      self.num_buckets, 0 if b is None else b.shape[0] // 2,
-                      _ptr(self.slopes), _ptr(self.times), _ptr(self.k_times))
-
-
-def _bias_arguments(table, buckets, heads, device):
-    """(float32 table, bucket ids, number of buckets) or Nones."""
-    _require((table is None) == (buckets is None), "bias_table and buckets go together")
-    if table is None:
-        return None, None, 0
-    _on_gpu("bias_table", table, device)
-    _on_gpu("buckets", buckets, device)
-    _require(table.dim() == 2 and table.shape[0] == heads,
-             "bias_table must be [heads, num_buckets]")
-    _require(table.dtype in _DTYPES, "bias_table must be float32, float16 or bfloat16")
-    if not 1 <= table.shape[1] <= MAX_BUCKETS:
-        raise ValueError(f"1 to {MAX_BUCKETS} buckets")
-    _check_ids(buckets)
-    return table.float().contiguous(), buckets.contiguous(), table.shape[1]
-
-
-def _check_ids(buckets):
-    _require(buckets.dtype == torch.int32 and buckets.dim() == 1 and buckets.shape[0] % 2 == 1,
-             "buckets must be an int32 tensor of 2 reach + 1 ids")
-    if buckets.shape[0] // 2 > MAX_REACH:
-        raise ValueError(f"reach must be 0 to {MAX_REACH}")
-
-
-def _check_qkv(q, k, v, dims):
-    _on_gpu("q", q)
-    _on_gpu("k", k, q.device)
-    _on_gpu("v", v, q.device)
-    if q.dim() != dims:
-        raise ValueError(f"q must have {dims} dimensions")
-    _require(k.shape == v.shape, "k and v must have the same shape")
-    _require(k.dim() == dims and q.shape[-1] == k.shape[-1], "q and k must have the same head size")
-    _require(q.dtype in _DTYPES, "q must be float32, float16 or bfloat16")
-    _require(q.dtype == k.dtype == v.dtype, "q, k and v must have the same type")
-    heads, kv_heads, dim = q.shape[-2], k.shape[-2], q.shape[-1]
-    _require(kv_heads > 0 and heads > 0 and heads % kv_heads == 0,
-             "heads must be a positive multiple of the key heads")
-    _require(0 < dim <= 128 and dim % 8 == 0, "the head size must be a multiple of 8 up to 128")
-    return heads, kv_heads, dim
-
-
-def _workspace(p, backward, device):
-    size = C.c_uint64()
-    _call(lib().trw_ops_attention_workspace, C.byref(p), backward, C.byref(size))
-    if not size.value:
-        return None
-    space = torch.empty(size.value, dtype=torch.uint8, device=device)
-    p.workspace, p.workspace_bytes = space.data_ptr(), size.value
-    return space
-
-
-class _WalkAttention(torch.autograd.Function):
-    """q, k, v: [walks, length, heads, dim] or [rows, heads, dim]."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, mask, terms):
-        shapes = q.shape, k.shape
-        if q.dim() == 4:
-            q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
-        q, k, v = _readable(q), _readable(k), _readable(v)
-        device = q.device
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        _, heads, dim = q.shape
-        p = _AttentionParams(
-            _DTYPES[q.dtype], heads, k.shape[1], dim, mask.q_rows, mask.k_rows, mask.q_info,
-            mask.k_info, mask.docs_info, mask.docs, mask.longest, mask.own_causal,
-            terms.struct(table), _rows(q), _rows(k), _rows(v), _rows(out))
-        stats = low = None
-        if any(ctx.needs_input_grad[:4]):
-            stats = torch.empty(2, heads, mask.q_rows, dtype=torch.float32, device=device)
-            p.stats = stats.data_ptr()
-            # Walks that go a wave each sum what the backward pass needs of the output there
-            if q.dtype is not torch.float32 and not 0 < mask.longest <= (96 if dim <= 64 else 64):
-                low = torch.empty_like(out)
-                p.out_low = _rows(low)
-        space = _workspace(p, 0, device)  # held until the call has queued
-        _queue(device, lib().trw_ops_attention_forward, C.byref(p))
-        del space
-        if stats is not None:
-            ctx.save_for_backward(q, k, v, table, out, stats, low)
-            ctx.mask, ctx.terms, ctx.params, ctx.shapes = mask, terms, p, shapes
-        return out.view(shapes[0])
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out):
-        q, k, v, table, *_ = ctx.saved_tensors
-        device = q.device
-        d_out = _readable(d_out.flatten(0, 1) if d_out.dim() == 4 else d_out)
-        d_q, d_k, d_v = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
-        d_table = None if table is None else torch.empty_like(table)
-        p = _AttentionParams.from_buffer_copy(ctx.params)
-        p.d_out, p.d_q, p.d_k, p.d_v = _rows(d_out), _rows(d_q), _rows(d_k), _rows(d_v)
-        p.d_table = _ptr(d_table)
-        p.workspace, p.workspace_bytes = None, 0
-        space = _workspace(p, 1, device)
-        _queue(device, lib().trw_ops_attention_backward, C.byref(p))
-        del space
-        q_shape, k_shape = ctx.shapes
-        return d_q.view(q_shape), d_k.view(k_shape), d_v.view(k_shape), d_table, None, None
+        return cls(_operators.packed_mask(offsets, rows, k_offsets, k_rows, kind, prefix), kind)
 
 
 def walk_attention(q, k, v, mask, *, scale=None, softcap=0.0, bias_table=None, buckets=None,
@@ -470,19 +135,10 @@ def walk_attention(q, k, v, mask, *, scale=None, softcap=0.0, bias_table=None, b
     (once).  Equal inputs give equal results, bit for bit.  A row that sees no
     key is zero.  Values that are not finite stay within their own walk."""
     _require(isinstance(mask, WalkMask), "mask must be a WalkMask")
-    heads, _, dim = _check_qkv(q, k, v, len(mask.q_shape) + 2)
-    _require(q.device == mask.device, "q is on another device than the mask")
-    if q.shape[:-2] != mask.q_shape:
-        raise ValueError(f"q must be {mask.q_shape} rows of heads")
-    if k.shape[:-2] != mask.k_shape:
-        raise ValueError(f"k must be {mask.k_shape} rows of heads")
-    table, buckets, num_buckets = _bias_arguments(bias_table, buckets, heads, q.device)
-    terms = _Terms(heads, q.device, dim, scale, softcap, buckets, num_buckets, slopes, times,
-                   k_times, (mask.q_shape, mask.k_shape))
-    return _WalkAttention.apply(q, k, v, table, mask, terms)
+    return _operators.walk_attention(q, k, v, mask._mask, scale, softcap, bias_table, buckets,
+                                     slopes, times, k_times)
 
 
-@torch.no_grad()
 def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=0.0,
                         bias_table=None, buckets=None, slopes=None, times=None, k_times=None):
     """One new event of each of a batch of walks: appends ``k`` and ``v``
@@ -498,69 +154,8 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
 
     A negative length is an idle row: output 0, caches untouched.  A full cache
     (``lens[b] >= capacity``) gives NaN and leaves the caches untouched."""
-    heads, kv_heads, dim = _check_qkv(q, k, v, 3)
-    batch, device = q.shape[0], q.device
-    _require(k.shape[0] == batch, "q and k must have the same batch")
-    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _on_gpu(name, x, device)
-        if (x.dtype is not q.dtype or x.dim() != 4 or x.shape[0] != batch
-                or x.shape[2:] != (kv_heads, dim)):
-            raise ValueError(f"{name} must be [batch, capacity, kv_heads, dim] of q's type")
-        if x.numel() and not _pieces(x):
-            raise ValueError(f"{name}'s rows must be 16-byte pieces")
-    _require(k_cache.shape == v_cache.shape, "k_cache and v_cache must have the same shape")
-    capacity = k_cache.shape[1]
-    lens = _ints("lens", lens, (batch,), device)
-    table, buckets, num_buckets = _bias_arguments(bias_table, buckets, heads, device)
-    _require((times is None) == (k_times is None), "times and k_times go together")
-    _require(k_times is None or k_times.is_contiguous(), "k_times must be contiguous")
-    terms = _Terms(heads, device, dim, scale, softcap, buckets, num_buckets, slopes, times,
-                   k_times, ((batch,), (batch, capacity)))
-    q, k, v = _readable(q), _readable(k), _readable(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    p = _StepParams(
-        _DTYPES[q.dtype], heads, kv_heads, dim, batch, capacity, lens.data_ptr(),
-        terms.struct(table), _rows(q), _rows(k), _rows(v), _rows(out), k_cache.data_ptr(),
-        v_cache.data_ptr(), *k_cache.stride()[:3], *v_cache.stride()[:3])
-    size = C.c_uint64()
-    _call(lib().trw_ops_attention_step_workspace, C.byref(p), C.byref(size))
-    if size.value:
-        space = torch.empty(size.value, dtype=torch.uint8, device=device)
-        p.workspace, p.workspace_bytes = space.data_ptr(), size.value
-    _queue(device, lib().trw_ops_attention_step, C.byref(p))
-    return out
-
-
-class _RelativeBias(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, buckets, q_len, k_len, q_offset):
-        table = table.contiguous()
-        heads, num_buckets = table.shape
-        out = torch.empty(heads, q_len, k_len, dtype=table.dtype, device=table.device)
-        p = _BiasParams(_DTYPES[table.dtype], heads, num_buckets, buckets.shape[0] // 2, q_len,
-                        k_len, q_offset, table.data_ptr(), buckets.data_ptr(), out.data_ptr())
-        _queue(table.device, lib().trw_ops_relative_bias, C.byref(p))
-        ctx.save_for_backward(table, buckets)
-        ctx.q_offset = q_offset
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out):
-        table, buckets = ctx.saved_tensors
-        if d_out.stride(-1) != 1:
-            d_out = d_out.contiguous()
-        d_table = torch.empty_like(table)
-        p = _BiasParams(_DTYPES[table.dtype], *table.shape, buckets.shape[0] // 2,
-                        d_out.shape[1], d_out.shape[2], ctx.q_offset, table.data_ptr(),
-                        buckets.data_ptr(), None, d_out.data_ptr(), d_out.stride(0),
-                        d_out.stride(1), d_table.data_ptr())
-        size = C.c_uint64()
-        _call(lib().trw_ops_relative_bias_workspace, C.byref(p), C.byref(size))
-        space = torch.empty(max(16, size.value), dtype=torch.uint8, device=table.device)
-        p.workspace, p.workspace_bytes = space.data_ptr(), size.value
-        _queue(table.device, lib().trw_ops_relative_bias_backward, C.byref(p))
-        return d_table, None, None, None, None
+    return _operators.walk_attention_step(q, k, v, k_cache, v_cache, lens, scale, softcap,
+                                          bias_table, buckets, slopes, times, k_times)
 
 
 def relative_bias(table, buckets, q_len, k_len, q_offset=0):
@@ -568,13 +163,4 @@ def relative_bias(table, buckets, q_len, k_len, q_offset=0):
     reach)]]``: the dense ``[heads, q_len, k_len]`` bias of a learned table
     ``[heads, num_buckets]``, in the table's type; differentiable by the table
     (once).  ``buckets``: as for :func:`walk_attention`."""
-    _on_gpu("table", table)
-    _on_gpu("buckets", buckets, table.device)
-    _require(table.dim() == 2 and table.shape[0] > 0, "table must be [heads, num_buckets]")
-    _require(table.dtype in _DTYPES, "table must be float32, float16 or bfloat16")
-    if not 1 <= table.shape[1] <= MAX_BUCKETS:
-        raise ValueError(f"1 to {MAX_BUCKETS} buckets")
-    _check_ids(buckets)
-    q_len, k_len, q_offset = int(q_len), int(k_len), int(q_offset)
-    _require(q_len >= 0 and k_len >= 0, "lengths must not be negative")
-    return _RelativeBias.apply(table, buckets.contiguous(), q_len, k_len, q_offset)
+    return _operators.relative_bias(table, buckets, q_len, k_len, q_offset)

@@ -1,0 +1,111 @@
+"""The C ABI of the operators (include/trw_operators.h) by ctypes, for callers
+with device pointers of their own.  Programs on PyTorch tensors use
+``temporal_random_walk.operators``."""
+from __future__ import annotations
+
+import ctypes as C
+import os
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+LIB_PATH = os.path.join(HERE, "libtrw_operators.so")
+ABI_VERSION = 1  # TRW_OPS_ABI_VERSION
+
+# every symbol the header declares
+EXPORTS = [
+    "trw_ops_walk_mask", "trw_ops_attention_workspace", "trw_ops_attention_forward",
+    "trw_ops_attention_backward", "trw_ops_attention_step_workspace", "trw_ops_attention_step",
+    "trw_ops_relative_bias", "trw_ops_relative_bias_workspace", "trw_ops_relative_bias_backward",
+    "trw_ops_last_error", "trw_ops_abi_version",
+]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class MaskParams(C.Structure):
+    _fields_ = [("docs", C.c_int64), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
+                ("q_length", C.c_int64), ("k_length", C.c_int64),
+                ("q_lens", C.c_void_p), ("k_lens", C.c_void_p),
+                ("q_offsets", C.c_void_p), ("k_offsets", C.c_void_p), ("prefix", C.c_void_p),
+                ("kind", C.c_int32), ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
+                ("docs_info", C.c_void_p)]
+
+
+class Score(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("table", C.c_void_p),
+                ("buckets", C.c_void_p), ("num_buckets", C.c_int32), ("reach", C.c_int32),
+                ("slopes", C.c_void_p), ("q_times", C.c_void_p), ("k_times", C.c_void_p)]
+
+
+class AttentionParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("dim", C.c_int32), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
+                ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
+                ("docs_info", C.c_void_p), ("docs", C.c_int64), ("longest", C.c_int64),
+                ("own_causal", C.c_int32),
+                ("score", Score),
+                ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("stats", C.c_void_p),
+                ("out_low", Rows), ("d_out", Rows), ("d_q", Rows), ("d_k", Rows), ("d_v", Rows),
+                ("d_table", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class StepParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("dim", C.c_int32), ("batch", C.c_int64), ("capacity", C.c_int64),
+                ("lens", C.c_void_p), ("score", Score),
+                ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows),
+                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("k_batch_stride", C.c_int64), ("k_pos_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_batch_stride", C.c_int64),
+                ("v_pos_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class BiasParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("num_buckets", C.c_int32),
+                ("reach", C.c_int32), ("q_len", C.c_int64), ("k_len", C.c_int64),
+                ("q_offset", C.c_int64), ("table", C.c_void_p), ("buckets", C.c_void_p),
+                ("out", C.c_void_p), ("d_out", C.c_void_p), ("d_out_head_stride", C.c_int64),
+                ("d_out_row_stride", C.c_int64), ("d_table", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+_lib = None
+
+
+def lib():
+    """Load libtrw_operators.so (raises if it has not been built)."""
+    global _lib
+    if _lib is None:
+        if not os.path.exists(LIB_PATH):
+            raise ImportError(f"{LIB_PATH} is missing: build it first "
+                              "(python temporal-random-walk_amd/build.py)")
+        L = C.CDLL(LIB_PATH)
+        P = C.c_void_p
+        size = C.POINTER(C.c_uint64)
+        L.trw_ops_walk_mask.argtypes = [C.POINTER(MaskParams), P]
+        L.trw_ops_attention_workspace.argtypes = [C.POINTER(AttentionParams), C.c_int32, size]
+        L.trw_ops_attention_forward.argtypes = [C.POINTER(AttentionParams), P]
+        L.trw_ops_attention_backward.argtypes = [C.POINTER(AttentionParams), P]
+        L.trw_ops_attention_step_workspace.argtypes = [C.POINTER(StepParams), size]
+        L.trw_ops_attention_step.argtypes = [C.POINTER(StepParams), P]
+        L.trw_ops_relative_bias.argtypes = [C.POINTER(BiasParams), P]
+        L.trw_ops_relative_bias_workspace.argtypes = [C.POINTER(BiasParams), size]
+        L.trw_ops_relative_bias_backward.argtypes = [C.POINTER(BiasParams), P]
+        L.trw_ops_last_error.restype = C.c_char_p
+        L.trw_ops_abi_version.restype = C.c_int32
+        if L.trw_ops_abi_version() != ABI_VERSION:
+            raise ImportError(f"{LIB_PATH} has ABI {L.trw_ops_abi_version()}, these bindings "
+                              f"expect {ABI_VERSION}: rebuild it")
+        _lib = L
+    return _lib
+
+
+def call(function, *args):
+    """A function of the library; a failure's status and message as an exception."""
+    rc = function(*args)
+    if rc != 0:
+        message = lib().trw_ops_last_error().decode()
+        raise {1: ValueError, 3: MemoryError}.get(rc, RuntimeError)(message)

@@ -19,28 +19,33 @@ def _ops():
     return operators
 
 
+def _abi():
+    from temporal_random_walk import operators_capi
+    return operators_capi
+
+
 def test_library_exports_every_declared_symbol():
-    ops = _ops()
+    ops, abi = _ops(), _abi()
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
     declared = sorted(set(re.findall(r"\b(trw_ops_[a-z_]+)\s*\(", text)))
-    assert declared == sorted(ops.EXPORTS)
-    lib = ops.lib()
+    assert declared == sorted(abi.EXPORTS)
+    lib = abi.lib()
     assert not [n for n in declared if not hasattr(lib, n)]
     version = int(re.search(r"#define TRW_OPS_ABI_VERSION (\d+)", open(HEADER).read()).group(1))
-    assert lib.trw_ops_abi_version() == ops.ABI_VERSION == version
-    assert b"gfx950" in open(ops.LIB_PATH, "rb").read()
+    assert lib.trw_ops_abi_version() == abi.ABI_VERSION == version
+    assert b"gfx950" in open(abi.LIB_PATH, "rb").read()
     limits = dict(re.findall(r"#define TRW_OPS_(MAX_\w+) (\d+)", open(HEADER).read()))
     assert {k: int(v) for k, v in limits.items()} == {"MAX_REACH": ops.MAX_REACH,
                                                       "MAX_BUCKETS": ops.MAX_BUCKETS}
 
 
-def _attention(ops, **changes):
+def _attention(abi, **changes):
     """Arguments that pass every check (their addresses are never followed: each test breaks one
     of them, or asks for a size only)."""
-    rows = lambda h: ops._Rows(4096, h * 64, 64)  # noqa: E731
-    p = ops._AttentionParams(dtype=2, heads=4, kv_heads=2, dim=64, q_rows=100, k_rows=100,
+    rows = lambda h: abi.Rows(4096, h * 64, 64)  # noqa: E731
+    p = abi.AttentionParams(dtype=2, heads=4, kv_heads=2, dim=64, q_rows=100, k_rows=100,
                              q_rows_info=4096, k_rows_info=4096,
-                             score=ops._Score(0.125, 0.0), q=rows(4), k=rows(2), v=rows(2),
+                             score=abi.Score(0.125, 0.0), q=rows(4), k=rows(2), v=rows(2),
                              out=rows(4), stats=4096, d_out=rows(4), d_q=rows(4), d_k=rows(2),
                              d_v=rows(2))
     for name, value in changes.items():
@@ -67,10 +72,10 @@ def _attention(ops, **changes):
     (dict(score__q_times=4096, score__k_times=4096), "slopes"),
 ])
 def test_attention_refusals(changes, message):
-    ops = _ops()
-    for function in (ops.lib().trw_ops_attention_forward, ops.lib().trw_ops_attention_backward):
+    abi = _abi()
+    for function in (abi.lib().trw_ops_attention_forward, abi.lib().trw_ops_attention_backward):
         with pytest.raises(ValueError, match=message):
-            ops._call(function, ctypes.byref(_attention(ops, **changes)), None)
+            abi.call(function, ctypes.byref(_attention(abi, **changes)), None)
 
 
 @pytest.mark.parametrize("changes,message", [
@@ -79,22 +84,22 @@ def test_attention_refusals(changes, message):
     (dict(score__table=4096, score__buckets=4096, score__num_buckets=4), "d_table"),
 ])
 def test_backward_refusals(changes, message):
-    ops = _ops()
+    abi = _abi()
     with pytest.raises(ValueError, match=message):
-        ops._call(ops.lib().trw_ops_attention_backward, ctypes.byref(_attention(ops, **changes)),
+        abi.call(abi.lib().trw_ops_attention_backward, ctypes.byref(_attention(abi, **changes)),
                   None)
 
 
 def test_null_arguments():
-    ops = _ops()
-    lib = ops.lib()
+    abi = _abi()
+    lib = abi.lib()
     for function in (lib.trw_ops_walk_mask, lib.trw_ops_attention_forward,
                      lib.trw_ops_attention_backward, lib.trw_ops_attention_step,
                      lib.trw_ops_relative_bias, lib.trw_ops_relative_bias_backward):
         with pytest.raises(ValueError, match="null"):
-            ops._call(function, None, None)
+            abi.call(function, None, None)
     with pytest.raises(ValueError, match="null"):
-        ops._call(lib.trw_ops_attention_workspace, ctypes.byref(_attention(ops)), 1, None)
+        abi.call(lib.trw_ops_attention_workspace, ctypes.byref(_attention(abi)), 1, None)
 
 
 @pytest.mark.parametrize("changes,message", [
@@ -104,13 +109,13 @@ def test_null_arguments():
     (dict(q_rows_info=4104), "aligned"),
 ])
 def test_mask_refusals(changes, message):
-    ops = _ops()
-    p = ops._MaskParams(docs=3, q_rows=30, k_rows=30, q_length=10, k_length=10, q_lens=4096,
+    abi = _abi()
+    p = abi.MaskParams(docs=3, q_rows=30, k_rows=30, q_length=10, k_length=10, q_lens=4096,
                         kind=1, q_rows_info=4096, k_rows_info=4096)
     for name, value in changes.items():
         setattr(p, name, value)
     with pytest.raises(ValueError, match=message):
-        ops._call(ops.lib().trw_ops_walk_mask, ctypes.byref(p), None)
+        abi.call(abi.lib().trw_ops_walk_mask, ctypes.byref(p), None)
 
 
 @pytest.mark.parametrize("changes,message", [
@@ -120,16 +125,16 @@ def test_mask_refusals(changes, message):
     (dict(batch=1 << 20), "too many"),
 ])
 def test_step_refusals(changes, message):
-    ops = _ops()
-    rows = lambda h: ops._Rows(4096, h * 64, 64)  # noqa: E731
-    p = ops._StepParams(dtype=2, heads=4, kv_heads=2, dim=64, batch=3, capacity=50, lens=4096,
-                        score=ops._Score(0.125, 0.0), q=rows(4), k=rows(2), v=rows(2), out=rows(4),
+    abi = _abi()
+    rows = lambda h: abi.Rows(4096, h * 64, 64)  # noqa: E731
+    p = abi.StepParams(dtype=2, heads=4, kv_heads=2, dim=64, batch=3, capacity=50, lens=4096,
+                        score=abi.Score(0.125, 0.0), q=rows(4), k=rows(2), v=rows(2), out=rows(4),
                         k_cache=4096, v_cache=4096, k_batch_stride=6400, k_pos_stride=128,
                         k_head_stride=64, v_batch_stride=6400, v_pos_stride=128, v_head_stride=64)
     for name, value in changes.items():
         setattr(p, name, value)
     with pytest.raises(ValueError, match=message):
-        ops._call(ops.lib().trw_ops_attention_step, ctypes.byref(p), None)
+        abi.call(abi.lib().trw_ops_attention_step, ctypes.byref(p), None)
 
 
 @pytest.mark.parametrize("changes,message", [
@@ -138,13 +143,13 @@ def test_step_refusals(changes, message):
     (dict(q_offset=1 << 40), "q_offset"), (dict(dtype=-1), "dtype"),
 ])
 def test_bias_refusals(changes, message):
-    ops = _ops()
-    p = ops._BiasParams(dtype=0, heads=2, num_buckets=4, reach=8, q_len=5, k_len=6, table=4096,
+    abi = _abi()
+    p = abi.BiasParams(dtype=0, heads=2, num_buckets=4, reach=8, q_len=5, k_len=6, table=4096,
                         buckets=4096, out=4096)
     for name, value in changes.items():
         setattr(p, name, value)
     with pytest.raises(ValueError, match=message):
-        ops._call(ops.lib().trw_ops_relative_bias, ctypes.byref(p), None)
+        abi.call(abi.lib().trw_ops_relative_bias, ctypes.byref(p), None)
 
 
 def test_tensors_on_the_cpu_are_refused():
