@@ -386,7 +386,8 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             check_status(trw_ops_attention_forward(&p, on.stream));
         }
         if (train) {
-            ctx->save_for_backward({q, k, v, table.value_or(Tensor()), out, stats, low});
+            // the output itself and no view of it, which would keep it, and so this node, alive
+            ctx->save_for_backward({q, k, v, table.value_or(Tensor()), result, stats, low});
             ctx->saved_data["call"] = c10::IValue::make_capsule(call);
         }
         return result;

@@ -653,3 +653,100 @@ def test_refusals(ops):
         ops.relative_bias(table, ids, -1, 4)
     with pytest.raises(ValueError, match="table"):
         ops.relative_bias(table[0], ids, 4, 4)
+
+
+def test_a_dropped_result_frees_its_memory(ops):
+    """The output's history holds nothing that holds the output."""
+    q, k, v = (torch.randn(2000, 4, 64, device="cuda", dtype=BF, requires_grad=True)
+               for _ in range(3))
+    table = torch.randn(4, 8, device="cuda", requires_grad=True)
+    ids = ops.distance_buckets(8, 16)
+    mask = ops.WalkMask.packed(torch.tensor([0, 700, 2000]).cuda(), 2000)
+
+    def both():
+        ops.walk_attention(q, k, v, mask, bias_table=table, buckets=ids)
+        ops.relative_bias(table, ids, 100, 100)
+
+    both()
+    held = torch.cuda.memory_allocated()
+    for _ in range(5):
+        both()
+    assert torch.cuda.memory_allocated() == held
+
+
+def test_gradients_are_differentiable_once(ops):
+    b = Batch([20, 5], dtype=SF)
+    q, k, v = (x.cuda().requires_grad_() for x in (b.q, b.k, b.v))
+    out = ops.walk_attention(q, k, v, b.mask(ops))
+    (d_q,) = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        d_q.sum().backward()
+    table = torch.randn(2, 4, device="cuda", requires_grad=True)
+    bias = ops.relative_bias(table, ops.distance_buckets(4, 3), 6, 6)
+    (d_table,) = torch.autograd.grad(bias.square().sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        d_table.sum().backward()
+
+
+def test_outputs_changed_in_place(ops):
+    """What the backward pass reads again must be as it was; the rest is the caller's."""
+    b = Batch([20, 5], dtype=SF)
+    want = b.run(ops)
+    q, k, v = (x.cuda().requires_grad_() for x in (b.q, b.k, b.v))
+    out = ops.walk_attention(q, k, v, b.mask(ops))
+    with torch.no_grad():
+        q.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(b.d_out.cuda())
+    with torch.no_grad():
+        q.copy_(b.q)
+    out = ops.walk_attention(q, k, v, b.mask(ops))
+    out.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(b.d_out.cuda())
+    out = ops.walk_attention(q, k, v, b.mask(ops)) * 1
+    out.mul_(1)
+    out.backward(b.d_out.cuda())
+    assert torch.equal(q.grad, want["d_q"])
+
+
+def test_no_memory(ops):
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.relative_bias(torch.zeros(1, 4, device="cuda"), ops.distance_buckets(4, 3),
+                          1 << 20, 1 << 20)
+
+
+def test_a_mask_on_another_stream(ops):
+    """A mask made on one stream, used on another and dropped at once."""
+    b = Batch([300, 60], heads=2, dtype=BF)
+    want = b.run(ops)["out"]
+    q, k, v = (x.cuda() for x in (b.q, b.k, b.v))
+    mask = b.mask(ops)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = ops.walk_attention(q, k, v, mask)
+    mask.record_stream(side)
+    del mask
+    for _ in range(8):  # would take the mask's place
+        b.mask(ops)._mask.info.zero_()
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_example():
+    """examples/walk_model.py at a small size: it learns, and its steps agree with one pass.  Both
+    paths round to bfloat16 six times a layer and twelve in all, each by at most 2^-8 of a value."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "walk_model.py")
+    spec = importlib.util.spec_from_file_location("walk_model", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, served, off, far = example.main(["--nodes", "200", "--walks", "400", "--length", "24",
+                                             "--batch", "200", "--steps", "30"])
+    assert losses[-1] < losses[0] - 1
+    assert served > 1000 and off < 12 * 2 ** -8
+    assert ((far >= 0) & (far < 24)).all()
