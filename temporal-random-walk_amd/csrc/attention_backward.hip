@@ -635,20 +635,21 @@ struct Layout {
 Layout layout_of(const trw_attention_params& p) {
     Layout l;
     uint64_t at = 0;
+    const int blocks = walk_blocks(p);
+    const bool tiles = blocks == 0 || walk_rest(p, blocks);  // else the walks' kernels do it all
     auto take = [&](uint64_t floats) {
         const uint64_t here = at;
         at += align256(floats * sizeof(float));
         return here;
     };
-    l.delta = take(static_cast<uint64_t>(p.heads) * p.q_rows);
+    l.delta = take(tiles ? static_cast<uint64_t>(p.heads) * p.q_rows : 0);
     if (p.score.table) {
         const uint64_t heads = p.heads, line = 2 * static_cast<uint64_t>(p.score.reach) + 1;
-        const int blocks = walk_blocks(p);
-        l.partial = take(heads * tiles_of(p.q_rows) * line);
+        l.partial = take(tiles ? heads * tiles_of(p.q_rows) * line : 0);
         l.walk_partial = take(blocks ? heads * p.docs * walk_line(p, blocks) : 0);
         l.lines = take(heads * 2 * kJoinGroups * line);
     }
-    const int splits = splits_of(p);
+    const int splits = tiles ? splits_of(p) : 1;
     const uint64_t part =
         splits > 1 ? static_cast<uint64_t>(splits) * p.k_rows * p.kv_heads * p.dim : 0;
     l.part_k = take(part);

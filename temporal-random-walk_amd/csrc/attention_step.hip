@@ -10,6 +10,8 @@
 // The new key and value are taken from the call's arguments, not from the
 // cache, by the workgroup whose positions include them, and written to the
 // cache by the walk's first workgroup: no launch and no wait between the two.
+#include <algorithm>
+
 #include "operators.h"
 
 namespace trw {
@@ -53,8 +55,13 @@ __device__ __forceinline__ void put_row(u32x4* tile, const T* row, int from, int
     }
 }
 
+// Two workgroups a compute unit where their tiles (66 KB at head size 128 in 16
+// bits) leave room: left to itself the compiler takes 298 registers there, one
+// workgroup, and 238 walks of 350 events (8 heads of 128, bfloat16) take 113 us
+// for 83 (4.1 TB/s).
 template <typename T, int DB>
-__global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DB <= 2 ? 2 : 1)
+void attention_step_kernel(StepArgs a) {
     typedef Tile<T, DB> G;
     constexpr size_t kTileBytes = G::bytes(kKeys);
     constexpr size_t kJoinBytes = kWaves * 32 * 33 * sizeof(float);
@@ -63,12 +70,16 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
     __shared__ u32x4 s_mem[kBytes / 16];
     __shared__ float s_m[kWaves][32], s_l[kWaves][32], s_times[kWaves][64];
 
-    const int split = blockIdx.x % a.splits;
-    int rest = blockIdx.x / a.splits;
+    // Consecutive workgroups go to the eight XCDs in turn: each takes all key
+    // heads of some positions, which lie side by side.
+    int rest = blockIdx.x / 8;
     const int col_group = rest % a.columns;
     rest /= a.columns;
     const int kv_head = rest % a.kv_heads;
-    const int b = rest / a.kv_heads;
+    const int item = rest / a.kv_heads * 8 + blockIdx.x % 8;
+    const int split = item % a.splits;
+    const int b = item / a.splits;
+    if (b >= a.batch) return;
     const int thread = threadIdx.x, lane = thread & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const Score& sc = a.score;
@@ -330,14 +341,21 @@ __global__ __launch_bounds__(kThreads) void join_step_kernel(StepArgs a) {
     *reinterpret_cast<t4*>(row_of<T>(a.out, b, head) + d) = out;
 }
 
-// Workgroups of one walk and key head: enough for four on each of the 256
-// compute units, each with at least four blocks a wave where the cache is full.
+// Workgroups of one walk and key head: each with at least four blocks a wave
+// where the cache is full.  Few walks: 1536 in all (768 where heads are large and
+// fewer fit), two or three times what the compute units hold, and no more, since
+// each has a sum to join: 3 histories of 100k events (2 key heads of 128) take 59
+// us with 768 and 66 with 1536, 50 walks of up to 58k (4 of 16) 228 with 1536 and
+// 334 with 512.  More walks: three each up to 3072 in all, which evens out their
+// lengths: 64 walks of up to 4k events (8 of 128) take 121 us with three each,
+// 131 with two.
 int splits_of(const trw_attention_step_params& p) {
     const int group = p.heads / p.kv_heads;
     const int64_t items = p.batch * p.kv_heads * ((group + 31) / 32);
     const int64_t most = (p.capacity + 4 * kWaves * kKeys - 1) / (4 * kWaves * kKeys);
-    const int64_t want = (1024 + items - 1) / (items > 0 ? items : 1);
-    return static_cast<int>(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+    const int64_t enough = p.dim > 64 ? 768 : 1536, n = std::max<int64_t>(items, 1);
+    const int64_t want = std::max((enough + n - 1) / n, std::min<int64_t>(3, 3072 / n));
+    return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
 }
 
 }  // namespace
@@ -378,7 +396,7 @@ void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
     a.partial = static_cast<float*>(p.workspace);
     a.part_stats = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(p.batch) * p.heads *
                                                              a.splits * p.dim);
-    const int64_t grid = p.batch * p.kv_heads * a.columns * a.splits;
+    const int64_t grid = xcd_grid(p.batch * a.splits) * p.kv_heads * a.columns;
     require(grid < (int64_t{1} << 31), "too many walks and heads");
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {
         typedef decltype(t) T;

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) void relative_bias_kernel(BiasArgs a) {
 // in LDS, distance d of it in slot (d % kElems) (line / kElems) + d / kElems, so
 // that lanes (kElems apart in distance) meet neither in a slot nor in a bank.
 template <typename T>
-__global__ __launch_bounds__(kThreads, 6) void relative_bias_backward_kernel(BiasArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void relative_bias_backward_kernel(BiasArgs a) {
     constexpr int kElems = 16 / sizeof(T);
     constexpr int kAhead = 2;  // pieces of a lane in flight
     extern __shared__ float s_lines[];  // [4][kElems * pieces]
