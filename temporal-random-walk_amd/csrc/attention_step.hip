@@ -10,6 +10,9 @@
 // The new key and value are taken from the call's arguments, not from the
 // cache, by the workgroup whose positions include them, and written to the
 // cache by the walk's first workgroup: no launch and no wait between the two.
+//
+// 64 walks of up to 4095 events (32 heads of 128 over 8 key heads, bfloat16) take
+// 123 us, 4.5 TB/s of cache; a large copy reaches 4.9, a sum 3.8.
 #include <algorithm>
 
 #include "operators.h"

@@ -15,6 +15,10 @@
 // P and dS are needed both with a lane per query row (for dq, as the registers
 // hold them) and with a lane per key (for dk and dv): they go through 2 KB
 // squares of LDS in the inputs' type and are read back transposed.
+//
+// 20000 walks of up to 80 rows (8 heads of 64, bfloat16) take 1.00 ms forward (4.9
+// TB/s of the rows' and the padding's bytes; a large copy reaches as much) and 2.6
+// backward (by length).
 #include <algorithm>
 
 #include "operators.h"
@@ -27,12 +31,15 @@ struct WalkArgs {
     Rows q, k, v, out, d_out, d_q, d_k, d_v;
     const int4* docs;  // two per document: q begin, len, rows, k begin | k len, rows, prefix, kind
     float* stats;      // as attention.hip writes them
-    float* partial;    // backward: [heads, docs, line] dS by distance
+    float* partial;    // backward: [heads, docs, stride] dS by distance
+    int stride;
     Score score;
     int heads, kv_heads, group, dim;
     int q_rows;
     int doc_count;
-    int limit;
+    int limit;     // this launch's walks: up to so many rows
+    int above;     // backward: and more than these
+    int last;      // backward: no launch takes longer ones
     int triangle;  // backward: a causal walk over its own keys has no tiles above the diagonal
     int time_at;   // backward: where in LDS the floats begin, in 16 bytes
 };
@@ -330,11 +337,12 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > (sizeof(T) == 4 ? 
     Score sc = a.score;
     sc.reach = walk_reach<kNB>(sc);
     const int line = 2 * sc.reach + 1;
-    if (max(d.q_len, d.k_len) > a.limit) {  // the tiles' kernels have it
-        if (sc.table)
+    if (max(d.q_len, d.k_len) <= a.above) return;  // another launch has it
+    if (max(d.q_len, d.k_len) > a.limit) {  // another launch or the tiles' kernels have it
+        if (sc.table && a.last)
             for (int h = first_head; h < first_head + a.group; ++h)
-                for (int n = threadIdx.x; n < line; n += 64 * kNB)
-                    a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * line + n] = 0.0f;
+                for (int n = threadIdx.x; n < a.stride; n += 64 * kNB)
+                    a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * a.stride + n] = 0.0f;
         return;
     }
     const uint32_t at_mem = lds_address(s_mem);
@@ -555,11 +563,14 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > (sizeof(T) == 4 ? 
             }
         }
         if (sc.table) {  // the waves' sums, by the first (they are in: two barriers ago)
-            float* out = a.partial + (static_cast<int64_t>(head) * a.doc_count + doc) * line;
-            for (int n = threadIdx.x; n < line; n += 64 * kNB) {
+            float* out = a.partial + (static_cast<int64_t>(head) * a.doc_count + doc) * a.stride;
+            for (int n = threadIdx.x; n < a.stride; n += 64 * kNB) {
+                const int at = n - (a.stride - line) / 2;
                 float sum = 0.0f;
+                if (at >= 0 && at < line) {
 #pragma unroll
-                for (int w = 0; w < kNB; ++w) sum += s_lut[(1 + w) * line + n];
+                    for (int w = 0; w < kNB; ++w) sum += s_lut[(1 + w) * line + at];
+                }
                 out[n] = sum;
             }
         }
@@ -581,12 +592,12 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > (sizeof(T) == 4 ? 
         if (wave == kNB / 2)
             zero_rows<T, DB>(a.d_q, d.q_begin, heads > 0 ? d.q_len : 0, d.q_rows, h, a.dim, lane);
         if (sc.table && heads == 0)
-            for (int n = threadIdx.x; n < line; n += 64 * kNB)
-                a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * line + n] = 0.0f;
+            for (int n = threadIdx.x; n < a.stride; n += 64 * kNB)
+                a.partial[(static_cast<int64_t>(h) * a.doc_count + doc) * a.stride + n] = 0.0f;
     }
 }
 
-WalkArgs make_args(const trw_attention_params& p, int limit) {
+WalkArgs make_args(const trw_attention_params& p) {
     WalkArgs a;
     a.q = make_rows(p.q);
     a.k = make_rows(p.k);
@@ -599,6 +610,7 @@ WalkArgs make_args(const trw_attention_params& p, int limit) {
     a.docs = reinterpret_cast<const int4*>(p.docs_info);
     a.stats = p.stats;
     a.partial = nullptr;
+    a.stride = 0;
     a.score = make_score(p.score);
     a.heads = p.heads;
     a.kv_heads = p.kv_heads;
@@ -606,8 +618,26 @@ WalkArgs make_args(const trw_attention_params& p, int limit) {
     a.dim = p.dim;
     a.q_rows = static_cast<int>(p.q_rows);
     a.doc_count = static_cast<int>(p.docs);
-    a.limit = limit;
+    a.above = -1;
+    a.limit = 0;
+    a.last = 1;
+    a.triangle = 0;
+    a.time_at = 0;
     return a;
+}
+
+// Whether the backward pass goes by the length of walks, a launch for each number
+// of blocks of 32 rows.  A workgroup has a wave and 16 KB of LDS or more for each
+// block that a walk may have, and walks that have fewer leave them idle; a launch
+// costs each walk that is not its own a workgroup that reads its length and ends.
+// Backward alone, walks of up to 80 (8 key heads of 64, bfloat16): 8192 of them
+// 1155 us in one launch and 1058 by length, 2048 of them 295 and 301; walks of 50
+// to 60 in one of two launches: 1595 and 1635.  Packed walks of up to 40 (2 key
+// heads), of which the host knows the mean alone: 8192 of them 677 and 560 us,
+// 2048 203 and 161, 512 86 and 117.  (The forward pass, whose workgroups are one
+// wave either way: 435 and 484, 185 and 194 us; it has one launch.)
+bool by_length(const trw_attention_params& p) {
+    return p.docs * p.kv_heads >= (p.longest > 0 ? 65536 : 2048);
 }
 
 // f<T, DB, NB>() for the walks that go a wave each: up to 96 rows at head sizes
@@ -646,6 +676,17 @@ void walk_dispatch(int dtype, int dim, int blocks, F&& f) {
 // batch is the tiles' kernels' alone.  Lengths are the device's; the host
 // knows the padded length, or the mean of packed walks, whose double should
 // fit.  Longer walks of such a batch still go to the tiles.
+//
+// Where many walks have a few rows each, most of a wave's 32 columns would be
+// idle, and tiles that several walks share are better: 8192 walks (8 heads of 64
+// over 4 key heads, a bias, bfloat16), forward and backward, take 426 us with a
+// wave each and 185 with tiles at 4 rows, 457 and 371 at 8, 504 and 708 at 12; in
+// float32 at head size 128, 3.7 and 1.2 ms at 4 rows, 3.8 and 2.3 at 8, 3.9 and
+// 4.0 at 12.  64 such walks of 4 rows, which do not fill the device either way,
+// take 105 and 169 us there.
+constexpr int64_t kTinyRows = 8;
+constexpr int64_t kTinyGroups = 2048;
+
 int walk_blocks(const trw_attention_params& p) {
     if (p.docs == 0) return 0;
     const int db = (p.dim + 31) / 32;
@@ -653,6 +694,7 @@ int walk_blocks(const trw_attention_params& p) {
     const int64_t rows = std::max(p.q_rows, p.k_rows);
     const int64_t mean = (rows + p.docs - 1) / p.docs;
     const int64_t length = p.longest > 0 ? p.longest : 2 * mean;
+    if (mean <= kTinyRows && p.docs * p.kv_heads >= kTinyGroups) return 0;
     if (mean > 32 * most || (p.longest > 0 && p.longest > 32 * most)) return 0;
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>((length + 31) / 32, 1), most));
 }
@@ -663,7 +705,8 @@ bool walk_rest(const trw_attention_params& p, int blocks) {
 }
 
 void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream) {
-    const WalkArgs a = make_args(p, 32 * blocks);
+    WalkArgs a = make_args(p);
+    a.limit = 32 * blocks;
     const unsigned grid = walk_grid(p);
     walk_dispatch(p.dtype, p.dim, blocks, [&](auto t, auto db, auto nb) {
         hipLaunchKernelGGL(
@@ -678,26 +721,31 @@ int walk_line(const trw_attention_params& p, int blocks) {
 }
 
 void walk_backward(const trw_attention_params& p, int blocks, float* partial, hipStream_t stream) {
-    WalkArgs a = make_args(p, 32 * blocks);
+    WalkArgs a = make_args(p);
     a.partial = partial;
+    a.stride = walk_line(p, blocks);
     a.triangle = p.own_causal;
     const unsigned grid = walk_grid(p);
-    const int line = walk_line(p, blocks);
-    walk_dispatch(p.dtype, p.dim, blocks, [&](auto t, auto db, auto nb) {
-        typedef decltype(t) T;
-        constexpr int DB = decltype(db)::value, kNB = decltype(nb)::value;
-        constexpr int kBlock = 32 * Tile<T, DB>::kSlots, kTile = 32 * Tile<T, 1>::kSlots;
-        const int tiles = (a.triangle ? kNB * (kNB + 1) / 2 : kNB * kNB) * 2 * kTile;
-        a.time_at = 2 * kNB * kBlock + std::max(2 * kNB * kBlock, tiles);
-        size_t lds = a.time_at * size_t{16} + 64 * kNB * sizeof(float);
-        if (p.score.table) lds += ((1 + kNB) * line + kNB * kSquare) * sizeof(float);
-        if (a.group > 1)
-            hipLaunchKernelGGL((walk_backward_kernel<T, DB, kNB, true>), dim3(grid), dim3(64 * kNB),
-                               lds, stream, a);
-        else
-            hipLaunchKernelGGL((walk_backward_kernel<T, DB, kNB, false>), dim3(grid), dim3(64 * kNB),
-                               lds, stream, a);
-    });
+    for (int n = by_length(p) ? 1 : blocks; n <= blocks; ++n, a.above = a.limit) {
+        a.limit = 32 * n;
+        a.last = n == blocks;
+        const int line = walk_line(p, n);
+        walk_dispatch(p.dtype, p.dim, n, [&](auto t, auto db, auto nb) {
+            typedef decltype(t) T;
+            constexpr int DB = decltype(db)::value, kNB = decltype(nb)::value;
+            constexpr int kBlock = 32 * Tile<T, DB>::kSlots, kTile = 32 * Tile<T, 1>::kSlots;
+            const int tiles = (a.triangle ? kNB * (kNB + 1) / 2 : kNB * kNB) * 2 * kTile;
+            a.time_at = 2 * kNB * kBlock + std::max(2 * kNB * kBlock, tiles);
+            size_t lds = a.time_at * size_t{16} + 64 * kNB * sizeof(float);
+            if (p.score.table) lds += ((1 + kNB) * line + kNB * kSquare) * sizeof(float);
+            if (a.group > 1)
+                hipLaunchKernelGGL((walk_backward_kernel<T, DB, kNB, true>), dim3(grid),
+                                   dim3(64 * kNB), lds, stream, a);
+            else
+                hipLaunchKernelGGL((walk_backward_kernel<T, DB, kNB, false>), dim3(grid),
+                                   dim3(64 * kNB), lds, stream, a);
+        });
+    }
     check_launch("walk_backward");
 }
 

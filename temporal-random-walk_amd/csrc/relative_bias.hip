@@ -13,6 +13,10 @@
 // Backward: sums by distance first, in lanes' registers and lines of LDS that
 // one wave adds to in its own order; workgroups' lines are joined in a fixed
 // order, and distances become buckets once, at the end.
+//
+// 16 heads, 4096 rows of 4199 columns, bfloat16 (550 MB a direction): 90 us
+// forward (6.1 TB/s, a fill reaches 6.9), 180 us for the sums by distance (3.1
+// TB/s, a large sum reaches 3.8), 21 for the two joins.
 #include "operators.h"
 
 namespace trw {

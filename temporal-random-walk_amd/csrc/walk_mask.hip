@@ -7,6 +7,9 @@
 // intervals alone (a wave with a walk of its own, from the walk's spans).  One
 // thread per row of either side and per document; a packed row finds its
 // document by a binary search of the offsets.
+//
+// 32 bytes written per row: 3 us for a small batch (one launch), 14 us for 1.6
+// million rows of padded walks (3.6 TB/s), once for all layers of a batch.
 #include "operators.h"
 
 namespace trw {

@@ -374,8 +374,9 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             stats = at::empty({2, q.size(1), mask.q_rows}, q.options().dtype(at::kFloat));
             p.stats = pointer<float>(stats);
             // Walks that go a wave each sum there what the backward pass needs of the output
+            // (those of up to 8 rows may go through tiles)
             const int64_t wave = p.dim <= 64 ? 96 : 64;
-            if (p.dtype != TRW_F32 && !(mask.longest > 0 && mask.longest <= wave)) {
+            if (p.dtype != TRW_F32 && !(mask.longest > 8 && mask.longest <= wave)) {
                 low = at::empty_like(out);
                 p.out_low = rows_of(low);
             }

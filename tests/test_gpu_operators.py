@@ -134,6 +134,89 @@ def test_terms_of_the_score(ops, dtype, terms, kind):
                       buckets=buckets, num_buckets=n, seed=n, **terms))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group,most,kind", [(64, 2, 36, "causal"), (32, 1, 68, "prefix"),
+                                                 (96, 2, 66, "causal")])
+def test_many_walks_of_many_lengths(ops, dtype, dim, group, most, kind):
+    """So many packed walks that those of each number of 32 rows have a launch of their own in the
+    backward pass, and some that none of those takes."""
+    gen = torch.Generator().manual_seed(dim)
+    lens = torch.randint(0, most, (130,), generator=gen).tolist()
+    lens[40:52] = [0, 1, 31, 32, 33, 64, 65, 96, 97, 130, 200, 2]
+    prefix = [(5 * w) % (n + 2) for w, n in enumerate(lens)] if kind == "prefix" else None
+    _check(ops, Batch(lens, heads=16 * group, kv_heads=16, dim=dim, dtype=dtype, kind=kind,
+                      prefix=prefix, buckets=ops.distance_buckets(4, 50, device="cpu"),
+                      num_buckets=4, softcap=30.0))
+
+
+def _padded(x, lens, length):
+    rows = x.new_full((len(lens), length) + x.shape[1:], math.nan)
+    for w, part in enumerate(x.split(lens)):
+        rows[w, :lens[w]] = part
+    return rows
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["causal", "full"])
+@pytest.mark.parametrize("padded", [False, True])
+def test_many_tiny_walks(ops, dtype, kind, padded):
+    """Walks of a few rows share tiles; padding holds NaN."""
+    gen = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 9, (130,), generator=gen).tolist()
+    if not padded:
+        lens[100:104] = [40, 97, 0, 260]
+    b = Batch(lens, heads=32, kv_heads=16, dim=64, dtype=dtype, kind=kind, slopes=True,
+              buckets=ops.distance_buckets(4, 5, kind == "full", "cpu"), num_buckets=4)
+    if not padded:
+        return _check(ops, b)
+    q, k, v = (_padded(x, lens, 8).cuda().requires_grad_() for x in (b.q, b.k, b.v))
+    table = b.table.cuda().requires_grad_()
+    mask = ops.WalkMask.padded(torch.tensor(lens).cuda(), 8, kind=kind)
+    out = ops.walk_attention(q, k, v, mask, **b.terms(table))
+    out.backward(_padded(b.d_out, lens, 8).cuda())
+    seen = torch.arange(8) < torch.tensor(lens)[:, None]
+    got = {"out": out, "d_q": q.grad, "d_k": k.grad, "d_v": v.grad}
+    for name, (value, bound) in b.reference().items():
+        if name == "d_table":
+            wf.check(name, table.grad, value, bound)
+            continue
+        rows = got[name].detach().cpu()
+        assert not rows[~seen].any()
+        wf.check(name, rows[seen], value, bound)
+
+
+def test_many_padded_walks(ops):
+    """A batch with launches by length against the same walks in smaller batches without: one
+    float32 rounding of each of at most 80 terms either way, of values of the order of one."""
+    gen = torch.Generator().manual_seed(4)
+    n, length, heads = 8200, 40, 8
+    lens = torch.randint(0, length + 1, (n,), generator=gen).cuda()
+    x = torch.randn(4, n, length, heads, 8, generator=gen).cuda()
+    table = torch.randn(heads, 6, generator=gen).cuda()
+    buckets = ops.distance_buckets(6, 36)
+
+    def run(part):
+        q, k, v = (y[part].clone().requires_grad_() for y in x[:3])
+        t = table.clone().requires_grad_()
+        out = ops.walk_attention(q, k, v, ops.WalkMask.padded(lens[part], length), bias_table=t,
+                                 buckets=buckets)
+        out.backward(x[3][part])
+        return [out.detach(), q.grad, k.grad, v.grad], t.grad.double()
+
+    got, got_table = run(slice(0, n))
+    want_table = torch.zeros_like(got_table)
+    scale = torch.zeros_like(got_table)
+    for w in range(0, n, 2050):
+        part = slice(w, w + 2050)
+        want, t = run(part)
+        want_table += t
+        scale += t.abs()
+        for a, b in zip(got, want):
+            torch.testing.assert_close(a[part], b, rtol=1e-4, atol=2e-4)
+    # sums of a few million products, of which the float32 ones hold a few thousand each
+    assert ((got_table - want_table).abs() <= 1e-3 * (scale + 1.0)).all()
+
+
 @pytest.mark.parametrize("k_lens", [None, [50, 1, 400]])
 @pytest.mark.parametrize("reach,num", [(0, 1), (0, 3), (1, 3), (31, 7), (300, 256), (1024, 64)])
 def test_bias_reaches(ops, reach, num, k_lens):
