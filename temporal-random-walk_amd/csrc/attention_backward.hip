@@ -93,6 +93,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
     int4 info = {0, 0, 0, 0};
     if (i < a.q_rows) info = a.q_info[i];
     const bool mine = i < a.q_rows && tiled(info.w, a.walk_limit);
+    // Nothing here for most workgroups of a batch whose walks go a wave each
+    if (!__syncthreads_or(mine)) {
+        if (sc.table)
+            for (int n = thread; n < line; n += kThreads)
+                a.partial[(static_cast<int64_t>(head) * a.q_tiles + tile) * line + n] = 0.0f;
+        return;
+    }
     int lo = info.x, hi = mine ? max(info.x, min(info.y, a.k_rows)) : info.x;
     const int diag = info.z;
     const bool any = lo < hi;
@@ -111,12 +118,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
         s_reduce[wave][0] = w_lo;
         s_reduce[wave][1] = w_hi;
         s_reduce[wave][2] = w_last_lo;
-    }
-    if (!__syncthreads_or(mine)) {
-        if (sc.table)
-            for (int n = thread; n < line; n += kThreads)
-                a.partial[(static_cast<int64_t>(head) * a.q_tiles + tile) * line + n] = 0.0f;
-        return;
     }
     if (sc.table) {
         fill_bias(s_lut, sc, head, thread, kThreads);
