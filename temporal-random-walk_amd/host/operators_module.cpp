@@ -296,12 +296,15 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v, int64_t dims) 
 }
 
 // ---- attention ------------------------------------------------------------------------------------
-// What one call's passes share.
+// What one call's passes share.  The tensors are saved variables: with hooks on
+// those (checkpointing, offloading) the backward pass gets others than the
+// forward pass had, and the first ones may be gone.
 struct Call : torch::CustomClassHolder {
     MaskPtr mask;
     std::optional<Terms> terms;
     trw_attention_params params{};
     std::vector<int64_t> q_shape, k_shape;
+    bool tabled = false, with_low = false;
 };
 using CallPtr = c10::intrusive_ptr<Call>;
 
@@ -318,6 +321,17 @@ Tensor workspace(trw_attention_params& p, int backward, const Tensor& beside) {
 }
 
 Tensor as_rows(const Tensor& x) { return readable(x.dim() == 4 ? x.flatten(0, 1) : x); }
+
+// What was saved as a tensor of this shape, type and device, as a hook gave it
+// back.
+const Tensor& unpacked(const Tensor& x, at::IntArrayRef shape, at::ScalarType type,
+                       const Tensor& beside) {
+    if (!x.defined() || !has_shape(x, shape) || x.scalar_type() != type ||
+        x.device() != beside.device())
+        throw std::runtime_error(
+            "a saved tensor came back from its hook with another shape, type or device");
+    return x;
+}
 
 bool differentiable(const Tensor& grad) {
     return at::GradMode::is_enabled() && grad.requires_grad();
@@ -387,6 +401,8 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             check_status(trw_ops_attention_forward(&p, on.stream));
         }
         if (train) {
+            call->tabled = table.has_value();
+            call->with_low = low.defined();
             // the output itself and no view of it, which would keep it, and so this node, alive
             ctx->save_for_backward({q, k, v, table.value_or(Tensor()), result, stats, low});
             ctx->saved_data["call"] = c10::IValue::make_capsule(call);
@@ -397,15 +413,37 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3];
         const auto call = c10::static_intrusive_pointer_cast<Call>(
             ctx->saved_data["call"].toCapsule());
         const bool again = differentiable(grads[0]);
         at::AutoGradMode no_grad(false);
+        trw_attention_params p = call->params;
+        const at::ScalarType type = grads[0].scalar_type();
+        const auto back = [&](int n, at::IntArrayRef shape, at::ScalarType of) {
+            return unpacked(saved[n], shape, of, grads[0]);
+        };
+        const Tensor q = readable(back(0, {p.q_rows, p.heads, p.dim}, type));
+        const Tensor k = readable(back(1, {p.k_rows, p.kv_heads, p.dim}, type));
+        const Tensor v = readable(back(2, {p.k_rows, p.kv_heads, p.dim}, type));
+        const Tensor out = as_rows(back(4, call->q_shape, type));
+        const Tensor stats = back(5, {2, p.heads, p.q_rows}, at::kFloat).contiguous();
+        p.q = rows_of(q);
+        p.k = rows_of(k);
+        p.v = rows_of(v);
+        p.out = rows_of(out);
+        p.stats = pointer<float>(stats);
+        Tensor table, low;
+        if (call->tabled) {
+            table = back(3, {p.heads, p.score.num_buckets}, at::kFloat).contiguous();
+            p.score.table = pointer<float>(table);
+        }
+        if (call->with_low) {
+            low = readable(back(6, {p.q_rows, p.heads, p.dim}, type));
+            p.out_low = rows_of(low);
+        }
         const Tensor d_out = as_rows(grads[0]);
         Tensor d_q = at::empty(q.sizes(), q.options()), d_k = at::empty(k.sizes(), k.options()),
                d_v = at::empty(v.sizes(), v.options()), d_table;
-        trw_attention_params p = call->params;  // its pointers are the saved tensors'
         p.d_out = rows_of(d_out);
         p.d_q = rows_of(d_q);
         p.d_k = rows_of(d_k);
@@ -522,15 +560,21 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
         check_status(trw_ops_relative_bias(&p, on.stream));
         ctx->save_for_backward({table, buckets});
         ctx->saved_data["q_offset"] = q_offset;
+        ctx->saved_data["num_buckets"] = table.size(1);
+        ctx->saved_data["ids"] = buckets.size(0);
         return out;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &table = saved[0], &buckets = saved[1];
         const bool again = differentiable(grads[0]);
         at::AutoGradMode no_grad(false);
         Tensor d_out = grads[0];
+        const Tensor table =
+            unpacked(saved[0], {d_out.size(0), ctx->saved_data["num_buckets"].toInt()},
+                     d_out.scalar_type(), d_out).contiguous();
+        const Tensor buckets =
+            unpacked(saved[1], {ctx->saved_data["ids"].toInt()}, at::kInt, d_out).contiguous();
         if (d_out.stride(-1) != 1) d_out = d_out.contiguous();
         Tensor d_table = at::empty(table.sizes(), table.options());
         trw_relative_bias_params p = params(table, buckets, d_out.size(1), d_out.size(2),
