@@ -296,15 +296,15 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v, int64_t dims) 
 }
 
 // ---- attention ------------------------------------------------------------------------------------
-// What one call's passes share.  The tensors are saved variables: with hooks on
-// those (checkpointing, offloading) the backward pass gets others than the
-// forward pass had, and the first ones may be gone.
+// What one call's passes share.  The tensors are saved variables: changes between
+// the passes are noticed, and with hooks on them (checkpointing, offloading) the
+// backward pass gets others than the forward pass had, which may be gone.
 struct Call : torch::CustomClassHolder {
     MaskPtr mask;
-    std::optional<Terms> terms;
+    std::optional<Terms> terms;  // until they are saved
     trw_attention_params params{};
     std::vector<int64_t> q_shape, k_shape;
-    bool tabled = false, with_low = false;
+    bool tabled = false, with_low = false, sloped = false, timed = false;
 };
 using CallPtr = c10::intrusive_ptr<Call>;
 
@@ -404,7 +404,12 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             call->tabled = table.has_value();
             call->with_low = low.defined();
             // the output itself and no view of it, which would keep it, and so this node, alive
-            ctx->save_for_backward({q, k, v, table.value_or(Tensor()), result, stats, low});
+            const Terms& terms = *call->terms;
+            ctx->save_for_backward({q, k, v, table.value_or(Tensor()), result, stats, low,
+                                    terms.buckets, terms.slopes, terms.times, terms.k_times});
+            call->sloped = terms.slopes.defined();
+            call->timed = terms.times.defined();
+            call->terms.reset();
             ctx->saved_data["call"] = c10::IValue::make_capsule(call);
         }
         return result;
@@ -432,10 +437,22 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
         p.v = rows_of(v);
         p.out = rows_of(out);
         p.stats = pointer<float>(stats);
-        Tensor table, low;
+        Tensor table, low, buckets, slopes, times, k_times;
         if (call->tabled) {
             table = back(3, {p.heads, p.score.num_buckets}, at::kFloat).contiguous();
+            buckets = back(7, {2 * p.score.reach + 1}, at::kInt).contiguous();
             p.score.table = pointer<float>(table);
+            p.score.buckets = pointer<int32_t>(buckets);
+        }
+        if (call->sloped) {
+            slopes = back(8, {p.heads}, at::kFloat).contiguous();
+            p.score.slopes = pointer<float>(slopes);
+        }
+        if (call->timed) {
+            times = back(9, call->mask->q_shape, at::kFloat).contiguous();
+            k_times = back(10, call->mask->k_shape, at::kFloat).contiguous();
+            p.score.q_times = pointer<float>(times);
+            p.score.k_times = pointer<float>(k_times);
         }
         if (call->with_low) {
             low = readable(back(6, {p.q_rows, p.heads, p.dim}, type));

@@ -137,3 +137,31 @@ def test_hooks_that_give_back_something_else(ops, other):
     for x in (out, bias):
         with pytest.raises(RuntimeError, match="came back from its hook"):
             x.backward(torch.zeros_like(x))
+
+
+@pytest.mark.parametrize("lens", [[20, 3], [130, 200]])
+@pytest.mark.parametrize("name", ["times", "k_times", "slopes", "buckets"])
+def test_terms_changed_between_the_passes(ops, name, lens):
+    """The backward pass works the scores out again: a term that has changed is an error."""
+    case = Case(ops, SF, False, lens)
+    want = case.run()
+    case.terms["k_times"] = case.terms["times"].clone()
+    leaves = case.leaves()
+    out = case.attention(*leaves)
+    case.terms[name].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        case.grads(out, leaves)
+    case.terms[name].sub_(1)
+    out = case.attention(*leaves)
+    got = case.grads(out, leaves)
+    for x in want:
+        assert torch.allclose(got[x], want[x], rtol=0, atol=1e-3), x
+
+
+def test_buckets_changed_between_the_passes_of_the_bias(ops):
+    table = torch.randn(3, 5, device="cuda", requires_grad=True)
+    ids = ops.distance_buckets(5, 7)
+    out = ops.relative_bias(table, ids, 20, 30)
+    ids.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
