@@ -179,8 +179,9 @@ __global__ __launch_bounds__(kThreads, 8) void relative_bias_backward_kernel(Bia
                 for (int e = 0; e < kElems; ++e) {
                     const int at = mine - e;
                     const float value = static_cast<float>(now.t[e]);
+                    // each once, also where reach 0 makes the two ends one
                     before += at >= 2 * reach ? value : 0.0f;
-                    after += at <= 0 && reach > 0 ? value : 0.0f;
+                    after += at <= 0 && at < 2 * reach ? value : 0.0f;
                     const unsigned in = at > 0 && at < 2 * reach ? at : 0;  // 0: read only
                     slot[e] = in % kElems * pieces + in / kElems;
                     line_value[e] = s[slot[e]] + value;

@@ -1,0 +1,38 @@
+"""The operators at the ends of their ranges, against their formulas in float64."""
+import math
+
+import pytest
+import torch
+
+from tests import walk_formulas as wf
+from tests.test_gpu_operators import BF, DTYPES, HF, SF, Batch, _check, _normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from temporal_random_walk import operators
+    return operators
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reach", [0, 1, 2, 7, 8, 1024])
+@pytest.mark.parametrize("q_len,k_len,offset", [(10, 10, 0), (80, 80, 0), (90, 2500, 1200),
+                                                (90, 83, 1200), (130, 600, 0), (70, 65, -30)])
+def test_bias_gradient_of_every_reach(ops, dtype, reach, q_len, k_len, offset):
+    """Each pair counts once, keys after the query too where all distances share one bucket."""
+    gen = torch.Generator().manual_seed(reach + q_len)
+    num = min(256, 2 * reach + 2)
+    ids = (torch.arange(2 * reach + 1) * 7 % num).int()
+    leaf = _normal(gen, 2, num, dtype=dtype).cuda().requires_grad_()
+    # nothing cancels, and no sum leaves float16
+    d_out = ((torch.rand(2, q_len, k_len, generator=gen) + 0.5) / 16).to(dtype)
+    out = ops.relative_bias(leaf, ids.cuda(), q_len, k_len, offset)
+    (grad,) = torch.autograd.grad(out, leaf, d_out.cuda())
+    hop = torch.arange(q_len)[:, None] + offset - torch.arange(k_len)
+    bucket = ids.long()[hop.clamp(-reach, reach) + reach].flatten()
+    want = torch.stack([torch.bincount(bucket, d.flatten().double(), minlength=num) for d in d_out])
+    # A lane adds up to 64 rows of at most ten pieces of eight values in float32, then come its
+    # wave's and the workgroups' sums; all terms have one sign.
+    wf.check("d_table", grad, want, (wf.U[dtype] + 900 * wf.F32) * want.abs() + 1e-30)
