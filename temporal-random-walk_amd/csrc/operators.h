@@ -495,8 +495,9 @@ __device__ __forceinline__ void add_diagonals(const float (&v)[16], float* squar
         const int d = lo - 8 * g + at;
         if (mine && abs(d) < reach) line[d + reach] += sum;
         if (hi - 8 * g >= reach || lo - 8 * g - 7 <= -reach) {
+            // each once, also where reach 0 makes the two ends one
             float before = mine && d >= reach ? sum : 0.0f;
-            float after = mine && d <= -reach && reach ? sum : 0.0f;
+            float after = mine && d <= -reach && d < reach ? sum : 0.0f;
 #pragma unroll
             for (int o = 32; o; o >>= 1) {
                 before += __shfl_xor(before, o);

@@ -36,3 +36,17 @@ def test_bias_gradient_of_every_reach(ops, dtype, reach, q_len, k_len, offset):
     # A lane adds up to 64 rows of at most ten pieces of eight values in float32, then come its
     # wave's and the workgroups' sums; all terms have one sign.
     wf.check("d_table", grad, want, (wf.U[dtype] + 900 * wf.F32) * want.abs() + 1e-30)
+
+
+ONE_DISTANCE = [(0, 1), (0, 3), (1, 3)]
+
+
+@pytest.mark.parametrize("kind", ["full", "prefix", "causal"])
+@pytest.mark.parametrize("reach,num", ONE_DISTANCE)
+@pytest.mark.parametrize("lens", [[20, 1, 33, 40], [50, 1, 170], [260]])
+def test_table_gradient_of_one_distance(ops, kind, reach, num, lens):
+    """Where all distances share a bucket its gradient is a sum that cancels, so a pair that is
+    lost or counted twice shows.  float32: the bound is far below one pair's share."""
+    ids = torch.arange(2 * reach + 1).int() % num
+    prefix = [n // 2 for n in lens] if kind == "prefix" else None
+    _check(ops, Batch(lens, dtype=SF, kind=kind, prefix=prefix, buckets=ids, num_buckets=num))
