@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                         for (int r = 0; r < 16; ++r) {
                             const int d = diag - (j_lane + acc_row(r));
                             far_before += d >= sc.reach ? x[0][r] : 0.0f;
-                            far_after += d <= -sc.reach ? x[0][r] : 0.0f;
+                            far_after += d <= -sc.reach && d < sc.reach ? x[0][r] : 0.0f;
                             if (abs(d) < sc.reach) atomicAdd(&s_sum[d + sc.reach], x[0][r]);
                         }
                     }

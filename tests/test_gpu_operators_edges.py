@@ -50,3 +50,14 @@ def test_table_gradient_of_one_distance(ops, kind, reach, num, lens):
     ids = torch.arange(2 * reach + 1).int() % num
     prefix = [n // 2 for n in lens] if kind == "prefix" else None
     _check(ops, Batch(lens, dtype=SF, kind=kind, prefix=prefix, buckets=ids, num_buckets=num))
+
+
+@pytest.mark.parametrize("kind", ["full", "prefix", "causal"])
+@pytest.mark.parametrize("reach,num", ONE_DISTANCE)
+@pytest.mark.parametrize("q_lens,k_lens", [([5, 9, 4], [50, 20, 300]), ([100, 31, 2], [160, 31, 9])])
+def test_table_gradient_of_one_distance_over_caches(ops, kind, reach, num, q_lens, k_lens):
+    """Prompts of several walks in one wave, whose rows have no diagonal in common."""
+    ids = torch.arange(2 * reach + 1).int() % num
+    prefix = [n // 2 for n in k_lens] if kind == "prefix" else None
+    _check(ops, Batch(q_lens, k_lens, dtype=SF, kind=kind, prefix=prefix, buckets=ids,
+                      num_buckets=num))
