@@ -132,8 +132,9 @@ trw_status trw_ops_attention_backward(const trw_attention_params* params, void* 
 /* One new event of each of `batch` walks: its key and value go into the walk's
  * cache at position lens[b], and it attends to positions 0 .. lens[b].  A
  * negative length is an idle row: it writes nothing to the cache and its
- * output is 0; a length of `capacity` or more (no room) gives NaN, and writes
- * nothing to the cache either. */
+ * output is 0 (as it is where the table masks every position); a length of
+ * `capacity` or more (no room) gives NaN, and writes nothing to the cache
+ * either. */
 typedef struct trw_attention_step_params {
     int32_t dtype;
     int32_t heads, kv_heads, dim;

@@ -284,7 +284,9 @@ void attention_step_kernel(StepArgs a) {
                 t4 out;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float value = n < 0 ? 0.0f : idle ? NAN : sum[e] * scale;
+                    // a total of 0: the bias masks every position
+                    const float value =
+                        n < 0 ? 0.0f : idle ? NAN : total != 0.0f ? sum[e] * scale : 0.0f;
                     out[e] = static_cast<T>(value);
                 }
                 *reinterpret_cast<t4*>(row_of<T>(a.out, b, join_head) + d) = out;
@@ -342,7 +344,10 @@ __global__ __launch_bounds__(kThreads) void join_step_kernel(StepArgs a) {
     t4 out;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        out[e] = static_cast<T>(n < 0 ? 0.0f : n >= a.capacity ? NAN : sum[e] / total);
+        out[e] = static_cast<T>(n < 0              ? 0.0f
+                                : n >= a.capacity  ? NAN
+                                : total != 0.0f    ? sum[e] / total
+                                                   : 0.0f);
     *reinterpret_cast<t4*>(row_of<T>(a.out, b, head) + d) = out;
 }
 

@@ -152,7 +152,8 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
     a cache as well and is written at ``lens[b]``.  The other arguments are
     :func:`walk_attention`'s; there is no gradient.
 
-    A negative length is an idle row: output 0, caches untouched.  A full cache
+    A negative length is an idle row: output 0, caches untouched.  Where the
+    table masks every position the output is 0 too.  A full cache
     (``lens[b] >= capacity``) gives NaN and leaves the caches untouched."""
     return _operators.walk_attention_step(q, k, v, k_cache, v_cache, lens, scale, softcap,
                                           bias_table, buckets, slopes, times, k_times)

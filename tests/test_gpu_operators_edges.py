@@ -61,3 +61,59 @@ def test_table_gradient_of_one_distance_over_caches(ops, kind, reach, num, q_len
     prefix = [n // 2 for n in k_lens] if kind == "prefix" else None
     _check(ops, Batch(q_lens, k_lens, dtype=SF, kind=kind, prefix=prefix, buckets=ids,
                       num_buckets=num))
+
+
+def _masked_steps(ops, dtype, lens, capacity, table, ids, heads=4, kv_heads=2, dim=64):
+    """A step under a table that masks: against the formula, zeros where nothing is left."""
+    gen = torch.Generator().manual_seed(capacity)
+    n = len(lens)
+    q = _normal(gen, n, heads, dim, dtype=dtype)
+    k, v = (_normal(gen, n, kv_heads, dim, dtype=dtype) for _ in range(2))
+    kc, vc = (_normal(gen, n, capacity, kv_heads, dim, dtype=dtype) for _ in range(2))
+    out = ops.walk_attention_step(q.cuda(), k.cuda(), v.cuda(), kc.cuda(), vc.cuda(),
+                                  torch.tensor(lens).cuda(), bias_table=table.cuda(),
+                                  buckets=ids.cuda()).cpu()
+    reach = ids.shape[0] // 2
+    for b, m in enumerate(lens):
+        kc[b, m], vc[b, m] = k[b], v[b]
+        hop = (m - torch.arange(m + 1)).clamp(max=reach) + reach
+        left = torch.isfinite(table[:, ids.long()[hop]]).any(-1)
+        assert not out[b][~left].any()  # and no NaN
+        low = table.double().clamp_min(-1e9)
+        want = wf.attention(q[b:b + 1].double(), kc[b, :m + 1].double(), vc[b, :m + 1].double(),
+                            wf.documents("causal", [1], [m + 1]), table=low, buckets=ids,
+                            dtype=dtype)["out"]
+        wf.check(f"out[{b}] of {m}", out[b:b + 1, left], *(x[:, left] for x in want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("capacity", [100, 9000])  # one workgroup a walk, and several
+def test_steps_that_a_table_masks(ops, dtype, capacity):
+    """Head 0 does not see the own event, head 1 nothing, head 2 the own event alone, head 3 all but
+    what is far: an empty cache, every position masked, a whole workgroup's share masked."""
+    ids = torch.arange(9, dtype=torch.int32)  # reach 4: distances -4..4, 0 is id 4
+    inf = -math.inf
+    table = torch.zeros(4, 9)
+    table[0, 4] = inf
+    table[1] = inf
+    table[2, 5:] = inf
+    table[3, 8] = inf
+    lens = [n for n in (0, 1, 3, 31, 64, 99, 4000, 8999) if n < capacity]
+    _masked_steps(ops, dtype, lens, capacity, table, ids)
+
+
+def test_steps_agree_with_a_pass_where_a_table_masks(ops):
+    n, heads, dim = 12, 2, 32
+    gen = torch.Generator().manual_seed(7)
+    q, k, v = (_normal(gen, n, heads, dim).cuda() for _ in range(3))
+    table = torch.tensor([[-math.inf, 0.3], [-math.inf, -math.inf]]).cuda()
+    ids = torch.tensor([0, 0, 0, 0, 1], dtype=torch.int32).cuda()  # two events back or more
+    whole = ops.walk_attention(q, k, v, ops.WalkMask.packed(torch.tensor([0, n]).cuda(), n),
+                               bias_table=table, buckets=ids)
+    assert not whole[:2].any() and not whole[:, 1].any() and whole[2:, 0].any()
+    kc, vc = (torch.zeros(1, n, heads, dim, device="cuda") for _ in range(2))
+    for i in range(n):
+        out = ops.walk_attention_step(q[i:i + 1], k[i:i + 1], v[i:i + 1], kc, vc,
+                                      torch.tensor([i]).cuda(), bias_table=table, buckets=ids)
+        # float32, at most 12 keys: a few units in the last place of sums of terms up to 4
+        assert torch.allclose(out[0], whole[i], rtol=0, atol=1e-5), i
