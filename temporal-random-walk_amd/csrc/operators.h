@@ -21,6 +21,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "tile_rows.h"
 #include "trw_operators.h"
 
 namespace trw {
@@ -268,12 +269,11 @@ struct Loader {
             for (int n = 0; n < kMine; ++n) copy_to_lds(at, offset[n], to + n * kThreads * 16);
         } else {
             // rows as bytes from row `from`, kept between it and the last one
-            const int before = (from - first) * pitch, last = (end - 1 - from) * pitch;
+            const EdgeRows edge = edge_rows(first, from, end, kRows, pitch);
 #pragma unroll
             for (int n = 0; n < kMine; ++n) {
                 const int row = first_row + n * kStep * pitch;
-                const int near = min(max(row - before, 0), last);
-                copy_to_lds(at, offset[n] + (near - row), to + n * kThreads * 16);
+                copy_to_lds(at, offset[n] + (edge_row(edge, row) - row), to + n * kThreads * 16);
             }
         }
     }

@@ -117,3 +117,33 @@ def test_steps_agree_with_a_pass_where_a_table_masks(ops):
                                       torch.tensor([i]).cuda(), bias_table=table, buckets=ids)
         # float32, at most 12 keys: a few units in the last place of sums of terms up to 4
         assert torch.allclose(out[0], whole[i], rtol=0, atol=1e-5), i
+
+
+@pytest.mark.parametrize("dtype,gap", [(BF, 1 << 22), (SF, 1 << 21)])
+def test_not_finite_beside_a_walk_of_far_rows(ops, dtype, gap):
+    """Rows 8 MB apart, the furthest that are read in place: a walk of 300 rows is longer than 2^31
+    bytes.  Walks share tiles, and those of the second are taken alone where the first is not
+    finite: the second's results do not change."""
+    lens, dim = [40, 300], 8
+    n = sum(lens)
+    gen = torch.Generator().manual_seed(11)
+    values = _normal(gen, 4, n, 1, dim, dtype=dtype)
+    far = torch.empty(n, gap, dtype=dtype, device="cuda")  # 2.9 GB
+
+    def run(bad):
+        rows = [far[:, m * dim:(m + 1) * dim].unflatten(1, (1, dim)) for m in range(4)]
+        for x, y in zip(rows, values):
+            x.copy_(y)
+        if bad is not None:
+            rows[bad][7, 0, 3] = math.nan
+        leaves = [x.detach().requires_grad_() for x in rows[:3]]
+        mask = ops.WalkMask.packed(torch.tensor([0, 40, n]).cuda(), n, kind="full")
+        out = ops.walk_attention(*leaves, mask)
+        return [out.detach(), *torch.autograd.grad(out, leaves, rows[3])]
+
+    want = run(None)
+    for bad in range(4):
+        got = run(bad)
+        for x, y in zip(got, want):
+            assert torch.equal(x[40:], y[40:])
+        assert any(torch.isnan(x[:40]).any() for x in got)
