@@ -504,6 +504,11 @@ Tensor walk_attention(const Tensor& q, const Tensor& k, const Tensor& v, const M
     return WalkAttention::apply(q, k, v, table, call, train);
 }
 
+// A kernel wrote to the tensor: who saved it for a backward pass is to know.
+void wrote(const Tensor& x) {
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor walk_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_,
                            const Tensor& k_cache, const Tensor& v_cache, const Tensor& lens_,
                            std::optional<double> scale, double softcap,
@@ -562,6 +567,9 @@ Tensor walk_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_,
         p.workspace = space.data_ptr();
     }
     check_status(trw_ops_attention_step(&p, on.stream));
+    wrote(k_cache);
+    wrote(v_cache);
+    if (k_times) wrote(*k_times);
     return out;
 }
 

@@ -165,3 +165,38 @@ def test_buckets_changed_between_the_passes_of_the_bias(ops):
     ids.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+def _event(requires_grad=False, dtype=SF, times=False):
+    x = dict(q=torch.randn(3, 4, 64, dtype=dtype, device="cuda", requires_grad=requires_grad),
+             k=torch.randn(3, 2, 64, dtype=dtype, device="cuda"),
+             v=torch.randn(3, 2, 64, dtype=dtype, device="cuda"),
+             k_cache=torch.randn(3, 16, 2, 64, dtype=dtype, device="cuda"),
+             v_cache=torch.randn(3, 16, 2, 64, dtype=dtype, device="cuda"),
+             lens=torch.tensor([0, 5, -1]).cuda())
+    if times:
+        x.update(slopes=torch.ones(4, device="cuda"), times=torch.ones(3, device="cuda"),
+                 k_times=torch.zeros(3, 16, device="cuda"))
+    return x
+
+
+@pytest.mark.parametrize("name", ["k_cache", "v_cache", "k_times"])
+def test_a_step_changes_its_caches(ops, name):
+    """What saved a cache before a step learns that the step wrote to it."""
+    event = _event(times=True)
+    weight = torch.ones((), device="cuda", requires_grad=True)
+    product = weight * event[name]
+    ops.walk_attention_step(**event)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    product = weight * event["q"]  # what it only reads is as it was
+    ops.walk_attention_step(**event)
+    product.sum().backward()
+
+
+def test_a_step_in_inference_mode(ops):
+    with torch.inference_mode():
+        event = _event(times=True)
+        want = ops.walk_attention_step(**event)
+    with torch.no_grad():  # caches that track no versions
+        assert torch.equal(ops.walk_attention_step(**event), want)
