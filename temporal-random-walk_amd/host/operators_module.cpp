@@ -333,8 +333,8 @@ const Tensor& unpacked(const Tensor& x, at::IntArrayRef shape, at::ScalarType ty
     return x;
 }
 
-bool differentiable(const Tensor& grad) {
-    return at::GradMode::is_enabled() && grad.requires_grad();
+bool differentiable(const Tensor& x) {
+    return at::GradMode::is_enabled() && x.requires_grad();
 }
 // A backward pass's results, which say so where they are differentiated again.
 torch::autograd::variable_list once(torch::autograd::variable_list grads, bool again) {
@@ -504,6 +504,29 @@ Tensor walk_attention(const Tensor& q, const Tensor& k, const Tensor& v, const M
     return WalkAttention::apply(q, k, v, table, call, train);
 }
 
+constexpr char kNoGradient[] = "walk_attention_step has no gradient";
+
+// Which of the arguments a gradient is asked of.
+torch::autograd::variable_list differentiated_of(std::initializer_list<OptionalTensor> given) {
+    torch::autograd::variable_list which;
+    for (const OptionalTensor& x : given) {
+        if (!x || !x->defined()) continue;
+        if (x->_fw_grad(/*level=*/0).defined()) throw std::runtime_error(kNoGradient);
+        if (differentiable(*x)) which.push_back(*x);
+    }
+    return which;
+}
+// The result, which says that it has no gradient where one of those is reached
+// through it.
+Tensor without_gradient(const Tensor& out, const torch::autograd::variable_list& differentiated) {
+    if (differentiated.empty()) return out;
+    torch::autograd::variable_list all{out};
+    all.insert(all.end(), differentiated.begin(), differentiated.end());
+    torch::autograd::DelayedError error(kNoGradient, static_cast<int64_t>(all.size()));
+    at::AutoGradMode grad(true);
+    return error(std::move(all))[0];
+}
+
 // A kernel wrote to the tensor: who saved it for a backward pass is to know.
 void wrote(const Tensor& x) {
     if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
@@ -515,6 +538,8 @@ Tensor walk_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_,
                            const OptionalTensor& bias_table, const OptionalTensor& buckets,
                            const OptionalTensor& slopes, const OptionalTensor& times,
                            const OptionalTensor& k_times) {
+    const auto differentiated = differentiated_of(
+        {q_, k_, v_, k_cache, v_cache, bias_table, slopes, times, k_times});
     at::AutoGradMode no_grad(false);
     check_qkv(q_, k_, v_, 3);
     const int64_t batch = q_.size(0), heads = q_.size(1), kv_heads = k_.size(1), dim = q_.size(2);
@@ -570,7 +595,7 @@ Tensor walk_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_,
     wrote(k_cache);
     wrote(v_cache);
     if (k_times) wrote(*k_times);
-    return out;
+    return without_gradient(out, differentiated);
 }
 
 // ---- the dense bias ---------------------------------------------------------------------------------

@@ -150,7 +150,8 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
     view of another order will do; dim contiguous, rows 16-byte pieces).  With
     ``times`` (``[batch]``), ``k_times`` (``[batch, capacity]``, contiguous) is
     a cache as well and is written at ``lens[b]``.  The other arguments are
-    :func:`walk_attention`'s; there is no gradient.
+    :func:`walk_attention`'s; there is no gradient, and a result that is
+    differentiated says so.
 
     A negative length is an idle row: output 0, caches untouched.  Where the
     table masks every position the output is 0 too.  A full cache

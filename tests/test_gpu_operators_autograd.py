@@ -200,3 +200,34 @@ def test_a_step_in_inference_mode(ops):
         want = ops.walk_attention_step(**event)
     with torch.no_grad():  # caches that track no versions
         assert torch.equal(ops.walk_attention_step(**event), want)
+
+
+def test_a_step_has_no_gradient(ops):
+    """It says so where one is asked for."""
+    event = _event(requires_grad=True)
+    out = ops.walk_attention_step(**event)
+    with pytest.raises(RuntimeError, match="walk_attention_step has no gradient"):
+        out.sum().backward()
+    for name in ("k", "v", "k_cache", "v_cache", "bias_table"):
+        event = _event()
+        event.update(bias_table=torch.randn(4, 3, device="cuda"),
+                     buckets=torch.tensor([0, 1, 2], dtype=torch.int32).cuda())
+        event[name].requires_grad_()
+        with pytest.raises(RuntimeError, match="walk_attention_step has no gradient"):
+            ops.walk_attention_step(**event).sum().backward()
+    event = _event(requires_grad=True)  # also where the input is reached another way
+    loss = ops.walk_attention_step(**event).sum() + event["q"].sum()
+    with pytest.raises(RuntimeError, match="walk_attention_step has no gradient"):
+        torch.autograd.grad(loss, event["q"])
+    with torch.no_grad():
+        assert not ops.walk_attention_step(**_event(requires_grad=True)).requires_grad
+    assert not ops.walk_attention_step(**_event()).requires_grad
+
+
+def test_a_step_has_no_forward_derivative(ops):
+    import torch.autograd.forward_ad as fwad
+    event = _event()
+    with fwad.dual_level():
+        event["q"] = fwad.make_dual(event["q"], torch.ones_like(event["q"]))
+        with pytest.raises(RuntimeError, match="walk_attention_step has no gradient"):
+            ops.walk_attention_step(**event)
