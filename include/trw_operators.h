@@ -105,6 +105,8 @@ typedef struct trw_attention_params {
     int64_t docs;
     int64_t longest; /* no document has more queries or keys than this; 0: not known */
     int32_t own_causal; /* 1: the mask is causal, over the queries' own rows as keys */
+    int32_t covered; /* 1: every row is a document's, its padding included (a padded mask); 0: rows
+                        of no document are looked for, and left zero */
     trw_score score;
     trw_rows q, k, v, out;
     float* stats; /* [2, heads, q_rows], of the rows' softmax (base 2); written by the forward

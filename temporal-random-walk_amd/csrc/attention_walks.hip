@@ -699,9 +699,10 @@ int walk_blocks(const trw_attention_params& p) {
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>((length + 31) / 32, 1), most));
 }
 
-// Whether walks longer than those can be in the batch.
+// Whether walks longer than those can be in the batch, or rows of no walk, which
+// the tiles' kernels leave zero.
 bool walk_rest(const trw_attention_params& p, int blocks) {
-    return p.longest <= 0 || p.longest > 32 * blocks;
+    return !p.covered || p.longest <= 0 || p.longest > 32 * blocks;
 }
 
 void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream) {

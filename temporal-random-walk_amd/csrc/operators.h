@@ -562,8 +562,8 @@ inline size_t element_size(int dtype) { return dtype == TRW_F32 ? 4 : 2; }
 void walk_mask(const trw_walk_mask_params& p, hipStream_t stream);
 uint64_t attention_workspace(const trw_attention_params& p, bool backward);
 // Short walks (attention_walks.hip): how many blocks of 32 rows one may have
-// (0: none go there), whether longer ones may be in the batch, floats of one
-// line of the table's gradient.
+// (0: none go there), whether longer ones or rows of none may be in the batch,
+// floats of one line of the table's gradient.
 int walk_blocks(const trw_attention_params& p);
 bool walk_rest(const trw_attention_params& p, int blocks);
 int walk_line(const trw_attention_params& p, int blocks);

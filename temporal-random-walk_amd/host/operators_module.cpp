@@ -376,6 +376,7 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
         p.docs_info = mask.docs_info;
         p.docs = mask.docs;
         p.longest = mask.longest;
+        p.covered = mask.longest > 0;  // padded
         p.own_causal = mask.own_causal;
         p.score = call->terms->score;
         p.score.table = pointer<float>(table);

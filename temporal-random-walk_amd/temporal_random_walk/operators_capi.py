@@ -43,7 +43,7 @@ class AttentionParams(C.Structure):
                 ("dim", C.c_int32), ("q_rows", C.c_int64), ("k_rows", C.c_int64),
                 ("q_rows_info", C.c_void_p), ("k_rows_info", C.c_void_p),
                 ("docs_info", C.c_void_p), ("docs", C.c_int64), ("longest", C.c_int64),
-                ("own_causal", C.c_int32),
+                ("own_causal", C.c_int32), ("covered", C.c_int32),
                 ("score", Score),
                 ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("stats", C.c_void_p),
                 ("out_low", Rows), ("d_out", Rows), ("d_q", Rows), ("d_k", Rows), ("d_v", Rows),

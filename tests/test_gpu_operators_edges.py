@@ -147,3 +147,49 @@ def test_not_finite_beside_a_walk_of_far_rows(ops, dtype, gap):
         for x, y in zip(got, want):
             assert torch.equal(x[40:], y[40:])
         assert any(torch.isnan(x[:40]).any() for x in got)
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("longest", [0, 5])
+def test_rows_of_no_document(ops, dtype, longest):
+    """The C ABI with packed offsets and the longest document stated: rows before the first one and
+    after the last are zero, in every output."""
+    import ctypes
+
+    from temporal_random_walk import operators_capi as abi
+    lib, rows, heads, kv_heads, dim = abi.lib(), 20, 4, 2, 64
+    offsets = torch.tensor([2, 7, 8, 12]).cuda()
+    gen = torch.Generator().manual_seed(longest)
+    q, d_out = (_normal(gen, rows, heads, dim, dtype=dtype).cuda() for _ in range(2))
+    k, v = (_normal(gen, rows, kv_heads, dim, dtype=dtype).cuda() for _ in range(2))
+    out, d_q, low = (torch.full_like(q, math.nan) for _ in range(3))
+    d_k, d_v = (torch.full_like(k, math.nan) for _ in range(2))
+    info = torch.zeros(2, rows, 4, dtype=torch.int32, device="cuda")
+    docs = torch.zeros(3, 8, dtype=torch.int32, device="cuda")
+    stats = torch.zeros(2, heads, rows, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    mask = abi.MaskParams(docs=3, q_rows=rows, k_rows=rows, q_offsets=offsets.data_ptr(), kind=1,
+                          q_rows_info=info[0].data_ptr(), k_rows_info=info[1].data_ptr(),
+                          docs_info=docs.data_ptr())
+    abi.call(lib.trw_ops_walk_mask, ctypes.byref(mask), stream)
+    at = lambda x: abi.Rows(x.data_ptr(), x.stride(0), x.stride(1))  # noqa: E731
+    p = abi.AttentionParams(
+        dtype={SF: 0, BF: 2}[dtype], heads=heads, kv_heads=kv_heads, dim=dim, q_rows=rows,
+        k_rows=rows, q_rows_info=info[0].data_ptr(), k_rows_info=info[1].data_ptr(),
+        docs_info=docs.data_ptr(), docs=3, longest=longest, own_causal=1,
+        score=abi.Score(dim ** -0.5, 0.0), q=at(q), k=at(k), v=at(v), out=at(out),
+        out_low=at(low), stats=stats.data_ptr(), d_out=at(d_out), d_q=at(d_q), d_k=at(d_k),
+        d_v=at(d_v))
+    for backward, run in ((0, lib.trw_ops_attention_forward), (1, lib.trw_ops_attention_backward)):
+        size = ctypes.c_uint64()
+        abi.call(lib.trw_ops_attention_workspace, ctypes.byref(p), backward, ctypes.byref(size))
+        space = torch.empty(size.value + 16, dtype=torch.uint8, device="cuda")
+        p.workspace, p.workspace_bytes = space.data_ptr(), size.value
+        abi.call(run, ctypes.byref(p), stream)
+        torch.cuda.synchronize()
+    d = lambda x: x[2:12].double().cpu()  # noqa: E731
+    want = wf.attention(d(q), d(k), d(v), wf.documents("causal", [5, 1, 4], [5, 1, 4]),
+                        d_out=d(d_out), dtype=dtype)
+    for name, x in (("out", out), ("d_q", d_q), ("d_k", d_k), ("d_v", d_v)):
+        assert not x[:2].any() and not x[12:].any(), name
+        wf.check(name, x[2:12], *want[name])
