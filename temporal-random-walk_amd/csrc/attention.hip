@@ -362,6 +362,18 @@ uint64_t attention_workspace(const trw_attention_params& p, bool backward) {
            (p.q_rows + kTileRows - 1) / kTileRows * sizeof(int);
 }
 
+// Tiles' workgroups are shared between several only where they are few, so that
+// this holds for all their launches; of the walks' the backward pass has a wave
+// for each block.
+void require_grids(const trw_attention_params& p, bool backward) {
+    const int blocks = walk_blocks(p);
+    if (blocks) require_grid(walk_grid(p), 64 * (backward ? blocks : 1));
+    if (blocks && !walk_rest(p, blocks)) return;
+    const auto tiles = [](int64_t rows) { return (rows + kTileRows - 1) / kTileRows; };
+    require_grid(xcd_grid(tiles(p.q_rows) * p.heads), kThreads);
+    if (backward) require_grid(xcd_grid(tiles(p.k_rows) * p.kv_heads), kThreads);
+}
+
 void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     if (p.q_rows == 0) return;
     require(p.workspace_bytes >= attention_workspace(p, false), "workspace is too small");

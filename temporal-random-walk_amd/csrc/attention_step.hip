@@ -407,7 +407,7 @@ void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
     a.part_stats = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(p.batch) * p.heads *
                                                              a.splits * p.dim);
     const int64_t grid = xcd_grid(p.batch * a.splits) * p.kv_heads * a.columns;
-    require(grid < (int64_t{1} << 31), "too many walks and heads");
+    require_grid(grid, kThreads);
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {
         typedef decltype(t) T;
         hipLaunchKernelGGL((attention_step_kernel<T, decltype(db)::value>),

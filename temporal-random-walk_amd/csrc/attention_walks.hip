@@ -66,10 +66,6 @@ __device__ __forceinline__ int head_of(const WalkArgs& a, int id) { return id / 
 __device__ __forceinline__ int doc_of(const WalkArgs& a, int id) {
     return id / (8 * a.kv_heads) * 8 + id % 8;
 }
-inline unsigned walk_grid(const trw_attention_params& p) {
-    return static_cast<unsigned>((p.docs + 7) / 8 * 8 * p.kv_heads);
-}
-
 __device__ __forceinline__ Doc load_doc(const int4* docs, int doc) {
     const int4 a = docs[2 * doc], b = docs[2 * doc + 1];
     Doc d;
@@ -699,6 +695,9 @@ int walk_blocks(const trw_attention_params& p) {
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>((length + 31) / 32, 1), most));
 }
 
+// Workgroups over walks and key heads.
+int64_t walk_grid(const trw_attention_params& p) { return (p.docs + 7) / 8 * 8 * p.kv_heads; }
+
 // Whether walks longer than those can be in the batch, or rows of no walk, which
 // the tiles' kernels leave zero.
 bool walk_rest(const trw_attention_params& p, int blocks) {
@@ -708,7 +707,7 @@ bool walk_rest(const trw_attention_params& p, int blocks) {
 void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream) {
     WalkArgs a = make_args(p);
     a.limit = 32 * blocks;
-    const unsigned grid = walk_grid(p);
+    const unsigned grid = static_cast<unsigned>(walk_grid(p));
     walk_dispatch(p.dtype, p.dim, blocks, [&](auto t, auto db, auto nb) {
         hipLaunchKernelGGL(
             (walk_forward_kernel<decltype(t), decltype(db)::value, decltype(nb)::value>),
@@ -726,7 +725,7 @@ void walk_backward(const trw_attention_params& p, int blocks, float* partial, hi
     a.partial = partial;
     a.stride = walk_line(p, blocks);
     a.triangle = p.own_causal;
-    const unsigned grid = walk_grid(p);
+    const unsigned grid = static_cast<unsigned>(walk_grid(p));
     for (int n = by_length(p) ? 1 : blocks; n <= blocks; ++n, a.above = a.limit) {
         a.limit = 32 * n;
         a.last = n == blocks;

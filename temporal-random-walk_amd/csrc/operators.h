@@ -33,6 +33,10 @@ struct InvalidArgument : std::invalid_argument {
 inline void require(bool ok, const char* message) {
     if (!ok) throw InvalidArgument(message);
 }
+// A launch has fewer than 2^32 threads.
+inline void require_grid(int64_t groups, int threads) {
+    require(groups < (int64_t{1} << 32) / threads, "too many rows, documents or heads for a launch");
+}
 inline void check_launch(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
@@ -567,8 +571,11 @@ uint64_t attention_workspace(const trw_attention_params& p, bool backward);
 int walk_blocks(const trw_attention_params& p);
 bool walk_rest(const trw_attention_params& p, int blocks);
 int walk_line(const trw_attention_params& p, int blocks);
+int64_t walk_grid(const trw_attention_params& p);
 void walk_forward(const trw_attention_params& p, int blocks, hipStream_t stream);
 void walk_backward(const trw_attention_params& p, int blocks, float* partial, hipStream_t stream);
+// That every launch of a pass can be made, before the first one.
+void require_grids(const trw_attention_params& p, bool backward);
 void attention_forward(const trw_attention_params& p, hipStream_t stream);
 void attention_backward(const trw_attention_params& p, hipStream_t stream);
 // A table's gradient from sums by distance: join_lines adds up to `groups`

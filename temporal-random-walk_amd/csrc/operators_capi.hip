@@ -176,7 +176,8 @@ trw_status trw_ops_attention_workspace(const trw_attention_params* params, int32
                                        uint64_t* bytes) {
     return guarded([&] {
         require(bytes != nullptr, "null argument");
-        *bytes = trw::ops::attention_workspace(checked(params), backward != 0);
+        trw::ops::require_grids(checked(params), backward != 0);
+        *bytes = trw::ops::attention_workspace(*params, backward != 0);
     });
 }
 
@@ -185,6 +186,7 @@ trw_status trw_ops_attention_forward(const trw_attention_params* params, void* s
         const trw_attention_params& p = checked(params);
         check_forward(p);
         check_aligned(p.workspace, "workspace must be 16-byte aligned");
+        trw::ops::require_grids(p, false);
         trw::ops::attention_forward(p, static_cast<hipStream_t>(stream));
     });
 }
@@ -202,6 +204,7 @@ trw_status trw_ops_attention_backward(const trw_attention_params* params, void* 
         require(!p.score.table || p.d_table, "d_table is null");
         check_aligned(p.k_rows_info, "k_rows_info must be 16-byte aligned");
         check_aligned(p.workspace, "workspace must be 16-byte aligned");
+        trw::ops::require_grids(p, true);
         trw::ops::attention_backward(p, static_cast<hipStream_t>(stream));
     });
 }

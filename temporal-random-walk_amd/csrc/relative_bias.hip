@@ -331,6 +331,7 @@ void relative_bias(const trw_relative_bias_params& p, hipStream_t stream) {
     if (rows > fair) rows = fair < 4 ? 4 : fair;
     a.rows_per_group = static_cast<int>(rows);
     const int chunks = copy_chunks(p.reach, elems);
+    require_grid((p.q_len + rows - 1) / rows, kThreads);
     const dim3 grid(static_cast<unsigned>((p.q_len + rows - 1) / rows),
                     static_cast<unsigned>(p.heads));
     by_type(p.dtype, [&](auto t) {
