@@ -202,7 +202,7 @@ __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, u
                  "global_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(lds), "v"(offset), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
 // The same of 4 bytes a lane.
 __device__ __forceinline__ void copy_word_to_lds(const void* base, uint32_t offset, uint32_t lds) {
@@ -211,7 +211,7 @@ __device__ __forceinline__ void copy_word_to_lds(const void* base, uint32_t offs
                  "global_load_lds_dword %1, %2"
                  :
                  : "s"(lds), "v"(offset), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
 // The LDS address of a __shared__ array (pass the array itself: of a pointer
 // that came a longer way the compiler does not know that it is one).
