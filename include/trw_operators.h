@@ -39,6 +39,9 @@ extern "C" {
  * buckets) and most buckets of one. */
 #define TRW_OPS_MAX_REACH 1024
 #define TRW_OPS_MAX_BUCKETS 256
+/* 16-bit types: softcaps above this have kernels of their own (walks of any
+ * length go through those of tiles). */
+#define TRW_OPS_WIDE_CAP 256
 
 typedef enum trw_dtype { TRW_F32 = 0, TRW_F16 = 1, TRW_BF16 = 2 } trw_dtype;
 

@@ -68,7 +68,7 @@ __device__ __forceinline__ void store_stats(const ForwardArgs& a, int64_t stat, 
     if (apart) a.stats[static_cast<int64_t>(a.heads) * a.q_rows + stat] = log_l;
 }
 
-template <typename T, int DB>
+template <typename T, int DB, bool kWide>
 __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // of a tile
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(ForwardA
             }
             const int j_lane = j0 + 4 * half;  // register r's key: + 32 b + acc_row(r)
             if (!plain) {
-                cap_scores<T>(sc, s);
+                cap_scores<T, kWide>(sc, s);
                 add_biases(sc, s, s_lut, slope, diag, w_diag_lo, w_diag_hi, q_time, s_time, j0, half);
             }
             if (j0 < full_lo || j0 + kKeys > full_hi) {
@@ -406,8 +406,11 @@ void attention_forward(const trw_attention_params& p, hipStream_t stream) {
     const int64_t grid = xcd_grid(static_cast<int64_t>(a.tiles) * a.heads * a.splits);
     const size_t lds = p.score.table ? (2 * a.score.reach + 1) * sizeof(float) : 0;
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {
-        hipLaunchKernelGGL((attention_forward_kernel<decltype(t), decltype(db)::value>),
-                           dim3(static_cast<unsigned>(grid)), dim3(kThreads), lds, stream, a);
+        by_cap<decltype(t)>(p.dtype, p.score, [&](auto wide) {
+            hipLaunchKernelGGL(
+                (attention_forward_kernel<decltype(t), decltype(db)::value, decltype(wide)::value>),
+                dim3(static_cast<unsigned>(grid)), dim3(kThreads), lds, stream, a);
+        });
         check_launch("attention_forward");
         if (a.splits > 1) {
             const int64_t threads = rows * (a.dim / 4);

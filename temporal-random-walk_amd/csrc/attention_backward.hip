@@ -44,12 +44,12 @@ struct BackwardArgs {
 };
 
 // Scores in base 2 of one block's products, and the slope that the cap left.
-template <typename T>
+template <typename T, bool kWide>
 __device__ __forceinline__ void score_block(const Score& sc, const f32x16& product,
                                             float (&x)[1][16], float (&slope)[16]) {
     if (sc.softcap > 0) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[0][r] = capped<T>(sc, product[r], slope[r]);
+        for (int r = 0; r < 16; ++r) x[0][r] = capped<T, kWide>(sc, product[r], slope[r]);
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -66,7 +66,7 @@ __device__ __forceinline__ void score_block(const Score& sc, const f32x16& produ
 // past the reach are summed in registers.  Rows whose walks' queries and keys
 // are not one distance apart (prompts of several walks) have no common diagonals
 // and take float atomics on the wave's own line.
-template <typename T, int DB>
+template <typename T, int DB, bool kWide>
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(BackwardArgs a) {
     typedef Tile<T, DB> G;
     constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
                     dp = mma(G::row(s_v, lane & 31, st, half), d_o[st], dp);
                 }
                 float x[1][16], cap_slope[16];
-                score_block<T>(sc, product, x, cap_slope);
+                score_block<T, kWide>(sc, product, x, cap_slope);
                 const int j_lane = j0 + 4 * half;
                 if (sc.biased()) {
                     add_biases(sc, x, s_lut, slope, diag, w_diag_lo, w_diag_hi, q_time,
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_q_kernel(Backw
 //
 // A lane holds one key (column) and 16 query rows at a time; q and dO pass
 // through LDS and are read both ways.
-template <typename T, int DB>
+template <typename T, int DB, bool kWide>
 __global__ __launch_bounds__(kThreads, DB < 4 ? 2 : 1) void attention_backward_kv_kernel(
     BackwardArgs a) {
     typedef Tile<T, DB> G;
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(kThreads, DB < 4 ? 2 : 1) void attention_backward_k
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             float cap_slope;
-                            x[r] = capped<T>(sc, product[r], cap_slope);
+                            x[r] = capped<T, kWide>(sc, product[r], cap_slope);
                             dp[r] *= cap_slope;
                         }
                     } else {
@@ -709,19 +709,24 @@ void attention_backward(const trw_attention_params& p, hipStream_t stream) {
         dispatch(p.dtype, p.dim, [&](auto t, auto db) {
             typedef decltype(t) T;
             constexpr int DB = decltype(db)::value;
-            if (a.q_tiles)
-                hipLaunchKernelGGL((attention_backward_q_kernel<T, DB>),
-                                   dim3(static_cast<unsigned>(
-                                       xcd_grid(static_cast<int64_t>(a.q_tiles) * a.heads))),
-                                   dim3(kThreads),
-                                   line ? 5 * line + 4 * kSquare * sizeof(float) : 0, stream, a);
-            check_launch("attention_backward");
-            if (a.k_tiles)
-                hipLaunchKernelGGL((attention_backward_kv_kernel<T, DB>),
-                                   dim3(static_cast<unsigned>(xcd_grid(
-                                       static_cast<int64_t>(a.k_tiles) * p.kv_heads * a.splits))),
-                                   dim3(kThreads), line, stream, a);
-            check_launch("attention_backward");
+            by_cap<T>(p.dtype, p.score, [&](auto wide) {
+                constexpr bool kWide = decltype(wide)::value;
+                if (a.q_tiles)
+                    hipLaunchKernelGGL((attention_backward_q_kernel<T, DB, kWide>),
+                                       dim3(static_cast<unsigned>(
+                                           xcd_grid(static_cast<int64_t>(a.q_tiles) * a.heads))),
+                                       dim3(kThreads),
+                                       line ? 5 * line + 4 * kSquare * sizeof(float) : 0, stream,
+                                       a);
+                check_launch("attention_backward");
+                if (a.k_tiles)
+                    hipLaunchKernelGGL(
+                        (attention_backward_kv_kernel<T, DB, kWide>),
+                        dim3(static_cast<unsigned>(xcd_grid(
+                            static_cast<int64_t>(a.k_tiles) * p.kv_heads * a.splits))),
+                        dim3(kThreads), line, stream, a);
+                check_launch("attention_backward");
+            });
             if (a.k_tiles && a.splits > 1) {
                 const int64_t n = p.k_rows * p.kv_heads * (p.dim / 4);
                 hipLaunchKernelGGL((join_splits_kernel<T>),

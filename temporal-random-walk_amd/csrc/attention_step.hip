@@ -62,7 +62,7 @@ __device__ __forceinline__ void put_row(u32x4* tile, const T* row, int from, int
 // bits) leave room: left to itself the compiler takes 298 registers there, one
 // workgroup, and 238 walks of 350 events (8 heads of 128, bfloat16) take 113 us
 // for 83 (4.1 TB/s).
-template <typename T, int DB>
+template <typename T, int DB, bool kWide>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DB <= 2 ? 2 : 1)
 void attention_step_kernel(StepArgs a) {
     typedef Tile<T, DB> G;
@@ -166,7 +166,7 @@ void attention_step_kernel(StepArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float unused;
-            s[r] = sc.softcap > 0 ? capped<T>(sc, x[r], unused) : x[r] * sc.scale2;
+            s[r] = sc.softcap > 0 ? capped<T, kWide>(sc, x[r], unused) : x[r] * sc.scale2;
         }
         float time[16];
         if (k_times) {
@@ -410,8 +410,11 @@ void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
     require_grid(grid, kThreads);
     dispatch(p.dtype, p.dim, [&](auto t, auto db) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((attention_step_kernel<T, decltype(db)::value>),
-                           dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+        by_cap<T>(p.dtype, p.score, [&](auto wide) {
+            hipLaunchKernelGGL(
+                (attention_step_kernel<T, decltype(db)::value, decltype(wide)::value>),
+                dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+        });
         check_launch("attention_step");
         if (a.splits > 1)
             hipLaunchKernelGGL((join_step_kernel<T>), dim3(static_cast<unsigned>(a.batch * a.heads)),

@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * kNB, kShared && (DB * kNB > (sizeof(T) == 4 ? 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         float cap_slope;
-                        (void)capped<T>(sc, x[r], cap_slope);
+                        (void)capped<T, false>(sc, x[r], cap_slope);
                         dp[b][r] *= cap_slope;
                     }
                 }
@@ -680,11 +680,14 @@ void walk_dispatch(int dtype, int dim, int blocks, F&& f) {
 // float32 at head size 128, 3.7 and 1.2 ms at 4 rows, 3.8 and 2.3 at 8, 3.9 and
 // 4.0 at 12.  64 such walks of 4 rows, which do not fill the device either way,
 // take 105 and 169 us there.
+//
+// Wide caps of the 16-bit types, which nobody's scores come near, are the tiles'
+// too: their kernels for those would be as many again.
 constexpr int64_t kTinyRows = 8;
 constexpr int64_t kTinyGroups = 2048;
 
 int walk_blocks(const trw_attention_params& p) {
-    if (p.docs == 0) return 0;
+    if (p.docs == 0 || wide_cap(p.dtype, p.score)) return 0;
     const int db = (p.dim + 31) / 32;
     const int most = db <= 2 ? 3 : 2;
     const int64_t rows = std::max(p.q_rows, p.k_rows);

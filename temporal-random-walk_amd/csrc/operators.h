@@ -20,6 +20,7 @@
 
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "tile_rows.h"
 #include "trw_operators.h"
@@ -391,24 +392,49 @@ __device__ __forceinline__ void fill_bias(float* lut, const Score& s, int head, 
     for (int i = thread; i < 2 * s.reach + 1; i += threads) lut[i] = table_entry(s, head, i);
 }
 
-// log2 e softcap tanh(scale x / softcap), and 1 - tanh^2.  The 16-bit types
-// take tanh from exp2 and a reciprocal: its error of some 1e-7 is absolute, far
-// below what their scores carry; float32 calls tanhf.
-template <typename T>
+// log2 e softcap tanh(scale x / softcap), and 1 - tanh^2.  float32 calls tanhf.
+// The 16-bit types take tanh from exp2 and a reciprocal: its error of some 1e-7 is
+// absolute, so one of 1e-7 softcap in the score, far below what their scores
+// carry while the cap is not wide.  kWide: below 1/16 of the cap, the first terms
+// of tanh's series, as exact as x (the next is 17/315 (1/16)^6 < 2^-28 of it).
+// Kernels of their own: as a branch in the others it costs registers that they
+// need (8192 rows, 16 heads of 128, backward: 1.72 -> 1.90 ms, 1.48 -> 1.67
+// without a cap).
+template <typename T, bool kWide>
 __device__ __forceinline__ float capped(const Score& s, float x, float& slope) {
     if constexpr (sizeof(T) == 4) {
         const float t = tanhf(x * s.scale / s.softcap);
         slope = 1.0f - t * t;
         return s.cap_out * t;
     } else {
-        const float u = __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * s.cap_in));
+        const float in = x * s.cap_in;
+        const float u = __builtin_amdgcn_rcpf(1.0f + exp2_fast(in));
         slope = 4.0f * u * (1.0f - u);
-        return fmaf(-2.0f * s.cap_out, u, s.cap_out);
+        const float far = fmaf(-2.0f * s.cap_out, u, s.cap_out);
+        if (!kWide) return far;
+        const float y = in * (0.5f * kLn2), y2 = y * y;
+        const float series = fmaf(y2, fmaf(y2, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
+        return fabsf(y) < 0.0625f ? x * s.scale2 * series : far;
     }
 }
 
+inline bool wide_cap(int dtype, const trw_score& s) {
+    return dtype != TRW_F32 && s.softcap > TRW_OPS_WIDE_CAP;
+}
+// f(kWide) for a type and a score.
+template <typename T, typename F>
+void by_cap(int dtype, const trw_score& s, F&& f) {
+    if constexpr (sizeof(T) == 2) {
+        if (wide_cap(dtype, s)) {
+            f(std::true_type());
+            return;
+        }
+    }
+    f(std::false_type());
+}
+
 // Products to scores in base 2, without biases and mask.
-template <typename T, int kBlocks>
+template <typename T, bool kWide = false, int kBlocks>
 __device__ __forceinline__ void cap_scores(const Score& sc, float (&s)[kBlocks][16]) {
     if (sc.softcap > 0) {
 #pragma unroll
@@ -416,7 +442,7 @@ __device__ __forceinline__ void cap_scores(const Score& sc, float (&s)[kBlocks][
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float unused;
-                s[b][r] = capped<T>(sc, s[b][r], unused);
+                s[b][r] = capped<T, kWide>(sc, s[b][r], unused);
             }
     } else {
 #pragma unroll

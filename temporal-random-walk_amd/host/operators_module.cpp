@@ -389,9 +389,10 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             stats = at::empty({2, q.size(1), mask.q_rows}, q.options().dtype(at::kFloat));
             p.stats = pointer<float>(stats);
             // Walks that go a wave each sum there what the backward pass needs of the output
-            // (those of up to 8 rows may go through tiles)
+            // (those of up to 8 rows may go through tiles, under a wide cap all do)
             const int64_t wave = p.dim <= 64 ? 96 : 64;
-            if (p.dtype != TRW_F32 && !(mask.longest > 8 && mask.longest <= wave)) {
+            if (p.dtype != TRW_F32 && !(mask.longest > 8 && mask.longest <= wave &&
+                                        p.score.softcap <= TRW_OPS_WIDE_CAP)) {
                 low = at::empty_like(out);
                 p.out_low = rows_of(low);
             }

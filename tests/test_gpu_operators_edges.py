@@ -193,3 +193,34 @@ def test_rows_of_no_document(ops, dtype, longest):
     for name, x in (("out", out), ("d_q", d_q), ("d_k", d_k), ("d_v", d_v)):
         assert not x[:2].any() and not x[12:].any(), name
         wf.check(name, x[2:12], *want[name])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [3000.0, 1e6, 1e30])
+@pytest.mark.parametrize("lens", [[20, 1, 33, 40], [130, 260]])
+def test_caps_far_above_the_scores(ops, dtype, softcap, lens):
+    """cap(x) is then x but for its cube over 3 softcap^2, and as exact as x: within the bounds of the
+    formula without a cap."""
+    b = Batch(lens, dtype=dtype, softcap=softcap, scale=0.5)
+    got, want = b.run(ops), b.reference()
+    b.softcap = 0.0
+    for name, (_, bound) in b.reference().items():
+        wf.check(name, got[name], want[name][0], bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [3000.0, 1e6, 1e30])
+def test_step_caps_far_above_the_scores(ops, dtype, softcap):
+    gen = torch.Generator().manual_seed(5)
+    n, dim, lens = 3, 64, [0, 40, 299]
+    q, k, v = (_normal(gen, n, 2, dim, dtype=dtype) for _ in range(3))
+    kc, vc = (_normal(gen, n, 300, 2, dim, dtype=dtype) for _ in range(2))
+    out = ops.walk_attention_step(q.cuda(), k.cuda(), v.cuda(), kc.cuda(), vc.cuda(),
+                                  torch.tensor(lens).cuda(), softcap=softcap, scale=0.5).cpu()
+    for b, m in enumerate(lens):
+        kc[b, m], vc[b, m] = k[b], v[b]
+        args = (q[b:b + 1].double(), kc[b, :m + 1].double(), vc[b, :m + 1].double(),
+                wf.documents("causal", [1], [m + 1]))
+        want = wf.attention(*args, softcap=softcap, scale=0.5, dtype=dtype)["out"][0]
+        bound = wf.attention(*args, scale=0.5, dtype=dtype)["out"][1]
+        wf.check(f"out[{b}]", out[b:b + 1], want, bound)
