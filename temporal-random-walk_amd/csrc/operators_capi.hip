@@ -230,6 +230,12 @@ trw_status trw_ops_attention_step(const trw_attention_step_params* params, void*
                    "k_cache is null");
         check_rows(trw_rows{p.v_cache, p.v_pos_stride, p.v_head_stride}, p.dtype, slots,
                    "v_cache is null");
+        // Walks write their new rows at once: no two may be one.
+        const auto apart = [](int64_t n, int64_t stride) { return n <= 1 || stride != 0; };
+        require(apart(p.batch, p.k_batch_stride) && apart(p.batch, p.v_batch_stride) &&
+                    apart(p.capacity, p.k_pos_stride) && apart(p.capacity, p.v_pos_stride) &&
+                    apart(p.kv_heads, p.k_head_stride) && apart(p.kv_heads, p.v_head_stride),
+                "a cache's rows must not share memory");
         const int64_t piece = 16 / static_cast<int64_t>(trw::ops::element_size(p.dtype));
         require(p.k_batch_stride % piece == 0 && p.v_batch_stride % piece == 0,
                 "batch strides must be multiples of 16 bytes");

@@ -147,7 +147,8 @@ def walk_attention_step(q, k, v, k_cache, v_cache, lens, *, scale=None, softcap=
     to ``lens[b]``.  The caller counts ``lens`` up.
 
     ``k_cache``, ``v_cache``: ``[batch, capacity, kv_heads, dim]`` (a transposed
-    view of another order will do; dim contiguous, rows 16-byte pieces).  With
+    view of another order will do; dim contiguous, rows 16-byte pieces, none of
+    them shared: no expanded view).  With
     ``times`` (``[batch]``), ``k_times`` (``[batch, capacity]``, contiguous) is
     a cache as well and is written at ``lens[b]``.  The other arguments are
     :func:`walk_attention`'s; there is no gradient, and a result that is

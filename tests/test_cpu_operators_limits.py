@@ -1,5 +1,5 @@
-"""What a launch cannot take is refused as an argument, before anything is queued (no GPU needed: the
-addresses are never followed)."""
+"""What a launch or a cache cannot take is refused as an argument, before anything is queued (no GPU
+needed: the addresses are never followed)."""
 import ctypes
 
 import pytest
@@ -44,6 +44,22 @@ def test_bias_of_too_many_rows():
                        table=4096, buckets=4096, out=4096)
     with pytest.raises(ValueError, match="too many rows, documents or heads"):
         abi.call(abi.lib().trw_ops_relative_bias, ctypes.byref(p), None)
+
+
+@pytest.mark.parametrize("stride", ["k_batch_stride", "v_batch_stride", "k_pos_stride",
+                                    "v_pos_stride", "k_head_stride", "v_head_stride"])
+def test_caches_whose_rows_share_memory(stride):
+    """An expanded view: two walks would write to one row."""
+    abi = _abi()
+    rows = lambda h: abi.Rows(4096, h * 64, 64)  # noqa: E731
+    p = abi.StepParams(dtype=2, heads=4, kv_heads=2, dim=64, batch=3, capacity=50, lens=4096,
+                       score=abi.Score(0.125, 0.0), q=rows(4), k=rows(2), v=rows(2), out=rows(4),
+                       k_cache=4096, v_cache=4096, k_batch_stride=6400, k_pos_stride=128,
+                       k_head_stride=64, v_batch_stride=6400, v_pos_stride=128, v_head_stride=64,
+                       workspace=4096, workspace_bytes=1 << 40)
+    setattr(p, stride, 0)
+    with pytest.raises(ValueError, match="share memory"):
+        abi.call(abi.lib().trw_ops_attention_step, ctypes.byref(p), None)
 
 
 def test_sizes_below_the_limits():

@@ -224,3 +224,17 @@ def test_step_caps_far_above_the_scores(ops, dtype, softcap):
         want = wf.attention(*args, softcap=softcap, scale=0.5, dtype=dtype)["out"][0]
         bound = wf.attention(*args, scale=0.5, dtype=dtype)["out"][1]
         wf.check(f"out[{b}]", out[b:b + 1], want, bound)
+
+
+def test_steps_over_one_shared_row(ops):
+    """Caches that walks share are refused; one walk's has any stride there."""
+    q, kv = torch.randn(3, 2, 64, device="cuda"), torch.randn(3, 2, 64, device="cuda")
+    cache, lens = torch.randn(1, 8, 2, 64, device="cuda"), torch.tensor([1, 2, 3]).cuda()
+    own = cache.repeat(3, 1, 1, 1)
+    for caches in ((cache.expand(3, -1, -1, -1), own), (own, own[:, :, :1].expand(-1, -1, 2, -1))):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.walk_attention_step(q, kv, kv, *caches, lens)
+    want = ops.walk_attention_step(q, kv, kv, own.clone(), own.clone(), lens)
+    one = ops.walk_attention_step(q[:1], kv[:1], kv[:1], cache.as_strided(cache.shape, (0, 128, 64, 1)),
+                                  own[:1].clone(), lens[:1])
+    assert torch.equal(one, want[:1])
