@@ -322,6 +322,9 @@ Tensor workspace(trw_attention_params& p, int backward, const Tensor& beside) {
 
 Tensor as_rows(const Tensor& x) { return readable(x.dim() == 4 ? x.flatten(0, 1) : x); }
 
+// Autograd saves no tensors of the inference mode.
+Tensor saveable(const Tensor& x) { return x.defined() && x.is_inference() ? x.clone() : x; }
+
 // What was saved as a tensor of this shape, type and device, as a hook gave it
 // back.
 const Tensor& unpacked(const Tensor& x, at::IntArrayRef shape, at::ScalarType type,
@@ -408,7 +411,8 @@ struct WalkAttention : torch::autograd::Function<WalkAttention> {
             // the output itself and no view of it, which would keep it, and so this node, alive
             const Terms& terms = *call->terms;
             ctx->save_for_backward({q, k, v, table.value_or(Tensor()), result, stats, low,
-                                    terms.buckets, terms.slopes, terms.times, terms.k_times});
+                                    saveable(terms.buckets), saveable(terms.slopes),
+                                    saveable(terms.times), saveable(terms.k_times)});
             call->sloped = terms.slopes.defined();
             call->timed = terms.times.defined();
             call->terms.reset();
@@ -610,7 +614,7 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
         p.out = out.data_ptr();
         OnDevice on(table);
         check_status(trw_ops_relative_bias(&p, on.stream));
-        ctx->save_for_backward({table, buckets});
+        ctx->save_for_backward({table, saveable(buckets)});
         ctx->saved_data["q_offset"] = q_offset;
         ctx->saved_data["num_buckets"] = table.size(1);
         ctx->saved_data["ids"] = buckets.size(0);

@@ -231,3 +231,18 @@ def test_a_step_has_no_forward_derivative(ops):
         event["q"] = fwad.make_dual(event["q"], torch.ones_like(event["q"]))
         with pytest.raises(RuntimeError, match="walk_attention_step has no gradient"):
             ops.walk_attention_step(**event)
+
+
+def test_terms_of_the_inference_mode(ops):
+    """Constant terms that were made there serve a training pass too."""
+    case = Case(ops, SF, False, [20, 3])
+    want = case.run()
+    with torch.inference_mode():
+        case.terms.update({name: x.clone() for name, x in case.terms.items()
+                           if isinstance(x, torch.Tensor) and name != "bias_table"})
+    got = case.run()
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    table = torch.randn(3, 6, device="cuda", requires_grad=True)
+    ops.relative_bias(table, case.terms["buckets"], 20, 30).sum().backward()
+    assert table.grad is not None
