@@ -74,14 +74,16 @@ void check_buckets(const float* table, const int32_t* buckets, int num_buckets, 
     require(reach >= 0 && reach <= TRW_OPS_MAX_REACH, "reach must be 0 to 1024");
 }
 
-void check_score(const trw_score& s) {
+// Times of no rows may be NULL (an empty tensor's address is).
+void check_score(const trw_score& s, int64_t q_rows, int64_t k_rows) {
     require(std::isfinite(s.scale), "scale must be finite");
     require(std::isfinite(s.softcap) && s.softcap >= 0, "softcap must be finite and not negative");
     if (s.table || s.buckets)
         check_buckets(s.table, s.buckets, s.num_buckets, s.reach);
-    require((s.q_times == nullptr) == (s.k_times == nullptr),
+    const bool times = s.q_times || s.k_times;
+    require(!times || ((s.q_times || q_rows == 0) && (s.k_times || k_rows == 0)),
             "times are needed for the queries and the keys");
-    require(s.q_times == nullptr || s.slopes != nullptr, "times are for slopes");
+    require(!times || s.slopes, "times are for slopes");
 }
 
 const trw_attention_params& checked(const trw_attention_params* p) {
@@ -95,7 +97,7 @@ const trw_attention_params& checked(const trw_attention_params* p) {
     require(p->docs >= 0 && p->docs < kMaxRows && p->longest >= 0,
             "docs must be 0 to 2^30 - 1, longest not negative");
     require((p->docs + 7) * p->kv_heads < (int64_t{1} << 31), "too many documents and heads");
-    check_score(p->score);
+    check_score(p->score, p->q_rows, p->k_rows);
     return *p;
 }
 
@@ -118,7 +120,7 @@ const trw_attention_step_params& checked(const trw_attention_step_params* p) {
     require(p->batch >= 0 && p->batch < kMaxRows, "batch must be 0 to 2^30 - 1");
     require(p->capacity >= 0 && p->capacity < kMaxRows, "capacity must be 0 to 2^30 - 1");
     require(p->batch * p->heads < (int64_t{1} << 31) / 1024, "too many walks and heads");
-    check_score(p->score);
+    check_score(p->score, p->batch, p->batch * p->capacity);
     return *p;
 }
 

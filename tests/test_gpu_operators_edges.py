@@ -238,3 +238,21 @@ def test_steps_over_one_shared_row(ops):
     one = ops.walk_attention_step(q[:1], kv[:1], kv[:1], cache.as_strided(cache.shape, (0, 128, 64, 1)),
                                   own[:1].clone(), lens[:1])
     assert torch.equal(one, want[:1])
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [([3, 0], [0, 0]), ([0, 0], [5, 2]), ([0], [0])])
+def test_times_of_no_rows(ops, q_lens, k_lens):
+    """Queries without keys, keys without queries: an empty tensor of times is one."""
+    got = Batch(q_lens, k_lens, slopes=True, times=True, kind="full").run(ops)
+    assert got["out"].shape[0] == sum(q_lens) and got["d_k"].shape[0] == sum(k_lens)
+    assert not any(x.any() for x in got.values())
+
+
+def test_step_over_a_cache_of_no_slots(ops):
+    q, kv = torch.randn(2, 2, 64, device="cuda"), torch.randn(2, 2, 64, device="cuda")
+    caches = [torch.empty(2, 0, 2, 64, device="cuda") for _ in range(2)]
+    out = ops.walk_attention_step(q, kv, kv, *caches, torch.tensor([0, -1]).cuda(),
+                                  slopes=torch.ones(2, device="cuda"),
+                                  times=torch.ones(2, device="cuda"),
+                                  k_times=torch.empty(2, 0, device="cuda"))
+    assert torch.isnan(out[0]).all() and not out[1].any()
