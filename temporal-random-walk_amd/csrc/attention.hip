@@ -15,14 +15,14 @@
 // the inputs' type for the product with V (as the matrix instructions take
 // it), the sum l is of the unrounded values.
 //
-// Bound by the arithmetic per pair (exponential, bias, conversion) beside the
-// matrix units: 16384 rows in one causal walk (16 heads of 128 over 4 key heads, a
-// bias by distance, bfloat16) take 1.32 ms, 830 TFLOP/s, with the vector units
-// busy 0.63 of the time and the matrix units 0.35; a large library product reaches
-// 1260.  Tiles that reach LDS past the registers, two at a time, and tiles of few
-// rows sharing long keys took it from 3.3 ms.  Capped
-// scores with a bias cost as much again in arithmetic per pair: 23 walks of up to
-// 1999 rows (8 heads of 80, float16) take 168 us.
+// Arithmetic per pair (exponential, bias, conversion) and matrix products, and
+// the waits between them: 16384 rows in one causal walk (16 heads of 128 over 4 key
+// heads, a bias by distance, bfloat16) take 1.32 to 1.35 ms, 816 to 833 TFLOP/s, with
+// the vector units busy 0.63 of the time and the matrix units 0.35; a large library
+// product reaches 1260.  Tiles that reach LDS past the registers, two at a time, and
+// tiles of few rows sharing long keys took it from 3.3 ms.  23 walks of up to 1999
+// rows (8 heads of 80, capped scores with a bias, float16) take 170 us (0.47 and
+// 0.14 busy).
 #include <algorithm>
 
 #include "operators.h"

@@ -12,8 +12,8 @@
 // depends on the order they run in and no float32 copy of a gradient goes
 // through memory.  Heads that share keys are one sum in registers.
 //
-// Bound by the arithmetic per pair and by what two (over keys: one) workgroups a
-// compute unit can hide: one causal walk of 8192 rows (16 heads of 128 over 4 key
+// Bound by what two (over keys: one) workgroups a compute unit can hide of the
+// waits between products and arithmetic: one causal walk of 8192 rows (16 heads of 128 over 4 key
 // heads, capped scores, bfloat16) takes 0.78 ms over query rows (vector units busy
 // 0.45 of the time, matrix units 0.22) and 0.98 over keys (0.34 and 0.23), where
 // two operands and two sums of 128 columns leave room for one workgroup.

@@ -630,7 +630,8 @@ WalkArgs make_args(const trw_attention_params& p) {
 // 1155 us in one launch and 1058 by length, 2048 of them 295 and 301; walks of 50
 // to 60 in one of two launches: 1595 and 1635.  Packed walks of up to 40 (2 key
 // heads), of which the host knows the mean alone: 8192 of them 677 and 560 us,
-// 2048 203 and 161, 512 86 and 117.  (The forward pass, whose workgroups are one
+// 2048 203 and 161, 512 86 and 117.  Other head sizes and counts go by the same rule,
+// unmeasured.  (The forward pass, whose workgroups are one
 // wave either way: 435 and 484, 185 and 194 us; it has one launch.)
 bool by_length(const trw_attention_params& p) {
     return p.docs * p.kv_heads >= (p.longest > 0 ? 65536 : 2048);

@@ -15,6 +15,12 @@ They run hand-written gfx950 kernels (``libtrw_operators.so``, whose C ABI is
 stream of the tensors' device, wait for nothing, and follow PyTorch's rules for
 tensors used on several streams.  There is no CPU path.  Import ``torch`` before the engine in one process:
 PyTorch brings a HIP runtime of its own, which has to come up first.
+
+Scores, softmax, sums and gradients are float32 whatever the inputs' type.  The
+softmax's weights and their gradients are rounded to float16 or bfloat16 where
+those are the inputs' type, as operands of the matrix instructions, so results
+are up to 1.5 times as far from exact ones as if they had been rounded once, at
+the end.
 """
 from __future__ import annotations
 
@@ -128,11 +134,13 @@ def walk_attention(q, k, v, mask, *, scale=None, softcap=0.0, bias_table=None, b
     (``softcap`` 0: none), d is the distance in positions clamped to
     [-reach, reach] (``buckets``: int32 ids of 2 reach + 1 distances,
     :func:`distance_buckets`) and t are ``times`` and ``k_times`` (float32, of
-    the rows' shape; without them, positions).  ``scale``: 1 / sqrt(dim) unless
-    given.  -inf in the table masks.
+    the rows' shape; without them, positions; subtract an origin from integer
+    timestamps first, of which float32 holds 24 bits).  ``scale``: 1 / sqrt(dim)
+    unless given.  -inf in the table masks.
 
     Returns the output in q's shape; differentiable by q, k, v and bias_table
-    (once).  Equal inputs give equal results, bit for bit.  A row that sees no
+    (once), also under checkpointing.  Arguments that change between the passes
+    are an error, as PyTorch's own.  Equal inputs give equal results, bit for bit.  A row that sees no
     key is zero.  Values that are not finite stay within their own walk."""
     _require(isinstance(mask, WalkMask), "mask must be a WalkMask")
     return _operators.walk_attention(q, k, v, mask._mask, scale, softcap, bias_table, buckets,
