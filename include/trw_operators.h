@@ -1,7 +1,8 @@
 /*
  * trw_operators.h -- C ABI of the operators that consume walks: attention
- * inside each walk (forward, backward, one new event over a cache) and the
- * learned bias by distance buckets.
+ * inside each walk (forward, backward, one new event over a cache, dense or in
+ * pages), the learned bias by distance buckets, rows written to pages (8 bits
+ * or as they are) and read back, and beam search over a walk's next nodes.
  *
  * The sampler leaves walks padded in device memory; a sequence model over
  * them trains and answers through these calls.  They live in a library of
@@ -43,7 +44,15 @@ extern "C" {
  * length go through those of tiles). */
 #define TRW_OPS_WIDE_CAP 256
 
-typedef enum trw_dtype { TRW_F32 = 0, TRW_F16 = 1, TRW_BF16 = 2 } trw_dtype;
+/* Most beams of a group, and most that are chosen. */
+#define TRW_OPS_BEAMS 32
+
+typedef enum trw_dtype {
+    TRW_F32 = 0,
+    TRW_F16 = 1,
+    TRW_BF16 = 2,
+    TRW_E4M3 = 3 /* of pages only: 8 bits, with a scale for each row and head */
+} trw_dtype;
 
 typedef enum trw_mask_kind {
     TRW_MASK_FULL = 0,   /* every key of the walk */
@@ -177,6 +186,109 @@ trw_status trw_ops_relative_bias(const trw_relative_bias_params* params, void* s
 trw_status trw_ops_relative_bias_workspace(const trw_relative_bias_params* params,
                                            uint64_t* bytes);
 trw_status trw_ops_relative_bias_backward(const trw_relative_bias_params* params, void* stream);
+
+/* Caches of keys and values in pages of a pool: [pages, kv_heads, page_rows, D],
+ * the last three dimensions contiguous.  Position p of walk w is row
+ * p % page_rows of page table[w, p / page_rows]; an entry outside [0, pages) is
+ * no page: what would be written there is not, what would be read is 0, and
+ * steps do not see it.
+ *
+ * TRW_E4M3: a row of one head is D codes c (e4m3, no infinities) and one byte b,
+ * of the values c 2^(b - 127): the smallest power of two that brings the row's
+ * largest finite size to 448 or less, 10 <= b <= 247; values go to the nearest
+ * code, ties to the even one, and become NaN where they are not finite.  D is a
+ * multiple of 16. */
+typedef struct trw_pages {
+    int32_t dtype;
+    int32_t kv_heads, dim;
+    int32_t page_rows; /* a power of two, 16 to 1024 */
+    int64_t pages;     /* below 2^31 */
+    void *k, *v;
+    uint8_t *k_scale, *v_scale; /* TRW_E4M3: [pages, kv_heads, page_rows] */
+    int64_t k_stride, v_stride; /* elements from page to page, as are the scales' */
+    int64_t k_scale_stride, v_scale_stride;
+    const int32_t* table; /* [walks, table_pages] */
+    int64_t table_stride, table_pages, walks; /* table_pages * page_rows below 2^30 */
+} trw_pages;
+
+/* Rows of walks to their pages, or pages to rows.  Padded (offsets NULL): walk w
+ * has the first counts[w] of `length` rows (counts NULL: all).  Packed: the rows
+ * [offsets[w], offsets[w + 1]).  Its row i is position starts[w] + i (starts NULL:
+ * i); a walk of a negative start is left out.  What is read for rows of no walk
+ * and of no page is 0. */
+typedef struct trw_paged_copy_params {
+    trw_pages pages;
+    int32_t dtype; /* of the rows: the pages', or any with TRW_E4M3 */
+    int64_t rows, length;
+    const int64_t *counts, *offsets, *starts;
+    trw_rows k, v;  /* [rows, kv_heads, D] */
+    float* times;   /* [rows] or NULL */
+    float* k_times; /* [pages, page_rows], with times */
+} trw_paged_copy_params;
+trw_status trw_ops_paged_write(const trw_paged_copy_params* params, void* stream);
+trw_status trw_ops_paged_read(const trw_paged_copy_params* params, void* stream);
+
+/* trw_ops_attention_step over pages: the new row goes to position lens[b], and
+ * walk b sees positions first[b] .. lens[b] (first NULL: from 0; more than lens[b]:
+ * the new row alone), the new one as the pages hold it.  A negative length is an
+ * idle row (output 0, nothing written); where there is no page for the new row
+ * the output is NaN and nothing is written. */
+typedef struct trw_paged_step_params {
+    trw_pages pages; /* walks: the batch */
+    int32_t dtype;   /* of q, k, v and out: the pages', or any with TRW_E4M3 */
+    int32_t heads;
+    const int64_t *lens, *first;
+    trw_score score; /* q_times [batch]; k_times [pages, page_rows], written too */
+    trw_rows q, k, v, out;
+    void* workspace;
+    uint64_t workspace_bytes;
+} trw_paged_step_params;
+trw_status trw_ops_paged_step_workspace(const trw_paged_step_params* params, uint64_t* bytes);
+trw_status trw_ops_paged_step(const trw_paged_step_params* params, void* stream);
+
+/* The `width` best continuations of each group's beams: scores[g, b] + log
+ * softmax(logits[g, b])[x] over beams b and nodes x, greatest first, ties to the
+ * lowest b * nodes + x.  A beam that has ended continues as end_token alone, with
+ * its score.  Beams whose score is not finite, or whose logits hold NaN, +inf or
+ * nothing above -inf, have no continuations, nor have nodes of -inf.  Where there
+ * are fewer than `width`: score -inf, parent 0, token end_token (0 without one),
+ * ended. */
+typedef struct trw_beam_select_params {
+    int32_t dtype; /* of the logits */
+    int32_t beams, width; /* 1 to TRW_OPS_BEAMS */
+    int64_t groups, nodes; /* nodes: 1 to 2^30 - 1 */
+    const void* logits; /* [groups, beams, nodes], nodes contiguous */
+    int64_t group_stride, beam_stride;
+    const float* scores;  /* [groups, beams] */
+    const uint8_t* ended; /* [groups, beams], 0 or 1, or NULL */
+    int64_t end_token;    /* -1: none */
+    float* out_scores;    /* [groups, width], as are the others */
+    int64_t *out_tokens, *out_parents;
+    uint8_t* out_ended;
+    void* workspace;
+    uint64_t workspace_bytes;
+} trw_beam_select_params;
+trw_status trw_ops_beam_select_workspace(const trw_beam_select_params* params, uint64_t* bytes);
+trw_status trw_ops_beam_select(const trw_beam_select_params* params, void* stream);
+
+/* Groups of beams after a choice: child c of group g continues what row
+ * g * beams + parents[g, c] held.  Its full pages are the parent's.  The page that
+ * is filled next, and those after it, a parent's first child takes over; each
+ * further child takes those of a beam without children, with a copy of the
+ * parent's rows in the first.  So rows of a group that still grow need pages of
+ * their own from there on, and equal lengths; others may be shorter. */
+typedef struct trw_beam_reorder_params {
+    int32_t beams, page_rows, count;
+    int64_t groups, pages, table_pages, table_stride;
+    const int32_t* table;   /* [groups * beams, table_pages] */
+    int32_t* out_table;     /* the same, contiguous; not the same memory */
+    const int64_t* lens;    /* [groups * beams] */
+    int64_t* out_lens;      /* not the same memory */
+    const int64_t* parents; /* [groups, beams] */
+    const trw_pages* caches; /* host memory, [count]: caches of this table (their own is not read) */
+    float* k_times;         /* [pages, page_rows] or NULL */
+} trw_beam_reorder_params;
+trw_status trw_ops_beam_reorder(const trw_beam_reorder_params* params, void* stream);
 
 /* Message of the last failed call on this thread. */
 const char* trw_ops_last_error(void);

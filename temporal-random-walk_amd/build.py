@@ -5,7 +5,8 @@ Produces, inside ``temporal-random-walk_amd/temporal_random_walk/``:
 * ``libtrw_engine.so`` -- the HIP engine (gfx950 code objects) behind the
   C ABI of ``include/trw_engine.h``;
 * ``libtrw_operators.so`` -- the operators on walks (attention, its
-  single-event form, the distance bias) behind ``include/trw_operators.h``;
+  single-event form over dense caches and pages, the distance bias, pages,
+  beam search) behind ``include/trw_operators.h``;
 * ``_operators*.so`` -- the same operators on PyTorch tensors (only where
   PyTorch is installed);
 * ``_temporal_random_walk*.so`` -- the pybind11 module that mirrors the
@@ -52,7 +53,9 @@ HIP_FLAGS = [
 
 HIP_SOURCES = ["primitives.hip", "build.hip", "walk.hip", "handoff.hip", "pickers.hip", "capi.hip"]
 OPERATOR_SOURCES = ["walk_mask.hip", "attention.hip", "attention_backward.hip",
-                    "attention_walks.hip", "attention_step.hip", "relative_bias.hip", "operators_capi.hip"]
+                    "attention_walks.hip", "attention_step.hip", "relative_bias.hip",
+                    "paged_copy.hip", "attention_paged.hip", "beams.hip", "operators_capi.hip"]
+MODULE_SOURCES = ["operators_module.cpp", "serving_module.cpp"]
 PROBE_DIR = os.path.join(PKG_ROOT, "probe")
 
 
@@ -139,18 +142,22 @@ def build_operators_module():
     target = os.path.join(OUT_DIR, "_operators" + suffix)
     tmp = target + ".tmp"
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
-        "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_operators",
-        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-        f"-I{INCLUDE}", *(f"-I{d}" for d in include_paths()), "-I/opt/rocm/include",
-        f"-I{sysconfig.get_paths()['include']}",
-        os.path.join(HOST, "operators_module.cpp"),
-        f"-L{OUT_DIR}", "-ltrw_operators", "-Wl,-rpath,$ORIGIN",
-        f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-        "-o", tmp,
-    ]
-    _run(cmd)
+    os.makedirs(BUILD_DIR, exist_ok=True)
+
+    def compile_one(src):
+        obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-w",
+              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_operators",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              f"-I{INCLUDE}", *(f"-I{d}" for d in include_paths()), "-I/opt/rocm/include",
+              f"-I{sysconfig.get_paths()['include']}", "-c", os.path.join(HOST, src), "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(MODULE_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, MODULE_SOURCES))
+    _run(["g++", "-shared", *objs, f"-L{OUT_DIR}", "-ltrw_operators", "-Wl,-rpath,$ORIGIN",
+          f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+          "-o", tmp])
     os.replace(tmp, target)
     return target
 

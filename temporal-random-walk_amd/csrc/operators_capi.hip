@@ -4,7 +4,9 @@
 #include <cmath>
 #include <new>
 
+#include "beams.h"
 #include "operators.h"
+#include "pages.h"
 
 namespace {
 
@@ -133,6 +135,95 @@ const trw_relative_bias_params& checked(const trw_relative_bias_params* p) {
     require(p->q_offset > -kMaxRows && p->q_offset < kMaxRows, "q_offset is out of range");
     check_buckets(static_cast<const float*>(p->table), p->buckets, p->num_buckets, p->reach);
     return *p;
+}
+
+// table: with the walks' table.
+void check_pages(const trw_pages& p, bool table) {
+    if (p.dtype == TRW_E4M3)
+        require(p.dim % 16 == 0, "pages in 8 bits: the head size must be a multiple of 16");
+    else
+        check_dtype(p.dtype);
+    check_heads(TRW_F32, p.kv_heads, p.kv_heads, p.dim);
+    require(p.page_rows >= 16 && p.page_rows <= 1024 && (p.page_rows & (p.page_rows - 1)) == 0,
+            "page_rows must be a power of two, 16 to 1024");
+    require(p.pages >= 0 && p.pages < (int64_t{1} << 31), "pages must be 0 to 2^31 - 1");
+    const int64_t lines = int64_t{p.kv_heads} * p.page_rows;
+    const int64_t piece = 16 / static_cast<int64_t>(trw::ops::page_element_size(p.dtype));
+    if (p.pages > 0) {
+        require(p.k != nullptr && p.v != nullptr, "the pages are null");
+        check_aligned(p.k, "pages must be 16-byte aligned");
+        check_aligned(p.v, "pages must be 16-byte aligned");
+        require(p.k_stride >= lines * p.dim && p.v_stride >= lines * p.dim,
+                "pages must not share memory");
+        require(p.k_stride % piece == 0 && p.v_stride % piece == 0,
+                "page strides must be multiples of 16 bytes");
+        require(p.k_stride <= (int64_t{1} << 40) && p.v_stride <= (int64_t{1} << 40),
+                "page strides must be up to 2^40 elements");
+        if (p.dtype == TRW_E4M3) {
+            require(p.k_scale != nullptr && p.v_scale != nullptr, "the scales are null");
+            check_aligned(p.k_scale, "scales must be 16-byte aligned");
+            check_aligned(p.v_scale, "scales must be 16-byte aligned");
+            require(p.k_scale_stride >= lines && p.v_scale_stride >= lines,
+                    "pages must not share memory");
+            require(p.k_scale_stride % 16 == 0 && p.v_scale_stride % 16 == 0,
+                    "page strides must be multiples of 16 bytes");
+            require(p.k_scale_stride <= (int64_t{1} << 40) && p.v_scale_stride <= (int64_t{1} << 40),
+                    "page strides must be up to 2^40 elements");
+        }
+    }
+    if (!table) return;
+    require(p.walks >= 0 && p.walks < kMaxRows, "walks must be 0 to 2^30 - 1");
+    require(p.table_pages >= 0 && p.table_pages < kMaxRows / p.page_rows,
+            "a walk's pages must have fewer than 2^30 rows");
+    require(p.walks * p.table_pages == 0 || p.table, "table is null");
+    require(p.table_stride >= 0, "table_stride must not be negative");
+}
+
+const trw_paged_copy_params& checked(const trw_paged_copy_params* params) {
+    require(params != nullptr, "null argument");
+    const trw_paged_copy_params& p = *params;
+    check_pages(p.pages, true);
+    check_dtype(p.dtype);
+    require(p.pages.dtype == TRW_E4M3 || p.pages.dtype == p.dtype,
+            "rows must have the pages' type");
+    require(p.rows >= 0 && p.rows < kMaxRows, "rows must be 0 to 2^30 - 1");
+    if (p.offsets) {
+        require(!p.counts, "counts are for padded walks, offsets for packed ones");
+    } else {
+        require(p.length >= 0 && p.length < kMaxRows && (p.length > 0 || p.rows == 0) &&
+                    p.rows == p.pages.walks * p.length,
+                "rows must be walks * length");
+    }
+    check_rows(p.k, p.dtype, p.rows, "k is null");
+    check_rows(p.v, p.dtype, p.rows, "v is null");
+    require(!p.times == !p.k_times || p.rows == 0 || p.pages.pages == 0,
+            "times and k_times go together");
+    return p;
+}
+
+const trw_paged_step_params& checked(const trw_paged_step_params* params) {
+    require(params != nullptr, "null argument");
+    const trw_paged_step_params& p = *params;
+    check_pages(p.pages, true);
+    check_heads(p.dtype, p.heads, p.pages.kv_heads, p.pages.dim);
+    require(p.pages.dtype == TRW_E4M3 || p.pages.dtype == p.dtype,
+            "q, k and v must have the pages' type");
+    require(p.pages.walks * p.heads < (int64_t{1} << 31) / 1024, "too many walks and heads");
+    check_score(p.score, p.pages.walks, p.pages.pages);
+    return p;
+}
+
+const trw_beam_select_params& checked(const trw_beam_select_params* params) {
+    require(params != nullptr, "null argument");
+    const trw_beam_select_params& p = *params;
+    check_dtype(p.dtype);
+    require(p.beams >= 1 && p.beams <= TRW_OPS_BEAMS && p.width >= 1 && p.width <= TRW_OPS_BEAMS,
+            "beams and width must be 1 to 32");
+    require(p.groups >= 0 && p.groups < kMaxRows, "groups must be 0 to 2^30 - 1");
+    require(p.nodes >= 1 && p.nodes < kMaxRows, "nodes must be 1 to 2^30 - 1");
+    require(p.end_token >= -1 && p.end_token < p.nodes, "end_token must be a node");
+    require(!p.ended || p.end_token >= 0, "ended beams need an end_token");
+    return p;
 }
 
 }  // namespace
@@ -271,6 +362,86 @@ trw_status trw_ops_relative_bias_backward(const trw_relative_bias_params* params
         require(reinterpret_cast<uintptr_t>(p.d_out) % trw::ops::element_size(p.dtype) == 0,
                 "d_out is misaligned");
         trw::ops::relative_bias_backward(p, static_cast<hipStream_t>(stream));
+    });
+}
+
+trw_status trw_ops_paged_write(const trw_paged_copy_params* params, void* stream) {
+    return guarded([&] {
+        trw::ops::paged_copy(checked(params), true, static_cast<hipStream_t>(stream));
+    });
+}
+
+trw_status trw_ops_paged_read(const trw_paged_copy_params* params, void* stream) {
+    return guarded([&] {
+        trw::ops::paged_copy(checked(params), false, static_cast<hipStream_t>(stream));
+    });
+}
+
+trw_status trw_ops_paged_step_workspace(const trw_paged_step_params* params, uint64_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "null argument");
+        *bytes = trw::ops::paged_step_workspace(checked(params));
+    });
+}
+
+trw_status trw_ops_paged_step(const trw_paged_step_params* params, void* stream) {
+    return guarded([&] {
+        const trw_paged_step_params& p = checked(params);
+        const int64_t batch = p.pages.walks;
+        check_rows(p.q, p.dtype, batch, "q is null");
+        check_rows(p.k, p.dtype, batch, "k is null");
+        check_rows(p.v, p.dtype, batch, "v is null");
+        check_rows(p.out, p.dtype, batch, "out is null");
+        require(batch == 0 || p.lens, "lens is null");
+        check_aligned(p.workspace, "workspace must be 16-byte aligned");
+        trw::ops::paged_step(p, static_cast<hipStream_t>(stream));
+    });
+}
+
+trw_status trw_ops_beam_select_workspace(const trw_beam_select_params* params, uint64_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "null argument");
+        *bytes = trw::ops::beam_select_workspace(checked(params));
+    });
+}
+
+trw_status trw_ops_beam_select(const trw_beam_select_params* params, void* stream) {
+    return guarded([&] {
+        const trw_beam_select_params& p = checked(params);
+        require(p.groups == 0 || (p.logits && p.scores), "logits and scores must not be null");
+        require(p.groups == 0 || (p.out_scores && p.out_tokens && p.out_parents && p.out_ended),
+                "outputs must not be null");
+        require(reinterpret_cast<uintptr_t>(p.logits) % trw::ops::element_size(p.dtype) == 0,
+                "logits are misaligned");
+        check_aligned(p.workspace, "workspace must be 16-byte aligned");
+        trw::ops::beam_select(p, static_cast<hipStream_t>(stream));
+    });
+}
+
+trw_status trw_ops_beam_reorder(const trw_beam_reorder_params* params, void* stream) {
+    return guarded([&] {
+        require(params != nullptr, "null argument");
+        const trw_beam_reorder_params& p = *params;
+        require(p.beams >= 1 && p.beams <= TRW_OPS_BEAMS, "beams must be 1 to 32");
+        require(p.groups >= 0 && p.groups < kMaxRows / p.beams, "groups must be 0 to 2^30 / beams");
+        require(p.count >= 0 && (p.count == 0 || p.caches), "caches is null");
+        trw_pages shared{TRW_F32, 1, 8, p.page_rows};  // the table's own checks
+        shared.table = p.table;
+        shared.table_stride = p.table_stride;
+        shared.table_pages = p.table_pages;
+        shared.walks = p.groups * p.beams;
+        check_pages(shared, true);
+        require(p.pages >= 0 && p.pages < (int64_t{1} << 31), "pages must be 0 to 2^31 - 1");
+        for (int c = 0; c < p.count; ++c) {
+            check_pages(p.caches[c], false);
+            require(p.caches[c].pages == p.pages && p.caches[c].page_rows == p.page_rows,
+                    "caches of one table must have pages alike");
+        }
+        require(p.groups == 0 || (p.lens && p.out_lens && p.parents && p.out_lens != p.lens),
+                "lens, out_lens and parents must not be null, nor the lens one");
+        require(p.groups * p.table_pages == 0 || (p.out_table && p.out_table != p.table),
+                "out_table must be memory of its own");
+        trw::ops::beam_reorder(p, static_cast<hipStream_t>(stream));
     });
 }
 

@@ -8,7 +8,12 @@ spends its time in:
 * :func:`walk_attention_step` -- one new event of each walk over its cache;
 * :func:`relative_bias` -- a learned bias by buckets of distance as a dense
   array, for models with an attention of their own (the other two take the
-  table itself).
+  table itself);
+* :class:`Pages`, :func:`paged_write`, :func:`paged_read`,
+  :func:`paged_attention_step` -- caches in pages of a common pool, in 8 bits or
+  as they are, for walks of very different and growing lengths;
+* :func:`beam_select`, :func:`beam_reorder` -- forecasts of several events by
+  beam search, over such caches.
 
 They run hand-written gfx950 kernels (``libtrw_operators.so``, whose C ABI is
 ``include/trw_operators.h``; ``operators_capi`` has it by ctypes) on the current
@@ -26,6 +31,7 @@ from __future__ import annotations
 
 import math
 import os
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -38,6 +44,7 @@ from . import _operators  # noqa: E402
 
 MAX_REACH = 1024
 MAX_BUCKETS = 256
+MAX_BEAMS = 32
 
 
 def _require(ok, message):
@@ -175,3 +182,139 @@ def relative_bias(table, buckets, q_len, k_len, q_offset=0):
     ``[heads, num_buckets]``, in the table's type; differentiable by the table
     (once).  ``buckets``: as for :func:`walk_attention`."""
     return _operators.relative_bias(table, buckets, q_len, k_len, q_offset)
+
+
+class Pages(NamedTuple):
+    """Keys and values of many walks in pages of one pool.
+
+    ``k``, ``v``: ``[pages, kv_heads, page_rows, dim]``, each page contiguous
+    (``page_rows``: a power of two, 16 to 1024).  Which pages are a walk's says a
+    table, int32 ``[walks, pages of a walk]``, that all layers share: position p
+    of walk w is row p % page_rows of page ``table[w, p // page_rows]``.  Entries
+    outside the pool (-1, say) are no pages: nothing is written there, 0 is read,
+    and steps do not see their positions.
+
+    Rows are kept as they are (float32, float16, bfloat16), or in 8 bits: ``k``
+    and ``v`` of ``torch.float8_e4m3fn``, and for each row and head a byte b of
+    ``k_scale`` or ``v_scale`` (uint8 ``[pages, kv_heads, page_rows]``); a value
+    is its code times 2^(b - 127), off by at most 1/16 of it or 2^-10 of that
+    power (for rows whose largest value is below 2^-109, of 2^-117).  What is not
+    finite becomes NaN.  ``dim`` is a multiple of 8 up to 128, of 16 in 8 bits."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+    @classmethod
+    def empty(cls, pages, page_rows, kv_heads, dim, *, dtype=torch.bfloat16, device="cuda"):
+        """A pool whose rows are still to be written; ``dtype``
+        ``torch.float8_e4m3fn`` for 8 bits."""
+        def one(*shape, of=dtype):
+            return torch.empty(pages, kv_heads, page_rows, *shape, dtype=of, device=device)
+
+        k, v = one(dim), one(dim)
+        if dtype != torch.float8_e4m3fn:
+            return cls(k, v)
+        return cls(k, v, one(of=torch.uint8), one(of=torch.uint8))
+
+    def record_stream(self, stream):
+        for x in self:
+            if x is not None:
+                x.record_stream(stream)
+
+
+def paged_write(pages, table, starts, k, v, *, counts=None, offsets=None, times=None, k_times=None):
+    """Rows of walks (prompts) to their pages: row i of walk w goes to position
+    ``starts[w] + i`` (``starts`` None: i).
+
+    ``k``, ``v``: ``[walks, length, kv_heads, dim]``, of which the first
+    ``counts[w]`` rows are walk w's (None: all), or ``[rows, kv_heads, dim]`` with
+    ``offsets`` (walk w has the rows ``offsets[w]`` up to ``offsets[w + 1]``).  Any
+    of the three types goes to 8 bits, else the pages' own.  ``times`` (float32, of
+    the rows' shape) go to ``k_times`` (``[pages, page_rows]``, contiguous).
+
+    A walk of a negative start is left out, as are positions that have no page.
+    Walks that are written at once need pages of their own there.  There is no
+    gradient."""
+    _operators.paged_write(pages, table, starts, k, v, counts, offsets, times, k_times)
+
+
+def paged_read(pages, table, *, lens=None, length=None, offsets=None, rows=None, dtype=None,
+               k_times=None):
+    """Pages back to rows, as :func:`walk_attention` takes them for prompts over
+    what is cached: ``k`` and ``v`` ``[walks, length, kv_heads, dim]`` of the first
+    ``lens[w]`` positions of each walk, or ``[rows, kv_heads, dim]`` where walk w
+    has the rows ``offsets[w]`` up to ``offsets[w + 1]``, from position 0 on; and,
+    with ``k_times``, their times as a third tensor.  Rows of no walk, and of
+    positions without a page, are 0.
+
+    ``dtype``: what 8 bits are read as (bfloat16 unless given, which is exact); else
+    the pages' own."""
+    k, v, times = _operators.paged_read(pages, table, lens, length, offsets, rows, dtype, k_times)
+    return (k, v) if times is None else (k, v, times)
+
+
+def paged_attention_step(q, k, v, pages, table, lens, *, first=None, scale=None, softcap=0.0,
+                         bias_table=None, buckets=None, slopes=None, times=None, k_times=None):
+    """:func:`walk_attention_step` over pages: appends ``k`` and ``v``
+    (``[batch, kv_heads, dim]``) at position ``lens[b]`` and returns the attention
+    of ``q`` (``[batch, heads, dim]``) over positions ``first[b]`` (None: 0) to
+    ``lens[b]``, the new one as the pages hold it.  The caller counts ``lens`` up.
+
+    ``first``: for windows; what lies before is not read, and its pages may be
+    another walk's by then.  More than ``lens[b]`` leaves the new event alone.
+    ``table``: a row for each of the batch.  ``k_times``: ``[pages, page_rows]``,
+    written at the new position.  The other arguments are
+    :func:`walk_attention`'s; there is no gradient, and a result that is
+    differentiated says so.
+
+    A negative length is an idle row: output 0, nothing written.  Where there is
+    no page for the new event the output is NaN, and nothing is written.  Rows of
+    a batch may share pages but not the one that they write."""
+    return _operators.paged_attention_step(q, k, v, pages, table, lens, first, scale, softcap,
+                                           bias_table, buckets, slopes, times, k_times)
+
+
+class BeamChoice(NamedTuple):
+    """What :func:`beam_select` chose, ``[groups, width]``: scores (float32),
+    nodes and parent beams (int64), and whether a beam has ended (bool)."""
+    scores: torch.Tensor
+    tokens: torch.Tensor
+    parents: torch.Tensor
+    ended: torch.Tensor
+
+
+def beam_select(logits, scores, width, *, ended=None, end_token=None):
+    """The ``width`` best continuations of each group's beams, best first.
+
+    ``logits``: ``[groups, beams, nodes]`` of any of the three types (-inf: not a
+    next node), ``scores``: float32 ``[groups, beams]``, each beam's log
+    probability (-inf: no beam; a group that starts has one).  A continuation of
+    beam b by node x scores ``scores[b] + log softmax(logits[b])[x]``; equal ones
+    come by their beam, then by their node.  ``ended`` (bool ``[groups, beams]``):
+    beams that have come to ``end_token`` continue as themselves, token
+    ``end_token``.  Up to 32 beams and 32 of a width.
+
+    A beam whose score is not finite, or whose logits hold NaN, +inf or nothing
+    above -inf, has no continuations.  Where a group has fewer than ``width``: score -inf,
+    parent 0, token ``end_token`` (0 without one), ended.  Scores are summed in
+    float64; there is no gradient."""
+    return BeamChoice(*_operators.beam_select(logits, scores, width, ended, end_token))
+
+
+def beam_reorder(table, lens, parents, caches, *, k_times=None):
+    """Makes the rows of a table, and their pages, those of chosen beams.
+
+    Row ``g * beams + b`` of ``table`` and ``lens`` is beam b of group g; after it
+    has been called, row ``g * beams + c`` of the table and lengths that it returns
+    holds what beam ``parents[g, c]`` (``[groups, beams]``) held.  ``caches``: the
+    :class:`Pages` of every layer, ``k_times`` as for
+    :func:`paged_attention_step`.
+
+    Beams share the full pages of their common past.  The page that is filled next,
+    and those after it, go to a parent's first child; a further child takes those
+    of a beam without children, with a copy of the rows: nothing else moves.  So
+    each row of a group starts with pages of its own (a prompt is written to one
+    row of each group, and ``parents`` 0 spreads it), and rows of a group have equal
+    lengths, but for beams that have ended, which may be shorter."""
+    return _operators.beam_reorder(table, lens, parents, list(caches), k_times)

@@ -15,6 +15,9 @@ EXPORTS = [
     "trw_ops_walk_mask", "trw_ops_attention_workspace", "trw_ops_attention_forward",
     "trw_ops_attention_backward", "trw_ops_attention_step_workspace", "trw_ops_attention_step",
     "trw_ops_relative_bias", "trw_ops_relative_bias_workspace", "trw_ops_relative_bias_backward",
+    "trw_ops_paged_write", "trw_ops_paged_read", "trw_ops_paged_step_workspace",
+    "trw_ops_paged_step", "trw_ops_beam_select_workspace", "trw_ops_beam_select",
+    "trw_ops_beam_reorder",
     "trw_ops_last_error", "trw_ops_abi_version",
 ]
 
@@ -72,6 +75,48 @@ class BiasParams(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
+class Pages(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32),
+                ("page_rows", C.c_int32), ("pages", C.c_int64), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("k_scale_stride", C.c_int64), ("v_scale_stride", C.c_int64),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int64),
+                ("walks", C.c_int64)]
+
+
+class PagedCopyParams(C.Structure):
+    _fields_ = [("pages", Pages), ("dtype", C.c_int32), ("rows", C.c_int64),
+                ("length", C.c_int64), ("counts", C.c_void_p), ("offsets", C.c_void_p),
+                ("starts", C.c_void_p), ("k", Rows), ("v", Rows), ("times", C.c_void_p),
+                ("k_times", C.c_void_p)]
+
+
+class PagedStepParams(C.Structure):
+    _fields_ = [("pages", Pages), ("dtype", C.c_int32), ("heads", C.c_int32),
+                ("lens", C.c_void_p), ("first", C.c_void_p), ("score", Score),
+                ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class BeamSelectParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("beams", C.c_int32), ("width", C.c_int32),
+                ("groups", C.c_int64), ("nodes", C.c_int64), ("logits", C.c_void_p),
+                ("group_stride", C.c_int64), ("beam_stride", C.c_int64),
+                ("scores", C.c_void_p), ("ended", C.c_void_p), ("end_token", C.c_int64),
+                ("out_scores", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("out_parents", C.c_void_p), ("out_ended", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class BeamReorderParams(C.Structure):
+    _fields_ = [("beams", C.c_int32), ("page_rows", C.c_int32), ("count", C.c_int32),
+                ("groups", C.c_int64), ("pages", C.c_int64), ("table_pages", C.c_int64),
+                ("table_stride", C.c_int64), ("table", C.c_void_p), ("out_table", C.c_void_p),
+                ("lens", C.c_void_p), ("out_lens", C.c_void_p), ("parents", C.c_void_p),
+                ("caches", C.POINTER(Pages)), ("k_times", C.c_void_p)]
+
+
 _lib = None
 
 
@@ -94,6 +139,13 @@ def lib():
         L.trw_ops_relative_bias.argtypes = [C.POINTER(BiasParams), P]
         L.trw_ops_relative_bias_workspace.argtypes = [C.POINTER(BiasParams), size]
         L.trw_ops_relative_bias_backward.argtypes = [C.POINTER(BiasParams), P]
+        L.trw_ops_paged_write.argtypes = [C.POINTER(PagedCopyParams), P]
+        L.trw_ops_paged_read.argtypes = [C.POINTER(PagedCopyParams), P]
+        L.trw_ops_paged_step_workspace.argtypes = [C.POINTER(PagedStepParams), size]
+        L.trw_ops_paged_step.argtypes = [C.POINTER(PagedStepParams), P]
+        L.trw_ops_beam_select_workspace.argtypes = [C.POINTER(BeamSelectParams), size]
+        L.trw_ops_beam_select.argtypes = [C.POINTER(BeamSelectParams), P]
+        L.trw_ops_beam_reorder.argtypes = [C.POINTER(BeamReorderParams), P]
         L.trw_ops_last_error.restype = C.c_char_p
         L.trw_ops_abi_version.restype = C.c_int32
         if L.trw_ops_abi_version() != ABI_VERSION:
