@@ -2,10 +2,17 @@
 //
 // Per walk and key head: read the pages once, at memory speed.  The query heads
 // that share a key head are the columns of the products, 16 of them; a wave takes
-// blocks of 32 positions (two halves of 16, each in one page), four waves and,
-// where walks are few, many workgroups share a walk: each keeps a maximum, a sum
-// and an output of its own, joined at the end.  Positions that the walk does not
-// see are never read.
+// blocks of 32 positions (two halves of 16, each in one page), four waves share a
+// walk, each with a maximum, a sum and an output of its own, joined at the end.
+// Positions that the walk does not see are never read.
+//
+// Walks differ in length, and only the device knows how much, so the positions of
+// all walks are put in one line and dealt out evenly to as many workgroups as the
+// device holds at once.  Where that cuts a walk, its parts are joined by a second
+// launch.  With walks' own workgroups, three of them each, 64 walks of 100 to 4095
+// events (8 heads of 128, 8 bits) took 76.7 us, OURS so.  Many walks, and walks of
+// up to 512, have a workgroup each: there is no second launch, and the device
+// evens them out.
 //
 // v_mfma_f32_16x16x32 with keys as rows leaves lane l with keys 4 (l / 16) .. + 4
 // of column l & 15.  Two halves give eight, which are the B operand of the next
@@ -25,7 +32,6 @@
 #include <algorithm>
 
 #include "pages.h"
-#include "step_join.h"
 
 namespace trw {
 namespace ops {
@@ -43,10 +49,30 @@ struct PagedArgs {
     const int64_t *lens, *first;
     float* k_times;  // [pages, page_rows]
     Score score;
-    int batch, heads, kv_heads, group, columns, dim, splits;
-    float* partial;      // [batch, heads, splits, dim]
-    float2* part_stats;  // [batch, heads, splits]
+    int batch, heads, kv_heads, group, columns, dim;
+    int even;            // workgroups of a key head that share all walks evenly; 0: one a walk
+    // of walks that are cut: each workgroup's first and last part
+    float* partial;      // [workgroups, 2, columns, dim]
+    float2* part_stats;  // [workgroups, 2, columns]: maximum (base 2) and sum
+    int64_t* begins;     // [batch + 1] where each walk begins in the line of units
 };
+
+constexpr int kUnit = kWaves;  // blocks that a workgroup takes at once
+
+// Units of a walk: one at least, which writes what an idle one answers.
+struct Length {
+    int n, first, units;  // the new event's position, the first that is seen
+    bool in;              // whether the table has a place for the new event
+};
+__device__ __forceinline__ Length length_of(const PagedArgs& a, int64_t b) {
+    const int64_t at = a.lens[b], begin = a.first ? a.first[b] : 0;
+    Length r;
+    r.in = at >= 0 && at < static_cast<int64_t>(a.pages.table_pages) << a.pages.shift;
+    r.n = r.in ? static_cast<int>(at) : 0;
+    r.first = static_cast<int>(min(max(begin, int64_t{0}), static_cast<int64_t>(r.n)));
+    r.units = (r.n / kKeys - r.first / kKeys) / kUnit + 1;
+    return r;
+}
 
 __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -235,13 +261,29 @@ __device__ __forceinline__ void reads_done() {
     asm volatile("" ::: "memory");
 }
 
+// The kernel's arguments once more, from memory: what is not needed all the time is not
+// held in registers all the time (held, the arguments took more scalar registers than
+// there are, and some 700 moves between them and vector registers).
+typedef __attribute__((address_space(4))) const PagedArgs* ArgsAgain;
+__device__ __forceinline__ ArgsAgain args_again() {
+    ArgsAgain p = (ArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // Rows lo .. hi - 1 of a half as bits.
 __device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
     return hi > lo ? ((1u << hi) - 1) & ~((1u << lo) - 1) : 0u;
 }
 
+// Workgroups that a compute unit holds: their tiles' room in LDS, and registers.
+template <typename T, int DB, bool kEight>
+constexpr int kResident = kEight           ? (DB <= 2 ? 4 : 3)
+                          : sizeof(T) == 2 ? (DB <= 2 ? 4 : 2)
+                                           : (DB == 1 ? 4 : DB == 2 ? 2 : 1);
+
 template <typename T, int DB, bool kWide, bool kEight>
-__global__ __launch_bounds__(kThreads, kEight ? (DB <= 2 ? 4 : 3) : sizeof(T) == 2 ? (DB <= 2 ? 4 : 2) : 1)
+__global__ __launch_bounds__(kThreads, (kResident<T, DB, kEight>))
 void paged_step_kernel(PagedArgs a) {
     typedef std::conditional_t<kEight, Eight<DB>, Wide<T, DB>> In;
     typedef typename In::G G;
@@ -255,6 +297,9 @@ void paged_step_kernel(PagedArgs a) {
     __shared__ float s_m[kWaves][kColumns], s_l[kWaves][kColumns];
     __shared__ float s_times[kWaves][64];
     __shared__ uint32_t s_scales[kEight ? kWaves : 1][64];  // keys' 32 bytes, values' 32
+    __shared__ int64_t s_sums[kWaves];
+    __shared__ int64_t s_start;
+    __shared__ int s_walk;
 
     // Consecutive workgroups go to the eight XCDs in turn: each takes all key
     // heads of some positions.
@@ -263,78 +308,87 @@ void paged_step_kernel(PagedArgs a) {
     rest /= a.columns;
     const int kv_head = rest % a.kv_heads;
     const int item = rest / a.kv_heads * 8 + blockIdx.x % 8;
-    const int split = item % a.splits;
-    const int b = item / a.splits;
-    if (b >= a.batch) return;
     const int thread = threadIdx.x, lane = thread & 63, quarter = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
-    const Score& sc = a.score;
-    const Pages& pages = a.pages;
-    const int shift = pages.shift, page_mask = (1 << shift) - 1;
-
-    const int64_t at_n = a.lens[b];  // position of the new event
-    const int64_t room = static_cast<int64_t>(pages.table_pages) << shift;
-    const int new_page = at_n >= 0 && at_n < room ? pages.page_of(b, at_n) : -1;
-    const bool idle = new_page < 0;
-    const int n = idle ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(at_n));
-    const int64_t at_first = a.first ? a.first[b] : 0;
-    const int first = __builtin_amdgcn_readfirstlane(
-        static_cast<int>(min(max(at_first, int64_t{0}), static_cast<int64_t>(n))));
+    const int shift = a.pages.shift, page_mask = (1 << shift) - 1, dim = a.dim;
     const int col = col_group * kColumns + (lane & 15);
     const int head = kv_head * a.group + col;
-    const bool any = !idle && col < a.group;
-    const T* fresh_k = row_of<const T>(a.k, b, kv_head);
-    const T* fresh_v = row_of<const T>(a.v, b, kv_head);
-    const float q_time = sc.q_times ? sc.q_times[b] : 0.0f;
-
-    // The new row as codes, eight of them in each lane by its number in 16.
-    u32x2 codes_k = {0, 0}, codes_v = {0, 0};
-    int byte_k = 0, byte_v = 0;
-    auto encode = [&]() {
-        const int from = (lane & 15) * 8;
-        float k[8] = {}, v[8] = {}, k_top = 0.0f, v_top = 0.0f;
-        if (from < a.dim) {
-            load8(fresh_k + from, k);
-            load8(fresh_v + from, v);
-        }
+    const bool any = col < a.group;
+    const bool biased = a.score.table, sloped = a.score.slopes, timed = a.k_times;
+    const float softcap = a.score.softcap, scale2 = a.score.scale2;
+    const float slope = sloped && any ? a.score.slopes[head] * kLog2e : 0.0f;
+    const float far_bias = biased && any ? table_entry(a.score, head, 2 * a.score.reach) : 0.0f;
+    const int pitch = dim * kBytes;
+    uint32_t offset[G::kHalfCopies];  // bytes from a half's first row
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            k_top = fmaxf(k_top, size_of(k[e]));
-            v_top = fmaxf(v_top, size_of(v[e]));
-        }
-        byte_k = scale_byte(group_max<16>(k_top));
-        byte_v = scale_byte(group_max<16>(v_top));
-        codes_k = eight_codes(k, inverse_power(byte_k));
-        codes_v = eight_codes(v, inverse_power(byte_v));
-    };
-
-    if (!idle && split == 0 && col_group == 0 && wave == 0) {
-        const int64_t line = (static_cast<int64_t>(kv_head) << shift) + (n & page_mask);
-        char* k_row = pages.k + new_page * pages.k_page + line * a.dim * kBytes;
-        char* v_row = pages.v + new_page * pages.v_page + line * a.dim * kBytes;
-        if constexpr (kEight) {
-            encode();
-            if (lane * 8 < a.dim) {
-                *reinterpret_cast<u32x2*>(k_row + lane * 8) = codes_k;
-                *reinterpret_cast<u32x2*>(v_row + lane * 8) = codes_v;
-            }
-            if (lane == 0) {
-                pages.k_scale[new_page * pages.k_scale_page + line] = byte_k;
-                pages.v_scale[new_page * pages.v_scale_page + line] = byte_v;
-            }
-        } else if (lane * G::kElems < a.dim) {
-            reinterpret_cast<u32x4*>(k_row)[lane] = reinterpret_cast<const u32x4*>(fresh_k)[lane];
-            reinterpret_cast<u32x4*>(v_row)[lane] = reinterpret_cast<const u32x4*>(fresh_v)[lane];
-        }
-        if (a.k_times && kv_head == 0 && lane == 0)
-            a.k_times[(static_cast<int64_t>(new_page) << shift) + (n & page_mask)] = q_time;
+    for (int c = 0; c < G::kHalfCopies; ++c) {
+        const int row = lane / G::kSlots + c * G::kStep;
+        const int chunk = (lane % G::kSlots) ^ G::swizzle(row);
+        offset[c] = row * pitch + (chunk * 16 < pitch ? chunk * 16 : 0);
     }
 
-    // this workgroup's blocks of positions
-    const int first_block = first / kKeys;
-    const int64_t blocks = idle ? 0 : n / kKeys + 1 - first_block;
-    const int block_begin = first_block + static_cast<int>(blocks * split / a.splits);
-    const int block_end = first_block + static_cast<int>(blocks * (split + 1) / a.splits);
+    // Units [unit, unit + left) of this workgroup, counted from walk b's first.
+    int b = item;
+    int64_t unit = 0, left = INT64_MAX;
+    if (a.even) {
+        if (item >= a.even) return;
+        // each thread some walks one after the other
+        const int each = (a.batch + kThreads - 1) / kThreads;
+        const int walk = min(thread * each, a.batch), end = min(walk + each, a.batch);
+        int64_t mine = 0;
+        for (int w = walk; w < end; ++w) mine += length_of(a, w).units;
+        int64_t before = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t other = __shfl_up(static_cast<long long>(before), o);
+            if (lane >= o) before += other;
+        }
+        if (lane == 63) s_sums[wave] = before;
+        __syncthreads();
+        int64_t all = 0;
+        before -= mine;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) before += s_sums[w];
+            all += s_sums[w];
+        }
+        const int64_t begin = all * item / a.even, stop = all * (item + 1) / a.even;
+        const bool notes = item == 0 && kv_head == 0 && col_group == 0;
+        if (notes && thread == 0) a.begins[a.batch] = all;
+        for (int w = walk; w < end; ++w) {
+            const int units = length_of(a, w).units;
+            if (notes) a.begins[w] = before;
+            if (before <= begin && begin < before + units) {
+                s_walk = w;
+                s_start = begin - before;
+            }
+            before += units;
+        }
+        if (begin >= stop) return;
+        __syncthreads();
+        b = s_walk;
+        unit = s_start;
+        left = stop - begin;
+    } else if (item >= a.batch) {
+        return;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+
+  for (int part = 0; left > 0; part = 1) {
+    const Length length = length_of(a, b);
+    const int n = __builtin_amdgcn_readfirstlane(length.n);
+    const int first = __builtin_amdgcn_readfirstlane(length.first);
+    const int units = __builtin_amdgcn_readfirstlane(length.units);
+    const int from_unit = __builtin_amdgcn_readfirstlane(static_cast<int>(unit));
+    const int till_unit =
+        __builtin_amdgcn_readfirstlane(static_cast<int>(min(unit + left, static_cast<int64_t>(units))));
+    const bool idle = !length.in;
+    const float q_time = timed ? a.score.q_times[b] : 0.0f;
+
+    // this part's blocks of positions
+    const int first_block = first / kKeys, last_block = idle ? first_block : n / kKeys + 1;
+    const int block_begin = first_block + from_unit * kUnit;
+    const int block_end = min(last_block, first_block + till_unit * kUnit);
 
     F q[DB][kParts];
     {
@@ -343,13 +397,10 @@ void paged_step_kernel(PagedArgs a) {
         for (int st = 0; st < DB; ++st) {
             const int at = 32 * st + 8 * quarter;
             float x[8] = {};
-            if (any && at < a.dim) load8(row + at, x);
+            if (any && at < dim) load8(row + at, x);
             in_parts<kParts>(x, q[st]);
         }
     }
-    const float slope = sc.slopes && any ? sc.slopes[head] * kLog2e : 0.0f;
-    const float far_bias = sc.table && any ? table_entry(sc, head, 2 * sc.reach) : 0.0f;
-
     f32x4 o[2 * DB];
 #pragma unroll
     for (int c = 0; c < 2 * DB; ++c) o[c] = f32x4{0, 0, 0, 0};
@@ -363,23 +414,21 @@ void paged_step_kernel(PagedArgs a) {
     u32x4* s_v = s_k + G::kSize / 16;
     const uint32_t at_k = lds_address(s_mem) + wave * 2 * static_cast<uint32_t>(G::kSize);
     const uint32_t at_v = at_k + static_cast<uint32_t>(G::kSize);
-    const int pitch = a.dim * kBytes;
     constexpr int kCopies = 2 * G::kHalfCopies;
-    uint32_t offset[G::kHalfCopies];  // bytes from a half's first row
-#pragma unroll
-    for (int c = 0; c < G::kHalfCopies; ++c) {
-        const int row = lane / G::kSlots + c * G::kStep;
-        const int chunk = (lane % G::kSlots) ^ G::swizzle(row);
-        offset[c] = row * pitch + (chunk * 16 < pitch ? chunk * 16 : 0);
-    }
 
     // Pages of the wave's next 64 blocks, one block's two halves a lane.
     int ids[2];
     auto fetch_ids = [&](int block) {
+        const ArgsAgain g = args_again();
+        const int32_t* table = g->pages.table + b * g->pages.table_stride;
+        const int table_pages = g->pages.table_pages, pages = g->pages.pages;
         const int64_t j = (static_cast<int64_t>(block) + lane * kWaves) * kKeys;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            ids[h] = j + kHalf * h <= n ? pages.page_of(b, j + kHalf * h) : -1;
+        for (int h = 0; h < 2; ++h) {
+            const int64_t at = (j + kHalf * h) >> shift;
+            const int id = j + kHalf * h <= n && at < table_pages ? table[at] : -1;
+            ids[h] = id < pages ? id : -1;
+        }
     };
     // The rows of a half that are in the pages and seen: [lo, hi), none where hi <= lo.
     struct Span {
@@ -393,228 +442,301 @@ void paged_step_kernel(PagedArgs a) {
         s.hi = s.page < 0 ? 0 : min(n - j, kHalf);
         return s;
     };
-    // Copies of one half; rows that are not seen repeat the nearest one that is,
-    // and a half without any asks for the query's first 16 bytes, which nothing reads.
-    auto fetch_half = [&](const Span& s, const char* pool, int64_t page_bytes, int j, uint32_t to) {
-        const bool none = s.hi <= s.lo;
-        const int64_t line = (static_cast<int64_t>(kv_head) << shift) + (j & page_mask);
-        const char* base = uniform(none ? a.q.data + static_cast<int64_t>(b) * a.q.row * sizeof(T)
-                                        : pool + s.page * page_bytes + line * pitch);
-        if (s.lo == 0 && s.hi == kHalf) {
+    // A head's row of a page, in rows.
+    auto line_of = [&](int j) { return (static_cast<int64_t>(kv_head) << shift) + (j & page_mask); };
+    // Copies of a block's keys or values; rows that are not seen repeat the nearest one
+    // that is, and a half without any asks for the query's first 16 bytes, which nothing
+    // reads.
+    auto fetch = [&](const Span (&s)[2], const char* pool, int64_t page_bytes, int j0, uint32_t to) {
+        const ArgsAgain g = args_again();
+        const char* nothing = g->q.data + static_cast<int64_t>(b) * g->q.row * sizeof(T);
 #pragma unroll
-            for (int c = 0; c < G::kHalfCopies; ++c) copy_to_lds(base, offset[c], to + c * 1024);
-        } else {
+        for (int h = 0; h < 2; ++h) {
+            const bool none = s[h].hi <= s[h].lo;
+            const char* base = uniform(
+                none ? nothing : pool + s[h].page * page_bytes + line_of(j0 + kHalf * h) * pitch);
+            uint32_t at[G::kHalfCopies];
 #pragma unroll
-            for (int c = 0; c < G::kHalfCopies; ++c) {
-                const int row = lane / G::kSlots + c * G::kStep;
-                const int near = min(max(row, s.lo), s.hi - 1);
-                copy_to_lds(base, none ? 0u : offset[c] + (near - row) * pitch, to + c * 1024);
+            for (int c = 0; c < G::kHalfCopies; ++c) at[c] = offset[c];
+            if (s[h].lo > 0 || s[h].hi < kHalf) {
+#pragma unroll
+                for (int c = 0; c < G::kHalfCopies; ++c) {
+                    const int row = lane / G::kSlots + c * G::kStep;
+                    const int near = min(max(row, s[h].lo), s[h].hi - 1);
+                    at[c] = none ? 0u : offset[c] + (near - row) * pitch;
+                }
             }
+#pragma unroll
+            for (int c = 0; c < G::kHalfCopies; ++c)
+                copy_to_lds(base, at[c], __builtin_amdgcn_readfirstlane(
+                                             to + (h * G::kHalfCopies + c) * 1024));
         }
     };
     auto fetch_k = [&](const Span (&s)[2], int j0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            fetch_half(s[h], pages.k, pages.k_page, j0 + kHalf * h,
-                       __builtin_amdgcn_readfirstlane(at_k + h * (uint32_t(G::kSize) / 2)));
+        const ArgsAgain g = args_again();
+        fetch(s, g->pages.k, g->pages.k_page, j0, at_k);
         if constexpr (kEight) {
             // lanes 0 .. 3 and 4 .. 7: four keys' scales each, of the two halves; 8 .. 15:
             // values'; the rest repeat them
-            const int h = (lane >> 2) & 1;
-            const Span mine = h ? s[1] : s[0];
-            const int64_t line = (static_cast<int64_t>(kv_head) << shift) +
-                                 ((j0 + kHalf * h) & page_mask) + 4 * (lane & 3);
-            const uint8_t* from = lane & 8 ? pages.v_scale + mine.page * pages.v_scale_page + line
-                                           : pages.k_scale + mine.page * pages.k_scale_page + line;
-            if (mine.page < 0) from = reinterpret_cast<const uint8_t*>(a.lens + b);
+            const int h = (lane >> 2) & 1, page = h ? s[1].page : s[0].page;
+            const int64_t line = line_of(j0 + kHalf * h) + 4 * (lane & 3);
+            const uint8_t* from = lane & 8 ? g->pages.v_scale + page * g->pages.v_scale_page + line
+                                           : g->pages.k_scale + page * g->pages.k_scale_page + line;
+            if (page < 0) from = reinterpret_cast<const uint8_t*>(g->lens + b);
             copy_far_word_to_lds(from, __builtin_amdgcn_readfirstlane(
                                            lds_address(s_scales) + wave * 256));
         }
-        if (a.k_times) {
-            const int h = (lane >> 4) & 1;
-            const Span mine = h ? s[1] : s[0];
-            const float* from = a.k_times + (static_cast<int64_t>(mine.page) << shift) +
+        if (timed) {
+            const int h = (lane >> 4) & 1, page = h ? s[1].page : s[0].page;
+            const float* from = g->k_times + (static_cast<int64_t>(page) << shift) +
                                 ((j0 + kHalf * h) & page_mask) + (lane & 15);
-            if (mine.page < 0) from = sc.q_times + b;
+            if (page < 0) from = g->score.q_times + b;
             copy_far_word_to_lds(
                 from, __builtin_amdgcn_readfirstlane(lds_address(s_times) + wave * 256));
         }
     };
     auto fetch_v = [&](const Span (&s)[2], int j0) {
+        const ArgsAgain g = args_again();
+        fetch(s, g->pages.v, g->pages.v_page, j0, at_v);
+    };
+    // The new row takes its place in the wave's tiles, and every place after it, and goes
+    // to its page.
+    auto put_new = [&](int from, int page, int at_lane) {
+        const ArgsAgain g = args_again();
+        const T* fresh_k = reinterpret_cast<const T*>(g->k.data) + static_cast<int64_t>(b) * g->k.row +
+                           kv_head * g->k.head;
+        const T* fresh_v = reinterpret_cast<const T*>(g->v.data) + static_cast<int64_t>(b) * g->v.row +
+                           kv_head * g->v.head;
+        const bool writes = col_group == 0 && page >= 0;
+        const int64_t line = line_of(n);
+        char* k_row = g->pages.k + page * g->pages.k_page + line * pitch;
+        char* v_row = g->pages.v + page * g->pages.v_page + line * pitch;
+        if constexpr (kEight) {
+            // eight codes in each lane, by its number in 16
+            const int at = at_lane & 15;
+            float k[8] = {}, v[8] = {}, k_top = 0.0f, v_top = 0.0f;
+            if (at * 8 < dim) {
+                load8(fresh_k + at * 8, k);
+                load8(fresh_v + at * 8, v);
+            }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            fetch_half(s[h], pages.v, pages.v_page, j0 + kHalf * h,
-                       __builtin_amdgcn_readfirstlane(at_v + h * (uint32_t(G::kSize) / 2)));
+            for (int e = 0; e < 8; ++e) {
+                k_top = fmaxf(k_top, size_of(k[e]));
+                v_top = fmaxf(v_top, size_of(v[e]));
+            }
+            const int byte_k = scale_byte(group_max<16>(k_top));
+            const int byte_v = scale_byte(group_max<16>(v_top));
+            const u32x2 codes_k = eight_codes(k, inverse_power(byte_k));
+            const u32x2 codes_v = eight_codes(v, inverse_power(byte_v));
+            for (int row = from + (at_lane >> 4); row < kKeys; row += 4) {
+                if (at < G::kSlots * 2) {
+                    const int byte = G::slot(row, at >> 1) * 16 + (at & 1) * 8;
+                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_k) + byte) = codes_k;
+                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_v) + byte) = codes_v;
+                }
+                uint8_t* scales = reinterpret_cast<uint8_t*>(s_scales[wave]);
+                scales[row] = byte_k;
+                scales[32 + row] = byte_v;
+            }
+            if (writes && at_lane * 8 < dim) {
+                *reinterpret_cast<u32x2*>(k_row + at_lane * 8) = codes_k;
+                *reinterpret_cast<u32x2*>(v_row + at_lane * 8) = codes_v;
+            }
+            if (writes && at_lane == 0) {
+                g->pages.k_scale[page * g->pages.k_scale_page + line] = byte_k;
+                g->pages.v_scale[page * g->pages.v_scale_page + line] = byte_v;
+            }
+        } else {
+            const u32x4* k_from = reinterpret_cast<const u32x4*>(fresh_k);
+            const u32x4* v_from = reinterpret_cast<const u32x4*>(fresh_v);
+            for (int c = from * G::kSlots + at_lane; c < kKeys * G::kSlots; c += 64) {
+                const int row = c / G::kSlots, chunk = c % G::kSlots;
+                const int at = chunk * G::kElems < dim ? chunk : 0;
+                s_k[G::slot(row, chunk)] = k_from[at];
+                s_v[G::slot(row, chunk)] = v_from[at];
+            }
+            if (writes && at_lane * G::kElems < dim) {
+                reinterpret_cast<u32x4*>(k_row)[at_lane] = k_from[at_lane];
+                reinterpret_cast<u32x4*>(v_row)[at_lane] = v_from[at_lane];
+            }
+        }
+        if (writes && timed && kv_head == 0 && at_lane == 0)
+            g->k_times[(static_cast<int64_t>(page) << shift) + (n & page_mask)] = q_time;
     };
 
-    int block = block_begin + wave, number = 0;
-    Span span[2];
-    if (block < block_end) {
-        fetch_ids(block);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) span[h] = span_of(0, h, block * kKeys);
-        fetch_k(span, block * kKeys);
-        fetch_v(span, block * kKeys);
-    }
+    // Each round works on a block and asks for the next; the first one only asks (so
+    // that the code is there once, which matters where a call is short).
+    int block = block_begin + wave - kWaves, number = -1;
+    if (block + kWaves < block_end) fetch_ids(block + kWaves);
+    Span span[2] = {};
+    int works = 0;
 #pragma unroll 1
-    for (; block < block_end; block += kWaves) {
+    for (;;) {
         const int j0 = block * kKeys, j1 = j0 + kWaves * kKeys;
         const bool more = block + kWaves < block_end;
         int at_lane = lane;  // LDS addresses are not held over the loop
         asm volatile("" : "+v"(at_lane));
-        // keys that count: those of the pages, and the new one
-        const uint32_t seen = bits_of(span[0].lo, span[0].hi) | bits_of(span[1].lo, span[1].hi) << 16 |
-                              (n - j0 < kKeys ? 1u << (n - j0) : 0u);
-        copies_landed<kCopies>();  // keys; the values, asked for last, may be on their way
-        if (seen != 0xffffffffu || n - j0 < kKeys) {
-            copies_landed<0>();
-            // Values of rows that are not seen meet a weight of 0: they may not be NaN.
+        uint32_t seen = 0;
+        uint32_t scales[2][2] = {};  // of keys and values: four bytes a half
+        float s[8] = {}, time[8] = {};
+        if (works) {
+            // keys that count: those of the pages, and the new one
+            const bool news = n - j0 < kKeys;
+            seen = bits_of(span[0].lo, span[0].hi) | bits_of(span[1].lo, span[1].hi) << 16 |
+                   (news ? 1u << (n - j0) : 0u);
+            copies_landed<kCopies>();  // keys; the values, asked for last, may be on their way
+            if (seen != 0xffffffffu || news) {
+                copies_landed<0>();
+                // Values of rows that are not seen meet a weight of 0: they may not be NaN.
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (span[h].hi <= span[h].lo)
-                    for (int c = at_lane; c < kHalf * G::kSlots; c += 64)
-                        s_v[h * kHalf * G::kSlots + c] = u32x4{0, 0, 0, 0};
-            if (n - j0 < kKeys) {  // the new row, from its place on
-                const int from = n - j0;
-                if constexpr (kEight) {
-                    encode();
-                    const int at = at_lane & 15;
-                    for (int row = from + (at_lane >> 4); row < kKeys; row += 4) {
-                        if (at < G::kSlots * 2) {
-                            const int byte = G::slot(row, at >> 1) * 16 + (at & 1) * 8;
-                            *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_k) + byte) = codes_k;
-                            *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_v) + byte) = codes_v;
-                        }
-                        uint8_t* scales = reinterpret_cast<uint8_t*>(s_scales[wave]);
-                        scales[row] = byte_k;
-                        scales[32 + row] = byte_v;
-                    }
-                } else {
-                    for (int c = from * G::kSlots + at_lane; c < kKeys * G::kSlots; c += 64) {
-                        const int row = c / G::kSlots, chunk = c % G::kSlots;
-                        const int at = chunk * G::kElems < a.dim ? chunk : 0;
-                        s_k[G::slot(row, chunk)] = reinterpret_cast<const u32x4*>(fresh_k)[at];
-                        s_v[G::slot(row, chunk)] = reinterpret_cast<const u32x4*>(fresh_v)[at];
-                    }
+                for (int h = 0; h < 2; ++h)
+                    if (span[h].hi <= span[h].lo)
+                        for (int c = at_lane; c < kHalf * G::kSlots; c += 64)
+                            s_v[h * kHalf * G::kSlots + c] = u32x4{0, 0, 0, 0};
+                if (news) {
+                    const int page = n - j0 < kHalf ? span[0].page : span[1].page;
+                    put_new(n - j0, page, at_lane);
+                    if (page < 0) l = NAN;  // no page for the new event: no answer
                 }
             }
-        }
-        f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int st = 0; st < DB; ++st)
+            for (int st = 0; st < DB; ++st)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const F k = In::row(s_k, kHalf * h + (at_lane & 15), st, at_lane >> 4);
+                for (int h = 0; h < 2; ++h) {
+                    const F k = In::row(s_k, kHalf * h + (at_lane & 15), st, at_lane >> 4);
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) x[h] = mma16(k, q[st][p], x[h]);
+                    for (int p = 0; p < kParts; ++p) x[h] = mma16(k, q[st][p], x[h]);
+                }
+            if constexpr (kEight) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    scales[0][h] = s_scales[wave][4 * h + (at_lane >> 4)];
+                    scales[1][h] = s_scales[wave][8 + 4 * h + (at_lane >> 4)];
+                }
             }
-        uint32_t scales[2][2];  // of keys and values: four bytes a half
-        if constexpr (kEight) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                scales[0][h] = s_scales[wave][4 * h + (at_lane >> 4)];
-                scales[1][h] = s_scales[wave][8 + 4 * h + (at_lane >> 4)];
+            for (int r = 0; r < 8; ++r) {
+                s[r] = x[r >> 2][r & 3];
+                if constexpr (kEight) s[r] *= power_of((scales[0][r >> 2] >> (8 * (r & 3))) & 255);
             }
-        }
-        float s[8];
+            if (timed) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            float product = x[r >> 2][r & 3];
-            if constexpr (kEight) product *= power_of((scales[0][r >> 2] >> (8 * (r & 3))) & 255);
-            float unused;
-            s[r] = sc.softcap > 0 ? capped<T, kWide>(sc, product, unused) : product * sc.scale2;
+                for (int r = 0; r < 8; ++r)
+                    time[r] = s_times[wave][kHalf * (r >> 2) + 4 * (at_lane >> 4) + (r & 3)];
+            }
+            reads_done();  // so the next keys may come
         }
-        float time[8];
-        if (a.k_times) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                time[r] = s_times[wave][kHalf * (r >> 2) + 4 * (at_lane >> 4) + (r & 3)];
-        }
-        reads_done();
         if (more) {
             number = (number + 1) & 63;
-            if (number == 0) fetch_ids(block + kWaves);
+            if (number == 0 && works) fetch_ids(block + kWaves);
 #pragma unroll
             for (int h = 0; h < 2; ++h) span[h] = span_of(number, h, j1);
             fetch_k(span, j1);
         }
-        // distances from the new event of register r's key: last_d - at(r)
-        const int last_d = n - j0 - 4 * quarter;
-        auto at = [](int r) { return kHalf * (r >> 2) + (r & 3); };
-        if (sc.table) {
-            if (n - (j0 + kKeys - 1) >= sc.reach) {
+        if (works) {
+            if (softcap > 0) {
+                const ArgsAgain g = args_again();
+                Score sc;
+                sc.cap_in = g->score.cap_in;
+                sc.cap_out = g->score.cap_out;
+                sc.scale = g->score.scale;
+                sc.scale2 = scale2;
+                sc.softcap = softcap;
+                float unused;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) s[r] += far_bias;
-            } else if (any) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int d = min(max(last_d - at(r), 0), sc.reach);
-                    s[r] += table_entry(sc, head, d + sc.reach);
-                }
-            }
-        }
-        if (sc.slopes) {
-            if (a.k_times) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    // the new event's own time is not in the pages yet: it is 0 away
-                    const float gap = q_time - time[r];
-                    s[r] = fmaf(-slope, last_d == at(r) ? 0.0f : fabsf(gap), s[r]);
-                }
+                for (int r = 0; r < 8; ++r) s[r] = capped<T, kWide>(sc, s[r], unused);
             } else {
-                const float from = static_cast<float>(last_d);
 #pragma unroll
-                for (int r = 0; r < 8; ++r) s[r] = fmaf(-slope, fabsf(from - at(r)), s[r]);
+                for (int r = 0; r < 8; ++r) s[r] *= scale2;
             }
-        }
-        const uint32_t mine = seen >> (4 * quarter);
-        if (seen != 0xffffffffu) {
+            // distances from the new event of register r's key: last_d - at(r)
+            const int last_d = n - j0 - 4 * quarter;
+            auto at = [](int r) { return kHalf * (r >> 2) + (r & 3); };
+            if (biased) {
+                const ArgsAgain g = args_again();
+                Score sc;
+                sc.table = g->score.table;
+                sc.buckets = g->score.buckets;
+                sc.num_buckets = g->score.num_buckets;
+                sc.reach = g->score.reach;
+                if (n - (j0 + kKeys - 1) >= sc.reach) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (!(mine >> at(r) & 1)) s[r] = -INFINITY;
-        }
-        float top = s[0];
+                    for (int r = 0; r < 8; ++r) s[r] += far_bias;
+                } else if (any) {
 #pragma unroll
-        for (int r = 1; r < 8; ++r) top = fmaxf(top, s[r]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > m)) {
-            const float grown = fmaxf(m, top);
-            const float by = exp2_fast(m - grown);
-            m = grown;
-            l *= by;
+                    for (int r = 0; r < 8; ++r) {
+                        const int d = min(max(last_d - at(r), 0), sc.reach);
+                        s[r] += table_entry(sc, head, d + sc.reach);
+                    }
+                }
+            }
+            if (sloped) {
+                if (timed) {
 #pragma unroll
-            for (int c = 0; c < 2 * DB; ++c)
+                    for (int r = 0; r < 8; ++r) {
+                        // the new event's own time is not in the pages yet: it is 0 away
+                        const float gap = q_time - time[r];
+                        s[r] = fmaf(-slope, last_d == at(r) ? 0.0f : fabsf(gap), s[r]);
+                    }
+                } else {
+                    const float from = static_cast<float>(last_d);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[c][r] *= by;
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            s[r] = exp2_fast(s[r] - m);
-            l += s[r];
-        }
-        if constexpr (kEight) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                s[r] *= power_of((scales[1][r >> 2] >> (8 * (r & 3))) & 255);
-            if (seen != 0xffffffffu) {  // whatever is in the place of a scale
+                    for (int r = 0; r < 8; ++r) s[r] = fmaf(-slope, fabsf(from - at(r)), s[r]);
+                }
+            }
+            const uint32_t mine = seen >> (4 * quarter);
+            if (seen != 0xffffffffu) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
-                    if (!(mine >> at(r) & 1)) s[r] = 0.0f;
+                    if (!(mine >> at(r) & 1)) s[r] = -INFINITY;
             }
-        }
-        F p[kParts];
-        in_parts<kParts>(s, p);
-        if (more) copies_landed<kCopies>();  // values; the next keys may be on their way
-        else copies_landed<0>();
+            float top = s[0];
 #pragma unroll
-        for (int c = 0; c < 2 * DB; ++c) {
-            const F v = In::columns(s_v, c, at_lane);
+            for (int r = 1; r < 8; ++r) top = fmaxf(top, s[r]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m)) {
+                const float grown = fmaxf(m, top);
+                const float by = exp2_fast(m - grown);
+                m = grown;
+                l *= by;
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) o[c] = mma16(v, p[part], o[c]);
+                for (int c = 0; c < 2 * DB; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[c][r] *= by;
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                s[r] = exp2_fast(s[r] - m);
+                l += s[r];
+            }
+            if constexpr (kEight) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    s[r] *= power_of((scales[1][r >> 2] >> (8 * (r & 3))) & 255);
+                if (seen != 0xffffffffu) {  // whatever is in the place of a scale
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (!(mine >> at(r) & 1)) s[r] = 0.0f;
+                }
+            }
+            F p[kParts];
+            in_parts<kParts>(s, p);
+            if (more) copies_landed<kCopies>();  // values; the next keys may be on their way
+            else copies_landed<0>();
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) {
+                const F v = In::columns(s_v, c, at_lane);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) o[c] = mma16(v, p[part], o[c]);
+            }
+            reads_done();
         }
-        reads_done();
-        if (more) fetch_v(span, j1);
+        if (!more) break;
+        fetch_v(span, j1);
+        block += kWaves;
+        asm volatile("s_mov_b32 %0, 1" : "=s"(works));
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -632,7 +754,7 @@ void paged_step_kernel(PagedArgs a) {
                                   4 * quarter) = o[c];
     __syncthreads();
     const int columns = min(a.group - col_group * kColumns, kColumns);
-    const int pieces = a.dim / 4;
+    const int pieces = dim / 4;
     for (int i = thread; i < columns * pieces; i += kThreads) {
         const int jc = i / pieces, d = i % pieces * 4;
         float top = s_m[0][jc], total = 0.0f;
@@ -648,14 +770,13 @@ void paged_step_kernel(PagedArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, part[e], sum[e]);
         }
-        // no page for the new event: no answer
-        if (idle && at_n >= 0) total = NAN;
-        const int join_head = kv_head * a.group + col_group * kColumns + jc;
-        const int64_t part = (static_cast<int64_t>(b) * a.heads + join_head) * a.splits + split;
-        if (a.splits > 1) {
-            *reinterpret_cast<f32x4*>(a.partial + part * a.dim + d) = sum;
-            if (d == 0) a.part_stats[part] = make_float2(top, total);
+        if (idle && a.lens[b] >= 0) total = NAN;  // no room for the new event: no answer
+        if (from_unit > 0 || till_unit < units) {
+            const int64_t at = (static_cast<int64_t>(blockIdx.x) * 2 + part) * kColumns + jc;
+            *reinterpret_cast<f32x4*>(a.partial + at * dim + d) = sum;
+            if (d == 0) a.part_stats[at] = make_float2(top, total);
         } else {
+            const int join_head = kv_head * a.group + col_group * kColumns + jc;
             typedef T t4 __attribute__((ext_vector_type(4)));
             t4 out;
 #pragma unroll
@@ -664,28 +785,109 @@ void paged_step_kernel(PagedArgs a) {
             *reinterpret_cast<t4*>(row_of<T>(a.out, b, join_head) + d) = out;
         }
     }
+    if (!a.even) return;
+    left -= till_unit - from_unit;
+    unit = 0;
+    ++b;
+    __syncthreads();  // the join's room is the next part's tiles
+  }
 }
 
-// Workgroups of one walk and key head: each with at least four blocks a wave
-// where the table is full; few walks: 1536 workgroups in all, more: three each up
-// to 3072, which evens out their lengths.
-int splits_of(const trw_paged_step_params& p) {
+// Joins the parts of one walk and head that was cut: 32 threads for the elements, four
+// each, and eight shares of the parts.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedArgs a) {
+    __shared__ f32x4 s_sum[8][32];
+    __shared__ float s_total[8], s_top[4];
+    const int head = blockIdx.x % a.heads;
+    const int b = blockIdx.x / a.heads;
+    const int64_t begin = a.begins[b], end = a.begins[b + 1], all = a.begins[a.batch];
+    // the workgroup that has unit x: the last that begins at x or before
+    auto owner = [&](int64_t x) { return static_cast<int>(((x + 1) * a.even - 1) / all); };
+    const int first = owner(begin), parts = owner(end - 1) - first + 1;
+    if (parts == 1) return;
+    const int kv_head = head / a.group, col = head % a.group;
+    // The first workgroup's part is its last one, unless the walk begins it; the others'
+    // is their first one.
+    const int begun = all * first / a.even < begin;
+    auto part_of = [&](int s) {
+        const int item = first + s;
+        const int64_t block =
+            (static_cast<int64_t>(item / 8 * a.kv_heads + kv_head) * a.columns + col / kColumns) * 8 +
+            item % 8;
+        return (block * 2 + (s == 0 ? begun : 0)) * kColumns + col % kColumns;
+    };
+    const int thread = threadIdx.x, share = thread >> 5, d = (thread & 31) * 4;
+    float top = kFloor;
+    for (int s = thread; s < parts; s += kThreads) top = fmaxf(top, a.part_stats[part_of(s)].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((thread & 63) == 0) s_top[thread >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    float total = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+    // No branch inside, so that several parts' loads are in flight: threads past the
+    // head size read its last elements again and store nothing.
+    const int from = min(d, a.dim - 4);
+#pragma unroll 4
+    for (int s = share; s < parts; s += 8) {
+        const int64_t at = part_of(s);
+        const float2 st = a.part_stats[at];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.partial + at * a.dim + from);
+        const float by = exp2_fast(st.x - top);
+        total = fmaf(by, st.y, total);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, x[e], sum[e]);
+    }
+    s_sum[share][thread & 31] = sum;
+    if ((thread & 31) == 0) s_total[share] = total;
+    __syncthreads();
+    if (share || d >= a.dim) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+        total += s_total[w];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += s_sum[w][thread & 31][e];
+    }
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(total != 0.0f ? sum[e] / total : 0.0f);
+    *reinterpret_cast<t4*>(row_of<T>(a.out, b, head) + d) = out;
+}
+
+// Workgroups of a key head among which all walks are evened out; 0: one a walk.
+int even_of(const trw_paged_step_params& p, int resident) {
     const int group = p.heads / p.pages.kv_heads;
-    const int64_t items = p.pages.walks * p.pages.kv_heads * ((group + kColumns - 1) / kColumns);
-    const int64_t capacity = p.pages.table_pages * p.pages.page_rows;
-    const int64_t most = (capacity + 4 * kWaves * kKeys - 1) / (4 * kWaves * kKeys);
-    const int64_t n = std::max<int64_t>(items, 1);
-    const int64_t want = std::max((1536 + n - 1) / n, std::min<int64_t>(3, 3072 / n));
-    return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
+    const int64_t heads = int64_t{p.pages.kv_heads} * ((group + kColumns - 1) / kColumns);
+    const int64_t slots = 256 * resident;
+    if (p.pages.table_pages * p.pages.page_rows <= 4 * kUnit * kKeys) return 0;
+    if (p.pages.walks * heads >= 4 * slots) return 0;
+    return static_cast<int>(std::max<int64_t>(1, slots / heads));
+}
+int even_of(const trw_paged_step_params& p) {
+    int even = 0;
+    dispatch(p.dtype, p.pages.dim, [&](auto t, auto db) {
+        typedef decltype(t) T;
+        constexpr int DB = decltype(db)::value;
+        even = even_of(p, p.pages.dtype == TRW_E4M3 ? kResident<T, DB, true> : kResident<T, DB, false>);
+    });
+    return even;
+}
+int64_t grid_of(const trw_paged_step_params& p, int even) {
+    const int group = p.heads / p.pages.kv_heads;
+    const int columns = (group + kColumns - 1) / kColumns;
+    return xcd_grid(even ? even : p.pages.walks) * p.pages.kv_heads * columns;
 }
 
 }  // namespace
 
 uint64_t paged_step_workspace(const trw_paged_step_params& p) {
-    const int splits = splits_of(p);
-    if (splits == 1) return 0;
-    return static_cast<uint64_t>(p.pages.walks) * p.heads * splits * (p.pages.dim + 2) *
-           sizeof(float);
+    const int even = even_of(p);
+    if (!even) return 0;
+    return grid_of(p, even) * 2 * kColumns * (p.pages.dim + 2) * sizeof(float) +
+           (p.pages.walks + 1) * sizeof(int64_t);
 }
 
 void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
@@ -708,11 +910,12 @@ void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
     a.group = p.heads / p.pages.kv_heads;
     a.columns = (a.group + kColumns - 1) / kColumns;
     a.dim = p.pages.dim;
-    a.splits = splits_of(p);
-    a.partial = static_cast<float*>(p.workspace);
-    a.part_stats = reinterpret_cast<float2*>(a.partial + batch * p.heads * a.splits * a.dim);
-    const int64_t grid = xcd_grid(batch * a.splits) * a.kv_heads * a.columns;
+    a.even = even_of(p);
+    const int64_t grid = grid_of(p, a.even);
     require_grid(grid, kThreads);
+    a.partial = static_cast<float*>(p.workspace);
+    a.part_stats = reinterpret_cast<float2*>(a.partial + grid * 2 * kColumns * a.dim);
+    a.begins = reinterpret_cast<int64_t*>(a.part_stats + grid * 2 * kColumns);
     dispatch(p.dtype, a.dim, [&](auto t, auto db) {
         typedef decltype(t) T;
         by_cap<T>(p.dtype, p.score, [&](auto wide) {
@@ -726,10 +929,9 @@ void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
                                    dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
         });
         check_launch("paged_attention_step");
-        if (a.splits > 1) {
-            const StepJoin join{a.partial, a.part_stats, a.out, nullptr, 0, a.heads, a.dim, a.splits};
-            hipLaunchKernelGGL((join_step_kernel<T>), dim3(static_cast<unsigned>(batch * a.heads)),
-                               dim3(kJoinThreads), 0, stream, join);
+        if (a.even) {
+            hipLaunchKernelGGL((join_parts_kernel<T>), dim3(static_cast<unsigned>(batch * a.heads)),
+                               dim3(kThreads), 0, stream, a);
             check_launch("paged_attention_step");
         }
     });

@@ -16,7 +16,6 @@
 #include <algorithm>
 
 #include "operators.h"
-#include "step_join.h"
 
 namespace trw {
 namespace ops {
@@ -298,6 +297,60 @@ void attention_step_kernel(StepArgs a) {
         a.part_stats[part] = make_float2(top, total);
 }
 
+// Joins the workgroups of one walk and head: 32 threads for the elements, four
+// each, and eight shares of the workgroups.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_step_kernel(StepArgs a) {
+    __shared__ f32x4 s_sum[8][32];
+    __shared__ float s_total[8], s_top[4];
+    const int head = blockIdx.x % a.heads;
+    const int b = blockIdx.x / a.heads;
+    const int thread = threadIdx.x, share = thread >> 5, d = (thread & 31) * 4;
+    const int64_t part = (static_cast<int64_t>(b) * a.heads + head) * a.splits;
+    float top = kFloor;
+    for (int s = thread; s < a.splits; s += kThreads) top = fmaxf(top, a.part_stats[part + s].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((thread & 63) == 0) s_top[thread >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    float total = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+    // No branch inside, so that eight workgroups' loads are in flight (128 of them:
+    // 4.8 us, 9.4 with a branch): threads past the head size read its last elements
+    // again and store nothing.
+    const float* from = a.partial + part * a.dim + min(d, a.dim - 4);
+#pragma unroll 8
+    for (int s = share; s < a.splits; s += 8) {
+        const float2 st = a.part_stats[part + s];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(s) * a.dim);
+        const float by = exp2_fast(st.x - top);
+        total = fmaf(by, st.y, total);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, x[e], sum[e]);
+    }
+    s_sum[share][thread & 31] = sum;
+    if ((thread & 31) == 0) s_total[share] = total;
+    __syncthreads();
+    if (share || d >= a.dim) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+        total += s_total[w];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += s_sum[w][thread & 31][e];
+    }
+    const int64_t n = a.lens[b];
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        out[e] = static_cast<T>(n < 0              ? 0.0f
+                                : n >= a.capacity  ? NAN
+                                : total != 0.0f    ? sum[e] / total
+                                                   : 0.0f);
+    *reinterpret_cast<t4*>(row_of<T>(a.out, b, head) + d) = out;
+}
+
 // Workgroups of one walk and key head: each with at least four blocks a wave
 // where the cache is full.  Few walks: 1536 in all (768 where heads are large and
 // fewer fit), two or three times what the compute units hold, and no more, since
@@ -363,12 +416,9 @@ void attention_step(const trw_attention_step_params& p, hipStream_t stream) {
                 dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
         });
         check_launch("attention_step");
-        if (a.splits > 1) {
-            const StepJoin join{a.partial, a.part_stats, a.out,  a.lens,
-                                a.capacity, a.heads,    a.dim, a.splits};
+        if (a.splits > 1)
             hipLaunchKernelGGL((join_step_kernel<T>), dim3(static_cast<unsigned>(a.batch * a.heads)),
-                               dim3(kJoinThreads), 0, stream, join);
-        }
+                               dim3(kThreads), 0, stream, a);
         check_launch("attention_step");
     });
 }

@@ -640,86 +640,137 @@ bool fused(const trw_beam_select_params& p) { return p.beams * chunks_of(p) <= k
 // ---- reordering ----------------------------------------------------------------------------------
 constexpr int kCaches = 8;  // of one launch
 
-struct Cache {
-    char *k, *v;
-    uint8_t *k_scale, *v_scale;
-    int64_t k_page, v_page, k_scale_page, v_scale_page;
+struct Matrix {  // keys or values of one cache
+    char* data;
+    uint8_t* scale;  // or null
+    int64_t page, scale_page;
     int row_bytes, heads;
 };
 struct ReorderArgs {
-    Cache caches[kCaches];
+    Matrix matrix[2 * kCaches];
     const int32_t* table;
     int64_t table_stride;
     int32_t* out_table;
     const int64_t *lens, *parents;
     int64_t* out_lens;
     float* k_times;
-    int beams, table_pages, pages, shift, count, first;
+    int beams, table_pages, pages, shift, first, matrices, heads, share;
 };
 
-__device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes, int thread) {
-    for (int at = thread * 16; at < bytes; at += kThreads * 16)
-        *reinterpret_cast<u32x4*>(to + at) = *reinterpret_cast<const u32x4*>(from + at);
-}
-
-// One child of a group, and (grid y) one head of one cache; y = 0 writes the table too.
+// `share` workgroups a group.  Every wave works out the group's plan, a child a lane;
+// the rows that move, of every head of every cache's keys and values, are then dealt
+// out to the workgroups piece by piece, which evens out how many children a group's
+// parents have.
 __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
-    const int child = blockIdx.x % a.beams;
-    const int64_t group = static_cast<int64_t>(blockIdx.x / a.beams) * a.beams;
+    const int part = blockIdx.x % a.share;
+    const int64_t group = static_cast<int64_t>(blockIdx.x / a.share) * a.beams;
     const int thread = threadIdx.x, lane = thread & 63;
-    int parent_of = -1;  // this lane's child's
+    int parent = -1;
+    int64_t len = 0;  // of this lane's beam, then of its child
     if (lane < a.beams) {
         const int64_t p = a.parents[group + lane];
-        parent_of = static_cast<int>(min(max(p, int64_t{0}), static_cast<int64_t>(a.beams - 1)));
+        len = a.lens[group + lane];
+        parent = static_cast<int>(min(max(p, int64_t{0}), static_cast<int64_t>(a.beams - 1)));
     }
     // beams without children, and children that are not their parent's first
     uint32_t childless = 0, further = 0;
     for (int b = 0; b < a.beams; ++b) {
-        const uint32_t children = static_cast<uint32_t>(__ballot(parent_of == b));
+        const uint32_t children = static_cast<uint32_t>(__ballot(parent == b));
         if (!children) childless |= 1u << b;
         further |= children & (children - 1);
     }
-    const int parent = __builtin_amdgcn_readlane(parent_of, child);
-    const bool moves = further >> child & 1;
-    int taken = parent;
-    if (moves) {  // as many beams are without children as children are further ones
-        uint32_t left = childless;
-        for (int n = __popc(further & ((1u << child) - 1)); n; --n) left &= left - 1;
-        taken = __ffs(left) - 1;
-    }
-    const int64_t len = a.lens[group + parent];
-    const int64_t full = len > 0 ? len >> a.shift : 0;
-    const int32_t* from = a.table + (group + parent) * a.table_stride;
-    const int32_t* rest = a.table + (group + taken) * a.table_stride;
-    if (blockIdx.y == 0 && a.first) {
-        int32_t* to = a.out_table + (group + child) * a.table_pages;
-        for (int p = thread; p < a.table_pages; p += kThreads) to[p] = p < full ? from[p] : rest[p];
-        if (thread == 0) a.out_lens[group + child] = len;
-    }
+    len = __shfl(len, max(parent, 0));
+    const int full = len > 0 ? static_cast<int>(min(len >> a.shift, static_cast<int64_t>(a.table_pages)))
+                             : 0;
     const int rows = len > 0 ? static_cast<int>(len & ((1 << a.shift) - 1)) : 0;
-    if (!moves || !rows || full >= a.table_pages) return;
-    const int source = from[full], target = rest[full];
-    if (source < 0 || source >= a.pages || target < 0 || target >= a.pages || source == target) return;
-    if (blockIdx.y == 0 && a.first && a.k_times)
-        for (int r = thread; r < rows; r += kThreads)
-            a.k_times[(static_cast<int64_t>(target) << a.shift) + r] =
-                a.k_times[(static_cast<int64_t>(source) << a.shift) + r];
-    int head = blockIdx.y, c = 0;
-    while (c < a.count && head >= a.caches[c].heads) head -= a.caches[c++].heads;
-    if (c == a.count) return;
-    const Cache& cache = a.caches[c];
-    const int64_t line = static_cast<int64_t>(head) << a.shift;
-    const int bytes = rows * cache.row_bytes;
-    copy_bytes(cache.k + target * cache.k_page + line * cache.row_bytes,
-               cache.k + source * cache.k_page + line * cache.row_bytes, bytes, thread);
-    copy_bytes(cache.v + target * cache.v_page + line * cache.row_bytes,
-               cache.v + source * cache.v_page + line * cache.row_bytes, bytes, thread);
-    if (cache.k_scale)
-        for (int r = thread; r < rows; r += kThreads) {
-            cache.k_scale[target * cache.k_scale_page + line + r] =
-                cache.k_scale[source * cache.k_scale_page + line + r];
-            cache.v_scale[target * cache.v_scale_page + line + r] =
-                cache.v_scale[source * cache.v_scale_page + line + r];
+    int taken = parent, source = -1, target = -1;
+    if (lane < a.beams && further >> lane & 1) {
+        // as many beams are without children as children are further ones
+        uint32_t left = childless;
+        for (int n = __popc(further & ((1u << lane) - 1)); n; --n) left &= left - 1;
+        taken = __ffs(left) - 1;
+        if (rows && full < a.table_pages) {
+            source = a.table[(group + parent) * a.table_stride + full];
+            target = a.table[(group + taken) * a.table_stride + full];
+        }
+    }
+    // what moves: between pages of the pool
+    const u64 moving = __ballot(source >= 0 && source < a.pages && target >= 0 && target < a.pages &&
+                                source != target);
+
+    if (a.first) {
+        for (int child = part; child < a.beams; child += a.share) {
+            const int whole = __builtin_amdgcn_readlane(full, child);
+            const int32_t* from =
+                a.table + (group + __builtin_amdgcn_readlane(parent, child)) * a.table_stride;
+            const int32_t* rest =
+                a.table + (group + __builtin_amdgcn_readlane(taken, child)) * a.table_stride;
+            int32_t* to = a.out_table + (group + child) * a.table_pages;
+            for (int p = thread; p < a.table_pages; p += kThreads)
+                to[p] = p < whole ? from[p] : rest[p];
+        }
+        if (part == 0 && thread < a.beams) a.out_lens[group + thread] = len;
+    }
+
+    const int each = a.matrices * a.heads, items = __popcll(moving) * each;
+    constexpr int kAtOnce = 4;
+    for (int i0 = part; i0 < items; i0 += kAtOnce * a.share) {
+        const char* read[kAtOnce];
+        char* write[kAtOnce];
+        const uint8_t* read_scale[kAtOnce];
+        uint8_t* write_scale[kAtOnce];
+        u32x4 data[kAtOnce];
+        uint8_t scale[kAtOnce];
+        int pieces[kAtOnce], scales[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {  // all on their way at once
+            const int item = i0 + i * a.share;
+            pieces[i] = scales[i] = 0;
+            if (item >= items) continue;
+            u64 left = moving;
+            for (int n = item / each; n; --n) left &= left - 1;
+            const int child = __ffsll(left) - 1, head = item % each % a.heads;
+            const Matrix& x = a.matrix[item % each / a.heads];
+            if (head >= x.heads) continue;
+            const int from = __builtin_amdgcn_readlane(source, child);
+            const int to = __builtin_amdgcn_readlane(target, child);
+            const int count = __builtin_amdgcn_readlane(rows, child);
+            const int64_t line = static_cast<int64_t>(head) << a.shift;
+            read[i] = x.data + from * x.page + line * x.row_bytes;
+            write[i] = x.data + to * x.page + line * x.row_bytes;
+            pieces[i] = count * x.row_bytes / 16;
+            if (thread < pieces[i]) data[i] = reinterpret_cast<const u32x4*>(read[i])[thread];
+            if (x.scale) {
+                read_scale[i] = x.scale + from * x.scale_page + line;
+                write_scale[i] = x.scale + to * x.scale_page + line;
+                scales[i] = count;
+                if (thread < count) scale[i] = read_scale[i][thread];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (thread < pieces[i]) reinterpret_cast<u32x4*>(write[i])[thread] = data[i];
+            if (thread < scales[i]) write_scale[i][thread] = scale[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {  // what is more than a thread's piece
+#pragma unroll 4
+            for (int n = thread + kThreads; n < pieces[i]; n += kThreads)
+                reinterpret_cast<u32x4*>(write[i])[n] = reinterpret_cast<const u32x4*>(read[i])[n];
+            for (int n = thread + kThreads; n < scales[i]; n += kThreads)
+                write_scale[i][n] = read_scale[i][n];
+        }
+    }
+    if (a.first && a.k_times)
+        for (int n = part; n < __popcll(moving); n += a.share) {
+            u64 left = moving;
+            for (int i = n; i; --i) left &= left - 1;
+            const int child = __ffsll(left) - 1;
+            const int64_t from = __builtin_amdgcn_readlane(source, child);
+            const int64_t to = __builtin_amdgcn_readlane(target, child);
+            const int count = __builtin_amdgcn_readlane(rows, child);
+            for (int r = thread; r < count; r += kThreads)
+                a.k_times[(to << a.shift) + r] = a.k_times[(from << a.shift) + r];
         }
 }
 
@@ -788,26 +839,32 @@ void beam_reorder(const trw_beam_reorder_params& p, hipStream_t stream) {
     a.pages = static_cast<int>(p.pages);
     a.shift = 0;
     while ((1 << a.shift) < p.page_rows) ++a.shift;
-    const int64_t rows = p.groups * p.beams;
     int done = 0;
     do {
-        a.count = std::min(kCaches, p.count - done);
+        const int count = std::min(kCaches, p.count - done);
         a.first = done == 0;
-        int heads = 0;
-        for (int c = 0; c < a.count; ++c) {
+        int heads = 1;
+        for (int c = 0; c < count; ++c) {
             const trw_pages& from = p.caches[done + c];
             const Pages pages = make_pages(from);
-            a.caches[c] = Cache{pages.k, pages.v, pages.k_scale, pages.v_scale, pages.k_page,
-                                pages.v_page, pages.k_scale_page, pages.v_scale_page,
-                                static_cast<int>(from.dim * page_element_size(from.dtype)),
-                                from.kv_heads};
-            heads += from.kv_heads;
+            const int row_bytes = static_cast<int>(from.dim * page_element_size(from.dtype));
+            a.matrix[2 * c] = Matrix{pages.k,      pages.k_scale, pages.k_page, pages.k_scale_page,
+                                  row_bytes, from.kv_heads};
+            a.matrix[2 * c + 1] = Matrix{pages.v,      pages.v_scale, pages.v_page, pages.v_scale_page,
+                                      row_bytes, from.kv_heads};
+            heads = std::max(heads, from.kv_heads);
         }
-        require_grid(rows * std::max(heads, 1), kThreads);
-        hipLaunchKernelGGL(reorder_kernel, dim3(static_cast<unsigned>(rows), std::max(heads, 1)),
+        // As many workgroups as the device holds at once: 32 groups of 8 beams, 4 caches of
+        // 8 heads, 46 MB: TIMES
+        a.matrices = 2 * count;
+        a.heads = heads;
+        const int64_t most = static_cast<int64_t>(std::max(1, p.beams - 1)) * a.matrices * heads;
+        a.share = static_cast<int>(std::min(most, std::max<int64_t>(1, 2048 / p.groups)));
+        require_grid(p.groups * a.share, kThreads);
+        hipLaunchKernelGGL(reorder_kernel, dim3(static_cast<unsigned>(p.groups * a.share)),
                            dim3(kThreads), 0, stream, a);
         check_launch("beam_reorder");
-        done += a.count;
+        done += count;
     } while (done < p.count);
 }
 

@@ -424,7 +424,7 @@ trw_status trw_ops_beam_reorder(const trw_beam_reorder_params* params, void* str
         const trw_beam_reorder_params& p = *params;
         require(p.beams >= 1 && p.beams <= TRW_OPS_BEAMS, "beams must be 1 to 32");
         require(p.groups >= 0 && p.groups < kMaxRows / p.beams, "groups must be 0 to 2^30 / beams");
-        require(p.count >= 0 && (p.count == 0 || p.caches), "caches is null");
+        require(p.count >= 1 && p.caches, "pages of at least one cache are needed");
         trw_pages shared{TRW_F32, 1, 8, p.page_rows};  // the table's own checks
         shared.table = p.table;
         shared.table_stride = p.table_stride;
