@@ -22,9 +22,13 @@
 //
 // 8 bits: codes are exact in bfloat16, and the products are bfloat16's whatever
 // the type of q.  Keys' scales multiply scores and values' scales the softmax's
-// weights, in float32 and exactly (they are powers of two).  q and the weights of
-// longer types go as two (float16) or three (float32) bfloat16 parts, which lose
-// nothing of q and 2^-16 and 2^-24 of a weight.
+// weights, in float32 and exactly (they are powers of two).  q of longer types goes
+// as two (float16) or three (float32) bfloat16 parts, which lose nothing.
+//
+// The softmax's weights go as two bfloat16 parts as well, or three where q is
+// float32, so that nothing but the output is rounded as far as bfloat16 is (one part:
+// outputs up to 1.75 times as far from exact ones; it costs no time that is seen, the
+// kernel waits for memory).  Pages of float16 take float16 weights.
 //
 // The new row is taken from the call's arguments by the workgroup whose positions
 // include it (in 8 bits as the codes that the pages get), and written to the pages
@@ -261,6 +265,42 @@ __device__ __forceinline__ void reads_done() {
     asm volatile("" ::: "memory");
 }
 
+// How `all` units are dealt out to `many` workgroups: the first ones get one more.
+struct Share {
+    int64_t each, more;
+    __device__ __forceinline__ Share(int64_t all, int many) {
+        if (all < (int64_t{1} << 31)) {  // a division of 32 bits
+            each = static_cast<uint32_t>(all) / static_cast<uint32_t>(many);
+        } else {
+            each = all / many;
+        }
+        more = all - each * many;
+    }
+    __device__ __forceinline__ int64_t begin(int item) const {
+        return item * each + min(static_cast<int64_t>(item), more);
+    }
+    // Who has unit x.
+    __device__ __forceinline__ int owner(int64_t x) const {
+        const int64_t big = more * (each + 1);
+        return static_cast<int>(x < big ? x / (each + 1) : more + (x - big) / each);
+    }
+};
+
+// Sums of the lanes up to each: by shifts inside rows of 16, then the rows' sums.
+template <int kMove, int kRows>
+__device__ __forceinline__ int moved(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, kMove, kRows, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);
+    x += moved<0x143, 0xc>(x);
+    return x;
+}
+
 // The kernel's arguments once more, from memory: what is not needed all the time is not
 // held in registers all the time (held, the arguments took more scalar registers than
 // there are, and some 700 moves between them and vector registers).
@@ -289,7 +329,9 @@ void paged_step_kernel(PagedArgs a) {
     typedef typename In::G G;
     typedef typename In::F F;
     constexpr int kBytes = kEight ? 1 : sizeof(T);
-    constexpr int kParts = !kEight ? 1 : sizeof(T) == 4 ? 3 : std::is_same<T, __bf16>::value ? 1 : 2;
+    constexpr bool kShort = std::is_same<T, __bf16>::value;
+    constexpr int kParts = !kEight || kShort ? 1 : sizeof(T) == 4 ? 3 : 2;  // of q
+    constexpr int kWeights = kShort ? 2 : kParts;  // parts of a weight
     constexpr int kJoinPitch = 32 * DB + 4;
     constexpr size_t kJoinBytes = size_t(kWaves) * kColumns * kJoinPitch * sizeof(float);
     constexpr size_t kTileBytes = 2 * kWaves * G::kSize;
@@ -330,52 +372,77 @@ void paged_step_kernel(PagedArgs a) {
     // Units [unit, unit + left) of this workgroup, counted from walk b's first.
     int b = item;
     int64_t unit = 0, left = INT64_MAX;
+    const bool few = a.even && a.batch <= 64;  // a walk a lane
+    Length mine{};
     if (a.even) {
         if (item >= a.even) return;
-        // each thread some walks one after the other
-        const int each = (a.batch + kThreads - 1) / kThreads;
-        const int walk = min(thread * each, a.batch), end = min(walk + each, a.batch);
-        int64_t mine = 0;
-        for (int w = walk; w < end; ++w) mine += length_of(a, w).units;
-        int64_t before = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t other = __shfl_up(static_cast<long long>(before), o);
-            if (lane >= o) before += other;
-        }
-        if (lane == 63) s_sums[wave] = before;
-        __syncthreads();
-        int64_t all = 0;
-        before -= mine;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) before += s_sums[w];
-            all += s_sums[w];
-        }
-        const int64_t begin = all * item / a.even, stop = all * (item + 1) / a.even;
         const bool notes = item == 0 && kv_head == 0 && col_group == 0;
-        if (notes && thread == 0) a.begins[a.batch] = all;
-        for (int w = walk; w < end; ++w) {
-            const int units = length_of(a, w).units;
-            if (notes) a.begins[w] = before;
-            if (before <= begin && begin < before + units) {
-                s_walk = w;
-                s_start = begin - before;
+        if (few) {
+            if (lane < a.batch) mine = length_of(a, lane);
+            const int till = wave_scan(mine.units);
+            const int all = __builtin_amdgcn_readlane(till, 63);
+            const Share share(all, a.even);
+            const int begin = static_cast<int>(share.begin(item));
+            left = share.begin(item + 1) - begin;
+            if (notes && thread < a.batch) a.begins[thread] = till - mine.units;
+            if (notes && thread == 0) a.begins[a.batch] = all;
+            if (left <= 0) return;
+            b = __popcll(__ballot(till <= begin));
+            unit = begin - __builtin_amdgcn_readlane(till - mine.units, b);
+        } else {
+            // each thread some walks one after the other
+            const int each = (a.batch + kThreads - 1) / kThreads;
+            const int walk = min(thread * each, a.batch), end = min(walk + each, a.batch);
+            int64_t sum = 0;
+            for (int w = walk; w < end; ++w) sum += length_of(a, w).units;
+            int64_t before = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t other = __shfl_up(static_cast<long long>(before), o);
+                if (lane >= o) before += other;
             }
-            before += units;
+            if (lane == 63) s_sums[wave] = before;
+            __syncthreads();
+            int64_t all = 0;
+            before -= sum;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if (w < wave) before += s_sums[w];
+                all += s_sums[w];
+            }
+            const Share share(all, a.even);
+            const int64_t begin = share.begin(item);
+            left = share.begin(item + 1) - begin;
+            if (notes && thread == 0) a.begins[a.batch] = all;
+            for (int w = walk; w < end; ++w) {
+                const int units = length_of(a, w).units;
+                if (notes) a.begins[w] = before;
+                if (before <= begin && begin < before + units) {
+                    s_walk = w;
+                    s_start = begin - before;
+                }
+                before += units;
+            }
+            if (left <= 0) return;
+            __syncthreads();
+            b = s_walk;
+            unit = s_start;
         }
-        if (begin >= stop) return;
-        __syncthreads();
-        b = s_walk;
-        unit = s_start;
-        left = stop - begin;
     } else if (item >= a.batch) {
         return;
     }
     b = __builtin_amdgcn_readfirstlane(b);
 
   for (int part = 0; left > 0; part = 1) {
-    const Length length = length_of(a, b);
+    Length length;
+    if (few) {
+        length.n = __builtin_amdgcn_readlane(mine.n, b);
+        length.first = __builtin_amdgcn_readlane(mine.first, b);
+        length.units = __builtin_amdgcn_readlane(mine.units, b);
+        length.in = __builtin_amdgcn_readlane(mine.in, b);
+    } else {
+        length = length_of(a, b);
+    }
     const int n = __builtin_amdgcn_readfirstlane(length.n);
     const int first = __builtin_amdgcn_readfirstlane(length.first);
     const int units = __builtin_amdgcn_readfirstlane(length.units);
@@ -390,17 +457,6 @@ void paged_step_kernel(PagedArgs a) {
     const int block_begin = first_block + from_unit * kUnit;
     const int block_end = min(last_block, first_block + till_unit * kUnit);
 
-    F q[DB][kParts];
-    {
-        const T* row = row_of<const T>(a.q, b, any ? head : 0);
-#pragma unroll
-        for (int st = 0; st < DB; ++st) {
-            const int at = 32 * st + 8 * quarter;
-            float x[8] = {};
-            if (any && at < dim) load8(row + at, x);
-            in_parts<kParts>(x, q[st]);
-        }
-    }
     f32x4 o[2 * DB];
 #pragma unroll
     for (int c = 0; c < 2 * DB; ++c) o[c] = f32x4{0, 0, 0, 0};
@@ -568,6 +624,17 @@ void paged_step_kernel(PagedArgs a) {
     // that the code is there once, which matters where a call is short).
     int block = block_begin + wave - kWaves, number = -1;
     if (block + kWaves < block_end) fetch_ids(block + kWaves);
+    F q[DB][kParts];
+    {
+        const T* row = row_of<const T>(a.q, b, any ? head : 0);
+#pragma unroll
+        for (int st = 0; st < DB; ++st) {
+            const int at = 32 * st + 8 * quarter;
+            float x[8] = {};
+            if (any && at < dim) load8(row + at, x);
+            in_parts<kParts>(x, q[st]);
+        }
+    }
     Span span[2] = {};
     int works = 0;
 #pragma unroll 1
@@ -721,15 +788,15 @@ void paged_step_kernel(PagedArgs a) {
                         if (!(mine >> at(r) & 1)) s[r] = 0.0f;
                 }
             }
-            F p[kParts];
-            in_parts<kParts>(s, p);
+            F p[kWeights];
+            in_parts<kWeights>(s, p);
             if (more) copies_landed<kCopies>();  // values; the next keys may be on their way
             else copies_landed<0>();
 #pragma unroll
             for (int c = 0; c < 2 * DB; ++c) {
                 const F v = In::columns(s_v, c, at_lane);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part) o[c] = mma16(v, p[part], o[c]);
+                for (int w = 0; w < kWeights; ++w) o[c] = mma16(v, p[w], o[c]);
             }
             reads_done();
         }
@@ -793,23 +860,25 @@ void paged_step_kernel(PagedArgs a) {
   }
 }
 
-// Joins the parts of one walk and head that was cut: 32 threads for the elements, four
-// each, and eight shares of the parts.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedArgs a) {
-    __shared__ f32x4 s_sum[8][32];
-    __shared__ float s_total[8], s_top[4];
-    const int head = blockIdx.x % a.heads;
-    const int b = blockIdx.x / a.heads;
+// Joins the parts of walks that were cut: 32 threads for the elements of a head, four
+// each, and kShares shares of the parts.
+template <typename T, int kShares, int kSize>
+__global__ __launch_bounds__(kSize) void join_parts_kernel(PagedArgs a) {
+    constexpr int kHeads = kSize / 32 / kShares;
+    __shared__ f32x4 s_sum[kHeads][kShares][32];
+    __shared__ float s_total[kHeads][kShares];
+    const int thread = threadIdx.x, lane = thread & 31, share = thread / 32 % kShares;
+    const int mine = thread / 32 / kShares, groups = (a.heads + kHeads - 1) / kHeads;
+    const int b = blockIdx.x / groups;
+    const int head = min(static_cast<int>(blockIdx.x % groups) * kHeads + mine, a.heads - 1);
     const int64_t begin = a.begins[b], end = a.begins[b + 1], all = a.begins[a.batch];
-    // the workgroup that has unit x: the last that begins at x or before
-    auto owner = [&](int64_t x) { return static_cast<int>(((x + 1) * a.even - 1) / all); };
-    const int first = owner(begin), parts = owner(end - 1) - first + 1;
+    const Share share_of(all, a.even);
+    const int first = share_of.owner(begin), parts = share_of.owner(end - 1) - first + 1;
     if (parts == 1) return;
     const int kv_head = head / a.group, col = head % a.group;
     // The first workgroup's part is its last one, unless the walk begins it; the others'
     // is their first one.
-    const int begun = all * first / a.even < begin;
+    const int begun = share_of.begin(first) < begin;
     auto part_of = [&](int s) {
         const int item = first + s;
         const int64_t block =
@@ -817,21 +886,18 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedArgs a) {
             item % 8;
         return (block * 2 + (s == 0 ? begun : 0)) * kColumns + col % kColumns;
     };
-    const int thread = threadIdx.x, share = thread >> 5, d = (thread & 31) * 4;
+    const int d = lane * 4;
     float top = kFloor;
-    for (int s = thread; s < parts; s += kThreads) top = fmaxf(top, a.part_stats[part_of(s)].x);
+    for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_stats[part_of(s)].x);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((thread & 63) == 0) s_top[thread >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     float total = 0.0f;
     f32x4 sum = {0, 0, 0, 0};
     // No branch inside, so that several parts' loads are in flight: threads past the
     // head size read its last elements again and store nothing.
     const int from = min(d, a.dim - 4);
 #pragma unroll 4
-    for (int s = share; s < parts; s += 8) {
+    for (int s = share; s < parts; s += kShares) {
         const int64_t at = part_of(s);
         const float2 st = a.part_stats[at];
         const f32x4 x = *reinterpret_cast<const f32x4*>(a.partial + at * a.dim + from);
@@ -840,16 +906,19 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, x[e], sum[e]);
     }
-    s_sum[share][thread & 31] = sum;
-    if ((thread & 31) == 0) s_total[share] = total;
-    __syncthreads();
-    if (share || d >= a.dim) return;
+    if constexpr (kShares > 1) {
+        s_sum[mine][share][lane] = sum;
+        if (lane == 0) s_total[mine][share] = total;
+        __syncthreads();
+        if (share) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) {
-        total += s_total[w];
+        for (int w = 1; w < kShares; ++w) {
+            total += s_total[mine][w];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += s_sum[w][thread & 31][e];
+            for (int e = 0; e < 4; ++e) sum[e] += s_sum[mine][w][lane][e];
+        }
     }
+    if (d >= a.dim) return;
     typedef T t4 __attribute__((ext_vector_type(4)));
     t4 out;
 #pragma unroll
@@ -930,8 +999,17 @@ void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
         });
         check_launch("paged_attention_step");
         if (a.even) {
-            hipLaunchKernelGGL((join_parts_kernel<T>), dim3(static_cast<unsigned>(batch * a.heads)),
-                               dim3(kThreads), 0, stream, a);
+            // Parts of a walk: a head's by 32 shares where there are many (3 walks of 100k
+            // events, 128 parts: TIMES), else eight heads a workgroup.
+            const bool many = a.even > 8 * batch;
+            const int64_t joins = batch * (many ? a.heads : (a.heads + 7) / 8);
+            require_grid(joins, many ? 1024 : 256);
+            if (many)
+                hipLaunchKernelGGL((join_parts_kernel<T, 32, 1024>),
+                                   dim3(static_cast<unsigned>(joins)), dim3(1024), 0, stream, a);
+            else
+                hipLaunchKernelGGL((join_parts_kernel<T, 1, 256>),
+                                   dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, a);
             check_launch("paged_attention_step");
         }
     });
