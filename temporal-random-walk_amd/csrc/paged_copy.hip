@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(CopyArgs a) {
     if (kWrite && !mine) return;  // (whole groups: a group has one row)
     if (!kWrite && row >= a.rows) return;
 
-    if (a.k_times && blockIdx.y == 0 && sub == 0) {
+    if (a.times && blockIdx.y == 0 && sub == 0) {
         float* held = a.k_times + (static_cast<int64_t>(page) << a.pages.shift) + slot;
         if (kWrite) *held = a.times[row];
         else a.times[row] = mine ? *held : 0.0f;

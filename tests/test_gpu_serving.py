@@ -720,6 +720,9 @@ def test_nothing_at_all(ops):
     assert (out[0] == 0).all() and torch.isnan(out[1:]).all()
     got = ops.beam_select(torch.zeros(0, 2, 9, device="cuda"), torch.zeros(0, 2, device="cuda"), 3)
     assert got.scores.shape == (0, 3)
+    got = ops.paged_read(pages, table.new_zeros(2, 3), lens=torch.tensor([2, 5]).cuda(), length=4,
+                         k_times=torch.zeros(0, 16, device="cuda"))
+    assert all((x == 0).all() for x in got) and got[2].shape == (2, 4)
     a, b = ops.beam_reorder(table, none, torch.zeros(0, 2, dtype=torch.int64).cuda(), [pages])
     assert a.shape == (0, 0) and b.shape == (0,)
 
