@@ -10,9 +10,17 @@
 // all walks are put in one line and dealt out evenly to as many workgroups as the
 // device holds at once.  Where that cuts a walk, its parts are joined by a second
 // launch.  With walks' own workgroups, three of them each, 64 walks of 100 to 4095
-// events (8 heads of 128, 8 bits) took 76.7 us, OURS so.  Many walks, and walks of
+// events (8 heads of 128, 8 bits) took 76.7 us, 67.3 so.  Many walks, and walks of
 // up to 512, have a workgroup each: there is no second launch, and the device
-// evens them out.
+// evens them out (512 walks of 0 to 511 events: 87 us, dealt out 93).
+//
+// Measured, both launches: 64 walks of 4095 events each, 5.2 TB/s in 16 bits and 4.9 in
+// 8 (a large copy: 5.17).  Of the mixed 64 above, 283 MB and 54.7 us at a copy's rate,
+// the walk over the pages takes 64.3 us and the join 4.7; 3 walks of 260k events
+// together, 135 MB and 26.2 us, 39.5 and 7.8.  What is over is the start (four loads
+// one after the other before the first tile, 5 to 7 us) and the second launch.  In 8
+// bits the vector units are busy 0.37 of the time, the matrix units 0.08.  Heads of up
+// to 64 use part of a tile's width: 32 columns in 8 bits read at 2.2 TB/s.
 //
 // v_mfma_f32_16x16x32 with keys as rows leaves lane l with keys 4 (l / 16) .. + 4
 // of column l & 15.  Two halves give eight, which are the B operand of the next
@@ -999,8 +1007,9 @@ void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
         });
         check_launch("paged_attention_step");
         if (a.even) {
-            // Parts of a walk: a head's by 32 shares where there are many (3 walks of 100k
-            // events, 128 parts: TIMES), else eight heads a workgroup.
+            // Parts of a walk: a head's by 32 shares where there are many (3 walks of
+            // 260k events together, 128 parts each: 7.8 us), else eight heads a workgroup
+            // (64 walks over 96 workgroups: 4.7 us).
             const bool many = a.even > 8 * batch;
             const int64_t joins = batch * (many ? a.heads : (a.heads + 7) / 8);
             require_grid(joins, many ? 1024 : 256);
