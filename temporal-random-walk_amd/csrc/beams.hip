@@ -18,7 +18,8 @@
 //
 // Order.  A beam's pages but the last one are full, so beams share them by their table
 // alone.  The last page is written to next, so each beam owns its own: a parent's first
-// child keeps it, further children copy its rows to the pages of beams without children.
+// child keeps it, further children copy its rows to the pages of beams without children
+// (unless another beam's past lies there, which no beam's that still grows does).
 #include <algorithm>
 #include <cmath>
 
@@ -688,11 +689,12 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
         if (!children) childless |= 1u << b;
         further |= children & (children - 1);
     }
+    const int held = static_cast<int>(
+        min(max(len, int64_t{0}) >> a.shift, static_cast<int64_t>(a.table_pages)));
     len = __shfl(len, max(parent, 0));
-    const int full = len > 0 ? static_cast<int>(min(len >> a.shift, static_cast<int64_t>(a.table_pages)))
-                             : 0;
+    const int full = __shfl(held, max(parent, 0));
     const int rows = len > 0 ? static_cast<int>(len & ((1 << a.shift) - 1)) : 0;
-    int taken = parent, source = -1, target = -1;
+    int taken = parent, source = -1, target = -1, kept = full;
     if (lane < a.beams && further >> lane & 1) {
         // as many beams are without children as children are further ones
         uint32_t left = childless;
@@ -701,6 +703,17 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
         if (rows && full < a.table_pages) {
             source = a.table[(group + parent) * a.table_stride + full];
             target = a.table[(group + taken) * a.table_stride + full];
+            // A parent that ended before others: the page may be part of what another beam
+            // holds.  Then the child reads the parent's, which grows no more.
+            bool others = false;
+#pragma unroll 4
+            for (int b = 0; b < a.beams; ++b)
+                if (!(childless >> b & 1) && __builtin_amdgcn_readlane(held, b) >= full)
+                    others |= a.table[(group + b) * a.table_stride + full] == target;
+            if (others) {
+                target = -1;
+                kept = full + 1;
+            }
         }
     }
     // what moves: between pages of the pool
@@ -709,7 +722,7 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
 
     if (a.first) {
         for (int child = part; child < a.beams; child += a.share) {
-            const int whole = __builtin_amdgcn_readlane(full, child);
+            const int whole = __builtin_amdgcn_readlane(kept, child);
             const int32_t* from =
                 a.table + (group + __builtin_amdgcn_readlane(parent, child)) * a.table_stride;
             const int32_t* rest =

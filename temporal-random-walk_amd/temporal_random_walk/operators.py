@@ -316,5 +316,6 @@ def beam_reorder(table, lens, parents, caches, *, k_times=None):
     of a beam without children, with a copy of the rows: nothing else moves.  So
     each row of a group starts with pages of its own (a prompt is written to one
     row of each group, and ``parents`` 0 spreads it), and rows of a group have equal
-    lengths, but for beams that have ended, which may be shorter."""
+    lengths, but for beams that have ended, which may be shorter (their children share
+    their last page where a copy would take one that another beam's past lies in)."""
     return _operators.beam_reorder(table, lens, parents, list(caches), k_times)

@@ -511,6 +511,33 @@ def test_reorder_out_of_range(ops):
     assert (pages.k == 1).all() and (pages.v == 1).all()
 
 
+@pytest.mark.parametrize("lens,table", [
+    # Beam 0 has ended early; beams 1 to 3 went on together, from page 1 on.
+    ([10, 40, 40, 40], [[0, 4, 5], [1, 6, 7], [1, 6, 8], [1, 9, 10]]),
+    # Beam 2 holds what ended beam 1 does, and beam 3, the longest, is dropped.
+    ([25, 20, 20, 50], [[0, 4, 5, 11], [1, 6, 7, 12], [1, 6, 8, 13], [2, 9, 10, 14]]),
+    # Nothing is shared: a short beam's rows are copied.
+    ([10, 40, 40, 40], [[0, 4, 5], [1, 6, 7], [2, 9, 8], [3, 11, 10]])])
+def test_more_children_of_a_short_beam(ops, lens, table):
+    """A choice of fewer than its width names beam 0 as the rest's parent, which may have ended
+    before the others: its children take no page that another child's history lies in."""
+    gen = torch.Generator().manual_seed(3)
+    pages = ops.Pages(*(_normal(gen, 15, 2, 16, 64, dtype=BF).cuda() for _ in "kv"))
+    times = torch.rand(15, 16, generator=gen).cuda()
+    table = torch.tensor(table, dtype=torch.int32).cuda()
+    lens = torch.tensor(lens).cuda()
+    read = lambda t, n: ops.paged_read(pages, t, lens=n, length=64, k_times=times)  # noqa: E731
+    before = read(table, lens)
+    for parents in ([0, 1, 0, 0], [1, 0, 0, 0]):
+        chosen = torch.tensor(parents).cuda()
+        new, new_lens = ops.beam_reorder(table, lens, chosen[None], [pages], k_times=times)
+        after = read(new, new_lens)
+        for x, y in zip(before, after):
+            assert torch.equal(y, x[chosen])
+        assert new_lens.tolist() == lens[chosen].tolist()
+        table, lens, before = new, new_lens, after
+
+
 # ---- together ---------------------------------------------------------------------------------------
 def _model(gen, nodes, heads, kv_heads, dim):
     """A layer of its own for a walk's last node: rows of q, k, v, and logits of an output."""
