@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(CopyArgs a) {
                 else end = mid;
             }
             number = row - a.offsets[walk];
-            mine = mine && number >= 0 && row < a.offsets[walk + 1];
+            mine = mine && number >= 0 && number < a.rows && row < a.offsets[walk + 1];
         } else {
             mine = false;
         }

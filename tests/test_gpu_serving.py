@@ -538,6 +538,23 @@ def test_more_children_of_a_short_beam(ops, lens, table):
         table, lens, before = new, new_lens, after
 
 
+def test_offsets_of_no_walk(ops):
+    """Offsets that are not walks' write nothing, and what is read for their rows is 0."""
+    pages = ops.Pages.empty(4, 16, 1, 8)
+    for x in pages[:2]:
+        x.fill_(1.0)
+    table = torch.arange(4, dtype=torch.int32).cuda().view(2, 2)
+    rows = torch.full((6, 1, 8), 2.0, dtype=BF, device="cuda")
+    far = (1 << 63) - 1
+    for offsets in ([-far, -far, -far], [-far, 0, 0], [far, far, far], [-far, -far, 6], [5, -9, far]):
+        offsets = torch.tensor(offsets).cuda()
+        k, v = ops.paged_read(pages, table, offsets=offsets, rows=6)
+        assert ((k == 0) | (k == 1)).all() and torch.equal(k, v)
+        if offsets[1] != -9:
+            ops.paged_write(pages, table, torch.tensor([7, 8]).cuda(), rows, rows, offsets=offsets)
+            assert (k == 0).all() and (pages.k == 1).all() and (pages.v == 1).all()
+
+
 # ---- together ---------------------------------------------------------------------------------------
 def _model(gen, nodes, heads, kv_heads, dim):
     """A layer of its own for a walk's last node: rows of q, k, v, and logits of an output."""
@@ -791,6 +808,7 @@ def test_refusals(ops):
                           lens), "contiguous|heads"),
             (lambda: step(new, new, new, ops.Pages(p.k[:1].expand_as(p.v), p.v), table, lens),
              "share memory"),
+            (lambda: step(new, new, new, ops.Pages(p.k, p.k), table, lens), "share memory"),
             (lambda: step(new, new, new, ops.Pages.empty(4, 24, 2, 64), table, lens), "power of two"),
             (lambda: step(new[..., :24].contiguous(), new[..., :24].contiguous(),
                           new[..., :24].contiguous(), ops.Pages.empty(4, 16, 2, 24, dtype=E8), table,
