@@ -700,21 +700,26 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
         uint32_t left = childless;
         for (int n = __popc(further & ((1u << lane) - 1)); n; --n) left &= left - 1;
         taken = __ffs(left) - 1;
-        if (rows && full < a.table_pages) {
-            source = a.table[(group + parent) * a.table_stride + full];
-            target = a.table[(group + taken) * a.table_stride + full];
-            // A parent that ended before others: the page may be part of what another beam
-            // holds.  Then the child reads the parent's, which grows no more.
-            bool others = false;
-#pragma unroll 4
-            for (int b = 0; b < a.beams; ++b)
-                if (!(childless >> b & 1) && __builtin_amdgcn_readlane(held, b) >= full)
-                    others |= a.table[(group + b) * a.table_stride + full] == target;
-            if (others) {
-                target = -1;
-                kept = full + 1;
-            }
+    }
+    // Further children's copies, those of equal lengths at once: a lane a beam's page.
+    const u64 fill = __ballot(rows && full < a.table_pages) & further;
+    for (u64 left = fill; left;) {
+        const int at = __builtin_amdgcn_readlane(full, __ffsll(left) - 1);
+        const u64 these = left & __ballot(full == at);
+        const int page = lane < a.beams ? a.table[(group + lane) * a.table_stride + at] : -1;
+        const int from = __shfl(page, max(parent, 0)), to = __shfl(page, max(taken, 0));
+        // A parent that ended before others: the page may be part of what another beam with
+        // children holds.  Then the child reads the parent's, which grows no more.
+        bool others = false;
+        for (u64 b = __ballot(lane < a.beams && held >= at) & ~childless; b; b &= b - 1)
+            others |= __builtin_amdgcn_readlane(page, __ffsll(b) - 1) == to;
+        others = others && to >= 0 && to < a.pages;
+        if (these >> lane & 1) {
+            source = from;
+            target = others ? -1 : to;
+            kept = full + others;
         }
+        left &= ~these;
     }
     // what moves: between pages of the pool
     const u64 moving = __ballot(source >= 0 && source < a.pages && target >= 0 && target < a.pages &&

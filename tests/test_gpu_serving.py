@@ -508,6 +508,10 @@ def test_reorder_out_of_range(ops):
     got, _ = ops.beam_reorder(table, torch.tensor([3, 1 << 50]).cuda(), torch.tensor([[7, 9]]).cuda(),
                               [pages])
     assert got.tolist() == [[1 << 30, 2], [1 << 30, 2]]
+    empty = torch.tensor([[0, 1], [2, -1], [3, -1]], dtype=torch.int32).cuda()
+    got, _ = ops.beam_reorder(empty, torch.full((3,), 20).cuda(), torch.tensor([[0, 0, 1]]).cuda(),
+                              [pages])
+    assert got.tolist() == [[0, 1], [0, -1], [2, -1]]
     assert (pages.k == 1).all() and (pages.v == 1).all()
 
 
