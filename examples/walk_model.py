@@ -9,7 +9,10 @@
 3. Serving: the caches are filled from the first events of some walks, then
    ``walk_attention_step`` takes one event of each walk at a time; the logits are
    compared with those of one pass over whole walks.
-4. A look inside: ``relative_bias`` gives the learned bias as a dense array, from
+4. A forecast: the histories of some walks go to pages of 8 bits
+   (``paged_write``), and a beam search names the likeliest ways on
+   (``paged_attention_step``, ``beam_select``, ``beam_reorder``).
+5. A look inside: ``relative_bias`` gives the learned bias as a dense array, from
    which plain tensor code shows how far back each head looks.
 """
 import argparse
@@ -30,6 +33,7 @@ from temporal_random_walk import operators as ops  # noqa: E402
 HEADS, KV_HEADS, DIM = 8, 2, 64
 WIDTH = HEADS * DIM
 BUCKETS, REACH = 32, 128
+GROUP = 20  # nodes that meet
 
 
 def sample_walks(nodes, group, walks, length, seed):
@@ -80,14 +84,17 @@ class WalkModel(nn.Module):
     def terms(self):
         return dict(bias_table=self.bias, buckets=self.buckets, slopes=self.slopes)
 
-    def forward(self, at, times, mask, caches=None):
-        """Logits at each event of padded walks; fills the caches' first positions if given."""
+    def forward(self, at, times, mask, caches=None, keep=None):
+        """Logits at each event of padded walks; fills the caches' first positions if given, or
+        has ``keep`` take each layer's keys and values."""
         x = self.embed(at)
         for i, layer in enumerate(self.layers):
             q, k, v = layer.project(x)
             if caches:
                 for cache, rows in zip(caches[i], (k, v)):
                     cache[:, :rows.shape[1]] = rows
+            if keep:
+                keep(i, k, v)
             x = layer.rest(x, ops.walk_attention(q, k, v, mask, times=times, **self.terms()))
         return self.head(self.norm(x))
 
@@ -98,6 +105,16 @@ class WalkModel(nn.Module):
             q, k, v = layer.project(x)
             x = layer.rest(x, ops.walk_attention_step(
                 q, k, v, k_cache, v_cache, lens, times=times, k_times=k_times, **self.terms()))
+        return self.head(self.norm(x))
+
+
+    def paged_step(self, at, times, caches, table, k_times, lens):
+        """The same over pages."""
+        x = self.embed(at)
+        for layer, pages in zip(self.layers, caches):
+            q, k, v = layer.project(x)
+            x = layer.rest(x, ops.paged_attention_step(
+                q, k, v, pages, table, lens, times=times, k_times=k_times, **self.terms()))
         return self.head(self.norm(x))
 
 
@@ -147,6 +164,48 @@ def serve(model, at, times, lens, prompt):
 
 
 @torch.no_grad()
+def forecast(model, at, times, lens, steps, beams=4, page_rows=16):
+    """The likeliest ways on from each walk: nodes [walks, beams, steps] and their log
+    probabilities.  Events to come are as far apart in time as the walk's were."""
+    walks, length = at.shape
+    each = -(-(length + steps) // page_rows)
+    rows = walks * beams
+    table = torch.arange(rows * each, dtype=torch.int32, device="cuda").view(rows, each)
+    caches = [ops.Pages.empty(rows * each, page_rows, KV_HEADS, DIM, dtype=torch.float8_e4m3fn)
+              for _ in model.layers]
+    k_times = torch.zeros(rows * each, page_rows, device="cuda")
+    # the walks' histories without their last event, each to the pages of its first beam
+    held = (lens - 1).clamp(min=0)
+
+    def keep(layer, k, v):
+        ops.paged_write(caches[layer], table[::beams], None, k, v, counts=held, times=times,
+                        k_times=k_times)
+
+    last = at.gather(1, held[:, None])[:, 0]
+    now = times.gather(1, held[:, None])[:, 0]
+    gap = (now - times[:, 0]) / held.clamp(min=1)
+    scores = torch.full((walks, beams), -math.inf, device="cuda")
+    scores[:, 0] = 0
+    nodes = last.repeat_interleave(beams)
+    path = nodes.new_empty(walks, beams, 0)
+    parents = torch.zeros(walks, beams, dtype=torch.int64, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16):
+        model(at, times.contiguous(), ops.WalkMask.padded(lens, length), keep=keep)
+        table, at_lens = ops.beam_reorder(table, held.repeat_interleave(beams), parents, caches,
+                                          k_times=k_times)
+        for n in range(steps):
+            when = (now + n * gap).repeat_interleave(beams)
+            logits = model.paged_step(nodes, when, caches, table, k_times, at_lens)
+            choice = ops.beam_select(logits.unflatten(0, (walks, beams)), scores, beams)
+            table, at_lens = ops.beam_reorder(table, at_lens + 1, choice.parents, caches,
+                                              k_times=k_times)
+            scores, nodes = choice.scores, choice.tokens.flatten()
+            path = path.gather(1, choice.parents[..., None].expand_as(path))
+            path = torch.cat([path, choice.tokens[..., None]], -1)
+    return path, scores
+
+
+@torch.no_grad()
 def look(model, at, times, lens):
     """How many events back each head of the first layer looks, on average."""
     length = at.shape[1]
@@ -171,7 +230,7 @@ def main(argv=None):
     parser.add_argument("--steps", type=int, default=50)
     args = parser.parse_args(argv)
     torch.manual_seed(0)
-    at, times, lens = sample_walks(args.nodes, 20, args.walks, args.length, seed=0)
+    at, times, lens = sample_walks(args.nodes, GROUP, args.walks, args.length, seed=0)
     print(f"{at.shape[0]} walks, {int(lens.sum())} events")
     model = WalkModel(args.nodes).cuda()
     torch.cuda.synchronize()
@@ -184,6 +243,10 @@ def main(argv=None):
     prompt = args.length // 2
     served, off = serve(model, at[some], times[some], lens[some], prompt)
     print(f"{served} events served from event {prompt} on: logits {off:.2e} from those of one pass")
+    path, scores = forecast(model, at[some], times[some], lens[some], 8)
+    within = (path // GROUP == at[some].gather(1, lens[some, None] - 1)[..., None] // GROUP)
+    print(f"likeliest 8 events to come: log probability {float(scores[:, 0].mean()):.2f}, "
+          f"{float(within[:, 0].float().mean()):.3f} of them in the walk's own group")
     far = look(model, at[some], times[some], lens[some])
     print("events that a head looks back:", " ".join(f"{x:.1f}" for x in far.tolist()))
     return losses, served, off, far

@@ -838,3 +838,20 @@ def test_refusals(ops):
              "pages alike")):
         with pytest.raises(ValueError, match=message):
             call()
+
+
+def test_example():
+    """The forecast of examples/walk_model.py runs: paths of nodes, distinct, best first."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "walk_model.py")
+    spec = importlib.util.spec_from_file_location("walk_model", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    at, times, lens = example.sample_walks(100, 20, 24, 20, seed=1)
+    model = example.WalkModel(100).cuda()
+    nodes, scores = example.forecast(model, at, times, lens, 5, beams=3)
+    assert nodes.shape == (at.shape[0], 3, 5) and ((nodes >= 0) & (nodes < 100)).all()
+    assert torch.isfinite(scores).all() and (scores[:, :-1] >= scores[:, 1:]).all()
+    assert all(len(set(map(tuple, x))) == 3 for x in nodes.tolist())
