@@ -36,7 +36,9 @@
 // The softmax's weights go as two bfloat16 parts as well, or three where q is
 // float32, so that nothing but the output is rounded as far as bfloat16 is (one part:
 // outputs up to 1.75 times as far from exact ones; it costs no time that is seen, the
-// kernel waits for memory).  Pages of float16 take float16 weights.
+// kernel waits for memory).  Over pages of float16 they go as two float16 parts, and the
+// largest weight is 2^15 instead of 1 (the sum too, so that it cancels): float16 ends at
+// 2^-24, and what many keys of less than that share would be lost next to one of 1.
 //
 // The new row is taken from the call's arguments by the workgroup whose positions
 // include it (in 8 bits as the codes that the pages get), and written to the pages
@@ -339,7 +341,9 @@ void paged_step_kernel(PagedArgs a) {
     constexpr int kBytes = kEight ? 1 : sizeof(T);
     constexpr bool kShort = std::is_same<T, __bf16>::value;
     constexpr int kParts = !kEight || kShort ? 1 : sizeof(T) == 4 ? 3 : 2;  // of q
-    constexpr int kWeights = kShort ? 2 : kParts;  // parts of a weight
+    // parts of a weight, and what the largest one is
+    constexpr int kWeights = sizeof(T) == 4 ? kParts : 2;
+    constexpr float kLargest = std::is_same<F, f16x8>::value ? 32768.0f : 1.0f;
     constexpr int kJoinPitch = 32 * DB + 4;
     constexpr size_t kJoinBytes = size_t(kWaves) * kColumns * kJoinPitch * sizeof(float);
     constexpr size_t kTileBytes = 2 * kWaves * G::kSize;
@@ -783,7 +787,7 @@ void paged_step_kernel(PagedArgs a) {
             }
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                s[r] = exp2_fast(s[r] - m);
+                s[r] = exp2_fast(s[r] - m) * kLargest;
                 l += s[r];
             }
             if constexpr (kEight) {
