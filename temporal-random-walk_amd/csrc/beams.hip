@@ -36,7 +36,9 @@ constexpr int kMost = TRW_OPS_BEAMS;
 constexpr int kJoinWaves = 16;    // of a group's workgroup, at most
 constexpr int kRanked = 256;      // chunks that are ranked without a bound
 constexpr float kMax = 3.402823466e38f;
-constexpr float kNear = 1e30f;  // logits up to here have products in base 2
+// Up to here a maximum's product with log2 e is off by 2^-13 at most, and its rounding
+// is taken from a sum of exponentials as (1 - ln2 rounding), good to 2^-27.
+constexpr float kNear = 2048.0f;
 
 typedef unsigned long long u64;
 
@@ -270,7 +272,8 @@ __device__ __forceinline__ void sum_chunk(const T* row, const uint8_t* ended, in
             for (int e = 0; e < kElems; ++e) sum += exp2_fast(fmaf(x[c].at(e), kLog2e, -base2));
         sum = fmaf(-kLn2 * fmaf(top, kLog2e, -base2), sum, sum);
     } else {
-        // -inf, and a chunk of nothing else, add 0
+        // differences first, which are exact where their exponentials are not 0; -inf, and a
+        // chunk of nothing else, add 0
         const float base = fmaxf(top, -kMax);
 #pragma unroll
         for (int c = 0; c < kPieces; ++c)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import walk_formulas as wf
-from tests.test_gpu_serving import DTYPES, Pool, ops  # noqa: F401
+from tests.test_gpu_serving import DTYPES, SIZES, Pool, _choose, _normal, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,39 @@ def test_step_of_small_weights(ops, dtype, eight, cached, capacity):  # noqa: F8
     # 2^-39 of the largest weight where the type has no smaller numbers
     bound = bound + (wf.U[dtype] + 2.0 ** -16) * o.abs() + cached * 2.0 ** -39 * 100.0
     wf.check("out", out, o, bound)
+
+
+# ---- choice among beams -----------------------------------------------------------------------------
+LOWS = [-(10.0 ** n) for n in range(3, 38)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("groups,beams,nodes,width", [(2, 3, 9000, 8), (1, 2, 70001, 5)])
+def test_choice_of_finitely_masked_nodes(ops, dtype, groups, beams, nodes, width):  # noqa: F811
+    """Masks of any size over whole chunks beside ordinary ones, and over whole rows."""
+    gen = torch.Generator().manual_seed(nodes)
+    x = _normal(gen, groups, beams, nodes, dtype=dtype, std=3.0)
+    scores = -torch.rand(groups, beams, generator=gen)
+    for low in LOWS:
+        if low < torch.finfo(dtype).min:
+            break
+        y = x.clone()
+        y[..., 4096:] = low
+        _choose(ops, y, scores, width)
+        y = torch.full_like(x, low)
+        y[..., 8200:8300] = x[..., 8200:8300]
+        _choose(ops, y, scores, width)
+        _choose(ops, torch.full_like(x, low), scores, width)
+        _choose(ops, torch.full_like(x, -low), scores, width)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("groups,beams,nodes,width", SIZES)
+@pytest.mark.parametrize("far", [100.0, 1e3, 3e3, 1e4, -1e4, 6e4, 1e6, -1e6, 1e8, -1e8])
+def test_choice_far_from_zero(ops, dtype, groups, beams, nodes, width, far):  # noqa: F811
+    """Rows shifted by a constant choose as they do around zero."""
+    if abs(far) > torch.finfo(dtype).max:
+        return
+    gen = torch.Generator().manual_seed(nodes)
+    x = (_normal(gen, groups, beams, nodes, std=3.0) + far).to(dtype)
+    _choose(ops, x, -torch.rand(groups, beams, generator=gen), width)
