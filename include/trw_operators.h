@@ -277,8 +277,8 @@ trw_status trw_ops_beam_select(const trw_beam_select_params* params, void* strea
  * further child takes those of a beam without children, with a copy of the
  * parent's rows in the first.  So rows of a group that still grow need pages of
  * their own from there on, and equal lengths; others may be shorter (where the page
- * to copy to is one that another beam with children reads, the further child of a
- * shorter parent has the parent's own). */
+ * to copy to is one that another beam with children reads, or that takes another
+ * child's rows, the further child of a shorter parent has the parent's own). */
 typedef struct trw_beam_reorder_params {
     int32_t beams, page_rows, count;
     int64_t groups, pages, table_pages, table_stride;

@@ -19,7 +19,8 @@
 // Order.  A beam's pages but the last one are full, so beams share them by their table
 // alone.  The last page is written to next, so each beam owns its own: a parent's first
 // child keeps it, further children copy its rows to the pages of beams without children
-// (unless another beam's past lies there, which no beam's that still grows does).
+// (unless another beam's past lies there, or another child's copy of other rows, which
+// is not so for a beam that still grows).
 #include <algorithm>
 #include <cmath>
 
@@ -712,10 +713,24 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
         const int page = lane < a.beams ? a.table[(group + lane) * a.table_stride + at] : -1;
         const int from = __shfl(page, max(parent, 0)), to = __shfl(page, max(taken, 0));
         // A parent that ended before others: the page may be part of what another beam with
-        // children holds.  Then the child reads the parent's, which grows no more.
-        bool others = false;
-        for (u64 b = __ballot(lane < a.beams && held >= at) & ~childless; b; b &= b - 1)
-            others |= __builtin_amdgcn_readlane(page, __ffsll(b) - 1) == to;
+        // children holds.  Then the child reads the parent's, which grows no more.  Beams without
+        // children may share a page as well: it takes one child's rows, and later children of
+        // other parents read their parents'.
+        const uint32_t reads = static_cast<uint32_t>(__ballot(lane < a.beams && held >= at)) & ~childless;
+        bool others = false, again = false;
+        for (int b = 0; b < a.beams; ++b) {
+            const bool same = __builtin_amdgcn_readlane(page, b) == to;
+            others |= same && (reads >> b & 1);
+            again |= same && b != taken;
+        }
+        if (__builtin_expect((__ballot(again && !others) & these) != 0, 0)) {
+            for (u64 b = these; b; b &= b - 1) {
+                const int n = __ffsll(b) - 1;
+                const bool copies = !__builtin_amdgcn_readlane(static_cast<int>(others), n);
+                others |= copies && lane > n && __builtin_amdgcn_readlane(to, n) == to &&
+                          __builtin_amdgcn_readlane(from, n) != from;
+            }
+        }
         others = others && to >= 0 && to < a.pages;
         if (these >> lane & 1) {
             source = from;

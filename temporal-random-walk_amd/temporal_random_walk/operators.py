@@ -317,5 +317,6 @@ def beam_reorder(table, lens, parents, caches, *, k_times=None):
     each row of a group starts with pages of its own (a prompt is written to one
     row of each group, and ``parents`` 0 spreads it), and rows of a group have equal
     lengths, but for beams that have ended, which may be shorter (their children share
-    their last page where a copy would take one that another beam's past lies in)."""
+    their last page where a copy would take one that another beam's past or another
+    child's copy lies in)."""
     return _operators.beam_reorder(table, lens, parents, list(caches), k_times)

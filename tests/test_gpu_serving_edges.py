@@ -1,10 +1,14 @@
 """Pages and beam search where rounding, masks and lengths are extreme, against their formulas in
-float64 (tests/serving_formulas.py, tests/walk_formulas.py)."""
+float64 (tests/serving_formulas.py, tests/walk_formulas.py, tests/beam_orders.py)."""
+import random
+
 import pytest
 import torch
 
+from tests import beam_orders as bo
 from tests import walk_formulas as wf
-from tests.test_gpu_serving import DTYPES, SIZES, Pool, _choose, _normal, ops  # noqa: F401
+from tests.test_cpu_beam_orders import TWO_SHORT
+from tests.test_gpu_serving import DTYPES, SF, SIZES, Pool, _choose, _normal, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +76,50 @@ def test_choice_far_from_zero(ops, dtype, groups, beams, nodes, width, far):  # 
     gen = torch.Generator().manual_seed(nodes)
     x = (_normal(gen, groups, beams, nodes, std=3.0) + far).to(dtype)
     _choose(ops, x, -torch.rand(groups, beams, generator=gen), width)
+
+
+# ---- reordering ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("table,lens,parents,page_rows", [
+    TWO_SHORT,
+    ([[0, 4, 5], [1, 6, 7], [2, 8, 9], [2, 8, 10]], [10, 12, 40, 40], [0, 0, 1, 1], 16),
+    # three short parents, and dropped beams of one past and of another
+    ([[0, 1], [2, 3], [4, 5], [6, 7], [6, 8], [9, 10]], [10, 12, 14, 20, 20, 30], [2, 1, 0, 0, 1, 2],
+     16)])
+def test_children_of_several_short_beams(ops, table, lens, parents, page_rows):  # noqa: F811
+    """Rows of different parents never go to one page."""
+    gen = torch.Generator().manual_seed(3)
+    pages = ops.Pages(*(_normal(gen, 16, 2, page_rows, 64).cuda() for _ in "kv"))
+    times = torch.rand(16, page_rows, generator=gen).cuda()
+    length = len(table[0]) * page_rows
+    read = lambda t, n: ops.paged_read(pages, t, lens=n, length=length, k_times=times)  # noqa: E731
+    rows, _, _ = bo.order(table, lens, parents, page_rows)
+    table, lens, chosen = torch.tensor(table).int().cuda(), torch.tensor(lens).cuda(), parents
+    before = read(table, lens)
+    new, new_lens = ops.beam_reorder(table, lens, torch.tensor([parents]).cuda(), [pages],
+                                     k_times=times)
+    assert new.tolist() == rows and new_lens.tolist() == lens[chosen].tolist()
+    for x, y in zip(before, read(new, new_lens)):
+        assert torch.equal(y, x[chosen])
+
+
+def test_any_parents(ops):  # noqa: F811
+    """Searches whose parents are any beams, those that ended early among them: tables are the
+    formula's, and every beam keeps its history."""
+    pages = ops.Pages.empty(64, 16, 1, 8, dtype=SF)
+    for seed in range(12):
+        gen = torch.Generator().manual_seed(seed)
+
+        def orders(table, lens, parents, page_rows):
+            want, want_lens, _ = bo.order(table, lens, parents, page_rows)
+            t, n = torch.tensor(table).int().cuda(), torch.tensor(lens).cuda()
+            for x in pages[:2]:
+                x.copy_(torch.randn(x.shape, generator=gen))
+            before = ops.paged_read(pages, t, lens=n, length=128)
+            new, new_lens = ops.beam_reorder(t, n, torch.tensor([parents]).cuda(), [pages])
+            assert new.tolist() == want and new_lens.tolist() == want_lens
+            for x, y in zip(before, ops.paged_read(pages, new, lens=new_lens, length=128)):
+                assert torch.equal(y, x[parents])
+            return want, want_lens, None
+
+        for _ in bo.search(random.Random(seed), orders, 16):
+            pass
