@@ -683,7 +683,10 @@ void paged_step_kernel(PagedArgs a) {
             for (int st = 0; st < DB; ++st)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const F k = In::row(s_k, kHalf * h + (at_lane & 15), st, at_lane >> 4);
+                    F k = In::row(s_k, kHalf * h + (at_lane & 15), st, at_lane >> 4);
+                    // Past the head size a row repeats its start: an infinity there times q's 0
+                    // would be NaN (in 8 bits it is NaN where it is).
+                    if (!kEight && st == DB - 1 && 32 * st + 8 * (at_lane >> 4) >= dim) k = F{};
 #pragma unroll
                     for (int p = 0; p < kParts; ++p) x[h] = mma16(k, q[st][p], x[h]);
                 }

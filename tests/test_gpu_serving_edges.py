@@ -42,6 +42,25 @@ def test_step_of_small_weights(ops, dtype, eight, cached, capacity):  # noqa: F8
     wf.check("out", out, o, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [8, 24, 40, 72, 104, 128])
+def test_step_over_infinite_keys(ops, dtype, dim):  # noqa: F811
+    """A key with an infinity against a query of the other sign has weight 0, at every head size."""
+    gen = torch.Generator().manual_seed(dim)
+    pool = Pool(ops, 1, 64, 1, dim, dtype=dtype)
+    q, k, v = (_normal(gen, 1, n, 1, dim, dtype=dtype) for n in (1, 41, 41))
+    q[..., 0] = 0.5 + q[..., 0].abs()
+    k[0, 7, 0, 0] = -torch.inf
+    ops.paged_write(pool.pages, pool.table, None, k[:, :-1].cuda(), v[:, :-1].cuda())
+    out = ops.paged_attention_step(q[0].cuda(), k[:, -1].cuda(), v[:, -1].cuda(), pool.pages,
+                                   pool.table, torch.tensor([40]).cuda())
+    seen = torch.arange(41) != 7
+    k[0, 7] = 0  # not seen: the formula's -inf
+    want = wf.attention(q[0].double(), k[0].double(), v[0].double(), [(40, 1, 41, seen[None])],
+                        dtype=dtype)["out"]
+    wf.check("out", out, *want)
+
+
 # ---- choice among beams -----------------------------------------------------------------------------
 LOWS = [-(10.0 ** n) for n in range(3, 38)]
 
