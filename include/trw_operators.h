@@ -191,7 +191,8 @@ trw_status trw_ops_relative_bias_backward(const trw_relative_bias_params* params
  * the last three dimensions contiguous.  Position p of walk w is row
  * p % page_rows of page table[w, p / page_rows]; an entry outside [0, pages) is
  * no page: what would be written there is not, what would be read is 0, and
- * steps do not see it.
+ * steps do not see it.  k, v and their scales share no memory (they may be parts of
+ * one record for each page, of one stride in bytes).
  *
  * TRW_E4M3: a row of one head is D codes c (e4m3, no infinities) and one byte b,
  * of the values c 2^(b - 127): the smallest power of two that brings the row's

@@ -976,8 +976,9 @@ uint64_t paged_step_workspace(const trw_paged_step_params& p) {
 
 void paged_step(const trw_paged_step_params& p, hipStream_t stream) {
     const int64_t batch = p.pages.walks;
+    require(batch == 0 || p.workspace_bytes >= paged_step_workspace(p), "workspace is too small");
+    require_apart(p.pages);
     if (batch == 0) return;
-    require(p.workspace_bytes >= paged_step_workspace(p), "workspace is too small");
     PagedArgs a;
     a.pages = make_pages(p.pages);
     a.q = make_rows(p.q);

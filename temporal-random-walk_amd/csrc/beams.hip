@@ -870,6 +870,7 @@ void beam_select(const trw_beam_select_params& p, hipStream_t stream) {
 }
 
 void beam_reorder(const trw_beam_reorder_params& p, hipStream_t stream) {
+    for (int c = 0; c < p.count; ++c) require_apart(p.caches[c]);
     if (p.groups == 0) return;
     ReorderArgs a;
     a.table = p.table;

@@ -166,6 +166,7 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(CopyArgs a) {
 }  // namespace
 
 void paged_copy(const trw_paged_copy_params& p, bool write, hipStream_t stream) {
+    require_apart(p.pages);
     if (p.rows == 0) return;
     CopyArgs a;
     a.pages = make_pages(p.pages);

@@ -54,6 +54,40 @@ inline Pages make_pages(const trw_pages& p) {
     return r;
 }
 
+// Whether blocks of a and of b, `count` of each and each `stride` bytes (its size or
+// more) from the next, share memory; where strides differ, whether the ranges do.
+inline bool share_memory(const void* a, int64_t a_size, int64_t a_stride, const void* b,
+                         int64_t b_size, int64_t b_stride, int64_t count) {
+    // (a range may not end inside the addresses that there are: __int128 holds its end)
+    const __int128 d = static_cast<__int128>(reinterpret_cast<uintptr_t>(b)) -
+                       static_cast<__int128>(reinterpret_cast<uintptr_t>(a));
+    if (d >= static_cast<__int128>(count - 1) * a_stride + a_size ||
+        -d >= static_cast<__int128>(count - 1) * b_stride + b_size)
+        return false;
+    if (count == 1 || a_stride != b_stride) return true;
+    const int64_t at = static_cast<int64_t>((d % a_stride + a_stride) % a_stride);
+    return at < a_size || at + b_size > a_stride;
+}
+// The last of the checks of pages that are written or read.
+inline void require_apart(const trw_pages& p) {
+    if (p.pages == 0) return;
+    const int64_t size = static_cast<int64_t>(page_element_size(p.dtype));
+    const int64_t lines = int64_t{p.kv_heads} * p.page_rows;
+    struct {
+        const void* at;
+        int64_t size, stride;
+    } const blocks[] = {{p.k, lines * p.dim * size, p.k_stride * size},
+                        {p.v, lines * p.dim * size, p.v_stride * size},
+                        {p.k_scale, lines, p.k_scale_stride},
+                        {p.v_scale, lines, p.v_scale_stride}};
+    const int count = p.dtype == TRW_E4M3 ? 4 : 2;
+    for (int i = 0; i < count; ++i)
+        for (int j = i + 1; j < count; ++j)
+            require(!share_memory(blocks[i].at, blocks[i].size, blocks[i].stride, blocks[j].at,
+                                  blocks[j].size, blocks[j].stride, p.pages),
+                    "k, v and their scales must not share memory");
+}
+
 // ---- rows in 8 bits ------------------------------------------------------------------------------
 // The exponents that a row may have: codes' smallest step stays a normal number
 // of float32 and bfloat16 (2^-9 2^-117), and 2^-e is one.

@@ -26,7 +26,6 @@ trw_pages pages_of(const PageTensors& t, const Tensor& beside) {
     REQUIRE(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
             "k and v of pages must be [pages, kv_heads, page_rows, dim] of one type");
     REQUIRE(pages_whole(k) && pages_whole(v), "a page must be contiguous");
-    REQUIRE(k.numel() == 0 || k.data_ptr() != v.data_ptr(), "k and v must not share memory");
     const bool eight = k.scalar_type() == at::kFloat8_e4m3fn;
     REQUIRE(k_scale.has_value() == eight && v_scale.has_value() == eight,
             "pages of float8_e4m3fn, and no others, have scales");

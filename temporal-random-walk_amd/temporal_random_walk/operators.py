@@ -188,7 +188,8 @@ class Pages(NamedTuple):
     """Keys and values of many walks in pages of one pool.
 
     ``k``, ``v``: ``[pages, kv_heads, page_rows, dim]``, each page contiguous
-    (``page_rows``: a power of two, 16 to 1024).  Which pages are a walk's says a
+    (``page_rows``: a power of two, 16 to 1024), of memory of their own or parts of
+    one record for each page.  Which pages are a walk's says a
     table, int32 ``[walks, pages of a walk]``, that all layers share: position p
     of walk w is row p % page_rows of page ``table[w, p // page_rows]``.  Entries
     outside the pool (-1, say) are no pages: nothing is written there, 0 is read,

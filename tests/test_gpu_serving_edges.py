@@ -8,7 +8,8 @@ import torch
 from tests import beam_orders as bo
 from tests import walk_formulas as wf
 from tests.test_cpu_beam_orders import TWO_SHORT
-from tests.test_gpu_serving import DTYPES, SF, SIZES, Pool, _choose, _normal, ops  # noqa: F401
+from tests.test_gpu_serving import (BF, DTYPES, E8, SF, SIZES, Pool, _choose, _normal,  # noqa: F401
+                                    ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +60,41 @@ def test_step_over_infinite_keys(ops, dtype, dim):  # noqa: F811
     want = wf.attention(q[0].double(), k[0].double(), v[0].double(), [(40, 1, 41, seen[None])],
                         dtype=dtype)["out"]
     wf.check("out", out, *want)
+
+
+def test_pages_as_records(ops):  # noqa: F811
+    """Keys, values and scales of a page in one record hold what they do in memory of their own;
+    scales of one memory are refused."""
+    gen = torch.Generator().manual_seed(5)
+    heads, rows, dim, count = 2, 32, 64, 9
+    sizes = [heads * rows * dim] * 2 + [heads * rows] * 2
+    pool = torch.zeros(count, sum(sizes), dtype=torch.uint8, device="cuda")
+    k, v, ks, vs = pool.split(sizes, 1)
+    shape = (heads, rows)
+    record = ops.Pages(*(x.view(E8).unflatten(1, (*shape, dim)) for x in (k, v)),
+                       *(x.unflatten(1, shape) for x in (ks, vs)))
+    whole = ops.Pages(*(None if x is None else x.contiguous() for x in record))
+    table = torch.randperm(count, generator=gen).int().view(3, 3).cuda()
+    lens = torch.tensor([90, 33, 64]).cuda()
+    kc, vc = (_normal(gen, 3, 90, heads, dim, dtype=BF).cuda() for _ in "kv")
+    q, new_k, new_v = (_normal(gen, 3, n, dim, dtype=BF).cuda() for n in (4, heads, heads))
+    got = []
+    for pages in (record, whole):
+        ops.paged_write(pages, table, None, kc, vc, counts=lens)
+        out = ops.paged_attention_step(q, new_k, new_v, pages, table, lens)
+        new, n = ops.beam_reorder(table, lens, torch.tensor([[1, 1, 0]]).cuda(), [pages])
+        got.append((out, *ops.paged_read(pages, new, lens=n, length=90)))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    for x, y in zip(record, whole):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    one = whole._replace(v_scale=whole.k_scale)
+    for call in (lambda: ops.paged_write(one, table, None, kc, vc),
+                 lambda: ops.paged_read(one, table, lens=lens, length=4),
+                 lambda: ops.paged_attention_step(q, new_k, new_v, one, table, lens),
+                 lambda: ops.beam_reorder(table, lens, torch.tensor([[1, 1, 0]]).cuda(), [one])):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
 
 
 # ---- choice among beams -----------------------------------------------------------------------------
