@@ -7,8 +7,10 @@
 // knows each beam's sum and the best continuation of every chunk, and the `width` best
 // ones are all in the `width` chunks whose best ones come first: of any other chunk's,
 // `width` come before.  Those few chunks are read again, and what reaches the last
-// one's best is ranked by counting.  Scores are added in float64, where candidates of
-// different beams meet.  Lanes hold the same nodes whatever the row's alignment, so that
+// one's best is ranked by counting.  What follows the chunks' sums is float64
+// (but for the exponentials that join them), for the order of candidates of different
+// beams: scores are 1.05 to 1.12 times as far from 64 bits as their last rounding, with
+// a logarithm of float32 1.25 to 1.7 times.  Lanes hold the same nodes whatever the row's alignment, so that
 // equal rows have equal sums and ties go to the lowest index.
 //
 // Measured: 64 groups of 8 beams over 50021 nodes in bfloat16 (51 MB, 9.9 us at a copy's
@@ -153,12 +155,6 @@ __device__ __forceinline__ double eight_sum(double x) {
     x += moved<0x4e>(x);
     return x + moved<0x141>(x);
 }
-// log x: float32's of the nearest float32, and the first term for what is left.
-__device__ __forceinline__ double log_of(double x) {
-    const float near = static_cast<float>(x);
-    return static_cast<double>(logf(near)) + (x - near) / near;
-}
-
 // The first `width` of `count` different keys in order, to `best` (may be `keys`), by
 // one wave.  count: width to kListed.
 __device__ __forceinline__ void take_best(const u64* keys, int count, u64* best, int width,
@@ -437,7 +433,7 @@ __device__ __forceinline__ void choose(const SelectArgs& a, int64_t group, const
         sum = eight_sum(sum);
         if (in && sub == 0) {
             double off = NAN;
-            if (grows && sum > 0.0) off = static_cast<double>(score) - log_of(sum);
+            if (grows && sum > 0.0) off = static_cast<double>(score) - log(sum);
             else if (is && ended) off = score;
             s.off[b] = off;
             s.top[b] = m;

@@ -298,8 +298,9 @@ def beam_select(logits, scores, width, *, ended=None, end_token=None):
 
     A beam whose score is not finite, or whose logits hold NaN, +inf or nothing
     above -inf, has no continuations.  Where a group has fewer than ``width``: score -inf,
-    parent 0, token ``end_token`` (0 without one), ended.  Scores are summed in
-    float64; there is no gradient."""
+    parent 0, token ``end_token`` (0 without one), ended.  Exponentials are float32's
+    and summed in float32, by parts of up to 4096 nodes; those sums' sum, its logarithm
+    and the scores are float64, rounded at the end.  There is no gradient."""
     return BeamChoice(*_operators.beam_select(logits, scores, width, ended, end_token))
 
 

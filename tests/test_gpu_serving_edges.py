@@ -1,5 +1,6 @@
 """Pages and beam search where rounding, masks and lengths are extreme, against their formulas in
 float64 (tests/serving_formulas.py, tests/walk_formulas.py, tests/beam_orders.py)."""
+import math
 import random
 
 import pytest
@@ -131,6 +132,16 @@ def test_choice_far_from_zero(ops, dtype, groups, beams, nodes, width, far):  # 
     gen = torch.Generator().manual_seed(nodes)
     x = (_normal(gen, groups, beams, nodes, std=3.0) + far).to(dtype)
     _choose(ops, x, -torch.rand(groups, beams, generator=gen), width)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nodes", [3, 10, 100, 777, 4097, 50021, 70001])
+def test_scores_are_rounded_once(ops, dtype, nodes):  # noqa: F811
+    """Rows of zeros have sums that float32 holds exactly: what is left is the result's rounding."""
+    scores = -20 * torch.rand(3, 4, generator=torch.Generator().manual_seed(nodes))
+    got = ops.beam_select(torch.zeros(3, 4, nodes, dtype=dtype).cuda(), scores.cuda(), 1)
+    want = scores.double().amax(1) - math.log(nodes)
+    assert ((got.scores[:, 0].cpu().double() - want).abs() <= want.abs() * (2.0 ** -24 + 1e-12)).all()
 
 
 # ---- reordering ----------------------------------------------------------------------------------------
