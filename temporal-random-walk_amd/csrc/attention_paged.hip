@@ -10,9 +10,9 @@
 // all walks are put in one line and dealt out evenly to as many workgroups as the
 // device holds at once.  Where that cuts a walk, its parts are joined by a second
 // launch.  With walks' own workgroups, three of them each, 64 walks of 100 to 4095
-// events (8 heads of 128, 8 bits) took 76.7 us, 67.3 so.  Many walks, and walks of
-// up to 512, have a workgroup each: there is no second launch, and the device
-// evens them out (512 walks of 0 to 511 events: 87 us, dealt out 93).
+// events (8 heads of 128, 8 bits) took 76.7 us, 67.3 so.  Where no walk can be long for
+// its batch, each has a workgroup and there is no second launch: the device evens them
+// out (512 walks of 0 to 511 events in tables of 512, 8 bits: 87 us, dealt out 93).
 //
 // Measured, both launches: 64 walks of 4095 events each, 5.2 TB/s in 16 bits and 4.9 in
 // 8 (a large copy: 5.17).  Of the mixed 64 above, 283 MB and 54.7 us at a copy's rate,
@@ -942,12 +942,22 @@ __global__ __launch_bounds__(kSize) void join_parts_kernel(PagedArgs a) {
 }
 
 // Workgroups of a key head among which all walks are evened out; 0: one a walk.
+// A workgroup takes some 20 ns for each position of a walk that it has alone, and tables say
+// how many that can be.  Evened out there is a second launch, and each workgroup adds up all
+// lengths, 5 ns a walk.  So walks have a workgroup each where none can have more than 512
+// positions, than 128 for each walk that a workgroup's place takes in turn (then one that
+// is that long adds up to 28 %), or than a quarter of the walks' number.  One each and
+// evened out, us in 16 bits with 8 heads of 128: 512 walks of 0 to 511 events, room for
+// 2048, 125 and 133, with one of 100,000 among them 1769 and 217; 512 of 0 to 2000 361 and
+// 366; 1024 of 0 to 1000 370 and 378; 1024 of 0 to 100 and one of 1900 152 and 119; 4096 of
+// 0 to 200 and one of 20,000 940 and 609; 100,000 of 0 to 100, one head of 64, 749 and 1244.
 int even_of(const trw_paged_step_params& p, int resident) {
     const int group = p.heads / p.pages.kv_heads;
     const int64_t heads = int64_t{p.pages.kv_heads} * ((group + kColumns - 1) / kColumns);
-    const int64_t slots = 256 * resident;
-    if (p.pages.table_pages * p.pages.page_rows <= 4 * kUnit * kKeys) return 0;
-    if (p.pages.walks * heads >= 4 * slots) return 0;
+    const int64_t slots = 256 * resident, walks = p.pages.walks;
+    const int64_t room = p.pages.table_pages * p.pages.page_rows;
+    if (room <= std::max({int64_t{4 * kUnit * kKeys}, 128 * walks * heads / slots, walks / 4}))
+        return 0;
     return static_cast<int>(std::max<int64_t>(1, slots / heads));
 }
 int even_of(const trw_paged_step_params& p) {

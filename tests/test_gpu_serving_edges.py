@@ -9,8 +9,8 @@ import torch
 from tests import beam_orders as bo
 from tests import walk_formulas as wf
 from tests.test_cpu_beam_orders import TWO_SHORT
-from tests.test_gpu_serving import (BF, DTYPES, E8, SF, SIZES, Pool, _choose, _normal,  # noqa: F401
-                                    ops)
+from tests.test_gpu_serving import (BF, DTYPES, E8, HF, SF, SIZES, Pool, _choose,  # noqa: F401
+                                    _normal, _step, ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -61,6 +61,14 @@ def test_step_over_infinite_keys(ops, dtype, dim):  # noqa: F811
     want = wf.attention(q[0].double(), k[0].double(), v[0].double(), [(40, 1, 41, seen[None])],
                         dtype=dtype)["out"]
     wf.check("out", out, *want)
+
+
+@pytest.mark.parametrize("dtype,eight", [(BF, False), (HF, True), (SF, False)])
+def test_step_of_a_long_walk_in_a_large_batch(ops, dtype, eight):  # noqa: F811
+    """Enough walks and heads for every place that a device has, several times, and one walk that is
+    longer than they are."""
+    _step(ops, dtype, [(7 * i) % 20 - 1 for i in range(520)] + [550], 560, 8, 8, 16, eight=eight)
+    _step(ops, dtype, [(7 * i) % 20 - 1 for i in range(520)], 520, 8, 8, 16, eight=eight)
 
 
 def test_pages_as_records(ops):  # noqa: F811
