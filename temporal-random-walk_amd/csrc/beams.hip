@@ -7,15 +7,15 @@
 // knows each beam's sum and the best continuation of every chunk, and the `width` best
 // ones are all in the `width` chunks whose best ones come first: of any other chunk's,
 // `width` come before.  Those few chunks are read again, and what reaches the last
-// one's best is ranked by counting.  What follows the chunks' sums is float64
-// (but for the exponentials that join them), for the order of candidates of different
-// beams: scores are 1.05 to 1.12 times as far from 64 bits as their last rounding, with
-// a logarithm of float32 1.25 to 1.7 times.  Lanes hold the same nodes whatever the row's alignment, so that
-// equal rows have equal sums and ties go to the lowest index.
+// one's best is ranked by counting.  What follows the chunks' sums is float64 (but for
+// the exponentials that join them), for the order of candidates of different beams:
+// scores are 1.05 to 1.12 times as far from 64 bits as their last rounding, with a
+// logarithm of float32 1.25 to 1.7 times.  Lanes hold the same nodes whatever the row's
+// alignment, so that equal rows have equal sums and ties go to the lowest index.
 //
 // Measured: 64 groups of 8 beams over 50021 nodes in bfloat16 (51 MB, 9.9 us at a copy's
 // rate) 20.3 us: 12.8 for the sums and 8.6 for the choice, whose few loads follow each
-// other.  Rows in a worse order for it, all equal or ascending, take 32 to 36.  4 groups
+// other.  Rows in a worse order for it, all equal or ascending, take 33 to 38.  4 groups
 // of 4 beams over 4000 nodes are one launch of 8.7 us.
 //
 // Order.  A beam's pages but the last one are full, so beams share them by their table
@@ -282,12 +282,17 @@ __device__ __forceinline__ void sum_chunk(const T* row, const uint8_t* ended, in
 }
 
 // The nodes of a chunk's pieces [first_piece, last_piece) whose logits are `from` or
-// above, `width` best ones at most, as keys; returns how many.
+// above, `width` best ones at most, as keys; returns how many.  Logits whose values
+// off + (logit - top) are one float64 are one logit, so that the lower node comes first.
 template <typename T>
 __device__ __forceinline__ int scan_chunk(const T* row, int nodes, int begin, int first_piece,
-                                          int last_piece, float from, int width, int lane,
-                                          u64* listed) {
+                                          int last_piece, float from, double off, double top,
+                                          int width, int lane, u64* listed) {
     constexpr int kElems = Piece<T>::kElems;
+    auto key_at = [&](float v, uint32_t node) {
+        const double value = off + (static_cast<double>(v) - top);
+        return key_of(static_cast<float>(value - off + top), node);
+    };
     Piece<T> x[kPieces];
     load_chunk(row, nodes, begin, lane, x, first_piece, last_piece);
     int count = 0;
@@ -305,7 +310,7 @@ __device__ __forceinline__ int scan_chunk(const T* row, int nodes, int begin, in
             if (!some) continue;
             if (v >= from)
                 listed[min(count + before_me(some), kListed - 1)] =
-                    key_of(v, begin + (c * 64 + lane) * kElems + e);
+                    key_at(v, begin + (c * 64 + lane) * kElems + e);
             count += __popcll(some);
         }
     }
@@ -323,7 +328,7 @@ __device__ __forceinline__ int scan_chunk(const T* row, int nodes, int begin, in
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int node = first + 64 * i;
-                const u64 key = key_of(v[i], node);
+                const u64 key = key_at(v[i], node);
                 const bool in = node < end && v[i] >= from && key > last;
                 const u64 some = __ballot(in);
                 if (in) listed[count + before_me(some)] = key;
@@ -567,7 +572,7 @@ __device__ __forceinline__ void choose(const SelectArgs& a, int64_t group, const
         u64* listed = s.listed[wave];
         const int found = scan_chunk<T>(row_of<T>(a, group, b), a.nodes, (n - b * a.chunks) * kChunk<T>,
                                         kPieces / shares * share, kPieces / shares * (share + 1),
-                                        from, a.width, lane, listed);
+                                        from, off, top, a.width, lane, listed);
         int place = 0;
         if (lane == 0) place = atomicAdd(&s.count[1], found);  // in any order: they are ranked
         place = __builtin_amdgcn_readfirstlane(place);

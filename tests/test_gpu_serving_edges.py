@@ -143,6 +143,31 @@ def test_choice_far_from_zero(ops, dtype, groups, beams, nodes, width, far):  # 
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nodes,width", [(100, 8), (9000, 5), (50021, 32)])
+@pytest.mark.parametrize("score", [-1e20, -1e30, -3e38])
+def test_choice_among_sums_that_round_to_one(ops, dtype, nodes, width, score):  # noqa: F811
+    """Scores, or a row's maximum, next to which the other logits are lost: equal sums come by their
+    beam, then by their node, whatever their logits are."""
+    gen = torch.Generator().manual_seed(nodes)
+    x = _normal(gen, 2, 3, nodes, dtype=dtype, std=3.0)
+    x[0, 0, 2:] = -math.inf  # the beam that counts has two ways on
+    scores = torch.tensor([[-0.5, score, score], [score, score, score]])
+    got = ops.beam_select(x.cuda(), scores.cuda(), width)
+    rest = list(range(width))
+    best = [0, 1] if x[0, 0, 0] >= x[0, 0, 1] else [1, 0]
+    assert got.tokens.tolist() == [best + rest[:-2], rest]
+    assert got.parents.tolist() == [[0, 0] + [1] * (width - 2), [0] * width]
+    assert (got.scores[:, 2:].cpu() == torch.tensor(score)).all()
+    if abs(score) <= torch.finfo(dtype).max:
+        x[..., nodes - 3] = -score  # of float32 and bfloat16: the rest is 1e20 and more below
+        got = ops.beam_select(x.cuda(), torch.zeros(2, 3).cuda(), width)
+        assert got.tokens.tolist() == [[nodes - 3] * 3 + rest[:2] + rest[:width - 5]] + [
+            [nodes - 3] * 3 + rest[:width - 3]]
+        assert got.parents.tolist() == [[0, 1, 2, 0, 0] + [1] * (width - 5),
+                                        [0, 1, 2] + [0] * (width - 3)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("nodes", [3, 10, 100, 777, 4097, 50021, 70001])
 def test_scores_are_rounded_once(ops, dtype, nodes):  # noqa: F811
     """Rows of zeros have sums that float32 holds exactly: what is left is the result's rounding."""
