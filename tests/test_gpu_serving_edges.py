@@ -71,6 +71,35 @@ def test_step_of_a_long_walk_in_a_large_batch(ops, dtype, eight):  # noqa: F811
     _step(ops, dtype, [(7 * i) % 20 - 1 for i in range(520)], 520, 8, 8, 16, eight=eight)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("cached,capacity", [(100, 128), (700, 768)])
+@pytest.mark.parametrize("low", ["-inf", "lowest"])
+def test_step_of_masked_distances(ops, dtype, eight, cached, capacity, low):  # noqa: F811
+    """A bias that masks some distances, those of the nearest events, and all of them: -inf leaves
+    nothing and the output is 0, the lowest finite value leaves equal weights."""
+    low = -math.inf if low == "-inf" else torch.finfo(SF).min
+    gen = torch.Generator().manual_seed(cached)
+    pool = Pool(ops, 1, capacity, 2, 64, dtype=dtype, eight=eight)
+    q, k, v = (_normal(gen, 1, m, n, 64, dtype=dtype) for m, n in
+               ((1, 4), (cached + 1, 2), (cached + 1, 2)))
+    ops.paged_write(pool.pages, pool.table, None, k[:, :-1].cuda(), v[:, :-1].cuda())
+    held = [pool.held(x[0]) for x in (k, v)]
+    ids = ops.distance_buckets(8, 64, device="cpu")
+    for masked in ([0], [0, 1, 2, 3, 4], [7], [2, 6], range(8)):
+        table = _normal(gen, 4, 8)
+        table[:, list(masked)] = low
+        table[0] = 1.0  # a head that sees everything
+        out = ops.paged_attention_step(q[0].cuda(), k[:, -1].cuda(), v[:, -1].cuda(), pool.pages,
+                                       pool.table, torch.tensor([cached]).cuda(),
+                                       bias_table=table.cuda(), buckets=ids.cuda())
+        want = wf.attention(q[0].double(), *held, wf.documents("causal", [1], [cached + 1]),
+                            table=table.double(), buckets=ids, dtype=dtype)["out"]
+        wf.check("out", out, *want)
+        if low == -math.inf and len(masked) == 8:
+            assert (out[:, 1:] == 0).all()
+
+
 def test_pages_as_records(ops):  # noqa: F811
     """Keys, values and scales of a page in one record hold what they do in memory of their own;
     scales of one memory are refused."""
