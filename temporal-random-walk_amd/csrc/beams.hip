@@ -718,12 +718,13 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
         // children may share a page as well: it takes one child's rows, and later children of
         // other parents read their parents'.
         const uint32_t reads = static_cast<uint32_t>(__ballot(lane < a.beams && held >= at)) & ~childless;
-        bool others = false, again = false;
-        for (int b = 0; b < a.beams; ++b) {
-            const bool same = __builtin_amdgcn_readlane(page, b) == to;
-            others |= same && (reads >> b & 1);
-            again |= same && b != taken;
-        }
+        uint32_t equal = 0;  // beams whose page is this child's
+        for (int b0 = 0; b0 < a.beams; b0 += 8)
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+                equal |= __builtin_amdgcn_readlane(page, b0 + b) == to ? 1u << (b0 + b) : 0u;
+        bool others = equal & reads;
+        const bool again = equal & childless & ~(1u << max(taken, 0));
         if (__builtin_expect((__ballot(again && !others) & these) != 0, 0)) {
             for (u64 b = these; b; b &= b - 1) {
                 const int n = __ffsll(b) - 1;
