@@ -16,11 +16,12 @@
 //
 // Measured, both launches: 64 walks of 4095 events each, 5.2 TB/s in 16 bits and 4.9 in
 // 8 (a large copy: 5.17).  Of the mixed 64 above, 283 MB and 54.7 us at a copy's rate,
-// the walk over the pages takes 64.3 us and the join 4.7; 3 walks of 260k events
-// together, 135 MB and 26.2 us, 39.5 and 7.8.  What is over is the start (four loads
+// the walk over the pages takes 64 to 66 us and the join 4.7; 3 walks of 260k events
+// together, 135 MB and 26.2 us, 39.0 and 7.9.  What is over is the start (four loads
 // one after the other before the first tile, 5 to 7 us) and the second launch.  In 8
-// bits the vector units are busy 0.37 of the time, the matrix units 0.08.  Heads of up
-// to 64 use part of a tile's width: 32 columns in 8 bits read at 2.2 TB/s.
+// bits the vector units are busy 0.37 of the time, the matrix units 0.08.  Tiles are 32,
+// 64 or 128 columns wide, in 8 bits 64 or 128; heads between those use part of one: 32
+// columns in 8 bits read at 2.2 TB/s, 96 in 16 bits at 3.85.
 //
 // v_mfma_f32_16x16x32 with keys as rows leaves lane l with keys 4 (l / 16) .. + 4
 // of column l & 15.  Two halves give eight, which are the B operand of the next
@@ -42,7 +43,8 @@
 //
 // The new row is taken from the call's arguments by the workgroup whose positions
 // include it (in 8 bits as the codes that the pages get), and written to the pages
-// by the walk's first workgroup: no launch and no wait between the two.
+// by the same one (of several for a key head's columns, the first): no launch and no
+// wait between the two.
 #include <algorithm>
 
 #include "pages.h"

@@ -14,9 +14,9 @@
 // alignment, so that equal rows have equal sums and ties go to the lowest index.
 //
 // Measured: 64 groups of 8 beams over 50021 nodes in bfloat16 (51 MB, 9.9 us at a copy's
-// rate) 20.3 us: 12.8 for the sums and 8.6 for the choice, whose few loads follow each
+// rate) 20.6 us: 12.9 for the sums and 8.8 for the choice, whose few loads follow each
 // other.  Rows in a worse order for it, all equal or ascending, take 33 to 38.  4 groups
-// of 4 beams over 4000 nodes are one launch of 8.7 us.
+// of 4 beams over 4000 nodes are one launch of 8.8 us.
 //
 // Order.  A beam's pages but the last one are full, so beams share them by their table
 // alone.  The last page is written to next, so each beam owns its own: a parent's first
@@ -904,7 +904,7 @@ void beam_reorder(const trw_beam_reorder_params& p, hipStream_t stream) {
         }
         // As many workgroups as the device holds at once: 32 groups of 8 beams, 4 caches of
         // 8 heads, 46 MB: 15.2 us with 2048, 17.4 with 1024, 17.5 with 4096 (before pages to
-        // copy to were looked up among other beams': 16.8 with it).
+        // copy to were looked up among other beams': 16.7 with it).
         a.matrices = 2 * count;
         a.heads = heads;
         const int64_t most = static_cast<int64_t>(std::max(1, p.beams - 1)) * a.matrices * heads;
