@@ -262,6 +262,57 @@ __device__ __forceinline__ void in_parts(const float (&x)[8], F (&parts)[kParts]
     }
 }
 
+// Weights as two operands whose sum they are, nearly, and both of which are positive where
+// the weight is, so that an infinity among the values stays one: the first is the greatest
+// number of fewer bits that is less than the weight.  (What is left is 2^-7 of it in
+// bfloat16 and 2^-10 in float16 at most, and rounded to half a step of as many bits; in
+// float16 both are its smallest number or more, 2^-39 of the largest weight.)
+__device__ __forceinline__ void in_positive_parts(const float (&x)[8], bf16x8 (&parts)[2]) {
+    union {
+        uint32_t u[4];
+        bf16x8 f;
+    } high;
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        uint32_t bits[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t all = __float_as_uint(x[e + i]);
+            bits[i] = (all - min(all, 1u)) & 0xffff0000u;
+            rest[e + i] = x[e + i] - __uint_as_float(bits[i]);
+        }
+        high.u[e / 2] = bits[0] >> 16 | bits[1];
+    }
+    parts[0] = high.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) parts[1][e] = static_cast<__bf16>(rest[e]);
+}
+__device__ __forceinline__ void in_positive_parts(const float (&x)[8], f16x8 (&parts)[2]) {
+    typedef __fp16 h16x2 __attribute__((ext_vector_type(2)));
+    union {
+        h16x2 h[4];
+        f16x8 f;
+    } high;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float below[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t all = __float_as_uint(x[e + i]);
+            below[i] = __uint_as_float(all - min(all, 1u));
+            if (x[e + i] > 0.0f) below[i] = fmaxf(below[i], 0x1p-24f);
+        }
+        high.h[e / 2] = __builtin_amdgcn_cvt_pkrtz(below[0], below[1]);  // towards 0
+    }
+    parts[0] = high.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float rest = x[e] - static_cast<float>(high.f[e]);
+        parts[1][e] = static_cast<_Float16>(x[e] > 0.0f ? fmaxf(rest, 0x1p-24f) : rest);
+    }
+}
+
 // A pointer that is the same in every lane, as a scalar.
 __device__ __forceinline__ const char* uniform(const char* p) {
     const uint64_t at = reinterpret_cast<uint64_t>(p);
@@ -569,9 +620,8 @@ void paged_step_kernel(PagedArgs a) {
         const ArgsAgain g = args_again();
         fetch(s, g->pages.v, g->pages.v_page, j0, at_v);
     };
-    // The new row takes its place in the wave's tiles, and every place after it, and goes
-    // to its page.
-    auto put_new = [&](int from, int page, int at_lane) {
+    // The new row takes its place in the wave's tiles, and goes to its page.
+    auto put_new = [&](int row, int page, int at_lane) {
         const ArgsAgain g = args_again();
         const T* fresh_k = reinterpret_cast<const T*>(g->k.data) + static_cast<int64_t>(b) * g->k.row +
                            kv_head * g->k.head;
@@ -598,13 +648,13 @@ void paged_step_kernel(PagedArgs a) {
             const int byte_v = scale_byte(group_max<16>(v_top));
             const u32x2 codes_k = eight_codes(k, inverse_power(byte_k));
             const u32x2 codes_v = eight_codes(v, inverse_power(byte_v));
-            for (int row = from + (at_lane >> 4); row < kKeys; row += 4) {
-                if (at < G::kSlots * 2) {
-                    const int byte = G::slot(row, at >> 1) * 16 + (at & 1) * 8;
-                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_k) + byte) = codes_k;
-                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_v) + byte) = codes_v;
-                }
-                uint8_t* scales = reinterpret_cast<uint8_t*>(s_scales[wave]);
+            if (at_lane < 16 && at < G::kSlots * 2) {
+                const int byte = G::slot(row, at >> 1) * 16 + (at & 1) * 8;
+                *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_k) + byte) = codes_k;
+                *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(s_v) + byte) = codes_v;
+            }
+            uint8_t* scales = reinterpret_cast<uint8_t*>(s_scales[wave]);
+            if (at_lane == 0) {
                 scales[row] = byte_k;
                 scales[32 + row] = byte_v;
             }
@@ -619,11 +669,10 @@ void paged_step_kernel(PagedArgs a) {
         } else {
             const u32x4* k_from = reinterpret_cast<const u32x4*>(fresh_k);
             const u32x4* v_from = reinterpret_cast<const u32x4*>(fresh_v);
-            for (int c = from * G::kSlots + at_lane; c < kKeys * G::kSlots; c += 64) {
-                const int row = c / G::kSlots, chunk = c % G::kSlots;
-                const int at = chunk * G::kElems < dim ? chunk : 0;
-                s_k[G::slot(row, chunk)] = k_from[at];
-                s_v[G::slot(row, chunk)] = v_from[at];
+            if (at_lane < G::kSlots) {
+                const int at = at_lane * G::kElems < dim ? at_lane : 0;
+                s_k[G::slot(row, at_lane)] = k_from[at];
+                s_v[G::slot(row, at_lane)] = v_from[at];
             }
             if (writes && at_lane * G::kElems < dim) {
                 reinterpret_cast<u32x4*>(k_row)[at_lane] = k_from[at_lane];
@@ -668,11 +717,12 @@ void paged_step_kernel(PagedArgs a) {
             copies_landed<kCopies>();  // keys; the values, asked for last, may be on their way
             if (seen != 0xffffffffu || news) {
                 copies_landed<0>();
-                // Values of rows that are not seen meet a weight of 0: they may not be NaN.
+                // Values of rows that are not seen meet a weight of 0: they may not be NaN,
+                // nor infinite.
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (span[h].hi <= span[h].lo)
-                        for (int c = at_lane; c < kHalf * G::kSlots; c += 64)
+                    for (int c = at_lane; c < kHalf * G::kSlots; c += 64)
+                        if (c / G::kSlots < span[h].lo || c / G::kSlots >= span[h].hi)
                             s_v[h * kHalf * G::kSlots + c] = u32x4{0, 0, 0, 0};
                 if (news) {
                     const int page = n - j0 < kHalf ? span[0].page : span[1].page;
@@ -806,7 +856,8 @@ void paged_step_kernel(PagedArgs a) {
                 }
             }
             F p[kWeights];
-            in_parts<kWeights>(s, p);
+            if constexpr (kEight || sizeof(T) == 4) in_parts<kWeights>(s, p);
+            else in_positive_parts(s, p);
             if (more) copies_landed<kCopies>();  // values; the next keys may be on their way
             else copies_landed<0>();
 #pragma unroll

@@ -135,6 +135,39 @@ def test_pages_as_records(ops):  # noqa: F811
             call()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [40, 64, 128])
+@pytest.mark.parametrize("capacity", [128, 768])
+def test_step_over_infinite_values(ops, dtype, dim, capacity):  # noqa: F811
+    """An infinity among the values that are seen makes its column that infinity, whatever its weight is
+    and wherever it lies, beside rows that are not seen too; other columns are as without it."""
+    gen = torch.Generator().manual_seed(dim)
+    lens, first = [100, 17, 64, 0, 40, 95], [0, 5, 33, 0, 40, 50]
+    walks = len(lens)
+    pool = Pool(ops, walks, capacity, 1, dim, dtype=dtype)
+    q, k, v = (_normal(gen, walks, m, 1, dim, dtype=dtype) for m in (1, 101, 101))
+    # the new event, the first and the last one that are cached; -26 and -40 are weights of 2^-38 and 2^-58
+    spots = [(w, j, c) for w in range(walks) for c, j in enumerate((lens[w], first[w], lens[w] - 1))
+             if j >= first[w]] + [(0, 50, 3), (0, 51, 4)]
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[0, 50, 0, 0], k[0, 51, 0, 0] = -26.0 * dim ** 0.5, -40.0 * dim ** 0.5
+
+    def run(x):
+        ops.paged_write(pool.pages, pool.table, None, k.cuda(), x.cuda(),
+                        counts=torch.tensor(lens).cuda())
+        new_k, new_v = (torch.stack([y[w, n] for w, n in enumerate(lens)]).cuda() for y in (k, x))
+        return ops.paged_attention_step(q[:, 0].cuda(), new_k, new_v, pool.pages, pool.table,
+                                        torch.tensor(lens).cuda(), first=torch.tensor(first).cuda())
+
+    fine = run(v)
+    assert torch.isfinite(fine).all()
+    for sign in (1, -1):
+        x, want = v.clone(), fine.clone()
+        for w, j, c in spots:
+            x[w, j, 0, c] = want[w, 0, c] = sign * math.inf
+        assert torch.equal(run(x), want)
+
+
 # ---- choice among beams -----------------------------------------------------------------------------
 LOWS = [-(10.0 ** n) for n in range(3, 38)]
 
