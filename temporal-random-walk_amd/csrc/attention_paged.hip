@@ -16,12 +16,12 @@
 //
 // Measured, both launches: 64 walks of 4095 events each, 5.2 TB/s in 16 bits and 4.9 in
 // 8 (a large copy: 5.17).  Of the mixed 64 above, 283 MB and 54.7 us at a copy's rate,
-// the walk over the pages takes 64 to 66 us and the join 4.7; 3 walks of 260k events
-// together, 135 MB and 26.2 us, 39.0 and 7.9.  What is over is the start (four loads
+// the walk over the pages takes 64.5 us and the join 4.9; 3 walks of 260k events
+// together, 135 MB and 26.2 us, 38.8 and 8.1.  What is over is the start (four loads
 // one after the other before the first tile, 5 to 7 us) and the second launch.  In 8
 // bits the vector units are busy 0.37 of the time, the matrix units 0.08.  Tiles are 32,
 // 64 or 128 columns wide, in 8 bits 64 or 128; heads between those use part of one: 32
-// columns in 8 bits read at 2.2 TB/s, 96 in 16 bits at 3.85.
+// columns in 8 bits read at 2.2 TB/s, 96 in 16 bits at 3.9.
 //
 // v_mfma_f32_16x16x32 with keys as rows leaves lane l with keys 4 (l / 16) .. + 4
 // of column l & 15.  Two halves give eight, which are the B operand of the next
